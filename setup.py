@@ -24,6 +24,10 @@ NVCC_FLAGS = [
 if os.environ.get("FT_KERNEL_CHECKS") == "1":
     NVCC_FLAGS.append("-DFT_KERNEL_CHECKS")
 
+# the C++ runtime that torch uses, even where the compiler ships only a static one: a second
+# copy inside the extension crashes when an error message formats a number
+LINK_FLAGS = ["-l:libstdc++.so.6"]
+
 sources = sorted(glob.glob(os.path.join(CSRC, "*.cu"))) + sorted(glob.glob(os.path.join(CSRC, "*.cpp")))
 
 setup(
@@ -36,6 +40,7 @@ setup(
             sources=sources,
             include_dirs=[os.path.join(HERE, CSRC)],
             extra_compile_args={"cxx": ["-O3", "-std=c++17"], "nvcc": NVCC_FLAGS},
+            extra_link_args=LINK_FLAGS,
         )
     ],
     cmdclass={"build_ext": BuildExtension.with_options(use_ninja=True)},

@@ -79,6 +79,20 @@ void flash_fwd_variant(const torch::Tensor& qkv, torch::Tensor& o, torch::Tensor
 void flash_bwd(const torch::Tensor& qkv, const torch::Tensor& o, const torch::Tensor& dout,
                const torch::Tensor& lse, torch::Tensor& dqkv, int64_t B, int64_t S, int64_t nq,
                int64_t nkv, int64_t D, torch::Tensor& err);
+void act8_quantize(const torch::Tensor& x, torch::Tensor& q, torch::Tensor& scale, int64_t group);
+void act8_dequantize(const torch::Tensor& q, const torch::Tensor& scale, torch::Tensor& x, int64_t group);
+void act8_rms_norm(const torch::Tensor& x, const torch::Tensor& w, torch::Tensor& y, torch::Tensor& rstd,
+                   torch::Tensor& q, torch::Tensor& scale, int64_t group, double eps);
+int64_t act8_norm_walkers(int64_t rows, int64_t H);
+void act8_rms_norm_bwd(const torch::Tensor& dy, const torch::Tensor& q, const torch::Tensor& scale,
+                       const torch::Tensor& w, const torch::Tensor& rstd, torch::Tensor& dx, torch::Tensor& y8,
+                       torch::Tensor& dw, torch::Tensor& part, int64_t group);
+void act8_swiglu(const torch::Tensor& gu, torch::Tensor& h, torch::Tensor& q, torch::Tensor& scale, int64_t group);
+void act8_swiglu_bwd(const torch::Tensor& dh, const torch::Tensor& q, const torch::Tensor& scale,
+                     torch::Tensor& dgu, torch::Tensor& h8, int64_t group);
+void rotary_qk(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& cos_t,
+               const torch::Tensor& sin_t, const c10::optional<torch::Tensor>& pos, torch::Tensor& oq,
+               torch::Tensor& ok, bool interleaved, bool inverse, torch::Tensor& err);
 }  // namespace ft
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -121,4 +135,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("flash_fwd", &ft::flash_fwd);
   m.def("flash_fwd_variant", &ft::flash_fwd_variant);
   m.def("flash_bwd", &ft::flash_bwd);
+  m.def("act8_quantize", &ft::act8_quantize, "groups of a row to int8 codes and fp32 scales");
+  m.def("act8_dequantize", &ft::act8_dequantize);
+  m.def("act8_rms_norm", &ft::act8_rms_norm, "RMSNorm that also keeps its input in 8 bits");
+  m.def("act8_norm_walkers", &ft::act8_norm_walkers, "rows of the act8_rms_norm_bwd workspace");
+  m.def("act8_rms_norm_bwd", &ft::act8_rms_norm_bwd, "RMSNorm backward from the 8-bit input");
+  m.def("act8_swiglu", &ft::act8_swiglu, "SwiGLU that also keeps gate and up in 8 bits");
+  m.def("act8_swiglu_bwd", &ft::act8_swiglu_bwd, "SwiGLU backward from 8-bit gate and up");
+  m.def("rotary_qk", &ft::rotary_qk, "rotary positions of q and k, half or interleaved");
 }

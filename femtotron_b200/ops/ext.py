@@ -16,10 +16,11 @@ _IMPORT_ERROR: Exception | None = None
 LAUNCHES = [0]
 
 # Kernels launched per call of an entry point when it is not exactly one: the flash backward
-# runs three (delta/LSE pre-pass, main, fp32 -> bf16 convert); the memory-management and
-# stream-memory-operation entry points launch none (copy engines, cuStreamWriteValue32).
+# runs three (delta/LSE pre-pass, main, fp32 -> bf16 convert), the 8-bit RMSNorm backward two
+# (main, weight-gradient sum); the memory-management and stream-memory-operation entry points
+# launch none (copy engines, cuStreamWriteValue32).
 KERNELS_PER_CALL = {
-    "flash_bwd": 3,
+    "flash_bwd": 3, "act8_rms_norm_bwd": 2, "act8_norm_walkers": 0,
     "symm_alloc": 0, "ipc_handle": 0, "ipc_open": 0, "ipc_close": 0, "tensor_at": 0,
     "copy_from_ptrs": 0, "stream_write": 0,
 }

@@ -93,6 +93,14 @@ void act8_swiglu_bwd(const torch::Tensor& dh, const torch::Tensor& q, const torc
 void rotary_qk(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& cos_t,
                const torch::Tensor& sin_t, const c10::optional<torch::Tensor>& pos, torch::Tensor& oq,
                torch::Tensor& ok, bool interleaved, bool inverse, torch::Tensor& err);
+std::vector<torch::Tensor> linear_xent_fwd(const torch::Tensor& h, const torch::Tensor& w,
+                                           const torch::Tensor& labels, int64_t vstart, int64_t ignore_index,
+                                           int64_t reduce, torch::Tensor& err);
+int64_t linear_xent_bwd(const torch::Tensor& h, const torch::Tensor& w, const torch::Tensor& labels,
+                        const torch::Tensor& lse, const torch::Tensor& grad, const torch::Tensor& factor,
+                        const c10::optional<torch::Tensor>& dh, const c10::optional<torch::Tensor>& dw,
+                        bool accumulate, int64_t vstart, int64_t ignore_index, int64_t workspace_bytes,
+                        torch::Tensor& err);
 }  // namespace ft
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -142,5 +150,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("act8_rms_norm_bwd", &ft::act8_rms_norm_bwd, "RMSNorm backward from the 8-bit input");
   m.def("act8_swiglu", &ft::act8_swiglu, "SwiGLU that also keeps gate and up in 8 bits");
   m.def("act8_swiglu_bwd", &ft::act8_swiglu_bwd, "SwiGLU backward from 8-bit gate and up");
+  m.def("linear_xent_fwd", &ft::linear_xent_fwd, "cross entropy of a linear head without its logits");
+  m.def("linear_xent_bwd", &ft::linear_xent_bwd, "its gradients, in pieces of the vocabulary");
   m.def("rotary_qk", &ft::rotary_qk, "rotary positions of q and k, half or interleaved");
 }

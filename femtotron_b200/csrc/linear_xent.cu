@@ -1,0 +1,548 @@
+// Softmax cross entropy of a linear head, x = h W^T, without the logits in memory (sm_100a).
+//
+//   lse_t = log sum_j exp x_tj,   loss_t = lse_t - x_t,label     (0 where the label is ignored)
+//   d_tj  = g_t (exp(x_tj - lse_t) - [j = label_t]),   dh = d W,   dW = d^T h
+//
+// Forward: the tcgen05 GEMM of gemm_core.cuh whose epilogue reduces each 256-column tile of
+// fp32 logits to (max, sum of exponentials) per row; a second kernel joins the tiles of a row.
+// The logits leave TMEM only as those two numbers.
+// Backward, in pieces of the vocabulary so that the workspace stays bounded: the product again,
+// with an epilogue that turns the fp32 logits into d (bf16, [T, piece]), then dW of the
+// piece's rows and the piece's share of dh from it.  The fourth product is the price of not
+// keeping the logits.
+//
+// d is rounded to bf16 because the tensor cores take it as an operand.  It is stored
+// without the upstream gradient's common factor, which is applied in fp32 to the products: the
+// entry of the label, close to -1, then keeps its leading digits exactly.
+// dh is summed over the pieces in fp32.  A product with too few tiles for the GPU (dh of a short
+// batch, whose sum runs over the vocabulary) is split over the sum into partial outputs that a
+// last kernel adds in a fixed order: no atomics, the same bits on every run.
+#include "gemm_core.cuh"
+
+namespace ft {
+namespace gemm {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// The tensor cores add each 16-deep step into their fp32 accumulator with truncation, which
+// draws a sum of n steps towards zero: a step loses a constant share a of the partial sum so far,
+// and partial sums that grow evenly (a run of like signs, or a random walk, in the mean) make
+// that a n / 2 of the result.  Measured against 64-bit products, a / 2 = 1.2e-8 (H = 64) to 1.54e-8
+// (H = 8192), 1.49e-8 = 2^-26 at H = 4096, where the loss was 2.0e-6 too small.  The logits of
+// both passes are therefore multiplied by 1 + 2^-26 n, folded into constants of the epilogues.
+__device__ __forceinline__ float untruncate(int K) {
+  return 1.f + 1.4901161e-8f * static_cast<float>((K + 15) / 16);
+}
+
+// (max, sum exp(x - max)) of a row's logits in this tile, and the label's logit.
+struct XentStatsEpi {
+  struct Args {
+    const int64_t* labels;
+    float2* part;   // [T, tiles_n]
+    float* target;  // [T]
+    int64_t vstart;
+    int tiles_n;
+  };
+  static constexpr bool kSplitK = false;
+  static constexpr bool kScales = false;
+  __device__ __forceinline__ static float f32_scale(const Args&) { return 1.f; }
+  template <int BN>
+  __device__ __forceinline__ static void tile(const Params& p, const Args& e, uint32_t tmem_acc, int q,
+                                              int lane, int row, int n0, int tn, int, bool) {
+    const bool row_ok = row < p.M;
+    const uint32_t tbase = tmem_acc + (static_cast<uint32_t>(q * 32) << 16);
+    int64_t at = -1;  // the label's column in this tile
+    if (row_ok) at = e.labels[row] - e.vstart - n0;
+    float m = -INFINITY, s = 0.f, tgt = 0.f;
+    const float fix = untruncate(p.K), unit = kLog2e * fix;
+#pragma unroll 1
+    for (int c = 0; c < BN / 32; ++c) {
+      const int valid = p.N - n0 - c * 32;
+      if (valid <= 0) break;  // the same for the whole warp
+      uint32_t r[32];
+      tmem_ld_32x32b_x32(tbase + c * 32, r);
+      tmem_wait_ld();
+      float v[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+      if (valid < 32) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (i >= valid) v[i] = -INFINITY;
+      }
+      const int64_t off = at - c * 32;
+      const bool hit = off >= 0 && off < 32 && off < valid;
+      if (__any_sync(0xffffffffu, hit)) {  // rare: V / 32 chunks, 32 labels
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (hit && off == i) tgt = v[i];
+      }
+      float m0 = v[0], m1 = v[1], m2 = v[2], m3 = v[3];
+#pragma unroll
+      for (int i = 4; i < 32; i += 4) {
+        m0 = fmaxf(m0, v[i]); m1 = fmaxf(m1, v[i + 1]);
+        m2 = fmaxf(m2, v[i + 2]); m3 = fmaxf(m3, v[i + 3]);
+      }
+      const float nm = fmaxf(m, fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)));
+      // a row of nothing but -inf keeps its sum at 0; NaN makes the sum NaN
+      const float base = nm == -INFINITY ? 0.f : nm * unit;
+      float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+#pragma unroll
+      for (int i = 0; i < 32; i += 4) {
+        s0 += ex2_approx(fmaf(v[i], unit, -base));
+        s1 += ex2_approx(fmaf(v[i + 1], unit, -base));
+        s2 += ex2_approx(fmaf(v[i + 2], unit, -base));
+        s3 += ex2_approx(fmaf(v[i + 3], unit, -base));
+      }
+      s = s * ex2_approx(fmaf(m, unit, -base)) + ((s0 + s1) + (s2 + s3));
+      m = nm;
+    }
+    if (row_ok) {
+      e.part[(int64_t)row * e.tiles_n + tn] = make_float2(m * fix, s);
+      if (at >= 0 && at < BN && at < p.N - n0) e.target[row] = tgt * fix;
+    }
+  }
+};
+
+// d (without the common factor) of this tile in bf16.
+struct XentGradEpi {
+  struct Args {
+    const int64_t* labels;
+    const float* lse;      // [T]
+    const float* weight;   // [T] relative row weights, or null: 1, and 0 where ignored
+    int64_t vstart;        // of this piece
+    int64_t ignore_index;
+  };
+  static constexpr bool kSplitK = false;
+  static constexpr bool kScales = false;
+  __device__ __forceinline__ static float f32_scale(const Args&) { return 1.f; }
+  template <int BN>
+  __device__ __forceinline__ static void tile(const Params& p, const Args& e, uint32_t tmem_acc, int q,
+                                              int lane, int row, int n0, int, int, bool) {
+    const bool row_ok = row < p.M;
+    const uint32_t tbase = tmem_acc + (static_cast<uint32_t>(q * 32) << 16);
+    int64_t at = -1;
+    float base = 0.f, g = 0.f;
+    const float unit = kLog2e * untruncate(p.K);
+    if (row_ok) {
+      const int64_t lab = e.labels[row];
+      at = lab - e.vstart - n0;
+      g = lab == e.ignore_index ? 0.f : (e.weight ? e.weight[row] : 1.f);
+      base = e.lse[row] * kLog2e;
+    }
+#pragma unroll 1
+    for (int c = 0; c < BN / 32; ++c) {
+      const int valid = p.N - n0 - c * 32;
+      if (valid <= 0) break;
+      uint32_t r[32];
+      tmem_ld_32x32b_x32(tbase + c * 32, r);
+      tmem_wait_ld();
+      float v[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = ex2_approx(fmaf(__uint_as_float(r[i]), unit, -base));
+      const int64_t off = at - c * 32;
+      const bool hit = off >= 0 && off < 32;
+      if (__any_sync(0xffffffffu, hit)) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (hit && off == i) v[i] -= 1.f;
+      }
+      if (row_ok) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = g == 0.f ? 0.f : v[i] * g;  // an ignored row's NaN stays out
+        // rows of D are padded to whole 32-column chunks
+        store_bf16x32(reinterpret_cast<__nv_bfloat16*>(p.D) + (int64_t)row * p.ldd + n0 + c * 32, v, 32);
+      }
+    }
+  }
+};
+
+// The products with d: scaled by the common factor a[0] * b[0], optionally split over K.
+struct XentProductEpi {
+  struct Args {
+    const float* a;  // null: no factor
+    const float* b;
+    int ksplit;
+  };
+  static constexpr bool kSplitK = true;
+  static constexpr bool kScales = true;
+  __device__ __forceinline__ static float f32_scale(const Args& e) {
+    return e.a ? e.a[0] * e.b[0] : 1.f;
+  }
+  template <int BN>
+  __device__ __forceinline__ static void tile(const Params& p, const Args& e, uint32_t tmem_acc, int q,
+                                              int lane, int row, int n0, int, int split, bool) {
+    const bool row_ok = row < p.M;
+    const uint32_t tbase = tmem_acc + (static_cast<uint32_t>(q * 32) << 16);
+    const float scale = f32_scale(e);
+    const int64_t at = ((int64_t)split * p.split_rows + row) * p.ldd;
+#pragma unroll 1
+    for (int c = 0; c < BN / 32; ++c) {
+      const int col0 = n0 + c * 32;
+      const int valid = min(32, p.N - col0);
+      if (valid <= 0) break;
+      uint32_t r[32];
+      tmem_ld_32x32b_x32(tbase + c * 32, r);
+      tmem_wait_ld();
+      float v[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]) * scale;
+      if (!row_ok) {
+      } else if (p.mode == EPI_STORE_BF16 || p.mode == EPI_ACC_BF16) {
+        __nv_bfloat16* d = reinterpret_cast<__nv_bfloat16*>(p.D) + at + col0;
+        if (p.mode == EPI_ACC_BF16) {
+          float o[32];
+          load_bf16x32(d, o, valid);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] += o[i];
+        }
+        store_bf16x32(d, v, valid);
+      } else {
+        float4* d4 = reinterpret_cast<float4*>(reinterpret_cast<float*>(p.D) + at + col0);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (j * 4 < valid) {
+            float4 x = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+            if (p.mode == EPI_ACC_F32) {
+              const float4 o = d4[j];
+              x.x += o.x; x.y += o.y; x.z += o.z; x.w += o.w;
+            }
+            d4[j] = x;
+          }
+        }
+      }
+    }
+  }
+};
+
+// ------------------------------------------------------------------ small kernels
+// One warp per row joins the tiles' (max, sum); stats[row] = (max, sum, target, has target).
+__global__ void __launch_bounds__(256) xent_join_kernel(const float2* __restrict__ part,
+                                                        const float* __restrict__ target,
+                                                        const int64_t* __restrict__ labels,
+                                                        float4* __restrict__ stats, float* __restrict__ lse,
+                                                        float* __restrict__ losses, int T, int tiles_n,
+                                                        int64_t vstart, int64_t V, int64_t ignore_index) {
+  const int row = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (row >= T) return;
+  const float2* p = part + (int64_t)row * tiles_n;
+  float m = -INFINITY, s = 0.f;
+  for (int i = lane; i < tiles_n; i += 32) {
+    const float2 v = p[i];
+    const float nm = fmaxf(m, v.x);
+    const float base = nm == -INFINITY ? 0.f : nm * kLog2e;
+    s = s * exp2f(fmaf(m, kLog2e, -base)) + v.y * exp2f(fmaf(v.x, kLog2e, -base));
+    m = nm;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float om = __shfl_xor_sync(0xffffffffu, m, o), os = __shfl_xor_sync(0xffffffffu, s, o);
+    const float nm = fmaxf(m, om);
+    const float base = nm == -INFINITY ? 0.f : nm * kLog2e;
+    s = s * exp2f(fmaf(m, kLog2e, -base)) + os * exp2f(fmaf(om, kLog2e, -base));
+    m = nm;
+  }
+  if (lane == 0) {
+    const int64_t lab = labels[row];
+    const bool has = lab >= vstart && lab < vstart + V;
+    const float tgt = has ? target[row] : 0.f;
+    const float l = m + logf(s);
+    stats[row] = make_float4(m, s, tgt, has ? 1.f : 0.f);
+    lse[row] = l;
+    // a label that no column answers to has no probability: its loss is not a number
+    losses[row] = lab == ignore_index ? 0.f : has ? l - tgt : __int_as_float(0x7fffffff);
+  }
+}
+
+// out = {sum of losses (divided by the number of rows that count, for `mean`), the factor of
+// its gradient: 1, or 1 / that number (0 for none)}: one block, a fixed order.
+__global__ void __launch_bounds__(1024) xent_total_kernel(const float* __restrict__ losses,
+                                                          const int64_t* __restrict__ labels,
+                                                          float* __restrict__ out, int T,
+                                                          int64_t ignore_index, int mean) {
+  __shared__ float ls[32];
+  __shared__ int ns[32];
+  float s = 0.f;
+  int n = 0;
+  for (int i = threadIdx.x; i < T; i += 1024) {
+    s += losses[i];
+    n += labels[i] != ignore_index;
+  }
+  s = warp_sum(s);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+  if (threadIdx.x % 32 == 0) { ls[threadIdx.x / 32] = s; ns[threadIdx.x / 32] = n; }
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    s = warp_sum(ls[threadIdx.x]);
+    n = ns[threadIdx.x];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    if (threadIdx.x == 0) {
+      out[0] = mean ? s / n : s;  // none that counts: 0 / 0, as the mean of nothing
+      out[1] = !mean ? 1.f : n ? 1.f / n : 0.f;
+    }
+  }
+}
+
+// Row gradients -> their largest magnitude (the common factor) and weights relative to it.
+__global__ void __launch_bounds__(1024) xent_weights_kernel(const float* __restrict__ g, float* __restrict__ weight,
+                                                            float* __restrict__ factor, int T) {
+  __shared__ float red[32];
+  float m = 0.f;
+  for (int i = threadIdx.x; i < T; i += 1024) m = fmaxf(m, fabsf(g[i]));
+  m = warp_max(m);
+  if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = m;
+  __syncthreads();
+  m = warp_max(red[threadIdx.x % 32]);
+  for (int i = threadIdx.x; i < T; i += 1024) weight[i] = m > 0.f ? g[i] / m : 0.f;
+  if (threadIdx.x == 0) { factor[0] = m; factor[1] = 1.f; }
+}
+
+// dh = factor * sum of the partial products, in order.
+__global__ void __launch_bounds__(256) xent_dh_kernel(const float* __restrict__ part, __nv_bfloat16* __restrict__ dh,
+                                                      const float* __restrict__ a, const float* __restrict__ b,
+                                                      int64_t quads, int64_t stride, int splits, int H4,
+                                                      int64_t lddh) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= quads) return;
+  const float f = a[0] * b[0];
+  float4 s = reinterpret_cast<const float4*>(part)[i];
+  for (int k = 1; k < splits; ++k) {
+    const float4 v = reinterpret_cast<const float4*>(part + k * stride)[i];
+    s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+  }
+  const int64_t row = i / H4;
+  const int c = static_cast<int>(i - row * H4) * 4;
+  *reinterpret_cast<uint2*>(dh + row * lddh + c) =
+      make_uint2(pack_bf16x2(s.x * f, s.y * f), pack_bf16x2(s.z * f, s.w * f));
+}
+
+// ------------------------------------------------------------------ host side
+constexpr auto kBF16 = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+
+static Params base_params(int M, int N, int K, torch::Tensor& err) {
+  Params p{};
+  p.M = M; p.N = N; p.K = K;
+  p.group_m = 8;
+  p.err = err.data_ptr<int>();
+  p.gate_row_elems = p.gate_chunk_elems = 1;
+  return p;
+}
+
+// x = h W^T into an epilogue (W: rows [v0, v0 + N) of the head).
+template <class Epi>
+static void logits_gemm(const torch::Tensor& h, const torch::Tensor& w, int64_t v0, int N, Params p,
+                        typename Epi::Args e, int bn, cudaStream_t st) {
+  const int T = h.size(0), H = h.size(1);
+  const bool pair = T > 128;
+  const auto* wp = reinterpret_cast<const __nv_bfloat16*>(w.data_ptr()) + v0 * w.stride(0);
+  CUtensorMap ta = make_tmap_2d(h.data_ptr(), kBF16, 2, H, T, h.stride(0), 64, 128, true);
+  CUtensorMap tb = make_tmap_2d(wp, kBF16, 2, H, N, w.stride(0), 64, pair ? bn / 2 : bn, true);
+  const int tiles = (T + (pair ? 255 : 127)) / (pair ? 256 : 128) * ((N + bn - 1) / bn);
+  if (pair) launch_pair<false, false, 256, Epi>(ta, tb, ta, p, tiles, st, e);
+  else if (bn == 256) launch<false, false, 256, 4, Epi>(ta, tb, p, tiles, st, e);
+  else launch<false, false, 128, 6, Epi>(ta, tb, p, tiles, st, e);
+}
+
+static int logits_bn(int T, int N) { return T > 128 ? 256 : (N > 128 * num_sms() ? 256 : 128); }
+
+// D = d W (a_mn false, D fp32 partials) or d^T h (a_mn true).
+template <bool A_MN>
+static void product(const void* A, int64_t lda, const void* B, int64_t ldb, int M, int N, int K, void* D,
+                    int64_t ldd, int mode, int ksplit, int split_rows, const float* fa, const float* fb,
+                    torch::Tensor& err, cudaStream_t st) {
+  Params p = base_params(M, N, K, err);
+  p.D = D;
+  p.ldd = ldd;
+  p.mode = mode;
+  p.split_rows = split_rows;
+  XentProductEpi::Args e{fa, fb, ksplit};
+  const bool pair = M > 128 && N > 128;
+  const bool f32 = mode == EPI_STORE_F32 || mode == EPI_ACC_F32;
+  int bn = N > 128 ? 256 : 128;
+  const long units = pair ? num_sms() / 2 : num_sms(), tm = (M + (pair ? 255 : 127)) / (pair ? 256 : 128);
+  if (bn == 256 && ksplit == 1) {  // the narrow tile where it fills the last wave better
+    const long kb = (K + BK - 1) / BK;
+    const long c256 = (tm * ((N + 255) / 256) + units - 1) / units * (256 * kb + 2048);
+    const long c128 = (tm * ((N + 127) / 128) + units - 1) / units * (128 * kb + 2048);
+    if (c128 * 105 < c256 * 100) bn = 128;
+  }
+  CUtensorMap ta = A_MN ? make_tmap_2d(A, kBF16, 2, M, K, lda, 64, 64, true)
+                        : make_tmap_2d(A, kBF16, 2, K, M, lda, 64, 128, true);
+  CUtensorMap tb = make_tmap_2d(B, kBF16, 2, N, K, ldb, 64, 64, true);
+  const int tiles = static_cast<int>(tm) * ((N + bn - 1) / bn) * ksplit;
+  if (pair) {
+    CUtensorMap td = f32 ? make_tmap_2d(D, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, N,
+                                        ksplit == 1 ? M : (uint64_t)ksplit * split_rows, ldd, 32, 32, true)
+                         : ta;
+    if (bn == 256) launch_pair<A_MN, true, 256, XentProductEpi>(ta, tb, td, p, tiles, st, e);
+    else launch_pair<A_MN, true, 128, XentProductEpi>(ta, tb, td, p, tiles, st, e);
+  } else if (bn == 256) {
+    launch<A_MN, true, 256, 4, XentProductEpi>(ta, tb, p, tiles, st, e);
+  } else {
+    launch<A_MN, true, 128, 6, XentProductEpi>(ta, tb, p, tiles, st, e);
+  }
+}
+
+static void check_operands(const torch::Tensor& h, const torch::Tensor& w, const torch::Tensor& labels,
+                           const torch::Tensor& err) {
+  TORCH_CHECK(h.dim() == 2 && w.dim() == 2, "linear_xent: h and w must be matrices");
+  TORCH_CHECK(h.size(1) == w.size(1) && h.size(1) >= 8 && h.size(1) % 8 == 0,
+              "linear_xent: h and w must agree in a hidden size that is a multiple of 8, got ", h.size(1), " and ",
+              w.size(1));
+  for (const torch::Tensor* t : {&h, &w})
+    TORCH_CHECK(t->is_cuda() && t->scalar_type() == at::kBFloat16 && t->stride(1) == 1 &&
+                    t->stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0,
+                "linear_xent: h and w must be bf16 CUDA matrices with 16-byte aligned rows");
+  TORCH_CHECK(labels.is_cuda() && labels.scalar_type() == at::kLong && labels.dim() == 1 && labels.is_contiguous() &&
+                  labels.size(0) == h.size(0),
+              "linear_xent: labels must be one int64 per row of h");
+  TORCH_CHECK(h.size(0) >= 1 && h.size(0) < (int64_t(1) << 30) && w.size(0) >= 1 && w.size(0) < (int64_t(1) << 30),
+              "linear_xent: rows out of range");
+  TORCH_CHECK(err.is_cuda() && err.scalar_type() == at::kInt);
+}
+
+}  // namespace gemm
+
+// {stats [T, 4] = (max, sum of exponentials, label's logit, whether the label lies in this
+// shard), lse [T], losses [T]} and, for reduce 1 (sum) or 2 (mean), {the loss, the factor of
+// its gradient (1, or 1 / rows that count)} as 0-d tensors.
+std::vector<torch::Tensor> linear_xent_fwd(const torch::Tensor& h, const torch::Tensor& w,
+                                           const torch::Tensor& labels, int64_t vstart, int64_t ignore_index,
+                                           int64_t reduce, torch::Tensor& err) {
+  using namespace gemm;
+  check_operands(h, w, labels, err);
+  const c10::cuda::CUDAGuard guard(h.device());
+  auto st = at::cuda::getCurrentCUDAStream();
+  const int T = h.size(0), V = w.size(0);
+  const int bn = logits_bn(T, V), tiles_n = (V + bn - 1) / bn;
+  const auto f32 = h.options().dtype(at::kFloat);
+  // one buffer: tiles' partials, target logits, then the results
+  torch::Tensor part = torch::empty({(int64_t)T * tiles_n * 2 + T}, f32);
+  torch::Tensor stats = torch::empty({T, 4}, f32), lse_t = torch::empty({T}, f32), losses = torch::empty({T}, f32);
+  float* target = part.data_ptr<float>() + (int64_t)T * tiles_n * 2;
+  Params p = base_params(T, V, h.size(1), err);
+  XentStatsEpi::Args e{labels.data_ptr<int64_t>(), reinterpret_cast<float2*>(part.data_ptr<float>()), target, vstart,
+                       tiles_n};
+  logits_gemm<XentStatsEpi>(h, w, 0, V, p, e, bn, st);
+  xent_join_kernel<<<(T + 7) / 8, 256, 0, st>>>(
+      reinterpret_cast<const float2*>(part.data_ptr<float>()), target, labels.data_ptr<int64_t>(),
+      reinterpret_cast<float4*>(stats.data_ptr<float>()), lse_t.data_ptr<float>(), losses.data_ptr<float>(), T, tiles_n,
+      vstart, V, ignore_index);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  if (reduce == 0) return {stats, lse_t, losses};
+  torch::Tensor total = torch::empty({2}, f32);
+  xent_total_kernel<<<1, 1024, 0, st>>>(losses.data_ptr<float>(), labels.data_ptr<int64_t>(), total.data_ptr<float>(),
+                                        T, ignore_index, reduce == 2);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {stats, lse_t, losses, total.select(0, 0), total.select(0, 1)};
+}
+
+// grad: fp32, one value (times factor: the gradient of a sum or mean) or one per row.
+// dh: bf16 [T, H] or none; dw: [V, H] bf16 or fp32 or none, stored or accumulated.
+// Returns the number of kernels launched.
+int64_t linear_xent_bwd(const torch::Tensor& h, const torch::Tensor& w, const torch::Tensor& labels,
+                        const torch::Tensor& lse, const torch::Tensor& grad, const torch::Tensor& factor,
+                        const c10::optional<torch::Tensor>& dh, const c10::optional<torch::Tensor>& dw,
+                        bool accumulate, int64_t vstart, int64_t ignore_index, int64_t workspace_bytes,
+                        torch::Tensor& err) {
+  using namespace gemm;
+  check_operands(h, w, labels, err);
+  const int T = h.size(0), H = h.size(1), V = w.size(0);
+  TORCH_CHECK(lse.is_cuda() && lse.scalar_type() == at::kFloat && lse.is_contiguous() && lse.numel() == T);
+  TORCH_CHECK(grad.is_cuda() && grad.scalar_type() == at::kFloat && grad.is_contiguous() &&
+                  (grad.dim() == 0 || grad.numel() == T),
+              "linear_xent_bwd: grad must be one fp32 value or one per row");
+  TORCH_CHECK(factor.is_cuda() && factor.scalar_type() == at::kFloat && factor.numel() == 1);
+  if (dh.has_value())
+    TORCH_CHECK(dh->is_cuda() && dh->scalar_type() == at::kBFloat16 && dh->is_contiguous() && dh->dim() == 2 &&
+                dh->size(0) == T && dh->size(1) == H);
+  int dw_mode = 0;
+  if (dw.has_value()) {
+    const bool f32 = dw->scalar_type() == at::kFloat;
+    TORCH_CHECK(dw->is_cuda() && (f32 || dw->scalar_type() == at::kBFloat16) && dw->dim() == 2 && dw->size(0) == V &&
+                    dw->size(1) == H && dw->stride(1) == 1 && dw->stride(0) % (f32 ? 4 : 8) == 0 &&
+                    reinterpret_cast<uintptr_t>(dw->data_ptr()) % 16 == 0,
+                "linear_xent_bwd: dw must be [V, H] bf16 or fp32 with 16-byte aligned rows");
+    dw_mode = f32 ? (accumulate ? EPI_ACC_F32 : EPI_STORE_F32) : (accumulate ? EPI_ACC_BF16 : EPI_STORE_BF16);
+  }
+  if (!dh.has_value() && !dw.has_value()) return 0;
+  const c10::cuda::CUDAGuard guard(h.device());
+  auto st = at::cuda::getCurrentCUDAStream();
+  const auto f32 = h.options().dtype(at::kFloat);
+  int64_t launches = 0;
+
+  // common factor and row weights
+  const float *fa = grad.data_ptr<float>(), *fb = factor.data_ptr<float>(), *weight = nullptr;
+  torch::Tensor weights;
+  if (grad.dim() > 0) {
+    weights = torch::empty({T + 2}, f32);
+    xent_weights_kernel<<<1, 1024, 0, st>>>(fa, weights.data_ptr<float>() + 2, weights.data_ptr<float>(), T);
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+    fa = weights.data_ptr<float>();
+    fb = fa + 1;
+    weight = fa + 2;
+    ++launches;
+  }
+
+  // pieces of the vocabulary: whole 256-column tiles, as even as they go
+  const int64_t most = std::max<int64_t>(256, workspace_bytes / (2 * (int64_t)T) / 256 * 256);
+  const int64_t pieces = (V + most - 1) / most;
+  const int64_t piece = ((V + pieces - 1) / pieces + 255) / 256 * 256;
+  const int64_t ldd = std::min<int64_t>(piece, (V + 31) / 32 * 32);
+  torch::Tensor d = torch::empty({T, ldd}, h.options());
+
+  // split of the dh product: the fewest partial outputs within 3% of the best fill of the GPU
+  const bool pair = T > 128 && H > 128;
+  const long units = pair ? num_sms() / 2 : num_sms();
+  const long tiles = (T + (pair ? 255 : 127)) / (pair ? 256 : 128) * ((H + 255) / 256);
+  const long kblocks = (std::min<int64_t>(piece, V) + BK - 1) / BK;
+  long ksplit = 1;
+  if (dh.has_value()) {
+    double best = 1e30;
+    for (long k = 1; k <= std::min<long>(32, std::max<long>(1, kblocks / 8)); ++k) {
+      const double cost = double((tiles * k + units - 1) / units) / k;
+      if (cost < best * 0.97) { best = cost; ksplit = k; }
+    }
+  }
+  const int64_t split_rows = (T + 255) / 256 * 256;
+  torch::Tensor acc;
+  if (dh.has_value()) acc = torch::empty({ksplit * split_rows, H}, f32);
+
+  for (int64_t v0 = 0; v0 < V; v0 += piece) {
+    const int n = static_cast<int>(std::min<int64_t>(piece, V - v0));
+    Params p = base_params(T, n, H, err);
+    p.D = d.data_ptr();
+    p.ldd = ldd;
+    XentGradEpi::Args e{labels.data_ptr<int64_t>(), lse.data_ptr<float>(), weight, vstart + v0, ignore_index};
+    logits_gemm<XentGradEpi>(h, w, v0, n, p, e, logits_bn(T, n), st);
+    ++launches;
+    if (dw.has_value()) {
+      char* out = reinterpret_cast<char*>(dw->data_ptr()) + v0 * dw->stride(0) * dw->element_size();
+      product<true>(d.data_ptr(), ldd, h.data_ptr(), h.stride(0), n, H, T, out, dw->stride(0), dw_mode, 1, 0, fa, fb,
+                    err, st);
+      ++launches;
+    }
+    if (dh.has_value()) {
+      const auto* wp = reinterpret_cast<const __nv_bfloat16*>(w.data_ptr()) + v0 * w.stride(0);
+      // every share needs a k-block: a short last piece adds to fewer partial outputs
+      const long shares = std::min<long>(ksplit, (n + BK - 1) / BK);
+      product<false>(d.data_ptr(), ldd, wp, w.stride(0), T, H, n, acc.data_ptr(), H,
+                     v0 == 0 ? EPI_STORE_F32 : EPI_ACC_F32, static_cast<int>(shares), static_cast<int>(split_rows),
+                     nullptr, nullptr, err, st);
+      ++launches;
+    }
+  }
+  if (dh.has_value()) {
+    const int64_t quads = (int64_t)T * (H / 4);
+    xent_dh_kernel<<<static_cast<unsigned>((quads + 255) / 256), 256, 0, st>>>(
+        acc.data_ptr<float>(), reinterpret_cast<__nv_bfloat16*>(dh->data_ptr()), fa, fb, quads, split_rows * H,
+        static_cast<int>(ksplit), H / 4, dh->stride(0));
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+    ++launches;
+  }
+  return launches;
+}
+
+}  // namespace ft

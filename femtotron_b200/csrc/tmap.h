@@ -42,11 +42,20 @@ inline CUtensorMap make_tmap_2d(const void* base, CUtensorMapDataType dtype, int
     throw std::runtime_error("femtotron_b200: TMA base address must be 16-byte aligned");
   if (strides[0] % 16 != 0)
     throw std::runtime_error("femtotron_b200: TMA row stride must be a multiple of 16 bytes");
-  CUresult r = encode_tiled_fn()(&m, dtype, 2, const_cast<void*>(base), dims, strides, box, estr,
-                                 CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                 swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
-                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  auto encode = [&] {
+    return encode_tiled_fn()(&m, dtype, 2, const_cast<void*>(base), dims, strides, box, estr,
+                             CU_TENSOR_MAP_INTERLEAVE_NONE,
+                             swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {
+    // a thread that has not called the runtime yet (autograd's, when a GEMM comes first in
+    // the backward) has no current context: bind its device's and try again
+    int dev = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = encode();
+  }
   if (r != CUDA_SUCCESS)
     throw std::runtime_error("femtotron_b200: cuTensorMapEncodeTiled failed with code " +
                              std::to_string(static_cast<int>(r)));

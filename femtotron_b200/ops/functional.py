@@ -26,6 +26,7 @@ import torch.distributed as dist
 from torch.autograd import Function
 
 from . import kernels as K
+from . import linear_xent as X
 from .matmul import gemm, linear_dgrad, linear_fwd, linear_wgrad
 
 
@@ -338,6 +339,72 @@ class LMHeadCrossEntropyFn(Function):
             write_weight_grad([ctx.param], lambda dst, acc: linear_wgrad(dlogits, h2, dst, acc))
         ctx.param = None
         return dh, None, None, None, None, None
+
+
+class LinearCrossEntropyFn(Function):
+    """Cross entropy of ``h @ w^T`` that never has the logits in memory: the forward keeps one
+    number per row, the backward computes the product again (``ops/linear_xent.py``)."""
+
+    @staticmethod
+    def forward(ctx, h, w, labels, vstart, tp_group, ignore_index, reduction, workspace_bytes):
+        h2 = _as2d(h)
+        lab = labels.reshape(-1).contiguous()
+        sharded = tp_group is not None and dist.get_world_size(tp_group) > 1
+        stats, lse, losses, loss, factor = X.forward(h2, w, lab, vstart, ignore_index,
+                                                     "none" if sharded else reduction, workspace_bytes)
+        if sharded:  # only [T, 4] numbers cross the group
+            ws = dist.get_world_size(tp_group)
+            allst = torch.empty(ws * stats.shape[0], 4, dtype=stats.dtype, device=stats.device)
+            dist.all_gather_into_tensor(allst, stats, group=tp_group)
+            lse, losses, loss, factor = X.combine(X.merge_shards(allst.view(ws, -1, 4)), lab, ignore_index,
+                                                  reduction)
+        ctx.save_for_backward(h2, w.detach(), lab, lse, lse.new_ones(()) if factor is None else factor)
+        ctx.param = w
+        ctx.meta = (vstart, ignore_index, workspace_bytes, reduction)
+        ctx.hshape = h.shape
+        return losses if reduction == "none" else loss
+
+    @staticmethod
+    def backward(ctx, dloss):
+        h2, w, lab, lse, factor = ctx.saved_tensors
+        vstart, ignore_index, workspace_bytes, reduction = ctx.meta
+        grad = dloss.float().contiguous()
+        dh = torch.empty_like(h2) if ctx.needs_input_grad[0] else None
+
+        def compute(dw, acc):
+            X.backward(h2, w, lab, lse, grad, factor, dh, dw, acc, vstart, ignore_index, workspace_bytes)
+        if ctx.needs_input_grad[1]:
+            write_weight_grad([ctx.param], compute)
+        else:
+            compute(None, False)
+        ctx.param = None
+        return dh.view(ctx.hshape) if dh is not None else None, None, None, None, None, None, None, None
+
+
+def linear_cross_entropy(h: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, *, vstart: int = 0, tp_group=None,
+                         ignore_index: int = -100, reduction: str = "mean",
+                         workspace_bytes: int = X.WORKSPACE_BYTES) -> torch.Tensor:
+    """Cross entropy of the head ``h [..., H] @ w [V, H]^T`` against ``labels`` (one per row of
+    h) without its logits in memory: the loss ("mean" over the labels that are not
+    ``ignore_index``, or "sum"), or one fp32 loss per row ("none", flat).  With ``tp_group``, w is
+    the vocabulary shard that starts at ``vstart``.  The weight gradient goes to w's gradient
+    sink; ``workspace_bytes`` bounds the backward's workspace.
+
+    The mean over no labels is NaN and its gradients are zero.  A label outside the vocabulary
+    makes its loss NaN.  On CUDA h and w are bf16 with a hidden size that is a multiple of 8."""
+    if reduction not in X.REDUCTIONS:
+        raise ValueError(f"linear_cross_entropy: reduction must be one of {tuple(X.REDUCTIONS)}, got {reduction!r}")
+    if w.dim() != 2 or h.dim() < 1 or h.shape[-1] != w.shape[1]:
+        raise ValueError(f"linear_cross_entropy: h {tuple(h.shape)} and w {tuple(w.shape)} do not match")
+    if labels.dtype != torch.int64 or labels.numel() != h.shape[:-1].numel():
+        raise ValueError(f"linear_cross_entropy: one int64 label per row is needed, got {labels.dtype} "
+                         f"{tuple(labels.shape)} for h {tuple(h.shape)}")
+    if h.dtype != w.dtype:
+        raise TypeError(f"linear_cross_entropy: h is {h.dtype}, w is {w.dtype}")
+    if labels.numel() == 0:
+        rows = h.reshape(0, h.shape[-1]).float().sum(-1)
+        return rows if reduction == "none" else rows.sum() if reduction == "sum" else rows.sum() / 0
+    return LinearCrossEntropyFn.apply(h, w, labels, vstart, tp_group, ignore_index, reduction, workspace_bytes)
 
 
 def shift_labels(labels: torch.Tensor, ignore_index: int = -100) -> torch.Tensor:

@@ -21,47 +21,111 @@
 namespace ft {
 namespace {
 
-constexpr int kChunk = 16;            // values per thread
+constexpr int kChunk = 16;                // values per thread
 constexpr float kTiny = 7.52316385e-37f;  // 2^-120
 constexpr float kInv127 = 1.0f / 127.0f;
 
-__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
 template <typename T> __device__ __forceinline__ T from_f(float v);
 template <> __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ float from_f(float v) { return v; }
 
-template <typename T> struct alignas(16) Vec16 { T v[16 / sizeof(T)]; };
+// How rows lie in memory: 16-value chunks on 32-byte boundaries (one 256-bit access per 16
+// bf16), on 16-byte ones, or neither.
+enum Rows { kRows32, kRows16, kRowsAny };
+
+// N 32-bit words of p, N = 4, 8 or 16.
+template <int N, Rows R>
+__device__ __forceinline__ void load_words(const void* p, uint32_t (&w)[N]) {
+  if constexpr (R == kRows32 && N >= 8) {
+#pragma unroll
+    for (int i = 0; i < N; i += 8)
+      asm("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+          : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]), "=r"(w[i + 4]), "=r"(w[i + 5]),
+            "=r"(w[i + 6]), "=r"(w[i + 7])
+          : "l"(__cvta_generic_to_global(static_cast<const uint32_t*>(p) + i))
+          : "memory");
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const uint32_t*>(p) + i);
+      w[i] = q.x; w[i + 1] = q.y; w[i + 2] = q.z; w[i + 3] = q.w;
+    }
+  }
+}
+template <int N, Rows R>
+__device__ __forceinline__ void store_words(void* p, const uint32_t (&w)[N]) {
+  if constexpr (R == kRows32 && N >= 8) {
+#pragma unroll
+    for (int i = 0; i < N; i += 8)
+      asm volatile("st.global.v8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(w[i]), "r"(w[i + 1]), "r"(w[i + 2]),
+                   "r"(w[i + 3]), "r"(w[i + 4]), "r"(w[i + 5]), "r"(w[i + 6]), "r"(w[i + 7]),
+                   "l"(__cvta_generic_to_global(static_cast<uint32_t*>(p) + i))
+                   : "memory");
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 4)
+      *reinterpret_cast<uint4*>(static_cast<uint32_t*>(p) + i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+  }
+}
+
+// 16 values and their packed words (two 16-bit values per word, the lower one first).
+__device__ __forceinline__ void unpack(const uint32_t (&w)[8], float (&v)[16], __nv_bfloat16) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    v[2 * i] = __uint_as_float(w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void unpack(const uint32_t (&w)[8], float (&v)[16], __half) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void unpack(const uint32_t (&w)[16], float (&v)[16], float) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(w[i]);
+}
+__device__ __forceinline__ void pack(const float (&v)[16], uint32_t (&w)[8], __nv_bfloat16) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+}
+__device__ __forceinline__ void pack(const float (&v)[16], uint32_t (&w)[8], __half) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+__device__ __forceinline__ void pack(const float (&v)[16], uint32_t (&w)[16], float) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(v[i]);
+}
 
 // Up to 16 values starting at p (`left` of them exist) as fp32, zeros after them.
-template <typename T, bool ALIGNED>
+template <typename T, Rows R>
 __device__ __forceinline__ void load16(const T* p, int left, float (&v)[16]) {
-  constexpr int PER = 16 / sizeof(T);
-  if (ALIGNED && left >= 16) {
-#pragma unroll
-    for (int j = 0; j < 16 / PER; ++j) {
-      const Vec16<T> q = *reinterpret_cast<const Vec16<T>*>(p + j * PER);
-#pragma unroll
-      for (int i = 0; i < PER; ++i) v[j * PER + i] = to_f(q.v[i]);
-    }
+  if (R != kRowsAny && left >= 16) {
+    uint32_t w[4 * sizeof(T)];
+    load_words<4 * sizeof(T), R>(p, w);
+    unpack(w, v, T{});
   } else {
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = i < left ? to_f(p[i]) : 0.f;
   }
 }
-template <typename T, bool ALIGNED>
+template <typename T, Rows R>
 __device__ __forceinline__ void store16(T* p, int left, const float (&v)[16]) {
-  constexpr int PER = 16 / sizeof(T);
-  if (ALIGNED && left >= 16) {
-#pragma unroll
-    for (int j = 0; j < 16 / PER; ++j) {
-      Vec16<T> q;
-#pragma unroll
-      for (int i = 0; i < PER; ++i) q.v[i] = from_f<T>(v[j * PER + i]);
-      *reinterpret_cast<Vec16<T>*>(p + j * PER) = q;
-    }
+  if (R != kRowsAny && left >= 16) {
+    uint32_t w[4 * sizeof(T)];
+    pack(v, w, T{});
+    store_words<4 * sizeof(T), R>(p, w);
   } else {
 #pragma unroll
     for (int i = 0; i < 16; ++i)
@@ -69,81 +133,105 @@ __device__ __forceinline__ void store16(T* p, int left, const float (&v)[16]) {
   }
 }
 
-// Largest magnitude over the `lanes` neighbouring threads that share a group.  NaN has to win,
+// Largest magnitude over the 2^lanes_log2 neighbouring threads that share a group.  NaN has to win,
 // so magnitudes are compared as their bit patterns (for non-negative floats the integer order
 // is the order of the values, with NaN above infinity).
-__device__ __forceinline__ float group_top(const float (&v)[16], int lanes) {
+__device__ __forceinline__ float group_top(const float (&v)[16], int lanes_log2) {
   uint32_t m = 0;
 #pragma unroll
   for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
-  for (int o = lanes >> 1; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) {  // groups have 2 to 16 threads
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, m, o);
+    if (o < (1 << lanes_log2)) m = max(m, other);
+  }
   return __uint_as_float(m);
 }
 
 // Codes of 16 values; returns the group's scale.  top = inf or NaN gives the scale NaN.
+// Adding 1.5 * 2^23 rounds the product to an integer (ties to even) whose two's complement is the
+// low byte of the sum: no conversion instruction, which would run at a quarter of the rate.
+// |x * mul| <= 127 (1 + 2^-22), so the codes need no clamp.
 __device__ __forceinline__ float encode16(const float (&v)[16], float top, uint4& out) {
   const bool fine = top < INFINITY;  // false for NaN
-  const float mul = (fine && top >= kTiny) ? __fmul_rn(__fdiv_rn(1.0f, top), 127.0f) : 0.f;
+  const bool kept = fine && top >= kTiny;
+  const float mul = kept ? __fmul_rn(__frcp_rn(top), 127.0f) : 0.f;
   uint32_t w[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    uint32_t x = 0;
+    uint32_t b[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int q = __float2int_rn(__fmul_rn(v[4 * j + i], mul));
-      x |= (static_cast<uint32_t>(min(127, max(-127, q))) & 0xffu) << (8 * i);
-    }
-    w[j] = x;
+    for (int i = 0; i < 4; ++i)
+      b[i] = __float_as_uint(__fadd_rn(__fmul_rn(v[4 * j + i], mul), 12582912.f));
+    w[j] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
   }
-  out = make_uint4(w[0], w[1], w[2], w[3]);
-  return fine ? (top >= kTiny ? __fmul_rn(top, kInv127) : 0.f) : __int_as_float(0x7fffffff);
+  out = kept ? make_uint4(w[0], w[1], w[2], w[3]) : make_uint4(0, 0, 0, 0);
+  return kept ? __fmul_rn(top, kInv127) : fine ? 0.f : __int_as_float(0x7fffffff);
 }
 
+// The reverse trick: a byte b + 128 under the exponent of 2^23 is the float 2^23 + b + 128.
+// Codes as floats, times `scale`.
 __device__ __forceinline__ void decode16(const uint4& q, float scale, float (&v)[16]) {
-  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+  const uint32_t w[4] = {q.x ^ 0x80808080u, q.y ^ 0x80808080u, q.z ^ 0x80808080u, q.w ^ 0x80808080u};
 #pragma unroll
   for (int j = 0; j < 4; ++j)
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      v[4 * j + i] = __fmul_rn(static_cast<float>(static_cast<int8_t>(w[j] >> (8 * i))), scale);
+      v[4 * j + i] = __fmul_rn(
+          __fadd_rn(__uint_as_float(__byte_perm(w[j], 0x4b000000u, 0x7440 + i)), -8388736.f), scale);
+}
+
+// Row and chunk of a thread (the launch has fewer than 2^31 threads).
+__device__ __forceinline__ void split_index(const FastDiv& slots, int64_t& row, int& slot) {
+  const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
+  const uint32_t r = slots.div(idx);
+  row = r;
+  slot = static_cast<int>(idx - r * slots.d);
+}
+
+__device__ __forceinline__ float sigmoid(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + __expf(-x)));
+  return r;
 }
 
 // ------------------------------------------------------------------ quantise / dequantise
-template <typename T, bool ALIGNED>
+template <typename T, Rows R>
 __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, int8_t* __restrict__ q,
                                                        float* __restrict__ scale, int64_t rows, int n,
-                                                       int64_t ldx, int64_t pitch, int groups, int lanes) {
-  const int slots = groups * lanes;  // threads per row, whole groups
-  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = idx / slots;
-  const int slot = static_cast<int>(idx - row * slots);
+                                                       int64_t ldx, int64_t pitch, int groups, int lanes_log2,
+                                                       FastDiv slots) {
+  // `slots` threads per row: whole groups
+  int64_t row;
+  int slot;
+  split_index(slots, row, slot);
   const int c = slot * kChunk;
   const int left = row < rows ? n - c : 0;
   float v[16];
-  load16<T, ALIGNED>(x + row * ldx + c, left, v);
-  const float top = group_top(v, lanes);
+  load16<T, R>(x + row * ldx + c, left, v);
+  const float top = group_top(v, lanes_log2);
   uint4 code;
   const float s = encode16(v, top, code);
   if (left > 0) {
     *reinterpret_cast<uint4*>(q + row * pitch + c) = code;
-    if (slot % lanes == 0) scale[row * groups + slot / lanes] = s;
+    if ((slot & ((1 << lanes_log2) - 1)) == 0) scale[row * groups + (slot >> lanes_log2)] = s;
   }
 }
 
-template <typename T, bool ALIGNED>
+template <typename T, Rows R>
 __global__ void __launch_bounds__(256) dequantize_kernel(const int8_t* __restrict__ q,
                                                          const float* __restrict__ scale,
                                                          T* __restrict__ x, int64_t rows, int n,
-                                                         int64_t ldx, int64_t pitch, int groups, int lanes) {
-  const int slots = (n + kChunk - 1) / kChunk;
-  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = idx / slots;
+                                                         int64_t ldx, int64_t pitch, int groups, int lanes_log2,
+                                                         FastDiv slots) {
+  int64_t row;
+  int slot;
+  split_index(slots, row, slot);
   if (row >= rows) return;
-  const int slot = static_cast<int>(idx - row * slots);
   const int c = slot * kChunk;
   float v[16];
-  decode16(*reinterpret_cast<const uint4*>(q + row * pitch + c), scale[row * groups + slot / lanes], v);
-  store16<T, ALIGNED>(x + row * ldx + c, n - c, v);
+  decode16(*reinterpret_cast<const uint4*>(q + row * pitch + c), scale[row * groups + (slot >> lanes_log2)], v);
+  store16<T, R>(x + row * ldx + c, n - c, v);
 }
 
 // ------------------------------------------------------------------ RMSNorm
@@ -164,12 +252,12 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
 
 // y = w x r, r = rsqrt(mean x^2 + eps), and the 8-bit copy of x, from one read of x.
 // NT threads share a row (VPT chunks each); blocks of max(NT, 128) threads.
-template <int NT, int VPT>
+template <int NT, int VPT, Rows R>
 __global__ void __launch_bounds__(NT > 128 ? NT : 128)
     rms_norm8_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ w,
                      __nv_bfloat16* __restrict__ y, float* __restrict__ rstd, int8_t* __restrict__ q,
                      float* __restrict__ scale, int64_t rows, int H, int64_t ldx, int64_t ldy,
-                     int64_t pitch, int groups, int lanes, float eps) {
+                     int64_t pitch, int groups, int lanes_log2, float eps) {
   __shared__ float red[NT / 32];
   constexpr int RPB = NT >= 128 ? 1 : 128 / NT;
   const int t = threadIdx.x % NT;
@@ -180,19 +268,19 @@ __global__ void __launch_bounds__(NT > 128 ? NT : 128)
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int c = (t + i * NT) * kChunk;
-    load16<__nv_bfloat16, true>(x + row * ldx + c, here ? H - c : 0, v[i]);
+    load16<__nv_bfloat16, R>(x + row * ldx + c, here ? H - c : 0, v[i]);
 #pragma unroll
     for (int j = 0; j < 16; ++j) ss += v[i][j] * v[i][j];
   }
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int slot = t + i * NT;
-    const float top = group_top(v[i], lanes);
+    const float top = group_top(v[i], lanes_log2);
     uint4 code;
     const float s = encode16(v[i], top, code);
     if (here && slot * kChunk < H) {
       *reinterpret_cast<uint4*>(q + row * pitch + slot * kChunk) = code;
-      if (slot % lanes == 0) scale[row * groups + slot / lanes] = s;
+      if ((slot & ((1 << lanes_log2) - 1)) == 0) scale[row * groups + (slot >> lanes_log2)] = s;
     }
   }
   ss = row_sum<NT>(ss, red);
@@ -203,50 +291,45 @@ __global__ void __launch_bounds__(NT > 128 ? NT : 128)
     const int c = (t + i * NT) * kChunk;
     if (!here || c >= H) continue;
     float wv[16];
-    load16<__nv_bfloat16, true>(w + c, H - c, wv);
+    load16<__nv_bfloat16, R>(w + c, H - c, wv);
 #pragma unroll
     for (int j = 0; j < 16; ++j) wv[j] *= v[i][j] * r;
-    store16<__nv_bfloat16, true>(y + row * ldy + c, H - c, wv);
+    store16<__nv_bfloat16, R>(y + row * ldy + c, H - c, wv);
   }
 }
 
 // n = x8 r,  dx = r (dy w - n mean(dy w n)),  y8 = n w,  dw = sum over rows of dy n.
-// A block walks a run of rows; its share of dw stays in registers and goes to part[block],
-// which dw_sum_kernel adds up in block order (no atomics: the same sums on every run).
-template <int NT, int VPT>
-__global__ void __launch_bounds__(NT > 128 ? NT : 128)
-    rms_norm8_bwd_kernel(const __nv_bfloat16* __restrict__ dy, const int8_t* __restrict__ q,
-                         const float* __restrict__ scale, const __nv_bfloat16* __restrict__ w,
-                         const float* __restrict__ rstd, __nv_bfloat16* __restrict__ dx,
-                         __nv_bfloat16* __restrict__ y8, float* __restrict__ part, int64_t rows, int H,
-                         int64_t lddy, int64_t lddx, int64_t ldy, int64_t pitch, int groups, int lanes,
-                         int rows_per_walker) {
-  __shared__ float red[NT / 32];
-  constexpr int RPB = NT >= 128 ? 1 : 128 / NT;
-  const int t = threadIdx.x % NT;
-  const int64_t walker = (int64_t)blockIdx.x * RPB + threadIdx.x / NT;
-  const int64_t r0 = walker * rows_per_walker;
+// A walker (NT threads) takes a run of rows; its share of dw stays in registers and goes to
+// part[walker], which dw_sum_kernel adds up in walker order (no atomics: the same sums on
+// every run).  This form is for short rows, one warp each.
+template <int VPT, Rows R>
+__global__ void __launch_bounds__(128)
+    rms_norm8_bwd_warp_kernel(const __nv_bfloat16* __restrict__ dy, const int8_t* __restrict__ q,
+                              const float* __restrict__ scale, const __nv_bfloat16* __restrict__ w,
+                              const float* __restrict__ rstd, __nv_bfloat16* __restrict__ dx,
+                              __nv_bfloat16* __restrict__ y8, float* __restrict__ part, int64_t rows, int H,
+                              int64_t lddy, int64_t pitch, int groups, int lanes_log2, int rows_per_walker) {
+  const int t = threadIdx.x % 32;
+  const int64_t walker = (int64_t)blockIdx.x * 4 + threadIdx.x / 32;
+  const int64_t r0 = walker * rows_per_walker, r1 = min(rows, r0 + rows_per_walker);
   float dw[VPT][16];
 #pragma unroll
   for (int i = 0; i < VPT; ++i)
 #pragma unroll
     for (int j = 0; j < 16; ++j) dw[i][j] = 0.f;
-  for (int k = 0; k < rows_per_walker; ++k) {
-    const int64_t row = r0 + k;
-    const bool here = row < rows;
-    if (!here && NT >= 32) break;  // the whole row's threads leave together
+  for (int64_t row = r0; row < r1; ++row) {
     const float r = rstd[row];
     float n[VPT][16], g[VPT][16];
     float dot = 0.f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int slot = t + i * NT;
+      const int slot = t + i * 32;
       const int c = slot * kChunk;
       if (c < H) {
-        decode16(*reinterpret_cast<const uint4*>(q + row * pitch + c), scale[row * groups + slot / lanes], n[i]);
-        load16<__nv_bfloat16, true>(dy + row * lddy + c, H - c, g[i]);
+        decode16(*reinterpret_cast<const uint4*>(q + row * pitch + c), scale[row * groups + (slot >> lanes_log2)], n[i]);
+        load16<__nv_bfloat16, R>(dy + row * lddy + c, H - c, g[i]);
         float wv[16];
-        load16<__nv_bfloat16, true>(w + c, H - c, wv);
+        load16<__nv_bfloat16, R>(w + c, H - c, wv);
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           n[i][j] *= r;
@@ -255,191 +338,380 @@ __global__ void __launch_bounds__(NT > 128 ? NT : 128)
           dot += g[i][j] * n[i][j];
           wv[j] *= n[i][j];
         }
-        store16<__nv_bfloat16, true>(y8 + row * ldy + c, H - c, wv);
+        store16<__nv_bfloat16, R>(y8 + row * H + c, H - c, wv);
       }
     }
-    dot = row_sum<NT>(dot, red) / H;
+    dot = warp_sum(dot) / H;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int c = (t + i * NT) * kChunk;
+      const int c = (t + i * 32) * kChunk;
       if (c < H) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) g[i][j] = r * (g[i][j] - n[i][j] * dot);
-        store16<__nv_bfloat16, true>(dx + row * lddx + c, H - c, g[i]);
+        store16<__nv_bfloat16, R>(dx + row * H + c, H - c, g[i]);
       }
     }
   }
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    const int c = (t + i * NT) * kChunk;
-    if (c < H && r0 < rows) store16<float, true>(part + walker * H + c, H - c, dw[i]);
+    const int c = (t + i * 32) * kChunk;
+    if (c < H && r0 < rows) store16<float, kRows16>(part + walker * H + c, H - c, dw[i]);
   }
 }
 
-// dw[c] = sum of part[0..walkers)[c]: 32 columns per block, 8 rows of threads.
-__global__ void __launch_bounds__(256) dw_sum_kernel(const float* __restrict__ part, float* __restrict__ dw,
-                                                     int walkers, int H) {
-  __shared__ float red[8][33];
+__device__ __forceinline__ uint64_t clock_ns() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
+
+// Long rows: a block per walker.  The rows' codes and dy come through a ring of kStages bulk
+// copies into shared memory, so the next rows are on their way during this one's reduction.
+// One barrier per row: the sums of the warps alternate between two buffers, and the stage that the
+// previous row used is refilled after this row's barrier.
+constexpr int kStages = 3;
+constexpr int kErrNormWait = 302;  // a bulk copy did not arrive
+
+template <int NT, int VPT, Rows R>
+__global__ void __launch_bounds__(NT, 512 / NT)
+    rms_norm8_bwd_kernel(const __nv_bfloat16* __restrict__ dy, const int8_t* __restrict__ q,
+                         const float* __restrict__ scale, const __nv_bfloat16* __restrict__ w,
+                         const float* __restrict__ rstd, __nv_bfloat16* __restrict__ dx,
+                         __nv_bfloat16* __restrict__ y8, float* __restrict__ part, int64_t rows, int H,
+                         int64_t lddy, int64_t pitch, int groups, int lanes_log2, int rows_per_walker,
+                         int* __restrict__ err) {
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ uint64_t full[kStages];
+  __shared__ float red[2][NT / 32];
+  const int t = threadIdx.x;
+  const int64_t r0 = (int64_t)blockIdx.x * rows_per_walker;
+  const int count = static_cast<int>(min(rows - r0, (int64_t)rows_per_walker));
+  const uint32_t code_bytes = static_cast<uint32_t>(pitch), dy_bytes = 2u * H;
+  const uint32_t stage_bytes = code_bytes + dy_bytes;
+  auto fetch = [&](int k) {  // one thread
+    uint8_t* s = ring + (k % kStages) * stage_bytes;
+    mbar_arrive_expect_tx(&full[k % kStages], stage_bytes);
+    bulk_load(s, q + (r0 + k) * pitch, code_bytes, &full[k % kStages]);
+    bulk_load(s + code_bytes, dy + (r0 + k) * lddy, dy_bytes, &full[k % kStages]);
+  };
+  if (t == 0) {
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) mbar_init(&full[i], 1);
+    fence_barrier_init();
+    for (int k = 0; k < min(count, kStages - 1); ++k) fetch(k);
+  }
+  uint32_t wq[VPT][8];
+  float dw[VPT][16], sc[VPT];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int slot = t + i * NT, c = slot * kChunk;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) wq[i][j] = 0;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) dw[i][j] = 0.f;
+    sc[i] = 0.f;
+    if (c < H) {
+      float wv[16];
+      load16<__nv_bfloat16, R>(w + c, H - c, wv);
+      pack(wv, wq[i], __nv_bfloat16{});
+      sc[i] = scale[r0 * groups + (slot >> lanes_log2)];
+    }
+  }
+  float r = rstd[r0];
+  __syncthreads();  // barriers are initialised
+  bool late = false;
+  for (int k = 0; k < count; ++k) {
+    const int64_t row = r0 + k;
+    const uint8_t* s = ring + (k % kStages) * stage_bytes;
+    // the next row's scalars
+    float sc_next[VPT], r_next = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int slot = t + i * NT;
+      sc_next[i] = (k + 1 < count && slot * kChunk < H) ? scale[(row + 1) * groups + (slot >> lanes_log2)] : 0.f;
+    }
+    if (k + 1 < count) r_next = rstd[row + 1];
+    if (!late && !mbar_try_wait(&full[k % kStages], (k / kStages) & 1)) {
+      const uint64_t start = clock_ns();
+      while (!mbar_try_wait(&full[k % kStages], (k / kStages) & 1)) {
+        if (clock_ns() - start > 2000000000ull) {  // give up waiting; the results are marked by err
+          atomicCAS(err, 0, kErrNormWait);
+          late = true;
+          break;
+        }
+      }
+    }
+    // n and dy w of a chunk; kept in registers over the barrier where one chunk is a thread's share
+    auto chunk = [&](int i, float (&n)[16], float (&g)[16]) {
+      const int c = (t + i * NT) * kChunk;
+      decode16(*reinterpret_cast<const uint4*>(s + c), sc[i] * r, n);
+      load16<__nv_bfloat16, kRows16>(reinterpret_cast<const __nv_bfloat16*>(s + code_bytes) + c, H - c, g);
+    };
+    float n[16], g[16];
+    float dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = (t + i * NT) * kChunk;
+      if (c < H) {
+        float wv[16], y[16];
+        chunk(i, n, g);
+        unpack(wq[i], wv, __nv_bfloat16{});
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          dw[i][j] += g[j] * n[j];
+          g[j] *= wv[j];
+          dot += g[j] * n[j];
+          y[j] = wv[j] * n[j];
+        }
+        store16<__nv_bfloat16, R>(y8 + row * H + c, H - c, y);
+      }
+    }
+    dot = warp_sum(dot);
+    if (t % 32 == 0) red[k & 1][t / 32] = dot;
+    __syncthreads();
+    if (t == 0 && k + kStages - 1 < count) fetch(k + kStages - 1);
+    dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < NT / 32; ++i) dot += red[k & 1][i];
+    dot /= H;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = (t + i * NT) * kChunk;
+      if (c < H) {
+        if (VPT > 1) {
+          float wv[16];
+          chunk(i, n, g);
+          unpack(wq[i], wv, __nv_bfloat16{});
+#pragma unroll
+          for (int j = 0; j < 16; ++j) g[j] *= wv[j];
+        }
+        float d[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) d[j] = r * (g[j] - n[j] * dot);
+        store16<__nv_bfloat16, R>(dx + row * H + c, H - c, d);
+      }
+      sc[i] = sc_next[i];
+    }
+    r = r_next;
+  }
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int c = (t + i * NT) * kChunk;
+    if (c < H) store16<float, kRows16>(part + (int64_t)blockIdx.x * H + c, H - c, dw[i]);
+  }
+}
+
+// dw[c] = sum of part[0..walkers)[c]: 32 columns per block, 32 rows of threads.
+__global__ void __launch_bounds__(1024) dw_sum_kernel(const float* __restrict__ part, float* __restrict__ dw,
+                                                      int walkers, int H) {
+  __shared__ float red[32][33];
   const int c = blockIdx.x * 32 + threadIdx.x % 32, k = threadIdx.x / 32;
   float s = 0.f;
   if (c < H)
-    for (int i = k; i < walkers; i += 8) s += part[(int64_t)i * H + c];
+    for (int i = k; i < walkers; i += 32) s += part[(int64_t)i * H + c];
   red[k][threadIdx.x % 32] = s;
   __syncthreads();
-  if (k == 0 && c < H) {
-#pragma unroll
-    for (int i = 1; i < 8; ++i) s += red[i][threadIdx.x];
-    dw[c] = s;
-  }
+  s = warp_sum(red[threadIdx.x % 32][k]);  // warp k adds column k
+  if (threadIdx.x % 32 == 0 && blockIdx.x * 32 + k < H) dw[blockIdx.x * 32 + k] = s;
 }
 
 // ------------------------------------------------------------------ SwiGLU
 // gu = [gate F | up F] -> h = silu(g) u, and the 8-bit copies of both halves (groups do not
 // cross from gate to up: each half is a row of its own in the code, pitch bytes apart).
-__global__ void __launch_bounds__(256) swiglu8_kernel(const __nv_bfloat16* __restrict__ gu,
+template <Rows R>
+__global__ void __launch_bounds__(256, 5) swiglu8_kernel(const __nv_bfloat16* __restrict__ gu,
                                                       __nv_bfloat16* __restrict__ h, int8_t* __restrict__ q,
                                                       float* __restrict__ scale, int64_t rows, int F,
                                                       int64_t ldgu, int64_t ldh, int64_t pitch, int groups,
-                                                      int lanes) {
-  const int slots = groups * lanes;
-  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = idx / slots;
-  const int slot = static_cast<int>(idx - row * slots);
+                                                      int lanes_log2, FastDiv slots) {
+  int64_t row;
+  int slot;
+  split_index(slots, row, slot);
   const int c = slot * kChunk;
   const int left = row < rows ? F - c : 0;
   float g[16], u[16];
-  load16<__nv_bfloat16, true>(gu + row * ldgu + c, left, g);
-  load16<__nv_bfloat16, true>(gu + row * ldgu + F + c, left, u);
-  const float tg = group_top(g, lanes), tu = group_top(u, lanes);
+  load16<__nv_bfloat16, R>(gu + row * ldgu + c, left, g);
+  load16<__nv_bfloat16, R>(gu + row * ldgu + F + c, left, u);
+  const float tg = group_top(g, lanes_log2), tu = group_top(u, lanes_log2);
   uint4 cg, cu;
   const float sg = encode16(g, tg, cg), su = encode16(u, tu, cu);
   if (left <= 0) return;
   *reinterpret_cast<uint4*>(q + 2 * row * pitch + c) = cg;
   *reinterpret_cast<uint4*>(q + (2 * row + 1) * pitch + c) = cu;
-  if (slot % lanes == 0) {
-    scale[2 * row * groups + slot / lanes] = sg;
-    scale[(2 * row + 1) * groups + slot / lanes] = su;
+  if ((slot & ((1 << lanes_log2) - 1)) == 0) {
+    scale[2 * row * groups + (slot >> lanes_log2)] = sg;
+    scale[(2 * row + 1) * groups + (slot >> lanes_log2)] = su;
   }
 #pragma unroll
-  for (int i = 0; i < 16; ++i) g[i] = g[i] * u[i] * __fdividef(1.f, 1.f + __expf(-g[i]));
-  store16<__nv_bfloat16, true>(h + row * ldh + c, left, g);
+  for (int i = 0; i < 16; ++i) g[i] = g[i] * u[i] * sigmoid(g[i]);
+  store16<__nv_bfloat16, R>(h + row * ldh + c, left, g);
 }
 
 // s = sigmoid(g8): dg = dh u8 s (1 + g8 (1 - s)), du = dh g8 s, h8 = g8 s u8.
+template <Rows R>
 __global__ void __launch_bounds__(256) swiglu8_bwd_kernel(const __nv_bfloat16* __restrict__ dh,
                                                           const int8_t* __restrict__ q,
                                                           const float* __restrict__ scale,
                                                           __nv_bfloat16* __restrict__ dgu,
                                                           __nv_bfloat16* __restrict__ h8, int64_t rows, int F,
                                                           int64_t lddh, int64_t lddgu, int64_t ldh,
-                                                          int64_t pitch, int groups, int lanes) {
-  const int slots = (F + kChunk - 1) / kChunk;
-  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = idx / slots;
+                                                          int64_t pitch, int groups, int lanes_log2,
+                                                          FastDiv slots) {
+  int64_t row;
+  int slot;
+  split_index(slots, row, slot);
   if (row >= rows) return;
-  const int slot = static_cast<int>(idx - row * slots);
   const int c = slot * kChunk;
   float d[16], g[16], u[16], hv[16];
-  load16<__nv_bfloat16, true>(dh + row * lddh + c, F - c, d);
-  decode16(*reinterpret_cast<const uint4*>(q + 2 * row * pitch + c), scale[2 * row * groups + slot / lanes], g);
+  load16<__nv_bfloat16, R>(dh + row * lddh + c, F - c, d);
+  decode16(*reinterpret_cast<const uint4*>(q + 2 * row * pitch + c), scale[2 * row * groups + (slot >> lanes_log2)], g);
   decode16(*reinterpret_cast<const uint4*>(q + (2 * row + 1) * pitch + c),
-           scale[(2 * row + 1) * groups + slot / lanes], u);
+           scale[(2 * row + 1) * groups + (slot >> lanes_log2)], u);
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    const float s = __fdividef(1.f, 1.f + __expf(-g[i]));
+    const float s = sigmoid(g[i]);
     const float gs = g[i] * s;
     hv[i] = gs * u[i];
     u[i] = d[i] * u[i] * s * (1.f + g[i] * (1.f - s));  // dg
     g[i] = d[i] * gs;                                   // du
   }
-  store16<__nv_bfloat16, true>(dgu + row * lddgu + c, F - c, u);
-  store16<__nv_bfloat16, true>(dgu + row * lddgu + F + c, F - c, g);
-  store16<__nv_bfloat16, true>(h8 + row * ldh + c, F - c, hv);
+  store16<__nv_bfloat16, R>(dgu + row * lddgu + c, F - c, u);
+  store16<__nv_bfloat16, R>(dgu + row * lddgu + F + c, F - c, g);
+  store16<__nv_bfloat16, R>(h8 + row * ldh + c, F - c, hv);
 }
 
 // ------------------------------------------------------------------ host side
-unsigned blocks_for(int64_t threads) {
-  const int64_t b = (threads + 255) / 256;
-  TORCH_CHECK(b < (int64_t(1) << 31), "act8: tensor too large for one launch");
-  return static_cast<unsigned>(b);
+unsigned blocks_for(int64_t threads) {  // 2^31 threads are 2^35 values
+  TORCH_CHECK_VALUE(threads < (int64_t(1) << 31) - 256, "act8: tensor too large for one launch");
+  return static_cast<unsigned>((threads + 255) / 256);
 }
 
-bool aligned16(const torch::Tensor& t) {
-  return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && (t.stride(0) * t.element_size()) % 16 == 0;
+int log2_lanes(int64_t group) { return group == 32 ? 1 : group == 64 ? 2 : group == 128 ? 3 : 4; }
+
+FastDiv divider(int64_t slots) {
+  FastDiv f;
+  f.set(static_cast<uint32_t>(slots));
+  return f;
+}
+
+Rows rows_of(const torch::Tensor& t) {
+  const auto p = reinterpret_cast<uintptr_t>(t.data_ptr());
+  const int64_t pitch = (t.dim() > 1 && t.size(0) > 1 ? t.stride(0) : 0) * t.element_size();
+  return p % 32 == 0 && pitch % 32 == 0 ? kRows32 : p % 16 == 0 && pitch % 16 == 0 ? kRows16 : kRowsAny;
+}
+
+void check_group(int64_t group) {
+  TORCH_CHECK_VALUE(group == 32 || group == 64 || group == 128 || group == 256,
+                    "act8: group must be 32, 64, 128 or 256, got ", group);
+}
+
+// x as rows over its last dimension, with a unit inner stride; `vec`: on 16-byte boundaries too.
+torch::Tensor as_rows(const torch::Tensor& x, const char* name, bool vec) {
+  TORCH_CHECK_VALUE(x.dim() >= 1, "act8: ", name, " needs at least one dimension");
+  TORCH_CHECK_VALUE(x.is_cuda(), "act8: ", name, " must be a CUDA tensor");
+  const int64_t n = x.size(-1);
+  int64_t rows = 1;
+  for (int i = 0; i + 1 < x.dim(); ++i) rows *= x.size(i);
+  torch::Tensor r = x.dim() == 2 ? x : x.reshape({rows, n});
+  if (n > 1 && r.stride(1) != 1) r = r.contiguous();
+  if (vec) {
+    TORCH_CHECK(x.scalar_type() == at::kBFloat16, "act8: ", name, " must be bf16 on CUDA, got ", x.scalar_type());
+    TORCH_CHECK(n >= 8 && n % 8 == 0, "act8: rows of ", name, " must hold a multiple of 8 values, got ", n);
+    if (rows_of(r) == kRowsAny) r = r.clone(at::MemoryFormat::Contiguous);
+  }
+  return r;
+}
+
+std::pair<torch::Tensor, torch::Tensor> code_buffers(const torch::Tensor& like, int64_t rows, int64_t n,
+                                                     int64_t group) {
+  return {torch::empty({rows, (n + 15) / 16 * 16}, like.options().dtype(at::kChar)),
+          torch::empty({rows, (n + group - 1) / group}, like.options().dtype(at::kFloat))};
 }
 
 void check_code(const torch::Tensor& q, const torch::Tensor& scale, int64_t code_rows, int64_t n, int64_t group) {
-  TORCH_CHECK(group == 32 || group == 64 || group == 128 || group == 256,
-              "act8: group must be 32, 64, 128 or 256, got ", group);
+  check_group(group);
   TORCH_CHECK(q.is_cuda() && scale.is_cuda() && q.scalar_type() == at::kChar && scale.scalar_type() == at::kFloat,
               "act8: codes must be int8 and scales fp32 CUDA tensors");
-  TORCH_CHECK(q.dim() == 2 && q.is_contiguous() && q.size(0) == code_rows && q.size(1) == (n + 15) / 16 * 16,
-              "act8: codes must be contiguous [rows, n rounded up to 16]");
+  TORCH_CHECK(q.dim() == 2 && q.is_contiguous() && q.size(0) == code_rows && q.size(1) == (n + 15) / 16 * 16 &&
+                  reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0,
+              "act8: codes must be contiguous [rows, n rounded up to 16] on a 16-byte boundary");
   TORCH_CHECK(scale.dim() == 2 && scale.is_contiguous() && scale.size(0) == code_rows &&
                   scale.size(1) == (n + group - 1) / group,
               "act8: scales must be contiguous [rows, groups]");
-  TORCH_CHECK(reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0, "act8: codes must be 16-byte aligned");
 }
 
-void check_rows(const torch::Tensor& t, int64_t rows, int64_t n, const char* name) {
-  TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kBFloat16 && t.dim() == 2 && t.size(0) == rows &&
-                  t.size(1) == n && t.stride(1) == 1 && aligned16(t),
-              "act8: ", name, " must be a bf16 CUDA tensor [", rows, ", ", n,
-              "] with unit inner stride and 16-byte aligned rows");
+torch::Tensor check_weight(const torch::Tensor& w, int64_t H) {
+  TORCH_CHECK(w.is_cuda() && w.scalar_type() == at::kBFloat16 && w.numel() == H,
+              "act8: the weight must be a bf16 CUDA vector of ", H, " values");
+  return w.is_contiguous() && rows_of(w) != kRowsAny ? w : w.clone(at::MemoryFormat::Contiguous);
+}
+
+const __nv_bfloat16* bf16(const torch::Tensor& t) { return reinterpret_cast<const __nv_bfloat16*>(t.data_ptr()); }
+__nv_bfloat16* bf16_out(torch::Tensor& t) { return reinterpret_cast<__nv_bfloat16*>(t.data_ptr()); }
+
+template <typename T>
+void launch_quantize(Rows r, unsigned grid, cudaStream_t st, const torch::Tensor& x, torch::Tensor& q,
+                     torch::Tensor& scale, int lanes) {
+  auto kern = r == kRows32 ? quantize_kernel<T, kRows32>
+                           : r == kRows16 ? quantize_kernel<T, kRows16> : quantize_kernel<T, kRowsAny>;
+  kern<<<grid, 256, 0, st>>>(reinterpret_cast<const T*>(x.data_ptr()), q.data_ptr<int8_t>(), scale.data_ptr<float>(),
+                             x.size(0), x.size(1), x.stride(0), q.size(1), scale.size(1), lanes,
+                             divider(scale.size(1) << lanes));
+}
+template <typename T>
+void launch_dequantize(Rows r, unsigned grid, cudaStream_t st, const torch::Tensor& q, const torch::Tensor& scale,
+                       torch::Tensor& x, int64_t rows, int n, int lanes) {
+  auto kern = r == kRows32 ? dequantize_kernel<T, kRows32>
+                           : r == kRows16 ? dequantize_kernel<T, kRows16> : dequantize_kernel<T, kRowsAny>;
+  kern<<<grid, 256, 0, st>>>(q.data_ptr<int8_t>(), scale.data_ptr<float>(), reinterpret_cast<T*>(x.data_ptr()), rows,
+                             n, n, q.size(1), scale.size(1), lanes, divider((n + kChunk - 1) / kChunk));
 }
 
 }  // namespace
 
-void act8_quantize(const torch::Tensor& x, torch::Tensor& q, torch::Tensor& scale, int64_t group) {
-  TORCH_CHECK(x.is_cuda() && x.dim() == 2 && (x.size(1) <= 1 || x.stride(1) == 1),
-              "act8_quantize: a 2-D CUDA tensor with unit inner stride is required");
-  const int64_t rows = x.size(0);
-  const int n = x.size(1);
-  check_code(q, scale, rows, n, group);
-  if (rows == 0 || n == 0) return;
+// (codes, scales) of x (bf16, fp16 or fp32), groups along its last dimension.
+std::tuple<torch::Tensor, torch::Tensor> act8_quantize(const torch::Tensor& x, int64_t group) {
+  check_group(group);
+  const auto type = x.scalar_type();
+  TORCH_CHECK(type == at::kBFloat16 || type == at::kHalf || type == at::kFloat,
+              "act8.quantize: bf16, fp16 or fp32 expected, got ", type);
   const c10::cuda::CUDAGuard guard(x.device());
+  const torch::Tensor r = as_rows(x, "x", false);
+  const int64_t rows = r.size(0), n = r.size(1);
+  TORCH_CHECK_VALUE(n < (int64_t(1) << 31), "act8: rows too long");
+  auto [q, scale] = code_buffers(r, rows, n, group);
+  if (rows == 0 || n == 0) return {q, scale};
   auto st = at::cuda::getCurrentCUDAStream();
-  const int lanes = group / kChunk, groups = scale.size(1);
-  const unsigned grid = blocks_for(rows * groups * lanes);
-  const bool al = aligned16(x);
-#define FT_Q(T, AL)                                                                                    \
-  quantize_kernel<T, AL><<<grid, 256, 0, st>>>(reinterpret_cast<const T*>(x.data_ptr()),               \
-                                               q.data_ptr<int8_t>(), scale.data_ptr<float>(), rows, n, \
-                                               x.stride(0), q.size(1), groups, lanes)
-#define FT_QA(T) do { if (al) FT_Q(T, true); else FT_Q(T, false); } while (0)
-  if (x.scalar_type() == at::kBFloat16) FT_QA(__nv_bfloat16);
-  else if (x.scalar_type() == at::kHalf) FT_QA(__half);
-  else if (x.scalar_type() == at::kFloat) FT_QA(float);
-  else TORCH_CHECK(false, "act8_quantize: bf16, fp16 or fp32 expected, got ", x.scalar_type());
-#undef FT_QA
-#undef FT_Q
+  const int lanes = log2_lanes(group);
+  const unsigned grid = blocks_for(rows * (scale.size(1) << lanes));
+  if (type == at::kBFloat16) launch_quantize<__nv_bfloat16>(rows_of(r), grid, st, r, q, scale, lanes);
+  else if (type == at::kHalf) launch_quantize<__half>(rows_of(r), grid, st, r, q, scale, lanes);
+  else launch_quantize<float>(rows_of(r), grid, st, r, q, scale, lanes);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {q, scale};
 }
 
-void act8_dequantize(const torch::Tensor& q, const torch::Tensor& scale, torch::Tensor& x, int64_t group) {
-  TORCH_CHECK(x.is_cuda() && x.dim() == 2 && (x.size(1) <= 1 || x.stride(1) == 1),
-              "act8_dequantize: a 2-D CUDA output with unit inner stride is required");
-  const int64_t rows = x.size(0);
-  const int n = x.size(1);
-  check_code(q, scale, rows, n, group);
-  if (rows == 0 || n == 0) return;
-  const c10::cuda::CUDAGuard guard(x.device());
+// The kept values as a contiguous tensor of `sizes` (rows of n values).
+torch::Tensor act8_dequantize(const torch::Tensor& q, const torch::Tensor& scale, const std::vector<int64_t>& sizes,
+                              int64_t n, torch::ScalarType dtype, int64_t group) {
+  check_code(q, scale, q.size(0), n, group);
+  TORCH_CHECK(dtype == at::kBFloat16 || dtype == at::kHalf || dtype == at::kFloat,
+              "act8.dequantize: bf16, fp16 or fp32 expected, got ", dtype);
+  const c10::cuda::CUDAGuard guard(q.device());
+  torch::Tensor x = torch::empty(sizes, q.options().dtype(dtype));
+  const int64_t rows = q.size(0);
+  TORCH_CHECK(x.numel() == rows * n, "act8.dequantize: codes of ", rows * n, " values do not fit ", x.sizes());
+  if (x.numel() == 0) return x;
   auto st = at::cuda::getCurrentCUDAStream();
-  const int lanes = group / kChunk, groups = scale.size(1);
+  const int lanes = log2_lanes(group);
   const unsigned grid = blocks_for(rows * ((n + kChunk - 1) / kChunk));
-  const bool al = aligned16(x);
-#define FT_D(T, AL)                                                                                        \
-  dequantize_kernel<T, AL><<<grid, 256, 0, st>>>(q.data_ptr<int8_t>(), scale.data_ptr<float>(),            \
-                                                 reinterpret_cast<T*>(x.data_ptr()), rows, n, x.stride(0), \
-                                                 q.size(1), groups, lanes)
-#define FT_DA(T) do { if (al) FT_D(T, true); else FT_D(T, false); } while (0)
-  if (x.scalar_type() == at::kBFloat16) FT_DA(__nv_bfloat16);
-  else if (x.scalar_type() == at::kHalf) FT_DA(__half);
-  else if (x.scalar_type() == at::kFloat) FT_DA(float);
-  else TORCH_CHECK(false, "act8_dequantize: bf16, fp16 or fp32 expected, got ", x.scalar_type());
-#undef FT_DA
-#undef FT_D
+  const int64_t pitch = n * x.element_size();  // the allocation itself starts on a 512-byte boundary
+  const Rows r = rows == 1 || pitch % 32 == 0 ? kRows32 : pitch % 16 == 0 ? kRows16 : kRowsAny;
+  if (dtype == at::kBFloat16) launch_dequantize<__nv_bfloat16>(r, grid, st, q, scale, x, rows, n, lanes);
+  else if (dtype == at::kHalf) launch_dequantize<__half>(r, grid, st, q, scale, x, rows, n, lanes);
+  else launch_dequantize<float>(r, grid, st, q, scale, x, rows, n, lanes);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return x;
 }
 
 // Threads per row and chunks per thread for a row of H values.
@@ -451,114 +723,131 @@ void act8_dequantize(const torch::Tensor& q, const torch::Tensor& scale, torch::
   else if (H <= 8192) LAUNCH(512, 1);   \
   else LAUNCH(512, 2)
 
-void act8_rms_norm(const torch::Tensor& x, const torch::Tensor& w, torch::Tensor& y, torch::Tensor& rstd,
-                   torch::Tensor& q, torch::Tensor& scale, int64_t group, double eps) {
-  const int64_t rows = x.size(0);
-  const int H = x.size(1);
-  TORCH_CHECK(H % 8 == 0 && H >= 8 && H <= 16384, "act8_rms_norm: H must be a multiple of 8, at most 16384");
-  check_rows(x, rows, H, "x");
-  check_rows(y, rows, H, "y");
-  check_code(q, scale, rows, H, group);
-  TORCH_CHECK(w.is_cuda() && w.scalar_type() == at::kBFloat16 && w.numel() == H && w.is_contiguous() &&
-                  reinterpret_cast<uintptr_t>(w.data_ptr()) % 16 == 0,
-              "act8_rms_norm: w must be a contiguous bf16 vector of H values");
-  TORCH_CHECK(rstd.is_cuda() && rstd.scalar_type() == at::kFloat && rstd.numel() == rows && rstd.is_contiguous());
-  if (rows == 0) return;
+// (y, rstd, codes, scales)
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> act8_rms_norm(const torch::Tensor& x,
+                                                                                     const torch::Tensor& weight,
+                                                                                     double eps, int64_t group) {
+  check_group(group);
   const c10::cuda::CUDAGuard guard(x.device());
+  const torch::Tensor r = as_rows(x, "x", true);
+  const int64_t rows = r.size(0);
+  const int H = r.size(1);
+  TORCH_CHECK(H <= 16384, "act8.rms_norm: at most 16384 values per row, got ", H);
+  const torch::Tensor w = check_weight(weight, H);
+  torch::Tensor y = torch::empty(x.sizes(), r.options());
+  torch::Tensor rstd = torch::empty({rows}, r.options().dtype(at::kFloat));
+  auto [q, scale] = code_buffers(r, rows, H, group);
+  if (rows == 0) return {y, rstd, q, scale};
   auto st = at::cuda::getCurrentCUDAStream();
-  const int lanes = group / kChunk, groups = scale.size(1);
-#define FT_L(NT, VPT)                                                                                       \
-  rms_norm8_kernel<NT, VPT><<<(rows + (NT >= 128 ? 1 : 128 / NT) - 1) / (NT >= 128 ? 1 : 128 / NT),         \
-                              NT >= 128 ? NT : 128, 0, st>>>(                                               \
-      reinterpret_cast<const __nv_bfloat16*>(x.data_ptr()),                                                 \
-      reinterpret_cast<const __nv_bfloat16*>(w.data_ptr()), reinterpret_cast<__nv_bfloat16*>(y.data_ptr()), \
-      rstd.data_ptr<float>(), q.data_ptr<int8_t>(), scale.data_ptr<float>(), rows, H, x.stride(0),          \
-      y.stride(0), q.size(1), groups, lanes, static_cast<float>(eps))
+  const int lanes = log2_lanes(group), groups = scale.size(1);
+  const bool wide = H % 16 == 0 && rows_of(r) == kRows32 && rows_of(w) == kRows32;
+#define FT_L(NT, VPT)                                                                                             \
+  do {                                                                                                            \
+    constexpr int rpb = NT >= 128 ? 1 : 128 / NT;                                                                 \
+    auto kern = wide ? rms_norm8_kernel<NT, VPT, kRows32> : rms_norm8_kernel<NT, VPT, kRows16>;                   \
+    kern<<<static_cast<unsigned>((rows + rpb - 1) / rpb), rpb * NT, 0, st>>>(                                     \
+        bf16(r), bf16(w), bf16_out(y), rstd.data_ptr<float>(), q.data_ptr<int8_t>(), scale.data_ptr<float>(), rows, \
+        H, r.stride(0), H, q.size(1), groups, lanes, static_cast<float>(eps));                                    \
+  } while (0)
   FT_NORM8_SIZES(FT_L);
 #undef FT_L
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {y, rstd, q, scale};
 }
 
-// Rows that may write a share of dw: the size of the workspace that act8_rms_norm_bwd needs.
-int64_t act8_norm_walkers(int64_t rows, int64_t H) {
-  const int64_t sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-  const int64_t most = H <= 1024 ? sms * 16 : H <= 2048 ? sms * 8 : H <= 4096 ? sms * 4 : sms * 2;
-  const int64_t per = (rows + most - 1) / most;
-  return rows == 0 ? 0 : (rows + per - 1) / per;
-}
-
-void act8_rms_norm_bwd(const torch::Tensor& dy, const torch::Tensor& q, const torch::Tensor& scale,
-                       const torch::Tensor& w, const torch::Tensor& rstd, torch::Tensor& dx, torch::Tensor& y8,
-                       torch::Tensor& dw, torch::Tensor& part, int64_t group) {
-  const int64_t rows = dy.size(0);
-  const int H = dy.size(1);
-  TORCH_CHECK(H % 8 == 0 && H >= 8 && H <= 16384, "act8_rms_norm_bwd: H must be a multiple of 8, at most 16384");
-  check_rows(dy, rows, H, "dy");
-  check_rows(dx, rows, H, "dx");
-  check_rows(y8, rows, H, "y8");
-  check_code(q, scale, rows, H, group);
-  TORCH_CHECK(w.is_cuda() && w.scalar_type() == at::kBFloat16 && w.numel() == H && w.is_contiguous() &&
-                  reinterpret_cast<uintptr_t>(w.data_ptr()) % 16 == 0);
-  TORCH_CHECK(rstd.is_cuda() && rstd.scalar_type() == at::kFloat && rstd.numel() == rows && rstd.is_contiguous());
-  TORCH_CHECK(dw.is_cuda() && dw.scalar_type() == at::kFloat && dw.numel() == H && dw.is_contiguous());
-  const int64_t walkers = act8_norm_walkers(rows, H);
-  TORCH_CHECK(part.is_cuda() && part.scalar_type() == at::kFloat && part.is_contiguous() &&
-                  part.numel() >= walkers * H && reinterpret_cast<uintptr_t>(part.data_ptr()) % 16 == 0,
-              "act8_rms_norm_bwd: workspace too small");
+// (dx, dw, y8)
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> act8_rms_norm_bwd(
+    const torch::Tensor& dy, const torch::Tensor& q, const torch::Tensor& scale, const torch::Tensor& weight,
+    const torch::Tensor& rstd, int64_t group, torch::Tensor& err) {
   const c10::cuda::CUDAGuard guard(dy.device());
+  const torch::Tensor g = as_rows(dy, "dy", true);
+  const int64_t rows = g.size(0);
+  const int H = g.size(1);
+  TORCH_CHECK(H <= 16384, "act8.rms_norm_bwd: at most 16384 values per row, got ", H);
+  check_code(q, scale, rows, H, group);
+  const torch::Tensor w = check_weight(weight, H);
+  TORCH_CHECK(rstd.is_cuda() && rstd.scalar_type() == at::kFloat && rstd.numel() == rows && rstd.is_contiguous());
+  const auto f32 = g.options().dtype(at::kFloat);
+  torch::Tensor dx = torch::empty(dy.sizes(), g.options()), y8 = torch::empty(dy.sizes(), g.options());
+  if (rows == 0) return {dx, torch::zeros({H}, f32), y8};
   auto st = at::cuda::getCurrentCUDAStream();
-  if (rows > 0) {
-    const int rpw = static_cast<int>((rows + walkers - 1) / walkers);
-    const int lanes = group / kChunk, groups = scale.size(1);
-#define FT_L(NT, VPT)                                                                                          \
-  rms_norm8_bwd_kernel<NT, VPT><<<(walkers + (NT >= 128 ? 1 : 128 / NT) - 1) / (NT >= 128 ? 1 : 128 / NT),     \
-                                  NT >= 128 ? NT : 128, 0, st>>>(                                              \
-      reinterpret_cast<const __nv_bfloat16*>(dy.data_ptr()), q.data_ptr<int8_t>(), scale.data_ptr<float>(),    \
-      reinterpret_cast<const __nv_bfloat16*>(w.data_ptr()), rstd.data_ptr<float>(),                            \
-      reinterpret_cast<__nv_bfloat16*>(dx.data_ptr()), reinterpret_cast<__nv_bfloat16*>(y8.data_ptr()),        \
-      part.data_ptr<float>(), rows, H, dy.stride(0), dx.stride(0), y8.stride(0), q.size(1), groups, lanes, rpw)
-    FT_NORM8_SIZES(FT_L);
+  // as many walkers as blocks (or, for short rows, warps) are resident, or one per row: 512
+  // threads per SM with everything in registers (49.1 us for 4096 x 8192) do better than 1024 that
+  // decode a row twice (55.0 us), and write half as many shares of dw
+  const int64_t sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  const int64_t most = H <= 1024 ? sms * 16 : H <= 2048 ? sms * 4 : H <= 4096 ? sms * 2 : sms;
+  const int64_t per = (rows + most - 1) / most, walkers = (rows + per - 1) / per;
+  torch::Tensor dw = torch::empty({H}, f32), part = torch::empty({walkers, H}, f32);
+  const int lanes = log2_lanes(group), groups = scale.size(1);
+  const bool wide = H % 16 == 0 && rows_of(g) == kRows32 && rows_of(w) == kRows32;
+  const int smem = kStages * static_cast<int>(q.size(1) + 2 * (int64_t)H);
+#define FT_ARGS                                                                                                  \
+  bf16(g), q.data_ptr<int8_t>(), scale.data_ptr<float>(), bf16(w), rstd.data_ptr<float>(), bf16_out(dx),         \
+      bf16_out(y8), part.data_ptr<float>(), rows, H, g.stride(0), q.size(1), groups, lanes, static_cast<int>(per)
+#define FT_L(NT, VPT)                                                                                            \
+  do {                                                                                                           \
+    if constexpr (NT == 32) {                                                                                    \
+      auto kern = wide ? rms_norm8_bwd_warp_kernel<VPT, kRows32> : rms_norm8_bwd_warp_kernel<VPT, kRows16>;      \
+      kern<<<static_cast<unsigned>((walkers + 3) / 4), 128, 0, st>>>(FT_ARGS);                                   \
+    } else {                                                                                                     \
+      constexpr int nt = NT < 128 ? 128 : NT;                                                                    \
+      auto kern = wide ? rms_norm8_bwd_kernel<nt, VPT, kRows32> : rms_norm8_bwd_kernel<nt, VPT, kRows16>;        \
+      static unsigned long long done[2] = {0, 0};                                                                \
+      smem_attr_once(kern, kStages * 3 * 16 * nt * VPT, done[wide]);                                             \
+      kern<<<static_cast<unsigned>(walkers), nt, smem, st>>>(FT_ARGS, err.data_ptr<int>());                      \
+    }                                                                                                            \
+  } while (0)
+  FT_NORM8_SIZES(FT_L);
 #undef FT_L
-    C10_CUDA_KERNEL_LAUNCH_CHECK();
-  }
-  dw_sum_kernel<<<(H + 31) / 32, 256, 0, st>>>(part.data_ptr<float>(), dw.data_ptr<float>(),
-                                               static_cast<int>(walkers), H);
+#undef FT_ARGS
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  dw_sum_kernel<<<(H + 31) / 32, 1024, 0, st>>>(part.data_ptr<float>(), dw.data_ptr<float>(),
+                                                static_cast<int>(walkers), H);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {dx, dw, y8};
 }
 
-void act8_swiglu(const torch::Tensor& gu, torch::Tensor& h, torch::Tensor& q, torch::Tensor& scale, int64_t group) {
-  const int64_t rows = h.size(0);
-  const int F = h.size(1);
-  TORCH_CHECK(F % 8 == 0 && F >= 8, "act8_swiglu: F must be a multiple of 8");
-  check_rows(gu, rows, 2 * (int64_t)F, "gu");
-  check_rows(h, rows, F, "h");
-  check_code(q, scale, 2 * rows, F, group);
-  if (rows == 0) return;
+// (h, codes, scales) of gu = [gate | up]
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> act8_swiglu(const torch::Tensor& gu, int64_t group) {
+  check_group(group);
   const c10::cuda::CUDAGuard guard(gu.device());
-  const int lanes = group / kChunk, groups = scale.size(1);
-  swiglu8_kernel<<<blocks_for(rows * groups * lanes), 256, 0, at::cuda::getCurrentCUDAStream()>>>(
-      reinterpret_cast<const __nv_bfloat16*>(gu.data_ptr()), reinterpret_cast<__nv_bfloat16*>(h.data_ptr()),
-      q.data_ptr<int8_t>(), scale.data_ptr<float>(), rows, F, gu.stride(0), h.stride(0), q.size(1), groups, lanes);
+  const torch::Tensor r = as_rows(gu, "gate and up", true);
+  const int64_t rows = r.size(0);
+  const int F = r.size(1) / 2;
+  TORCH_CHECK(r.size(1) % 16 == 0, "act8.swiglu: gate and up must hold a multiple of 8 values each, got ", r.size(1));
+  std::vector<int64_t> sizes = gu.sizes().vec();
+  sizes.back() = F;
+  torch::Tensor h = torch::empty(sizes, r.options());
+  auto [q, scale] = code_buffers(r, 2 * rows, F, group);
+  if (rows == 0) return {h, q, scale};
+  const int lanes = log2_lanes(group), groups = scale.size(1);
+  auto kern = F % 16 == 0 && rows_of(r) == kRows32 ? swiglu8_kernel<kRows32> : swiglu8_kernel<kRows16>;
+  kern<<<blocks_for(rows * ((int64_t)groups << lanes)), 256, 0, at::cuda::getCurrentCUDAStream()>>>(
+      bf16(r), bf16_out(h), q.data_ptr<int8_t>(), scale.data_ptr<float>(), rows, F, r.stride(0), F, q.size(1), groups,
+      lanes, divider((int64_t)groups << lanes));
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {h, q, scale};
 }
 
-void act8_swiglu_bwd(const torch::Tensor& dh, const torch::Tensor& q, const torch::Tensor& scale,
-                     torch::Tensor& dgu, torch::Tensor& h8, int64_t group) {
-  const int64_t rows = dh.size(0);
-  const int F = dh.size(1);
-  TORCH_CHECK(F % 8 == 0 && F >= 8, "act8_swiglu_bwd: F must be a multiple of 8");
-  check_rows(dh, rows, F, "dh");
-  check_rows(dgu, rows, 2 * (int64_t)F, "dgu");
-  check_rows(h8, rows, F, "h8");
-  check_code(q, scale, 2 * rows, F, group);
-  if (rows == 0) return;
+// (dgu, h8)
+std::tuple<torch::Tensor, torch::Tensor> act8_swiglu_bwd(const torch::Tensor& dh, const torch::Tensor& q,
+                                                         const torch::Tensor& scale, int64_t group) {
   const c10::cuda::CUDAGuard guard(dh.device());
-  const int lanes = group / kChunk, groups = scale.size(1);
-  swiglu8_bwd_kernel<<<blocks_for(rows * ((F + kChunk - 1) / kChunk)), 256, 0, at::cuda::getCurrentCUDAStream()>>>(
-      reinterpret_cast<const __nv_bfloat16*>(dh.data_ptr()), q.data_ptr<int8_t>(), scale.data_ptr<float>(),
-      reinterpret_cast<__nv_bfloat16*>(dgu.data_ptr()), reinterpret_cast<__nv_bfloat16*>(h8.data_ptr()), rows, F,
-      dh.stride(0), dgu.stride(0), h8.stride(0), q.size(1), groups, lanes);
+  const torch::Tensor r = as_rows(dh, "dh", true);
+  const int64_t rows = r.size(0);
+  const int F = r.size(1);
+  check_code(q, scale, 2 * rows, F, group);
+  std::vector<int64_t> sizes = dh.sizes().vec();
+  sizes.back() = 2 * F;
+  torch::Tensor dgu = torch::empty(sizes, r.options()), h8 = torch::empty(dh.sizes(), r.options());
+  if (rows == 0) return {dgu, h8};
+  const int lanes = log2_lanes(group), groups = scale.size(1);
+  auto kern = F % 16 == 0 && rows_of(r) == kRows32 ? swiglu8_bwd_kernel<kRows32> : swiglu8_bwd_kernel<kRows16>;
+  kern<<<blocks_for(rows * ((F + kChunk - 1) / kChunk)), 256, 0, at::cuda::getCurrentCUDAStream()>>>(
+      bf16(r), q.data_ptr<int8_t>(), scale.data_ptr<float>(), bf16_out(dgu), bf16_out(h8), rows, F, r.stride(0),
+      2 * (int64_t)F, F, q.size(1), groups, lanes, divider((F + kChunk - 1) / kChunk));
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {dgu, h8};
 }
 
 }  // namespace ft

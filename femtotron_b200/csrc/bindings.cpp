@@ -79,20 +79,22 @@ void flash_fwd_variant(const torch::Tensor& qkv, torch::Tensor& o, torch::Tensor
 void flash_bwd(const torch::Tensor& qkv, const torch::Tensor& o, const torch::Tensor& dout,
                const torch::Tensor& lse, torch::Tensor& dqkv, int64_t B, int64_t S, int64_t nq,
                int64_t nkv, int64_t D, torch::Tensor& err);
-void act8_quantize(const torch::Tensor& x, torch::Tensor& q, torch::Tensor& scale, int64_t group);
-void act8_dequantize(const torch::Tensor& q, const torch::Tensor& scale, torch::Tensor& x, int64_t group);
-void act8_rms_norm(const torch::Tensor& x, const torch::Tensor& w, torch::Tensor& y, torch::Tensor& rstd,
-                   torch::Tensor& q, torch::Tensor& scale, int64_t group, double eps);
-int64_t act8_norm_walkers(int64_t rows, int64_t H);
-void act8_rms_norm_bwd(const torch::Tensor& dy, const torch::Tensor& q, const torch::Tensor& scale,
-                       const torch::Tensor& w, const torch::Tensor& rstd, torch::Tensor& dx, torch::Tensor& y8,
-                       torch::Tensor& dw, torch::Tensor& part, int64_t group);
-void act8_swiglu(const torch::Tensor& gu, torch::Tensor& h, torch::Tensor& q, torch::Tensor& scale, int64_t group);
-void act8_swiglu_bwd(const torch::Tensor& dh, const torch::Tensor& q, const torch::Tensor& scale,
-                     torch::Tensor& dgu, torch::Tensor& h8, int64_t group);
-void rotary_qk(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& cos_t,
-               const torch::Tensor& sin_t, const c10::optional<torch::Tensor>& pos, torch::Tensor& oq,
-               torch::Tensor& ok, bool interleaved, bool inverse, torch::Tensor& err);
+std::tuple<torch::Tensor, torch::Tensor> act8_quantize(const torch::Tensor& x, int64_t group);
+torch::Tensor act8_dequantize(const torch::Tensor& q, const torch::Tensor& scale, const std::vector<int64_t>& sizes,
+                              int64_t n, torch::ScalarType dtype, int64_t group);
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> act8_rms_norm(const torch::Tensor& x,
+                                                                                     const torch::Tensor& weight,
+                                                                                     double eps, int64_t group);
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> act8_rms_norm_bwd(
+    const torch::Tensor& dy, const torch::Tensor& q, const torch::Tensor& scale, const torch::Tensor& weight,
+    const torch::Tensor& rstd, int64_t group, torch::Tensor& err);
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> act8_swiglu(const torch::Tensor& gu, int64_t group);
+std::tuple<torch::Tensor, torch::Tensor> act8_swiglu_bwd(const torch::Tensor& dh, const torch::Tensor& q,
+                                                         const torch::Tensor& scale, int64_t group);
+std::tuple<torch::Tensor, torch::Tensor> rotary_qk(const torch::Tensor& q, const torch::Tensor& k,
+                                                   const torch::Tensor& cos_t, const torch::Tensor& sin_t,
+                                                   const c10::optional<torch::Tensor>& pos, bool interleaved,
+                                                   bool inverse, bool inplace, torch::Tensor& err);
 std::vector<torch::Tensor> linear_xent_fwd(const torch::Tensor& h, const torch::Tensor& w,
                                            const torch::Tensor& labels, int64_t vstart, int64_t ignore_index,
                                            int64_t reduce, torch::Tensor& err);
@@ -146,7 +148,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("act8_quantize", &ft::act8_quantize, "groups of a row to int8 codes and fp32 scales");
   m.def("act8_dequantize", &ft::act8_dequantize);
   m.def("act8_rms_norm", &ft::act8_rms_norm, "RMSNorm that also keeps its input in 8 bits");
-  m.def("act8_norm_walkers", &ft::act8_norm_walkers, "rows of the act8_rms_norm_bwd workspace");
   m.def("act8_rms_norm_bwd", &ft::act8_rms_norm_bwd, "RMSNorm backward from the 8-bit input");
   m.def("act8_swiglu", &ft::act8_swiglu, "SwiGLU that also keeps gate and up in 8 bits");
   m.def("act8_swiglu_bwd", &ft::act8_swiglu_bwd, "SwiGLU backward from 8-bit gate and up");

@@ -386,6 +386,22 @@ FT_DEVICE float ex2_approx(float x) {
   return y;
 }
 
+// n / d for 0 <= n < 2^31 by one multiplication: with 2^(l-1) < d <= 2^l and
+// m = floor(2^(31+l) / d) + 1, the error of n m / 2^(31+l) stays below 1 / d.
+struct FastDiv {
+  uint32_t d = 1, m = 0x80000001u, shift = 31;
+  void set(uint32_t div) {
+    uint32_t l = 0;
+    while ((uint64_t(1) << l) < div) ++l;
+    d = div;
+    shift = 31 + l;
+    m = static_cast<uint32_t>((uint64_t(1) << shift) / div + 1);
+  }
+  FT_DEVICE uint32_t div(uint32_t n) const {
+    return static_cast<uint32_t>((static_cast<uint64_t>(n) * m) >> shift);
+  }
+};
+
 // Warp / block reductions
 FT_DEVICE float warp_sum(float v) {
 #pragma unroll

@@ -215,6 +215,114 @@ struct XentProductEpi {
   }
 };
 
+// ------------------------------------------------------------------ few tokens
+// The forward for at most kFewTokens tokens: one read of w, and nothing for the tensor cores to
+// win (a 128-row tile would be nearly empty).  A warp takes two vocabulary rows at a time, 2 x 4
+// packs of E values in flight per lane; h lies in shared memory in fp32, one plane per 4 of a
+// pack's E values, so that the lanes of a 16-byte read touch neighbouring words.  Every warp keeps a
+// running (max, sum) per token; a block leaves one pair per token, like a tile of the GEMM.
+constexpr int kFewTokens = 4;
+constexpr int kFewThreads = 256;
+
+template <int TOK, int E>  // E: 16 values per pack where rows lie on 32-byte boundaries, else 8
+__global__ void __launch_bounds__(kFewThreads, 2)
+    xent_few_kernel(const __nv_bfloat16* __restrict__ h, int64_t ldh, const __nv_bfloat16* __restrict__ w, int64_t ldw,
+                    const int64_t* __restrict__ labels, float2* __restrict__ part, float* __restrict__ target, int T,
+                    int V, int H, int64_t vstart) {
+  extern __shared__ __align__(16) float hs[];  // [TOK][E / 4][packs][4]
+  __shared__ float2 red[kFewThreads / 32][TOK];
+  constexpr int U = 4;
+  const int packs = H / E, lane = threadIdx.x % 32;
+  for (int i = threadIdx.x; i < TOK * H; i += kFewThreads) {
+    const int t = i / H, k = i - t * H, g = k / E, r = k - g * E;
+    hs[((t * (E / 4) + r / 4) * packs + g) * 4 + r % 4] =
+        t < T ? __bfloat162float(h[t * ldh + k]) : 0.f;
+  }
+  __syncthreads();
+  float m[TOK], s[TOK];
+#pragma unroll
+  for (int t = 0; t < TOK; ++t) { m[t] = -INFINITY; s[t] = 0.f; }
+  const int warps = gridDim.x * (kFewThreads / 32);
+  for (int row = 2 * (blockIdx.x * (kFewThreads / 32) + threadIdx.x / 32); row < V; row += 2 * warps) {
+    const __nv_bfloat16* wr[2] = {w + row * ldw, w + min(row + 1, V - 1) * ldw};
+    float acc[2][TOK];
+#pragma unroll
+    for (int t = 0; t < TOK; ++t) acc[0][t] = acc[1][t] = 0.f;
+    for (int g0 = lane; g0 < packs; g0 += 32 * U) {
+      uint32_t x[2][U][E / 2];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int g = g0 + 32 * u;
+          const __nv_bfloat16* at = wr[j] + g * E;
+#pragma unroll
+          for (int i = 0; i < E / 2; ++i) x[j][u][i] = 0;
+          if (g < packs) {
+            if constexpr (E == 16)
+              asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                           : "=r"(x[j][u][0]), "=r"(x[j][u][1]), "=r"(x[j][u][2]), "=r"(x[j][u][3]), "=r"(x[j][u][4]),
+                             "=r"(x[j][u][5]), "=r"(x[j][u][6]), "=r"(x[j][u][7])
+                           : "l"(__cvta_generic_to_global(at)));
+            else {
+              const uint4 q = *reinterpret_cast<const uint4*>(at);
+              x[j][u][0] = q.x; x[j][u][1] = q.y; x[j][u][2] = q.z; x[j][u][3] = q.w;
+            }
+          }
+        }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int g = min(g0 + 32 * u, packs - 1);  // past the end x is 0
+#pragma unroll
+        for (int q = 0; q < E / 4; ++q) {
+          float4 hv[TOK];
+#pragma unroll
+          for (int t = 0; t < TOK; ++t)
+            hv[t] = *reinterpret_cast<const float4*>(hs + ((t * (E / 4) + q) * packs + g) * 4);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint32_t a = x[j][u][2 * q], b = x[j][u][2 * q + 1];
+            const float a0 = __uint_as_float(a << 16), a1 = __uint_as_float(a & 0xffff0000u);
+            const float b0 = __uint_as_float(b << 16), b1 = __uint_as_float(b & 0xffff0000u);
+#pragma unroll
+            for (int t = 0; t < TOK; ++t)
+              acc[j][t] = fmaf(b1, hv[t].w, fmaf(b0, hv[t].z, fmaf(a1, hv[t].y, fmaf(a0, hv[t].x, acc[j][t]))));
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      if (row + j >= V) break;  // the same for the whole warp
+#pragma unroll
+      for (int t = 0; t < TOK; ++t) {
+        const float x = warp_sum(acc[j][t]);
+        const float nm = fmaxf(m[t], x);
+        const float base = nm == -INFINITY ? 0.f : nm * kLog2e;
+        s[t] = s[t] * ex2_approx(fmaf(m[t], kLog2e, -base)) + ex2_approx(fmaf(x, kLog2e, -base));
+        m[t] = nm;
+        if (lane == 0 && t < T && labels[t] == vstart + row + j) target[t] = x;
+      }
+    }
+  }
+  if (lane == 0) {
+#pragma unroll
+    for (int t = 0; t < TOK; ++t) red[threadIdx.x / 32][t] = make_float2(m[t], s[t]);
+  }
+  __syncthreads();
+  if (threadIdx.x < T) {
+    float2 v = red[0][threadIdx.x];
+    for (int i = 1; i < kFewThreads / 32; ++i) {
+      const float2 o = red[i][threadIdx.x];
+      const float nm = fmaxf(v.x, o.x);
+      const float base = nm == -INFINITY ? 0.f : nm * kLog2e;
+      v.y = v.y * ex2_approx(fmaf(v.x, kLog2e, -base)) + o.y * ex2_approx(fmaf(o.x, kLog2e, -base));
+      v.x = nm;
+    }
+    part[threadIdx.x * gridDim.x + blockIdx.x] = v;
+  }
+}
+
 // ------------------------------------------------------------------ small kernels
 // One warp per row joins the tiles' (max, sum); stats[row] = (max, sum, target, has target).
 __global__ void __launch_bounds__(256) xent_join_kernel(const float2* __restrict__ part,
@@ -415,17 +523,36 @@ std::vector<torch::Tensor> linear_xent_fwd(const torch::Tensor& h, const torch::
   check_operands(h, w, labels, err);
   const c10::cuda::CUDAGuard guard(h.device());
   auto st = at::cuda::getCurrentCUDAStream();
-  const int T = h.size(0), V = w.size(0);
-  const int bn = logits_bn(T, V), tiles_n = (V + bn - 1) / bn;
+  const int T = h.size(0), V = w.size(0), H = h.size(1);
+  // few tokens: a read of w by plain loads (see xent_few_kernel), while h fits beside two blocks
+  const int tok = T <= 1 ? 1 : T <= 2 ? 2 : 4;
+  const int few_bytes = tok * H * 4;
+  const bool few = T <= kFewTokens && few_bytes <= 96 * 1024;
+  const int bn = logits_bn(T, V);
+  const int tiles_n = few ? std::min((V + 15) / 16, 2 * num_sms()) : (V + bn - 1) / bn;
   const auto f32 = h.options().dtype(at::kFloat);
   // one buffer: tiles' partials, target logits, then the results
   torch::Tensor part = torch::empty({(int64_t)T * tiles_n * 2 + T}, f32);
   torch::Tensor stats = torch::empty({T, 4}, f32), lse_t = torch::empty({T}, f32), losses = torch::empty({T}, f32);
   float* target = part.data_ptr<float>() + (int64_t)T * tiles_n * 2;
-  Params p = base_params(T, V, h.size(1), err);
-  XentStatsEpi::Args e{labels.data_ptr<int64_t>(), reinterpret_cast<float2*>(part.data_ptr<float>()), target, vstart,
-                       tiles_n};
-  logits_gemm<XentStatsEpi>(h, w, 0, V, p, e, bn, st);
+  if (few) {
+    const bool wide = H % 16 == 0 && w.stride(0) % 16 == 0 && reinterpret_cast<uintptr_t>(w.data_ptr()) % 32 == 0;
+    auto kern = tok == 1   ? (wide ? xent_few_kernel<1, 16> : xent_few_kernel<1, 8>)
+                : tok == 2 ? (wide ? xent_few_kernel<2, 16> : xent_few_kernel<2, 8>)
+                           : (wide ? xent_few_kernel<4, 16> : xent_few_kernel<4, 8>);
+    static unsigned long long done[6] = {0, 0, 0, 0, 0, 0};
+    smem_attr_once(kern, 96 * 1024, done[(tok == 4 ? 4 : 2 * (tok - 1)) + wide]);
+    kern<<<tiles_n, kFewThreads, few_bytes, st>>>(
+        reinterpret_cast<const __nv_bfloat16*>(h.data_ptr()), h.stride(0),
+        reinterpret_cast<const __nv_bfloat16*>(w.data_ptr()), w.stride(0), labels.data_ptr<int64_t>(),
+        reinterpret_cast<float2*>(part.data_ptr<float>()), target, T, V, H, vstart);
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+  } else {
+    Params p = base_params(T, V, H, err);
+    XentStatsEpi::Args e{labels.data_ptr<int64_t>(), reinterpret_cast<float2*>(part.data_ptr<float>()), target, vstart,
+                         tiles_n};
+    logits_gemm<XentStatsEpi>(h, w, 0, V, p, e, bn, st);
+  }
   xent_join_kernel<<<(T + 7) / 8, 256, 0, st>>>(
       reinterpret_cast<const float2*>(part.data_ptr<float>()), target, labels.data_ptr<int64_t>(),
       reinterpret_cast<float4*>(stats.data_ptr<float>()), lse_t.data_ptr<float>(), losses.data_ptr<float>(), T, tiles_n,
@@ -454,7 +581,7 @@ int64_t linear_xent_bwd(const torch::Tensor& h, const torch::Tensor& w, const to
   TORCH_CHECK(grad.is_cuda() && grad.scalar_type() == at::kFloat && grad.is_contiguous() &&
                   (grad.dim() == 0 || grad.numel() == T),
               "linear_xent_bwd: grad must be one fp32 value or one per row");
-  TORCH_CHECK(factor.is_cuda() && factor.scalar_type() == at::kFloat && factor.numel() == 1);
+  TORCH_CHECK(factor.is_cuda() && factor.scalar_type() == at::kFloat && (grad.dim() > 0 || factor.numel() == 1));
   if (dh.has_value())
     TORCH_CHECK(dh->is_cuda() && dh->scalar_type() == at::kBFloat16 && dh->is_contiguous() && dh->dim() == 2 &&
                 dh->size(0) == T && dh->size(1) == H);

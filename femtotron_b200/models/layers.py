@@ -14,6 +14,15 @@ implementation whose forward runs:
 When the projections are tensor-parallel modules, the matching TP/SP collectives wrap the
 GEMMs.  If the projections are replaced by anything the fast path does not understand (a
 bias, custom modules), the layer falls back to calling the submodules one by one.
+
+Attributes that a user may set on the model config:
+
+    rotary_spec   dict of the general rotation (``ops/rotary.py``) in place of the plain one:
+                  "scaling" (a Hugging Face style rope_scaling dict, or None), "partial" (the
+                  share of a head that is rotated, 1.0), "interleaved" (False)
+    mlp_act8      True: the MLP block keeps what its backward needs in 8 bits
+                  (``functional.NormMLP8Fn``); without tensor parallelism
+    loss_keep_logits  False: the loss without the logits in memory
 """
 from __future__ import annotations
 
@@ -24,6 +33,7 @@ import torch.nn.functional as F
 from torch import nn
 
 from femtotron_b200.ops import functional as FN
+from femtotron_b200.ops import rotary
 from femtotron_b200.ops.kernels import rope_tables
 from femtotron_b200.parallel.tensor_parallel import comm_ops as C
 from femtotron_b200.parallel.tensor_parallel.linear import ColumnParallelLinear, RowParallelLinear
@@ -38,6 +48,21 @@ def _cfg(config, name, default=None):
 def head_dim_of(config) -> int:
     hd = getattr(config, "head_dim", None)
     return hd if hd else config.hidden_size // config.num_attention_heads
+
+
+def rotary_spec_of(config) -> dict | None:
+    """The config's ``rotary_spec`` with its defaults and "rot", the rotated values per head."""
+    spec = _cfg(config, "rotary_spec", None)
+    if spec is None:
+        return None
+    unknown = set(spec) - {"scaling", "partial", "interleaved"}
+    if unknown:
+        raise ValueError(f"rotary_spec: unknown keys {sorted(unknown)}")
+    partial = float(spec.get("partial", 1.0))
+    if not 0 < partial <= 1:
+        raise ValueError(f"rotary_spec: partial must be in (0, 1], got {partial}")
+    rot = int(head_dim_of(config) * partial) // 2 * 2
+    return {"scaling": spec.get("scaling"), "interleaved": bool(spec.get("interleaved", False)), "rot": rot}
 
 
 class LlamaRMSNorm(nn.Module):
@@ -72,6 +97,7 @@ class LlamaRotaryEmbedding(nn.Module):
         self.theta = float(_cfg(config, "rope_theta", None) or
                            (getattr(config, "rope_parameters", None) or {}).get("rope_theta", 10000.0))
         self.max_position_embeddings = int(_cfg(config, "max_position_embeddings", 2048))
+        self.spec = rotary_spec_of(config)
         self._cache: dict = {}
 
     def tables(self, device, dtype, length: int):
@@ -79,7 +105,11 @@ class LlamaRotaryEmbedding(nn.Module):
         key = (str(device), dtype, n)
         t = self._cache.get(key)
         if t is None:
-            t = rope_tables(self.head_dim, n, self.theta, device, dtype)
+            if self.spec is not None:
+                t = rotary.rotary_tables(self.spec["rot"], n, self.theta, self.spec["scaling"],
+                                         trained=self.max_position_embeddings, device=device)
+            else:
+                t = rope_tables(self.head_dim, n, self.theta, device, dtype)
             self._cache = {key: t}
         return t
 
@@ -156,6 +186,7 @@ class LlamaAttention(nn.Module):
         self.num_heads = config.num_attention_heads
         self.num_key_value_heads = _cfg(config, "num_key_value_heads", config.num_attention_heads)
         bias = bool(_cfg(config, "attention_bias", False))
+        self.rotary_spec = rotary_spec_of(config)
         H = config.hidden_size
         d = self.head_dim
         self.q_proj = nn.Linear(H, self.num_heads * d, bias=bias, device=device, dtype=dtype)
@@ -174,7 +205,7 @@ class LlamaAttention(nn.Module):
         nq = self.q_proj.weight.shape[0] // d
         nkv = self.k_proj.weight.shape[0] // d
         group, sp = _tp_info(self.q_proj)
-        comm = _sp_comm(x, group, sp, 0) if self._fusable() else None
+        comm = _sp_comm(x, group, sp, 0) if self._fusable() and self.rotary_spec is None else None
         if comm is not None and self.o_proj.weight.shape[0] == x.shape[-1]:
             from femtotron_b200.parallel.tensor_parallel.fused import SPColumnFn, SPRowFn
             qkv = SPColumnFn.apply(x, comm, "qkv_rope", (cos, sin, pos, nq + nkv, d, S),
@@ -183,8 +214,12 @@ class LlamaAttention(nn.Module):
             return SPRowFn.apply(o, residual, comm, self.o_proj.weight)
         if self._fusable():
             xin = _enter(x, group, sp)
-            qkv = FN.QKVRopeFn.apply(xin, cos, sin, pos, nq + nkv, d, S,
-                                     self.q_proj.weight, self.k_proj.weight, self.v_proj.weight)
+            if self.rotary_spec is not None:
+                qkv = FN.QKVRotaryFn.apply(xin, cos, sin, pos, nq, nkv, d, S, self.rotary_spec["interleaved"],
+                                           self.q_proj.weight, self.k_proj.weight, self.v_proj.weight)
+            else:
+                qkv = FN.QKVRopeFn.apply(xin, cos, sin, pos, nq + nkv, d, S,
+                                         self.q_proj.weight, self.k_proj.weight, self.v_proj.weight)
             o = causal_attention(qkv, B, S, nq, nkv, d)
             if group is None:
                 return FN.linear(o, self.o_proj.weight, residual=residual) if residual is not None \
@@ -195,7 +230,13 @@ class LlamaAttention(nn.Module):
         q2 = self.q_proj(x).reshape(-1, nq * d)
         k2 = self.k_proj(x).reshape(-1, nkv * d)
         v2 = self.v_proj(x).reshape(-1, nkv * d)
-        qk = _RopeFn.apply(torch.cat([q2, k2], -1), cos, sin, pos, nq + nkv, d, S)
+        if self.rotary_spec is not None:
+            q4, k4 = rotary.rotary(q2.view(-1, S, nq, d), k2.view(-1, S, nkv, d), cos, sin,
+                                   pos.view(-1, S) if pos is not None else None,
+                                   interleaved=self.rotary_spec["interleaved"])
+            qk = torch.cat([q4.reshape(-1, nq * d), k4.reshape(-1, nkv * d)], -1)
+        else:
+            qk = _RopeFn.apply(torch.cat([q2, k2], -1), cos, sin, pos, nq + nkv, d, S)
         qkv = torch.cat([qk, v2], -1).contiguous()
         o = causal_attention(qkv, B, S, nq, nkv, d)
         y = self.o_proj(o)
@@ -262,9 +303,16 @@ class LlamaDecoderLayer(nn.Module):
         self.layer_idx = layer_idx
         self.self_attn = LlamaAttention(config, layer_idx, device=device, dtype=dtype)
         self.mlp = LlamaMLP(config, device=device, dtype=dtype)
+        self.mlp_act8 = bool(_cfg(config, "mlp_act8", False))
         eps = float(_cfg(config, "rms_norm_eps", 1e-6))
         self.input_layernorm = LlamaRMSNorm(config.hidden_size, eps, device=device, dtype=dtype)
         self.post_attention_layernorm = LlamaRMSNorm(config.hidden_size, eps, device=device, dtype=dtype)
+
+    def _mlp8_applies(self, h: torch.Tensor) -> bool:
+        """The 8-bit block needs the fused projections without tensor parallelism, and a backward."""
+        return torch.is_grad_enabled() and self.mlp._fusable() and _tp_info(self.mlp.gate_proj)[0] is None and \
+            type(self.post_attention_layernorm) is LlamaRMSNorm and \
+            (not h.is_cuda or h.dtype == self.post_attention_layernorm.weight.dtype == torch.bfloat16)
 
     def forward(self, hidden_states: torch.Tensor, attention_mask=None, position_ids=None,
                 past_key_values=None, use_cache=False, position_embeddings=None,
@@ -280,6 +328,11 @@ class LlamaDecoderLayer(nn.Module):
         with nvtx_range(f"layer{self.layer_idx}"):
             n = self.input_layernorm(x)
             h = self.self_attn(n, position_embeddings, batch_shape, residual=x)
-            n2 = self.post_attention_layernorm(h)
-            out = self.mlp(n2, residual=h)
+            if self.mlp_act8 and self._mlp8_applies(h):
+                m, norm = self.mlp, self.post_attention_layernorm
+                out = FN.NormMLP8Fn.apply(h, norm.weight, norm.variance_epsilon, 128, m.gate_proj.weight,
+                                          m.up_proj.weight, m.down_proj.weight)
+            else:
+                n2 = self.post_attention_layernorm(h)
+                out = self.mlp(n2, residual=h)
         return out.view(shape)

@@ -39,7 +39,8 @@ class LlamaForTraining(nn.Module):
         hidden = self.model(input_ids)
         out: dict = {}
         if labels is not None:
-            out["loss"] = lm_head_loss(self.lm_head, hidden, labels)
+            out["loss"] = lm_head_loss(self.lm_head, hidden, labels,
+                                       keep_logits=getattr(self.config, "loss_keep_logits", True))
         want = materialize_logits if materialize_logits is not None else labels is None
         out["logits"] = full_logits(self.lm_head, hidden, tuple(input_ids.shape)) if want else None
         return out

@@ -24,7 +24,7 @@ from dataclasses import dataclass
 
 import torch
 
-from .ext import native
+from .ext import error_flag, native
 
 GROUPS = (32, 64, 128, 256)
 _TINY = 2.0 ** -120
@@ -49,13 +49,10 @@ class Act8:
 
     def dequantize(self, dtype: torch.dtype | None = None) -> torch.Tensor:
         """The kept values as a contiguous tensor of the original shape."""
-        x = torch.empty(self.shape, dtype=dtype or self.dtype, device=self.codes.device)
-        x2 = x.view(self.codes.shape[0], self.n)
-        if x.is_cuda:
-            native().act8_dequantize(self.codes, self.scales, x2, self.group)
-        else:
-            x2.copy_(_decode(self.codes, self.scales, self.n, self.group))
-        return x
+        if self.codes.is_cuda:
+            return native().act8_dequantize(self.codes, self.scales, self.shape, self.n, dtype or self.dtype,
+                                            self.group)
+        return _decode(self.codes, self.scales, self.n, self.group).to(dtype or self.dtype).view(self.shape)
 
 
 def _check_group(group: int) -> None:
@@ -92,31 +89,22 @@ def _decode(codes: torch.Tensor, scales: torch.Tensor, n: int, group: int) -> to
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
-    """x as 2-D rows with a unit inner stride (a view where its strides allow one)."""
-    x2 = x.reshape(x.shape[:-1].numel(), x.shape[-1])
-    return x2 if x2.shape[1] <= 1 or x2.stride(1) == 1 else x2.contiguous()
-
-
-def _rows16(x: torch.Tensor) -> torch.Tensor:
-    """``_rows`` whose rows start on 16-byte boundaries, as the fused kernels need."""
-    x2 = _rows(x)
-    if x2.is_cuda and (x2.data_ptr() % 16 or x2.stride(0) * x2.element_size() % 16):
-        x2 = x2.clone(memory_format=torch.contiguous_format)
-    return x2
+    """x as 2-D rows."""
+    return x.detach().reshape(x.shape[:-1].numel(), x.shape[-1])
 
 
 def quantize(x: torch.Tensor, group: int = 128) -> Act8:
     """Keep ``x`` (groups along its last dimension) in 8 bits."""
-    if x.dim() == 0:
-        raise ValueError("act8.quantize: x needs at least one dimension")
     if not x.is_floating_point():
         raise TypeError(f"act8.quantize: a floating tensor is required, got {x.dtype}")
-    x2 = _rows(x.detach())
-    codes, scales = _buffers(x2.shape[0], x2.shape[1], group, x.device)
     if x.is_cuda:
-        native().act8_quantize(x2, codes, scales, group)
-    else:
-        _encode(x2.float(), codes, scales, group)
+        codes, scales = native().act8_quantize(x, group)
+        return Act8(codes, scales, x.shape[-1], x.shape, x.dtype, group)
+    if x.dim() == 0:
+        raise ValueError("act8.quantize: x needs at least one dimension")
+    x2 = _rows(x)
+    codes, scales = _buffers(x2.shape[0], x2.shape[1], group, x.device)
+    _encode(x2.float(), codes, scales, group)
     return Act8(codes, scales, x2.shape[1], x.shape, x.dtype, group)
 
 
@@ -128,18 +116,15 @@ def dequantize(a: Act8, dtype: torch.dtype | None = None) -> torch.Tensor:
 def rms_norm(x: torch.Tensor, w: torch.Tensor, eps: float, group: int = 128):
     """``y = w x r`` with ``r = rsqrt(mean x^2 + eps)`` over the last dimension; returns
     (y, r [rows], x in 8 bits)."""
-    x2 = _rows16(x.detach())
+    if x.is_cuda:
+        y, rstd, codes, scales = native().act8_rms_norm(x, w, eps, group)
+        return y, rstd, Act8(codes, scales, x.shape[-1], x.shape, x.dtype, group)
+    x2 = _rows(x).float()
     T, H = x2.shape
     codes, scales = _buffers(T, H, group, x.device)
-    y = torch.empty(T, H, dtype=x.dtype, device=x.device)
-    rstd = torch.empty(T, dtype=torch.float32, device=x.device)
-    if x.is_cuda:
-        native().act8_rms_norm(x2, w, y, rstd, codes, scales, group, float(eps))
-    else:
-        xf = x2.float()
-        rstd.copy_(torch.rsqrt(xf.pow(2).mean(-1) + eps))
-        y.copy_(xf * rstd[:, None] * w.float())
-        _encode(xf, codes, scales, group)
+    rstd = torch.rsqrt(x2.pow(2).mean(-1) + eps)
+    y = (x2 * rstd[:, None] * w.float()).to(x.dtype)
+    _encode(x2, codes, scales, group)
     return y.view(x.shape), rstd, Act8(codes, scales, H, x.shape, x.dtype, group)
 
 
@@ -148,24 +133,14 @@ def rms_norm_bwd(dy: torch.Tensor, a: Act8, w: torch.Tensor, rstd: torch.Tensor)
     ``dw = sum dy n`` (fp32) and ``y8 = n w``; returns (dx, dw, y8)."""
     if dy.shape != a.shape:
         raise ValueError(f"act8.rms_norm_bwd: dy has shape {tuple(dy.shape)}, the input had {tuple(a.shape)}")
-    dy2 = _rows16(dy)
-    T, H = dy2.shape
-    dx = torch.empty(T, H, dtype=a.dtype, device=dy.device)
-    y8 = torch.empty(T, H, dtype=a.dtype, device=dy.device)
-    dw = torch.empty(H, dtype=torch.float32, device=dy.device)
     if dy.is_cuda:
-        m = native()
-        with torch.cuda.device(dy.device):
-            part = torch.empty(m.act8_norm_walkers(T, H), H, dtype=torch.float32, device=dy.device)
-        m.act8_rms_norm_bwd(dy2, a.codes, a.scales, w, rstd, dx, y8, dw, part, a.group)
-    else:
-        n = _decode(a.codes, a.scales, H, a.group) * rstd[:, None]
-        g = dy2.float()
-        dn = g * w.float()
-        dx.copy_(rstd[:, None] * (dn - n * (dn * n).mean(-1, keepdim=True)))
-        dw.copy_((g * n).sum(0))
-        y8.copy_(n * w.float())
-    return dx.view(a.shape), dw, y8.view(a.shape)
+        return native().act8_rms_norm_bwd(dy, a.codes, a.scales, w, rstd, a.group, error_flag(dy.device))
+    n = _decode(a.codes, a.scales, a.n, a.group) * rstd[:, None]
+    g = _rows(dy).float()
+    dn = g * w.float()
+    dx = (rstd[:, None] * (dn - n * (dn * n).mean(-1, keepdim=True))).to(a.dtype)
+    y8 = (n * w.float()).to(a.dtype)
+    return dx.view(a.shape), (g * n).sum(0), y8.view(a.shape)
 
 
 # ------------------------------------------------------------------------------ SwiGLU
@@ -173,16 +148,16 @@ def swiglu(gu: torch.Tensor, group: int = 128):
     """``h = silu(g) u`` of ``gu = [g | u]`` ([..., 2F]); returns (h [..., F], gu in 8 bits)."""
     if gu.shape[-1] % 2:
         raise ValueError("act8.swiglu: the last dimension must hold gate and up halves")
-    gu2 = _rows16(gu.detach())
-    T, F = gu2.shape[0], gu2.shape[1] // 2
-    codes, scales = _buffers(2 * T, F, group, gu.device)
-    h = torch.empty(T, F, dtype=gu.dtype, device=gu.device)
+    F = gu.shape[-1] // 2
     if gu.is_cuda:
-        native().act8_swiglu(gu2, h, codes, scales, group)
-    else:
-        g, u = gu2[:, :F].float(), gu2[:, F:].float()
-        h.copy_(g * torch.sigmoid(g) * u)
-        _encode(gu2.float().reshape(2 * T, F), codes, scales, group)
+        h, codes, scales = native().act8_swiglu(gu, group)
+        return h, Act8(codes, scales, F, gu.shape, gu.dtype, group)
+    gu2 = _rows(gu).float()
+    T = gu2.shape[0]
+    codes, scales = _buffers(2 * T, F, group, gu.device)
+    g, u = gu2[:, :F], gu2[:, F:]
+    h = (g * torch.sigmoid(g) * u).to(gu.dtype)
+    _encode(gu2.reshape(2 * T, F), codes, scales, group)
     return h.view(*gu.shape[:-1], F), Act8(codes, scales, F, gu.shape, gu.dtype, group)
 
 
@@ -190,17 +165,12 @@ def swiglu_bwd(dh: torch.Tensor, a: Act8):
     """Backward of ``swiglu`` from the 8-bit gate and up; returns (dgu [..., 2F], h8 [..., F])."""
     if (*dh.shape[:-1], 2 * dh.shape[-1]) != tuple(a.shape):
         raise ValueError(f"act8.swiglu_bwd: dh has shape {tuple(dh.shape)}, gate and up had {tuple(a.shape)}")
-    dh2 = _rows16(dh)
-    T, F = dh2.shape
-    dgu = torch.empty(T, 2 * F, dtype=a.dtype, device=dh.device)
-    h8 = torch.empty(T, F, dtype=a.dtype, device=dh.device)
     if dh.is_cuda:
-        native().act8_swiglu_bwd(dh2, a.codes, a.scales, dgu, h8, a.group)
-    else:
-        v = _decode(a.codes, a.scales, F, a.group).view(T, 2, F)
-        g, u, d = v[:, 0], v[:, 1], dh2.float()
-        s = torch.sigmoid(g)
-        dgu[:, :F] = (d * u * s * (1 + g * (1 - s))).to(dgu.dtype)
-        dgu[:, F:] = (d * g * s).to(dgu.dtype)
-        h8.copy_(g * s * u)
-    return dgu.view(a.shape), h8.view(dh.shape)
+        return native().act8_swiglu_bwd(dh, a.codes, a.scales, a.group)
+    F = a.n
+    d = _rows(dh).float()
+    v = _decode(a.codes, a.scales, F, a.group).view(-1, 2, F)
+    g, u = v[:, 0], v[:, 1]
+    s = torch.sigmoid(g)
+    dgu = torch.cat([d * u * s * (1 + g * (1 - s)), d * g * s], 1).to(a.dtype)
+    return dgu.view(a.shape), (g * s * u).to(a.dtype).view(dh.shape)

@@ -20,7 +20,7 @@ LAUNCHES = [0]
 # (main, weight-gradient sum); the memory-management and stream-memory-operation entry points
 # launch none (copy engines, cuStreamWriteValue32).
 KERNELS_PER_CALL = {
-    "flash_bwd": 3, "act8_rms_norm_bwd": 2, "act8_norm_walkers": 0,
+    "flash_bwd": 3, "act8_rms_norm_bwd": 2,
     "symm_alloc": 0, "ipc_handle": 0, "ipc_open": 0, "ipc_close": 0, "tensor_at": 0,
     "copy_from_ptrs": 0, "stream_write": 0,
 }

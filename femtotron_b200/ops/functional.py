@@ -21,12 +21,16 @@ without copying, so each of these projections is a single GEMM.
 """
 from __future__ import annotations
 
+from dataclasses import replace
+
 import torch
 import torch.distributed as dist
 from torch.autograd import Function
 
+from . import act8 as A8
 from . import kernels as K
 from . import linear_xent as X
+from . import rotary as R
 from .matmul import gemm, linear_dgrad, linear_fwd, linear_wgrad
 
 
@@ -94,6 +98,10 @@ def write_weight_grad(params, compute):
 
 
 def _write_weight_grad(params, compute):
+    if len(params) == 1:
+        dst, acc = _grad_target(params[0])
+        compute(dst.view(params[0].shape), acc)
+        return
     targets = [_grad_target(p) for p in params]
     dsts = [t.view(p.shape) for (t, _), p in zip(targets, params)]
     accs = [a for _, a in targets]
@@ -196,6 +204,43 @@ class QKVRopeFn(Function):
         return (dx, None, None, None, None, None, None) + (None,) * len(weights)
 
 
+class QKVRotaryFn(Function):
+    """QKVRopeFn with the general rotation of ``ops/rotary.py`` (fp32 tables, half or interleaved
+    layout, part of the head): qkv = x @ [Wq;Wk;Wv]^T, then q and k turned in place.  ``pos``:
+    one position per row of x, or None for 0, 1, ... in each sequence."""
+
+    @staticmethod
+    def _turn(qkv, cos, sin, pos, nq, nkv, d, S, interleaved, inverse):
+        rows = qkv.view(-1, S, qkv.shape[-1] // d, d)
+        R.rotary_qk(rows[:, :, :nq], rows[:, :, nq:nq + nkv], cos, sin,
+                    pos.view(-1, S) if pos is not None else None, interleaved=interleaved, inverse=inverse,
+                    inplace=True)
+
+    @staticmethod
+    def forward(ctx, x, cos, sin, pos, nq, nkv, head_dim, seq_len, interleaved, *weights):
+        x2 = _as2d(x)
+        qkv = linear_fwd(x2, cat_rows_view(weights))
+        ctx.meta = (nq, nkv, head_dim, seq_len, interleaved)
+        QKVRotaryFn._turn(qkv, cos, sin, pos, *ctx.meta, False)
+        ctx.save_for_backward(x2, cos, sin, pos if pos is not None else torch.empty(0),
+                              *[w.detach() for w in weights])
+        ctx.params = weights
+        ctx.has_pos = pos is not None
+        ctx.xshape = x.shape
+        return qkv
+
+    @staticmethod
+    def backward(ctx, dqkv):
+        x2, cos, sin, pos, *weights = ctx.saved_tensors
+        d = dqkv.contiguous().clone()
+        QKVRotaryFn._turn(d, cos, sin, pos if ctx.has_pos else None, *ctx.meta, True)
+        dx = linear_dgrad(d, cat_rows_view(weights)).view(ctx.xshape) if ctx.needs_input_grad[0] else None
+        if any(ctx.needs_input_grad[9:]):
+            write_weight_grad(ctx.params, lambda dst, acc: linear_wgrad(d, x2, dst, acc))
+        ctx.params = None
+        return (dx,) + (None,) * (8 + len(weights))
+
+
 # ------------------------------------------------------------------------------ gate/up + SwiGLU
 class GateUpSwiGLUFn(Function):
     """h = silu(x Wg^T) * (x Wu^T) as one GEMM whose tiles pair gate and up rows; the bf16
@@ -226,6 +271,47 @@ class GateUpSwiGLUFn(Function):
             write_weight_grad(ctx.params, lambda dst, acc: linear_wgrad(dgu, x2, dst, acc))
         ctx.params = None
         return dx, None, None
+
+
+class NormMLP8Fn(Function):
+    """out = x + down(silu(gate(n)) * up(n)), n = RMSNorm(x): the MLP block of a layer with what
+    its backward needs kept in 8 bits.  Of a row of x (H values) and of [gate | up] (2F values) one
+    byte per value is kept, instead of x, n, [gate | up] and the activation in the compute
+    dtype; the operands of the weight gradients are rebuilt from the same bytes."""
+
+    @staticmethod
+    def forward(ctx, x, w_norm, eps, group, w_gate, w_up, w_down):
+        x2 = _as2d(x)
+        n, rstd, x8 = A8.rms_norm(x2, w_norm, eps, group)
+        a, gu8 = A8.swiglu(linear_fwd(n, cat_rows_view([w_gate, w_up])), group)
+        out = linear_fwd(a, w_down, x2)
+        ctx.save_for_backward(x8.codes, x8.scales, rstd, gu8.codes, gu8.scales, w_norm.detach(),
+                              w_gate.detach(), w_up.detach(), w_down.detach())
+        ctx.kept = (x8, gu8)  # what the tensors above stand for; they are replaced on unpacking
+        x8.codes = x8.scales = gu8.codes = gu8.scales = None
+        ctx.params = (w_norm, w_gate, w_up, w_down)
+        ctx.xshape = x.shape
+        return out.view(x.shape)
+
+    @staticmethod
+    def backward(ctx, dout):
+        xc, xs, rstd, gc, gs, w_norm, w_gate, w_up, w_down = ctx.saved_tensors
+        x8, gu8 = (replace(a, codes=c, scales=s) for a, c, s in zip(ctx.kept, (xc, gc), (xs, gs)))
+        p_norm, p_gate, p_up, p_down = ctx.params
+        need = ctx.needs_input_grad
+        d = _as2d(dout)
+        dgu, a = A8.swiglu_bwd(linear_dgrad(d, w_down), gu8)
+        if need[6]:
+            write_weight_grad([p_down], lambda dst, acc: linear_wgrad(d, a, dst, acc))
+        del a
+        dn = linear_dgrad(dgu, cat_rows_view([w_gate, w_up]))
+        dx, dw, n = A8.rms_norm_bwd(dn, x8, w_norm, rstd)
+        if need[4] or need[5]:
+            write_weight_grad([p_gate, p_up], lambda dst, acc: linear_wgrad(dgu, n, dst, acc))
+        if need[1]:
+            write_vector_grad(p_norm, dw)
+        ctx.params = ctx.kept = None
+        return (dx + d).view(ctx.xshape) if need[0] else None, None, None, None, None, None, None
 
 
 # ------------------------------------------------------------------------------ RMSNorm
@@ -358,7 +444,7 @@ class LinearCrossEntropyFn(Function):
             dist.all_gather_into_tensor(allst, stats, group=tp_group)
             lse, losses, loss, factor = X.combine(X.merge_shards(allst.view(ws, -1, 4)), lab, ignore_index,
                                                   reduction)
-        ctx.save_for_backward(h2, w.detach(), lab, lse, lse.new_ones(()) if factor is None else factor)
+        ctx.save_for_backward(h2, w.detach(), lab, lse, lse if factor is None else factor)
         ctx.param = w
         ctx.meta = (vstart, ignore_index, workspace_bytes, reduction)
         ctx.hshape = h.shape

@@ -135,16 +135,9 @@ def rotary_qk(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Te
 
     On CUDA a position outside the tables gives NaN and is reported by
     ``check_kernel_errors`` (code 301); on the CPU it raises."""
-    pos = _check(q, k, cos, sin, pos)
     if q.is_cuda:
-        if q.shape[3] > 1 and (q.stride(3) != 1 or k.stride(3) != 1):
-            if inplace:
-                raise ValueError("rotary_qk: in place needs a unit inner stride")
-            q, k = q.contiguous(), k.contiguous()
-        oq, ok = (q, k) if inplace else (torch.empty_like(q, memory_format=torch.contiguous_format),
-                                         torch.empty_like(k, memory_format=torch.contiguous_format))
-        native().rotary_qk(q, k, cos, sin, pos, oq, ok, interleaved, inverse, error_flag(q.device))
-        return oq, ok
+        return native().rotary_qk(q, k, cos, sin, pos, interleaved, inverse, inplace, error_flag(q.device))
+    pos = _check(q, k, cos, sin, pos)
     if pos is None:
         pos = torch.arange(q.shape[1], device=q.device)[None]
     if pos.numel() and (int(pos.min()) < 0 or int(pos.max()) >= cos.shape[0]):

@@ -12,7 +12,11 @@ seq_len, tokenizer, data_dir, train_steps, micro_batch_size, lr, weight_decay, a
 adam_beta2, adam_eps, grad_clip, warmup_steps, min_lr_ratio, log_interval,
 checkpoint_interval, checkpoint_dir.  Additionally honoured: grad_accum_steps,
 num_microbatches and schedule (pipeline), sequence_parallel, rope_theta, rms_norm_eps,
-synthetic_data (uniform random tokens instead of a tokenised dataset), seed, metrics_path.
+synthetic_data (uniform random tokens instead of a tokenised dataset), seed, metrics_path, and
+for long sequences loss_keep_logits (false: the loss without its logits in memory), ac_bits (8:
+activation checkpoints in 8 bits), mlp_act8 (true: the MLP blocks keep 8-bit activations) and
+rope_scaling (a dict such as {rope_type: linear, factor: 4}, or "config" for the one of
+model_name's configuration), rope_partial, rope_interleaved.
 
 Unlike the reference script, pipeline parallelism (pp > 1) builds a PipelineRunner, gradient
 clipping and gradient accumulation are applied, and the vocabulary comes from the config
@@ -53,14 +57,15 @@ def parse_args(argv=None):
               "num_attention_heads", "num_key_value_heads", "vocab_size", "max_position_embeddings",
               "train_steps", "micro_batch_size",
               "seq_len", "warmup_steps", "num_samples", "log_interval", "checkpoint_interval",
-              "grad_accum_steps", "num_microbatches", "seed"):
+              "grad_accum_steps", "num_microbatches", "seed", "ac_bits"):
         p.add_argument(f"--{k}", type=int, default=None)
-    for k in ("lr", "grad_clip", "weight_decay", "min_lr_ratio", "init_std", "rope_theta", "rms_norm_eps"):
+    for k in ("lr", "grad_clip", "weight_decay", "min_lr_ratio", "init_std", "rope_theta", "rms_norm_eps",
+              "rope_partial"):
         p.add_argument(f"--{k}", type=float, default=None)
     for k in ("zero_wrap_policy", "ac_policy", "model_name", "dataset", "checkpoint_dir", "resume",
               "schedule", "metrics_path", "data_dir", "tokenizer"):
         p.add_argument(f"--{k}", type=str, default=None)
-    for k in ("ac_enabled", "sequence_parallel", "synthetic_data"):
+    for k in ("ac_enabled", "sequence_parallel", "synthetic_data", "loss_keep_logits", "mlp_act8", "rope_interleaved"):
         # `--ac_enabled true|false` as in the reference's CLI, or the bare flag for true
         p.add_argument(f"--{k}", type=_bool, nargs="?", const=True, default=None)
     return p.parse_args(argv)
@@ -77,7 +82,8 @@ DEFAULTS = dict(tp=1, pp=1, zero_stage=0, zero_wrap_policy="llama_decoder_layer"
                 checkpoint_dir="./checkpoints", grad_accum_steps=1, num_microbatches=1,
                 schedule="1f1b", sequence_parallel=False, rope_theta=10000.0, rms_norm_eps=1e-5,
                 synthetic_data=True, seed=1234, metrics_path=None, data_dir="./data", dataset=None,
-                tokenizer=None)
+                tokenizer=None, loss_keep_logits=True, ac_bits=16, mlp_act8=False, rope_scaling=None,
+                rope_partial=1.0, rope_interleaved=False)
 
 
 def load_config(args) -> dict:
@@ -98,6 +104,26 @@ def load_config(args) -> dict:
 
 
 def model_config_from(cfg: dict):
+    mc = _base_model_config(cfg)
+    # attributes only where they differ from the defaults: exported configurations stay plain
+    if not cfg.get("loss_keep_logits", True):
+        mc.loss_keep_logits = False
+    if cfg.get("mlp_act8", False):
+        mc.mlp_act8 = True
+    scaling = cfg.get("rope_scaling")
+    if scaling == "config":
+        scaling = getattr(mc, "rope_scaling", None) or getattr(mc, "rope_parameters", None)
+        if scaling is None:
+            raise ValueError("rope_scaling: config asked for, but the model configuration has none")
+    if scaling is not None and not isinstance(scaling, dict):
+        raise ValueError(f"rope_scaling must be a dict or 'config', got {scaling!r}")
+    partial, interleaved = cfg.get("rope_partial", 1.0), cfg.get("rope_interleaved", False)
+    if scaling is not None or partial != 1.0 or interleaved:
+        mc.rotary_spec = {"scaling": scaling, "partial": partial, "interleaved": interleaved}
+    return mc
+
+
+def _base_model_config(cfg: dict):
     from transformers import AutoConfig, LlamaConfig
     if cfg.get("model_name"):
         mc = AutoConfig.from_pretrained(cfg["model_name"])
@@ -170,8 +196,9 @@ def build_all(cfg: dict):
     if cfg["ac_enabled"]:
         n = apply_activation_checkpointing(model, get_ac_policy(cfg["ac_policy"]),
                                            use_reentrant=cfg["ac_use_reentrant"],
-                                           preserve_rng_state=cfg["ac_preserve_rng_state"])
-        log(f"activation checkpointing: {n} modules")
+                                           preserve_rng_state=cfg["ac_preserve_rng_state"],
+                                           bits=cfg.get("ac_bits", 16))
+        log(f"activation checkpointing: {n} modules" + (" in 8 bits" if cfg.get("ac_bits", 16) == 8 else ""))
     sched = create_lr_schedule(mp.inner, tc.warmup_steps, tc.train_steps, tc.min_lr_ratio)
     S, mb = cfg["seq_len"], cfg["micro_batch_size"]
     if cfg["synthetic_data"] or not cfg.get("dataset"):

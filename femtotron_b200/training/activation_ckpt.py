@@ -5,7 +5,12 @@ Selected modules are wrapped in :class:`ActivationCheckpointWrapper`, which runs
 module under ``torch.utils.checkpoint`` (non-reentrant by default).  State-dict hooks strip
 and re-add the wrapper prefix, so checkpoints keep the unwrapped parameter names.  The
 wrapped module object itself is reused, so hooks installed on it (e.g. ZeRO-3 unit hooks)
-stay inside the checkpointed region and fire again during the recomputation."""
+stay inside the checkpointed region and fire again during the recomputation.
+
+``bits=8`` keeps the wrapped module's first argument (the hidden states) in 8 bits
+(``ops/act8.py``) instead of its own dtype between forward and backward: half the memory of bf16
+checkpoints.  The forward runs on the exact values; the recomputation, and so the gradients,
+on the kept ones."""
 from __future__ import annotations
 
 from typing import Any
@@ -14,17 +19,57 @@ import torch
 from torch import nn
 from torch.utils.checkpoint import checkpoint
 
+from femtotron_b200.ops import act8
+
 _PREFIX = "_checkpoint_wrapped_module"
+
+
+class _Checkpoint8Fn(torch.autograd.Function):
+    """Runs ``fn(x)`` without a graph, keeps x in 8 bits, and runs fn again in the backward."""
+
+    @staticmethod
+    def forward(ctx, x, fn, preserve_rng_state):
+        ctx.fn = fn
+        ctx.devices = [x.device.index] if x.is_cuda else []
+        ctx.rng = None
+        if preserve_rng_state:
+            ctx.rng = (torch.get_rng_state(), [torch.cuda.get_rng_state(d) for d in ctx.devices])
+        ctx.autocast = (torch.is_autocast_enabled(x.device.type), torch.get_autocast_dtype(x.device.type))
+        a = act8.quantize(x)
+        ctx.save_for_backward(a.codes, a.scales)
+        ctx.kept = (a.n, a.shape, a.dtype, a.group)
+        with torch.no_grad():
+            return fn(x)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        x = act8.Act8(*ctx.saved_tensors, *ctx.kept).dequantize().requires_grad_()
+        on, dtype = ctx.autocast
+        with torch.random.fork_rng(ctx.devices, enabled=ctx.rng is not None), torch.enable_grad(), \
+                torch.autocast(x.device.type, dtype=dtype, enabled=on):
+            if ctx.rng is not None:
+                torch.set_rng_state(ctx.rng[0])
+                for d, state in zip(ctx.devices, ctx.rng[1]):
+                    torch.cuda.set_rng_state(state, d)
+            out = ctx.fn(x)
+        outs = out if isinstance(out, tuple) else (out,)
+        pairs = [(o, g) for o, g in zip(outs, grads) if torch.is_tensor(o) and o.requires_grad and g is not None]
+        torch.autograd.backward([o for o, _ in pairs], [g for _, g in pairs])
+        ctx.fn = None
+        return x.grad, None, None
 
 
 class ActivationCheckpointWrapper(nn.Module):
     def __init__(self, module: nn.Module, *, use_reentrant: bool = False,
-                 preserve_rng_state: bool = True, debug: bool = False):
+                 preserve_rng_state: bool = True, debug: bool = False, bits: int = 16):
         super().__init__()
+        if bits not in (8, 16):
+            raise ValueError(f"activation checkpoints are kept in 8 bits or as they are (16), got {bits}")
         self._checkpoint_wrapped_module = module
         self.use_reentrant = use_reentrant
         self.preserve_rng_state = preserve_rng_state
         self.debug = debug
+        self.bits = bits
         self._register_state_dict_hook(_post_state_dict_hook)
         self._register_load_state_dict_pre_hook(_pre_load_state_dict_hook, with_module=True)
 
@@ -35,6 +80,10 @@ class ActivationCheckpointWrapper(nn.Module):
     def forward(self, *args: Any, **kwargs: Any) -> Any:
         if not torch.is_grad_enabled():
             return self._checkpoint_wrapped_module(*args, **kwargs)
+        if self.bits == 8 and args and torch.is_tensor(args[0]) and args[0].is_floating_point() and \
+                args[0].requires_grad:
+            module, rest = self._checkpoint_wrapped_module, args[1:]
+            return _Checkpoint8Fn.apply(args[0], lambda x: module(x, *rest, **kwargs), self.preserve_rng_state)
         return checkpoint(self._checkpoint_wrapped_module, *args, use_reentrant=self.use_reentrant,
                           preserve_rng_state=self.preserve_rng_state, **kwargs)
 
@@ -45,17 +94,19 @@ class ActivationCheckpointWrapper(nn.Module):
             return getattr(self._checkpoint_wrapped_module, name)
 
     def extra_repr(self) -> str:
-        return f"use_reentrant={self.use_reentrant}, preserve_rng_state={self.preserve_rng_state}"
+        return f"use_reentrant={self.use_reentrant}, preserve_rng_state={self.preserve_rng_state}" + \
+            (f", bits={self.bits}" if self.bits != 16 else "")
 
 
 def apply_activation_checkpointing(model: nn.Module, policy, *, use_reentrant: bool = False,
-                                   preserve_rng_state: bool = True, debug: bool = False) -> int:
+                                   preserve_rng_state: bool = True, debug: bool = False,
+                                   bits: int = 16) -> int:
     """Wrap every module selected by `policy` (outermost match wins, no nesting); returns
-    the number of wrapped modules."""
+    the number of wrapped modules.  `bits=8` keeps their inputs in 8 bits."""
     targets = _collect_wrap_targets(model, policy)
     for parent, attr, mod in targets:
         w = ActivationCheckpointWrapper(mod, use_reentrant=use_reentrant,
-                                        preserve_rng_state=preserve_rng_state, debug=debug)
+                                        preserve_rng_state=preserve_rng_state, debug=debug, bits=bits)
         if isinstance(parent, (nn.ModuleList, nn.Sequential)) and attr.isdigit():
             parent[int(attr)] = w
         elif isinstance(parent, nn.ModuleDict):

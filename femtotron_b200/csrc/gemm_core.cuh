@@ -276,6 +276,7 @@ __device__ __forceinline__ void epilogue_tile(const Params& p, uint32_t tmem_acc
 //   kSplitK         whether the k-blocks of a tile are spread over Args::ksplit partial outputs
 //   tile<BN>()      consumes one accumulator tile, one output row per thread
 //   f32_scale()     factor of an fp32 output (1 unless the epilogue scales)
+//   kBf16Tma        whether the pair kernel may store bf16 tiles with tile_bf16_tma<BN>()
 struct StdEpi {
   struct Args {};
   static constexpr bool kSplitK = false;
@@ -285,6 +286,7 @@ struct StdEpi {
     epilogue_tile<BN>(p, tmem_acc, q, lane, row, n0, swiglu);
   }
   static constexpr bool kScales = false;
+  static constexpr bool kBf16Tma = false;
   __device__ __forceinline__ static float f32_scale(const Args&) { return 1.f; }
 };
 
@@ -524,6 +526,46 @@ __device__ __forceinline__ void epilogue_tile_f32_tma(const Params& p, const CUt
   }
 }
 
+// The same for bf16 outputs, 64 columns at a time (128-byte rows again): `f` turns the 64 fp32
+// accumulators of a row into the values to store.
+template <int PBN, class F>
+__device__ __forceinline__ void epilogue_tile_bf16_tma(const Params& p, const CUtensorMap* tma_d,
+                                                       float (*box)[32 * 32], uint32_t tmem_acc, int q,
+                                                       int lane, int row0, int n0, int& buf, F&& f) {
+  const uint32_t tbase = tmem_acc + (static_cast<uint32_t>(q * 32) << 16);
+#pragma unroll 1
+  for (int c = 0; c < PBN / 64; ++c) {
+    const int col0 = n0 + c * 64;
+    if (col0 >= p.N) break;  // uniform across the warp
+    uint32_t lo[32], hi[32];
+    tmem_ld_32x32b_x32(tbase + c * 64, lo);
+    tmem_ld_32x32b_x32(tbase + c * 64 + 32, hi);
+    tmem_wait_ld();
+    float v[64];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      v[i] = __uint_as_float(lo[i]);
+      v[32 + i] = __uint_as_float(hi[i]);
+    }
+    f(c * 64, v);
+    if (lane == 0) tma_store_wait_read_le1();  // box `buf` is free again
+    __syncwarp();
+    uint4* dst = reinterpret_cast<uint4*>(box[buf] + lane * 32);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      dst[j ^ (lane & 7)] =
+          make_uint4(pack_bf16x2(v[8 * j], v[8 * j + 1]), pack_bf16x2(v[8 * j + 2], v[8 * j + 3]),
+                     pack_bf16x2(v[8 * j + 4], v[8 * j + 5]), pack_bf16x2(v[8 * j + 6], v[8 * j + 7]));
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      tma_store_2d(tma_d, box[buf], col0, row0);
+      tma_store_commit();
+    }
+    buf ^= 1;
+  }
+}
+
 template <int BN, int STAGES>
 struct PairSmem {
   __nv_bfloat16 a[STAGES][128 * BK];
@@ -681,8 +723,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
     // ---------------- Epilogue (both CTAs) ----------------
     const int q = warp - EPI_WARP0;
     const bool f32_out = (p.mode == EPI_ACC_F32 || p.mode == EPI_STORE_F32);
+    const bool bf16_tma = Epi::kBf16Tma && p.mode == EPI_STORE_BF16;
     int epi_buf = 0;
-    if (f32_out && lane == 0) prefetch_tmap(&tma_d);
+    if ((f32_out || bf16_tma) && lane == 0) prefetch_tmap(&tma_d);
     const uint32_t acc_empty_leader0 = mapa_shared(smem_u32(&s.acc_empty[0]), 0);
     const uint32_t acc_empty_leader1 = mapa_shared(smem_u32(&s.acc_empty[1]), 0);
     int acc = 0;
@@ -701,7 +744,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
         epilogue_tile_f32_tma<PBN, Epi::kScales>(p, &tma_d, s.epi[q], tmem + acc * PBN, q, lane,
                                                  split * p.split_rows + m0 + q * 32, n0,
                                                  p.mode == EPI_ACC_F32, epi_buf, scale);
-      else
+      else if (bf16_tma) {
+        if constexpr (Epi::kBf16Tma)
+          Epi::template tile_bf16_tma<PBN>(p, e, &tma_d, s.epi[q], tmem + acc * PBN, q, lane, m0 + q * 32,
+                                           n0, epi_buf);
+      } else
         Epi::template tile<PBN>(p, e, tmem + acc * PBN, q, lane, m0 + q * 32 + lane, n0, tn, split,
                                 swiglu);
       tc_fence_before();
@@ -710,7 +757,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1;
     }
-    if (f32_out && lane == 0) tma_store_wait_all();  // bulk reductions done before exit
+    if ((f32_out || bf16_tma) && lane == 0) tma_store_wait_all();  // bulk reductions done before exit
   }
 
   tc_fence_before();

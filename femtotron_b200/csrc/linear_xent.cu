@@ -45,6 +45,7 @@ struct XentStatsEpi {
   };
   static constexpr bool kSplitK = false;
   static constexpr bool kScales = false;
+  static constexpr bool kBf16Tma = false;
   __device__ __forceinline__ static float f32_scale(const Args&) { return 1.f; }
   template <int BN>
   __device__ __forceinline__ static void tile(const Params& p, const Args& e, uint32_t tmem_acc, int q,
@@ -115,45 +116,64 @@ struct XentGradEpi {
   };
   static constexpr bool kSplitK = false;
   static constexpr bool kScales = false;
+  static constexpr bool kBf16Tma = true;
   __device__ __forceinline__ static float f32_scale(const Args&) { return 1.f; }
-  template <int BN>
-  __device__ __forceinline__ static void tile(const Params& p, const Args& e, uint32_t tmem_acc, int q,
-                                              int lane, int row, int n0, int, int, bool) {
-    const bool row_ok = row < p.M;
-    const uint32_t tbase = tmem_acc + (static_cast<uint32_t>(q * 32) << 16);
+
+  // What turns the logits of a row into its d: p = 2^(x unit - base), less 1 at column `at`, times g.
+  struct Row {
     int64_t at = -1;
-    float base = 0.f, g = 0.f;
-    const float unit = kLog2e * untruncate(p.K);
-    if (row_ok) {
+    float unit, base = 0.f, g = 0.f;
+    __device__ __forceinline__ Row(const Params& p, const Args& e, int row, int n0)
+        : unit(kLog2e * untruncate(p.K)) {
+      if (row >= p.M) return;
       const int64_t lab = e.labels[row];
       at = lab - e.vstart - n0;
       g = lab == e.ignore_index ? 0.f : (e.weight ? e.weight[row] : 1.f);
       base = e.lse[row] * kLog2e;
     }
+    template <int N>
+    __device__ __forceinline__ void apply(int col, float (&v)[N]) const {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = ex2_approx(fmaf(v[i], unit, -base));
+      const int64_t off = at - col;
+      const bool hit = off >= 0 && off < N;
+      if (__any_sync(0xffffffffu, hit)) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (hit && off == i) v[i] -= 1.f;
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = g == 0.f ? 0.f : v[i] * g;  // an ignored row's NaN stays out
+    }
+  };
+
+  template <int BN>
+  __device__ __forceinline__ static void tile(const Params& p, const Args& e, uint32_t tmem_acc, int q,
+                                              int lane, int row, int n0, int, int, bool) {
+    const uint32_t tbase = tmem_acc + (static_cast<uint32_t>(q * 32) << 16);
+    const Row turn(p, e, row, n0);
 #pragma unroll 1
     for (int c = 0; c < BN / 32; ++c) {
-      const int valid = p.N - n0 - c * 32;
-      if (valid <= 0) break;
+      if (n0 + c * 32 >= p.N) break;
       uint32_t r[32];
       tmem_ld_32x32b_x32(tbase + c * 32, r);
       tmem_wait_ld();
       float v[32];
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = ex2_approx(fmaf(__uint_as_float(r[i]), unit, -base));
-      const int64_t off = at - c * 32;
-      const bool hit = off >= 0 && off < 32;
-      if (__any_sync(0xffffffffu, hit)) {
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (hit && off == i) v[i] -= 1.f;
-      }
-      if (row_ok) {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = g == 0.f ? 0.f : v[i] * g;  // an ignored row's NaN stays out
-        // rows of D are padded to whole 32-column chunks
+      for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+      turn.apply(c * 32, v);
+      // rows of D are padded to whole 32-column chunks
+      if (row < p.M)
         store_bf16x32(reinterpret_cast<__nv_bfloat16*>(p.D) + (int64_t)row * p.ldd + n0 + c * 32, v, 32);
-      }
     }
+  }
+  template <int BN>
+  __device__ __forceinline__ static void tile_bf16_tma(const Params& p, const Args& e, const CUtensorMap* tma_d,
+                                                       float (*box)[32 * 32], uint32_t tmem_acc, int q, int lane,
+                                                       int row0, int n0, int& buf) {
+    const Row turn(p, e, row0 + lane, n0);
+    epilogue_tile_bf16_tma<BN>(p, tma_d, box, tmem_acc, q, lane, row0, n0, buf,
+                               [&](int col, float (&v)[64]) { turn.apply(col, v); });
   }
 };
 
@@ -166,6 +186,17 @@ struct XentProductEpi {
   };
   static constexpr bool kSplitK = true;
   static constexpr bool kScales = true;
+  static constexpr bool kBf16Tma = true;  // split K is for fp32 outputs only
+  template <int BN>
+  __device__ __forceinline__ static void tile_bf16_tma(const Params& p, const Args& e, const CUtensorMap* tma_d,
+                                                       float (*box)[32 * 32], uint32_t tmem_acc, int q, int lane,
+                                                       int row0, int n0, int& buf) {
+    const float scale = f32_scale(e);
+    epilogue_tile_bf16_tma<BN>(p, tma_d, box, tmem_acc, q, lane, row0, n0, buf, [&](int, float (&v)[64]) {
+#pragma unroll
+      for (int i = 0; i < 64; ++i) v[i] *= scale;
+    });
+  }
   __device__ __forceinline__ static float f32_scale(const Args& e) {
     return e.a ? e.a[0] * e.b[0] : 1.f;
   }
@@ -216,12 +247,13 @@ struct XentProductEpi {
 };
 
 // ------------------------------------------------------------------ few tokens
-// The forward for at most kFewTokens tokens: one read of w, and nothing for the tensor cores to
-// win (a 128-row tile would be nearly empty).  A warp takes two vocabulary rows at a time, 2 x 4
+// The forward for one or two tokens: one read of w, and nothing for the tensor cores to win (a
+// 128-row tile would be nearly empty).  Over 32000 words of 4096: 44.9 us for one token (5.8 TB/s)
+// and 51.5 us for two, where the GEMM takes 51 to 58 us up to 128 tokens; three took 71 us here.  A warp takes two vocabulary rows at a time, 2 x 4
 // packs of E values in flight per lane; h lies in shared memory in fp32, one plane per 4 of a
 // pack's E values, so that the lanes of a 16-byte read touch neighbouring words.  Every warp keeps a
 // running (max, sum) per token; a block leaves one pair per token, like a tile of the GEMM.
-constexpr int kFewTokens = 4;
+constexpr int kFewTokens = 2;
 constexpr int kFewThreads = 256;
 
 template <int TOK, int E>  // E: 16 values per pack where rows lie on 32-byte boundaries, else 8
@@ -448,7 +480,9 @@ static void logits_gemm(const torch::Tensor& h, const torch::Tensor& w, int64_t 
   CUtensorMap ta = make_tmap_2d(h.data_ptr(), kBF16, 2, H, T, h.stride(0), 64, 128, true);
   CUtensorMap tb = make_tmap_2d(wp, kBF16, 2, H, N, w.stride(0), 64, pair ? bn / 2 : bn, true);
   const int tiles = (T + (pair ? 255 : 127)) / (pair ? 256 : 128) * ((N + bn - 1) / bn);
-  if (pair) launch_pair<false, false, 256, Epi>(ta, tb, ta, p, tiles, st, e);
+  CUtensorMap td = ta;
+  if (pair && Epi::kBf16Tma) td = make_tmap_2d(p.D, kBF16, 2, N, T, p.ldd, 64, 32, true);
+  if (pair) launch_pair<false, false, 256, Epi>(ta, tb, td, p, tiles, st, e);
   else if (bn == 256) launch<false, false, 256, 4, Epi>(ta, tb, p, tiles, st, e);
   else launch<false, false, 128, 6, Epi>(ta, tb, p, tiles, st, e);
 }
@@ -483,7 +517,7 @@ static void product(const void* A, int64_t lda, const void* B, int64_t ldb, int 
   if (pair) {
     CUtensorMap td = f32 ? make_tmap_2d(D, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, N,
                                         ksplit == 1 ? M : (uint64_t)ksplit * split_rows, ldd, 32, 32, true)
-                         : ta;
+                         : make_tmap_2d(D, kBF16, 2, N, M, ldd, 64, 32, true);
     if (bn == 256) launch_pair<A_MN, true, 256, XentProductEpi>(ta, tb, td, p, tiles, st, e);
     else launch_pair<A_MN, true, 128, XentProductEpi>(ta, tb, td, p, tiles, st, e);
   } else if (bn == 256) {
@@ -525,7 +559,7 @@ std::vector<torch::Tensor> linear_xent_fwd(const torch::Tensor& h, const torch::
   auto st = at::cuda::getCurrentCUDAStream();
   const int T = h.size(0), V = w.size(0), H = h.size(1);
   // few tokens: a read of w by plain loads (see xent_few_kernel), while h fits beside two blocks
-  const int tok = T <= 1 ? 1 : T <= 2 ? 2 : 4;
+  const int tok = T <= 1 ? 1 : 2;
   const int few_bytes = tok * H * 4;
   const bool few = T <= kFewTokens && few_bytes <= 96 * 1024;
   const int bn = logits_bn(T, V);
@@ -537,11 +571,10 @@ std::vector<torch::Tensor> linear_xent_fwd(const torch::Tensor& h, const torch::
   float* target = part.data_ptr<float>() + (int64_t)T * tiles_n * 2;
   if (few) {
     const bool wide = H % 16 == 0 && w.stride(0) % 16 == 0 && reinterpret_cast<uintptr_t>(w.data_ptr()) % 32 == 0;
-    auto kern = tok == 1   ? (wide ? xent_few_kernel<1, 16> : xent_few_kernel<1, 8>)
-                : tok == 2 ? (wide ? xent_few_kernel<2, 16> : xent_few_kernel<2, 8>)
-                           : (wide ? xent_few_kernel<4, 16> : xent_few_kernel<4, 8>);
-    static unsigned long long done[6] = {0, 0, 0, 0, 0, 0};
-    smem_attr_once(kern, 96 * 1024, done[(tok == 4 ? 4 : 2 * (tok - 1)) + wide]);
+    auto kern = tok == 1 ? (wide ? xent_few_kernel<1, 16> : xent_few_kernel<1, 8>)
+                         : (wide ? xent_few_kernel<2, 16> : xent_few_kernel<2, 8>);
+    static unsigned long long done[4] = {0, 0, 0, 0};
+    smem_attr_once(kern, 96 * 1024, done[2 * (tok - 1) + wide]);
     kern<<<tiles_n, kFewThreads, few_bytes, st>>>(
         reinterpret_cast<const __nv_bfloat16*>(h.data_ptr()), h.stride(0),
         reinterpret_cast<const __nv_bfloat16*>(w.data_ptr()), w.stride(0), labels.data_ptr<int64_t>(),
@@ -620,17 +653,21 @@ int64_t linear_xent_bwd(const torch::Tensor& h, const torch::Tensor& w, const to
   const int64_t ldd = std::min<int64_t>(piece, (V + 31) / 32 * 32);
   torch::Tensor d = torch::empty({T, ldd}, h.options());
 
-  // split of the dh product: the fewest partial outputs within 3% of the best fill of the GPU
+  // split of the dh product, by the time that a model of it takes: whole waves of tiles at 20
+  // TFLOP/s per unit (a pair of SMs, or half of it), and the last kernel's read of the partial
+  // outputs at 6.5 TB/s.  1021 tokens of 5120, 32003 words: 80 tiles for 74 pairs, so unsplit
+  // the second wave is nearly empty: 422 us by the model, 262 us in 7 shares (measured: 264 in 12).
   const bool pair = T > 128 && H > 128;
   const long units = pair ? num_sms() / 2 : num_sms();
   const long tiles = (T + (pair ? 255 : 127)) / (pair ? 256 : 128) * ((H + 255) / 256);
   const long kblocks = (std::min<int64_t>(piece, V) + BK - 1) / BK;
   long ksplit = 1;
   if (dh.has_value()) {
+    const double tile_s = (pair ? 2.0 : 1.0) * 2 * 128 * 256 * double(V) / (pair ? 20e12 : 10e12);
     double best = 1e30;
     for (long k = 1; k <= std::min<long>(32, std::max<long>(1, kblocks / 8)); ++k) {
-      const double cost = double((tiles * k + units - 1) / units) / k;
-      if (cost < best * 0.97) { best = cost; ksplit = k; }
+      const double cost = double((tiles * k + units - 1) / units) / k * tile_s + k * (4.0 * T * H) / 6.5e12;
+      if (cost < best * 0.98) { best = cost; ksplit = k; }
     }
   }
   const int64_t split_rows = (T + 255) / 256 * 256;

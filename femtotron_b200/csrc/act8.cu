@@ -235,21 +235,6 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const int8_t* __restric
 }
 
 // ------------------------------------------------------------------ RMSNorm
-template <int NT>
-__device__ __forceinline__ float row_sum(float v, float* red) {
-  v = warp_sum(v);
-  if constexpr (NT > 32) {
-    const int w = threadIdx.x / 32;
-    __syncthreads();  // the previous use of red is over
-    if (threadIdx.x % 32 == 0) red[w] = v;
-    __syncthreads();
-    v = 0.f;
-#pragma unroll
-    for (int i = 0; i < NT / 32; ++i) v += red[i];
-  }
-  return v;
-}
-
 // y = w x r, r = rsqrt(mean x^2 + eps), and the 8-bit copy of x, from one read of x.
 // NT threads share a row (VPT chunks each); blocks of max(NT, 128) threads.
 template <int NT, int VPT, Rows R>
@@ -272,6 +257,9 @@ __global__ void __launch_bounds__(NT > 128 ? NT : 128)
 #pragma unroll
     for (int j = 0; j < 16; ++j) ss += v[i][j] * v[i][j];
   }
+  ss = warp_sum(ss);
+  if (NT > 32 && t % 32 == 0) red[t / 32] = ss;
+  // the codes need no sum: they are written while the row's warps come together
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int slot = t + i * NT;
@@ -283,7 +271,12 @@ __global__ void __launch_bounds__(NT > 128 ? NT : 128)
       if ((slot & ((1 << lanes_log2) - 1)) == 0) scale[row * groups + (slot >> lanes_log2)] = s;
     }
   }
-  ss = row_sum<NT>(ss, red);
+  if (NT > 32) {
+    __syncthreads();
+    ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < NT / 32; ++i) ss += red[i];
+  }
   const float r = rsqrtf(ss / H + eps);
   if (here && t == 0) rstd[row] = r;
 #pragma unroll

@@ -83,7 +83,12 @@ def error_flag(device: torch.device) -> torch.Tensor:
 
 
 class KernelTimeoutError(RuntimeError):
-    """A native kernel gave up on a bounded wait (see the error code)."""
+    """A native kernel gave up on a bounded wait, or met an argument that it could only check on
+    the device (see the error code)."""
+
+
+# codes that are not a bounded wait's
+_CODES = {301: "a rotary position outside the cosine and sine tables"}
 
 
 def check_kernel_errors(device: torch.device | None = None) -> None:
@@ -97,4 +102,5 @@ def check_kernel_errors(device: torch.device | None = None) -> None:
         code = int(t.item())
         if code != 0:
             t.zero_()
-            raise KernelTimeoutError(f"native kernel reported bounded-wait timeout, code {code}")
+            what = _CODES.get(code, "bounded-wait timeout")
+            raise KernelTimeoutError(f"native kernel reported {what}, code {code}")

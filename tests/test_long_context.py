@@ -158,27 +158,34 @@ def test_8_bit_block_is_left_out_without_a_backward(base):
         assert abs(float(model(ids, labels=ids)["loss"]) - loss) < 1e-5
 
 
-def test_training_command_runs_all_of_them_with_zero3(tmp_path):
-    """Two gloo ranks: ZeRO-3 gathers and shards each layer around its 8-bit checkpoint.  The first
-    loss is the plain run's (the forward is exact); later ones follow it."""
+def train(tmp_path, name, *extra):
+    """Losses of four steps of the training command on two gloo ranks, and its output."""
     import json
-    losses = []
-    for name, extra in (("all", []), ("plain", ["--ac_bits", "16", "--mlp_act8", "false", "--loss_keep_logits", "true"])):
-        metrics = tmp_path / f"{name}.jsonl"
-        cmd = [sys.executable, "-m", "torch.distributed.run", "--nproc-per-node", "2", "--master-addr", "127.0.0.1",
-               "--master-port", "29653", "-m", "femtotron_b200.scripts.train", "--config",
-               "configs/tiny_llama_long.yaml", "--seq_len", "64", "--micro_batch_size", "4", "--hidden_size", "64",
-               "--intermediate_size", "160", "--vocab_size", "256", "--num_hidden_layers", "2", "--num_samples", "200",
-               "--train_steps", "4", "--zero_stage", "3", "--warmup_steps", "1", "--metrics_path", str(metrics),
-               "--checkpoint_dir", str(tmp_path / name), "--checkpoint_interval", "1000", *extra]
-        r = subprocess.run(cmd, cwd=ROOT, env=dict(os.environ, CUDA_VISIBLE_DEVICES=""), capture_output=True,
-                           text=True, timeout=300)
-        assert r.returncode == 0, r.stderr[-2000:]
-        assert ("in 8 bits" in r.stdout) == (name == "all")
-        losses.append([json.loads(line)["loss"] for line in metrics.read_text().splitlines()])
-    assert len(losses[0]) == len(losses[1]) == 4
+    metrics = tmp_path / f"{name}.jsonl"
+    cmd = [sys.executable, "-m", "torch.distributed.run", "--nproc-per-node", "2", "--master-addr", "127.0.0.1",
+           "--master-port", "29653", "-m", "femtotron_b200.scripts.train", "--config", "configs/tiny_llama_long.yaml",
+           "--seq_len", "64", "--micro_batch_size", "4", "--hidden_size", "64", "--intermediate_size", "160",
+           "--vocab_size", "256", "--num_hidden_layers", "2", "--num_samples", "200", "--train_steps", "4",
+           "--warmup_steps", "1", "--metrics_path", str(metrics), "--checkpoint_dir", str(tmp_path / name),
+           "--checkpoint_interval", "1000", *extra]
+    r = subprocess.run(cmd, cwd=ROOT, env=dict(os.environ, CUDA_VISIBLE_DEVICES=""), capture_output=True, text=True,
+                       timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+    return [json.loads(line)["loss"] for line in metrics.read_text().splitlines()], r.stdout
+
+
+@pytest.mark.parametrize("layout", [["--zero_stage", "3"], ["--tp", "2"], ["--tp", "2", "--sequence_parallel", "true"]],
+                         ids=["zero3", "tp", "tp-sp"])
+def test_training_command_runs_all_of_them(tmp_path, layout):
+    """ZeRO-3 gathers and shards each layer around its 8-bit checkpoint; with tensor parallelism the
+    vocabulary shards join in the loss and the 8-bit MLP block stands aside.  The losses follow those
+    of the plain run."""
+    on, said = train(tmp_path, "all", *layout)
+    off, plain = train(tmp_path, "plain", *layout, "--ac_bits", "16", "--mlp_act8", "false", "--loss_keep_logits", "true")
+    assert "in 8 bits" in said and "in 8 bits" not in plain
+    assert len(on) == len(off) == 4
     # bf16 model: a rounding of the loss's inputs apart at most (2^-8 of a logit below 0.5)
-    assert all(abs(a - b) < 2e-3 for a, b in zip(*losses))
+    assert all(abs(a - b) < 2e-3 for a, b in zip(on, off))
 
 
 @pytest.mark.gpu

@@ -27,13 +27,14 @@ test:
 
 test-unit:
 	timeout $(TIMEOUT) $(PYTHON) -m pytest tests/test_units.py tests/test_model_vs_hf.py \
-		tests/test_bench_config.py tests/test_clocks.py -q
+		tests/test_bench_config.py tests/test_clocks.py tests/test_linear_xent.py tests/test_act8.py \
+		tests/test_rotary.py -q -m "not gpu"
 
 test-race:
 	timeout $(TIMEOUT) $(PYTHON) -m pytest tests/test_protocol_model.py -q
 
 test-integration:
-	timeout $(TIMEOUT) $(PYTHON) -m pytest tests/test_distributed_cpu.py tests/test_cli.py -q
+	timeout $(TIMEOUT) $(PYTHON) -m pytest tests/test_distributed_cpu.py tests/test_cli.py tests/test_long_context.py -q -m "not gpu"
 
 test-quick:
 	timeout $(TIMEOUT) $(PYTHON) -m pytest tests/test_units.py -q

@@ -310,7 +310,6 @@ class NormMLP8Fn(Function):
             write_weight_grad([p_gate, p_up], lambda dst, acc: linear_wgrad(dgu, n, dst, acc))
         if need[1]:
             write_vector_grad(p_norm, dw)
-        ctx.params = ctx.kept = None
         return (dx + d).view(ctx.xshape) if need[0] else None, None, None, None, None, None, None
 
 
@@ -463,7 +462,6 @@ class LinearCrossEntropyFn(Function):
             write_weight_grad([ctx.param], compute)
         else:
             compute(None, False)
-        ctx.param = None
         return dh.view(ctx.hshape) if dh is not None else None, None, None, None, None, None, None, None
 
 
@@ -474,7 +472,8 @@ def linear_cross_entropy(h: torch.Tensor, w: torch.Tensor, labels: torch.Tensor,
     h) without its logits in memory: the loss ("mean" over the labels that are not
     ``ignore_index``, or "sum"), or one fp32 loss per row ("none", flat).  With ``tp_group``, w is
     the vocabulary shard that starts at ``vstart``.  The weight gradient goes to w's gradient
-    sink; ``workspace_bytes`` bounds the backward's workspace.
+    sink; ``workspace_bytes`` bounds the part of d (the gradient of the logits) that the backward
+    has at a time, down to 256 columns of it; beside it stand fp32 sums of the hidden gradient.
 
     The mean over no labels is NaN and its gradients are zero.  A label outside the vocabulary
     makes its loss NaN.  On CUDA h and w are bf16 with a hidden size that is a multiple of 8."""

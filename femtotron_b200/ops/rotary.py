@@ -134,7 +134,10 @@ def rotary_qk(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Te
     q and k themselves turned in place.  ``pos``: [B, S] or [S], by default 0, 1, ...
 
     On CUDA a position outside the tables gives NaN and is reported by
-    ``check_kernel_errors`` (code 301); on the CPU it raises."""
+    ``check_kernel_errors`` (code 301); on the CPU it raises.  No autograd: ``rotary`` is the
+    differentiable form."""
+    if inplace and torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
+        raise ValueError("rotary_qk: in place on a tensor that autograd follows; use rotary()")
     if q.is_cuda:
         return native().rotary_qk(q, k, cos, sin, pos, interleaved, inverse, inplace, error_flag(q.device))
     pos = _check(q, k, cos, sin, pos)

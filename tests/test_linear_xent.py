@@ -198,6 +198,19 @@ def test_vocabulary_shards_join(device, world):
     close(total, dh, mh, 2.0 ** -7 + 2 * ex, 2.0 ** -7)
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_backward_twice(device):
+    """A kept graph gives the same gradient again, added to the first."""
+    h, w, lab = make(130, 64, 300, device)
+    h.requires_grad_()
+    w.requires_grad_()
+    loss = FN.linear_cross_entropy(h, w, lab, reduction="sum")
+    loss.backward(retain_graph=True)
+    one = h.grad.clone(), w.grad.clone()
+    loss.backward()
+    assert torch.equal(h.grad, 2 * one[0]) and torch.allclose(w.grad, 2 * one[1], rtol=2.0 ** -7, atol=0)
+
+
 def test_oracle_gradient_matches_differences():
     h, w, lab = make(4, 8, 12, "cpu", torch.float64, ignored=0.0)
     lab[1] = IGNORE

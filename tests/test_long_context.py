@@ -188,6 +188,13 @@ def test_training_command_runs_all_of_them(tmp_path, layout):
     assert all(abs(a - b) < 2e-3 for a, b in zip(on, off))
 
 
+def test_8_bit_mlp_block_under_zero3_without_checkpointing(tmp_path):
+    layout = ["--zero_stage", "3", "--ac_enabled", "false"]
+    on, _ = train(tmp_path, "on", *layout)
+    off, _ = train(tmp_path, "off", *layout, "--mlp_act8", "false", "--loss_keep_logits", "true")
+    assert len(on) == 4 and all(abs(a - b) < 2e-3 for a, b in zip(on, off))
+
+
 @pytest.mark.gpu
 def test_model_on_the_gpu_with_everything_on():
     from femtotron_b200.ops import attention, check_kernel_errors

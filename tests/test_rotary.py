@@ -175,6 +175,8 @@ def test_refusals(device):
         rotary.rotary_qk(q, k, cos, sin, torch.zeros(2, 4, dtype=torch.long, device=device))
     with pytest.raises(TypeError):
         rotary.rotary_qk(q, k, cos, sin, torch.zeros(2, 3, device=device))
+    with pytest.raises(ValueError):
+        rotary.rotary_qk(q.clone().requires_grad_(), k, cos, sin, inplace=True)
     for bad in ({"rope_type": "unheard-of"}, {"rope_type": "linear", "factor": 0.5}, {"rope_type": "yarn", "factor": 2.0}):
         with pytest.raises(ValueError):
             rotary.inv_frequencies(32, 10000.0, bad)

@@ -479,7 +479,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 //   full[s]      leader only: both CTAs' TMA bytes complete on it (expect_tx = 2 stages)
 //   empty[s]     both CTAs: the leader's commit multicasts to the pair when the stage is read
 //   acc_full[a]  both CTAs: commit multicast when accumulator a is complete
-//   acc_empty[a] leader only: 4 epilogue warps of each CTA arrive (8) when a is drained
+//   acc_empty[a] leader only: the epilogue warps of each CTA arrive (8 or 16) when a is drained
 // ------------------------------------------------------------------------------------------
 constexpr int PAIR_BN = 256;
 
@@ -566,11 +566,11 @@ __device__ __forceinline__ void epilogue_tile_bf16_tma(const Params& p, const CU
   }
 }
 
-template <int BN, int STAGES>
+template <int BN, int STAGES, int EW = 4>
 struct PairSmem {
   __nv_bfloat16 a[STAGES][128 * BK];
   __nv_bfloat16 b[STAGES][(BN / 2) * BK];
-  float epi[4][2][32 * 32];  // per epilogue warp: two 32x32 fp32 staging boxes (SW128 layout)
+  float epi[EW][2][32 * 32];  // per epilogue warp: two 32x32 fp32 staging boxes (SW128 layout)
   uint64_t full[STAGES];
   uint64_t empty[STAGES];
   uint64_t acc_full[2];
@@ -578,13 +578,15 @@ struct PairSmem {
   uint32_t tmem_base;
 };
 
-template <bool A_MN, bool B_MN, int PBN, int STAGES, class Epi = StdEpi>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
+// EW: epilogue warps, 4 or 8; with 8, two warps share the 32 rows of a quadrant and take half of
+// the columns each (for products whose few k-blocks leave the epilogue as the longer part).
+template <bool A_MN, bool B_MN, int PBN, int STAGES, class Epi = StdEpi, int EW = 4>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(128 + 32 * EW, 1)
     gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a,
                      const __grid_constant__ CUtensorMap tma_b,
                      const __grid_constant__ CUtensorMap tma_d, const Params p,
                      const typename Epi::Args e) {
-  using S = PairSmem<PBN, STAGES>;
+  using S = PairSmem<PBN, STAGES, EW>;
   extern __shared__ uint8_t smem_raw[];
   S& s = *reinterpret_cast<S*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
 
@@ -610,7 +612,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.acc_full[i], 1);
-      mbar_init(&s.acc_empty[i], 8);
+      mbar_init(&s.acc_empty[i], 2 * EW);
     }
     fence_barrier_init();
   }
@@ -721,7 +723,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
     }
   } else if (warp >= EPI_WARP0) {
     // ---------------- Epilogue (both CTAs) ----------------
-    const int q = warp - EPI_WARP0;
+    const int q = (warp - EPI_WARP0) & 3;
+    constexpr int EBN = PBN * 4 / EW;                   // columns of this warp
+    const int part = ((warp - EPI_WARP0) >> 2) * EBN;   // and the first of them
+    float(*box)[32 * 32] = s.epi[warp - EPI_WARP0];
     const bool f32_out = (p.mode == EPI_ACC_F32 || p.mode == EPI_STORE_F32);
     const bool bf16_tma = Epi::kBf16Tma && p.mode == EPI_STORE_BF16;
     int epi_buf = 0;
@@ -737,19 +742,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
       tile_coords(t, tiles_m, tiles_n, p.group_m, tm, tn);
       tm = rotate_m(tm, tiles_m, p.m_rot_rows, 256);
       const int m0 = tm * 256 + static_cast<int>(rank) * 128;
-      const int n0 = tn * out_cols;
+      const int n0 = tn * out_cols + part;
       if (!wait_bar(&s.acc_full[acc], acc_phase, p.err, 16)) break;
       tc_fence_after();
       if (f32_out)
-        epilogue_tile_f32_tma<PBN, Epi::kScales>(p, &tma_d, s.epi[q], tmem + acc * PBN, q, lane,
+        epilogue_tile_f32_tma<EBN, Epi::kScales>(p, &tma_d, box, tmem + acc * PBN + part, q, lane,
                                                  split * p.split_rows + m0 + q * 32, n0,
                                                  p.mode == EPI_ACC_F32, epi_buf, scale);
       else if (bf16_tma) {
         if constexpr (Epi::kBf16Tma)
-          Epi::template tile_bf16_tma<PBN>(p, e, &tma_d, s.epi[q], tmem + acc * PBN, q, lane, m0 + q * 32,
+          Epi::template tile_bf16_tma<EBN>(p, e, &tma_d, box, tmem + acc * PBN + part, q, lane, m0 + q * 32,
                                            n0, epi_buf);
       } else
-        Epi::template tile<PBN>(p, e, tmem + acc * PBN, q, lane, m0 + q * 32 + lane, n0, tn, split,
+        Epi::template tile<EBN>(p, e, tmem + acc * PBN + part, q, lane, m0 + q * 32 + lane, n0, tn, split,
                                 swiglu);
       tc_fence_before();
       __syncwarp();
@@ -807,17 +812,17 @@ static void launch(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
-template <bool A_MN, bool B_MN, int PBN, class Epi = StdEpi>
+template <bool A_MN, bool B_MN, int PBN, class Epi = StdEpi, int EW = 4>
 static void launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& td,
                         const Params& p, int num_tiles, cudaStream_t stream,
                         const typename Epi::Args& e = {}) {
-  constexpr int STAGES = PBN == 256 ? 6 : 7;
-  auto kern = gemm_pair_kernel<A_MN, B_MN, PBN, STAGES, Epi>;
-  const int smem = static_cast<int>(sizeof(PairSmem<PBN, STAGES>)) + 1024;
+  constexpr int STAGES = EW == 8 ? 4 : PBN == 256 ? 6 : 7;
+  auto kern = gemm_pair_kernel<A_MN, B_MN, PBN, STAGES, Epi, EW>;
+  const int smem = static_cast<int>(sizeof(PairSmem<PBN, STAGES, EW>)) + 1024;
   static unsigned long long configured = 0;  // per device, one mask per template instance
   smem_attr_once(kern, smem, configured);
   const int pairs = std::max(1, std::min(num_tiles, usable_sms(p) / 2));
-  kern<<<2 * pairs, NUM_THREADS, smem, stream>>>(ta, tb, td, p, e);
+  kern<<<2 * pairs, 128 + 32 * EW, smem, stream>>>(ta, tb, td, p, e);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 

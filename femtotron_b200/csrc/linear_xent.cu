@@ -11,6 +11,10 @@
 // piece's rows and the piece's share of dh from it.  The fourth product is the price of not
 // keeping the logits.
 //
+// Bound by the tensor cores for batches of a thousand tokens and more (81 to 87 % active in each
+// product, 0.94 of the sustained cuBLAS rate for 4096 tokens, 128256 words, hidden 4096: 12.9 ms for
+// the loss and both gradients), by the reads of w and the write of dw below that.
+//
 // d is rounded to bf16 because the tensor cores take it as an operand.  It is stored
 // without the upstream gradient's common factor, which is applied in fp32 to the products: the
 // entry of the label, close to -1, then keeps its leading digits exactly.
@@ -461,6 +465,14 @@ __global__ void __launch_bounds__(256) xent_dh_kernel(const float* __restrict__ 
 // ------------------------------------------------------------------ host side
 constexpr auto kBF16 = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
 
+// Where the k-blocks of a tile are over before four warps have drained the one before it, eight
+// epilogue warps (and four operand stages in place of six, to make room for their boxes) win.
+// Weight gradient of 32000 x 4096: 68.8 instead of 75.6 us for 64 tokens, 82.3 instead of 91.1 for
+// 256, but 116 instead of 112 for 512 and 262 instead of 235 for 1021 (of 5120).  d of 4096 tokens
+// over 32000 words: 101 instead of 117 us at a hidden size of 256, 125 instead of 140 at 512, 364
+// instead of 340 at 2048.
+constexpr int kFewKProduct = 256, kFewKLogits = 512;
+
 static Params base_params(int M, int N, int K, torch::Tensor& err) {
   Params p{};
   p.M = M; p.N = N; p.K = K;
@@ -482,7 +494,9 @@ static void logits_gemm(const torch::Tensor& h, const torch::Tensor& w, int64_t 
   const int tiles = (T + (pair ? 255 : 127)) / (pair ? 256 : 128) * ((N + bn - 1) / bn);
   CUtensorMap td = ta;
   if (pair && Epi::kBf16Tma) td = make_tmap_2d(p.D, kBF16, 2, N, T, p.ldd, 64, 32, true);
-  if (pair) launch_pair<false, false, 256, Epi>(ta, tb, td, p, tiles, st, e);
+  if (pair && Epi::kBf16Tma && H <= kFewKLogits)
+    launch_pair<false, false, 256, Epi, Epi::kBf16Tma ? 8 : 4>(ta, tb, td, p, tiles, st, e);
+  else if (pair) launch_pair<false, false, 256, Epi>(ta, tb, td, p, tiles, st, e);
   else if (bn == 256) launch<false, false, 256, 4, Epi>(ta, tb, p, tiles, st, e);
   else launch<false, false, 128, 6, Epi>(ta, tb, p, tiles, st, e);
 }
@@ -515,10 +529,12 @@ static void product(const void* A, int64_t lda, const void* B, int64_t ldb, int 
   CUtensorMap tb = make_tmap_2d(B, kBF16, 2, N, K, ldb, 64, 64, true);
   const int tiles = static_cast<int>(tm) * ((N + bn - 1) / bn) * ksplit;
   if (pair) {
+    const bool few_k = bn == 256 && ksplit == 1 && K <= kFewKProduct;
     CUtensorMap td = f32 ? make_tmap_2d(D, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, N,
                                         ksplit == 1 ? M : (uint64_t)ksplit * split_rows, ldd, 32, 32, true)
                          : make_tmap_2d(D, kBF16, 2, N, M, ldd, 64, 32, true);
-    if (bn == 256) launch_pair<A_MN, true, 256, XentProductEpi>(ta, tb, td, p, tiles, st, e);
+    if (few_k) launch_pair<A_MN, true, 256, XentProductEpi, 8>(ta, tb, td, p, tiles, st, e);
+    else if (bn == 256) launch_pair<A_MN, true, 256, XentProductEpi>(ta, tb, td, p, tiles, st, e);
     else launch_pair<A_MN, true, 128, XentProductEpi>(ta, tb, td, p, tiles, st, e);
   } else if (bn == 256) {
     launch<A_MN, true, 256, 4, XentProductEpi>(ta, tb, p, tiles, st, e);

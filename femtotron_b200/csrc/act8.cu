@@ -139,6 +139,42 @@ __device__ __forceinline__ void store16(T* p, int left, const float (&v)[16]) {
   }
 }
 
+// Rows on no 16-byte boundary: the warp takes its lanes' chunks two at a time, 16 lanes on
+// neighbouring values of one, and hands them over through shared memory (17 words per chunk: no bank
+// conflicts).  Every lane of the warp takes part, with left <= 0 where it has no chunk.
+template <typename T>
+__device__ __forceinline__ void load16_any(const T* p, int left, float (&v)[16], float* box) {
+  const int lane = threadIdx.x % 32;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int from = 2 * i + lane / 16, k = lane % 16;
+    const T* q = reinterpret_cast<const T*>(
+        __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(p), from));
+    const int have = __shfl_sync(0xffffffffu, left, from);
+    v[i] = k < have ? to_f(q[k]) : 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) box[(2 * i + lane / 16) * 17 + lane % 16] = v[i];
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = box[lane * 17 + i];
+}
+template <typename T>
+__device__ __forceinline__ void store16_any(T* p, int left, const float (&v)[16], float* box) {
+  const int lane = threadIdx.x % 32;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) box[lane * 17 + i] = v[i];
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int from = 2 * i + lane / 16, k = lane % 16;
+    T* q = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(p), from));
+    const int have = __shfl_sync(0xffffffffu, left, from);
+    if (k < have) q[k] = from_f<T>(box[from * 17 + k]);
+  }
+}
+template <Rows R> constexpr int kBoxes = R == kRowsAny ? 8 * 32 * 17 : 1;
+
 // Largest magnitude over the 2^lanes_log2 neighbouring threads that share a group.  NaN has to win,
 // so magnitudes are compared as their bit patterns (for non-negative floats the integer order
 // is the order of the values, with NaN above infinity).
@@ -214,7 +250,12 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, 
   const int c = slot * kChunk;
   const int left = row < rows ? n - c : 0;
   float v[16];
-  load16<T, R>(x + row * ldx + c, left, v);
+  if constexpr (R == kRowsAny) {
+    __shared__ float boxes[kBoxes<R>];
+    load16_any(x + row * ldx + c, left, v, boxes + threadIdx.x / 32 * (32 * 17));
+  } else {
+    load16<T, R>(x + row * ldx + c, left, v);
+  }
   const float top = group_top(v, lanes_log2);
   uint4 code;
   const float s = encode16(v, top, code);
@@ -233,11 +274,22 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const int8_t* __restric
   int64_t row;
   int slot;
   split_index(slots, row, slot);
-  if (row >= rows) return;
   const int c = slot * kChunk;
+  const int left = row < rows ? n - c : 0;
+  if (R != kRowsAny && left <= 0) return;
   float v[16];
-  decode16(*reinterpret_cast<const uint4*>(q + row * pitch + c), scale[row * groups + (slot >> lanes_log2)], v);
-  store16<T, R>(x + row * ldx + c, n - c, v);
+  if (left > 0)
+    decode16(*reinterpret_cast<const uint4*>(q + row * pitch + c), scale[row * groups + (slot >> lanes_log2)], v);
+  if constexpr (R == kRowsAny) {
+    __shared__ float boxes[kBoxes<R>];
+    if (left <= 0) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = 0.f;
+    }
+    store16_any(x + row * ldx + c, left, v, boxes + threadIdx.x / 32 * (32 * 17));
+  } else {
+    store16<T, R>(x + row * ldx + c, left, v);
+  }
 }
 
 // ------------------------------------------------------------------ RMSNorm

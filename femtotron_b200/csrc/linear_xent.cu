@@ -38,13 +38,10 @@ __device__ __forceinline__ float untruncate(int K) {
   return 1.f + 1.4901161e-8f * static_cast<float>((K + 15) / 16);
 }
 
-// (max, sum exp(x - max)) of a row's logits in this tile, and the label's logit.
+// (max, sum exp(x - max)) of a row's logits in this tile.
 struct XentStatsEpi {
   struct Args {
-    const int64_t* labels;
     float2* part;   // [T, tiles_n]
-    float* target;  // [T]
-    int64_t vstart;
     int tiles_n;
   };
   static constexpr bool kSplitK = false;
@@ -56,9 +53,7 @@ struct XentStatsEpi {
                                               int lane, int row, int n0, int tn, int, bool) {
     const bool row_ok = row < p.M;
     const uint32_t tbase = tmem_acc + (static_cast<uint32_t>(q * 32) << 16);
-    int64_t at = -1;  // the label's column in this tile
-    if (row_ok) at = e.labels[row] - e.vstart - n0;
-    float m = -INFINITY, s = 0.f, tgt = 0.f;
+    float m = -INFINITY, s = 0.f;
     const float fix = untruncate(p.K), unit = kLog2e * fix;
 #pragma unroll 1
     for (int c = 0; c < BN / 32; ++c) {
@@ -74,13 +69,6 @@ struct XentStatsEpi {
 #pragma unroll
         for (int i = 0; i < 32; ++i)
           if (i >= valid) v[i] = -INFINITY;
-      }
-      const int64_t off = at - c * 32;
-      const bool hit = off >= 0 && off < 32 && off < valid;
-      if (__any_sync(0xffffffffu, hit)) {  // rare: V / 32 chunks, 32 labels
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (hit && off == i) tgt = v[i];
       }
       float m0 = v[0], m1 = v[1], m2 = v[2], m3 = v[3];
 #pragma unroll
@@ -102,10 +90,7 @@ struct XentStatsEpi {
       s = s * ex2_approx(fmaf(m, unit, -base)) + ((s0 + s1) + (s2 + s3));
       m = nm;
     }
-    if (row_ok) {
-      e.part[(int64_t)row * e.tiles_n + tn] = make_float2(m * fix, s);
-      if (at >= 0 && at < BN && at < p.N - n0) e.target[row] = tgt * fix;
-    }
+    if (row_ok) e.part[(int64_t)row * e.tiles_n + tn] = make_float2(m * fix, s);
   }
 };
 
@@ -263,8 +248,7 @@ constexpr int kFewThreads = 256;
 template <int TOK, int E>  // E: 16 values per pack where rows lie on 32-byte boundaries, else 8
 __global__ void __launch_bounds__(kFewThreads, 2)
     xent_few_kernel(const __nv_bfloat16* __restrict__ h, int64_t ldh, const __nv_bfloat16* __restrict__ w, int64_t ldw,
-                    const int64_t* __restrict__ labels, float2* __restrict__ part, float* __restrict__ target, int T,
-                    int V, int H, int64_t vstart) {
+                    float2* __restrict__ part, int T, int V, int H) {
   extern __shared__ __align__(16) float hs[];  // [TOK][E / 4][packs][4]
   __shared__ float2 red[kFewThreads / 32][TOK];
   constexpr int U = 4;
@@ -337,7 +321,6 @@ __global__ void __launch_bounds__(kFewThreads, 2)
         const float base = nm == -INFINITY ? 0.f : nm * kLog2e;
         s[t] = s[t] * ex2_approx(fmaf(m[t], kLog2e, -base)) + ex2_approx(fmaf(x, kLog2e, -base));
         m[t] = nm;
-        if (lane == 0 && t < T && labels[t] == vstart + row + j) target[t] = x;
       }
     }
   }
@@ -360,19 +343,45 @@ __global__ void __launch_bounds__(kFewThreads, 2)
 }
 
 // ------------------------------------------------------------------ small kernels
-// One warp per row joins the tiles' (max, sum); stats[row] = (max, sum, target, has target).
+// Per row one warp joins the tiles' (max, sum) and another takes the label's logit, side by side;
+// stats[row] = (max, sum, target, has target).
+// The label's logit is summed again here in fp32: the loss is a difference of two numbers, and what
+// the tensor cores' truncation leaves of an error in one logit does not average out of this one
+// (at a hidden size of 8192 it was most of 1.1e-6 of the loss).
 __global__ void __launch_bounds__(256) xent_join_kernel(const float2* __restrict__ part,
-                                                        const float* __restrict__ target,
+                                                        const __nv_bfloat16* __restrict__ h, int64_t ldh,
+                                                        const __nv_bfloat16* __restrict__ w, int64_t ldw, int H,
                                                         const int64_t* __restrict__ labels,
                                                         float4* __restrict__ stats, float* __restrict__ lse,
                                                         float* __restrict__ losses, int T, int tiles_n,
                                                         int64_t vstart, int64_t V, int64_t ignore_index) {
-  const int row = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
-  if (row >= T) return;
-  const float2* p = part + (int64_t)row * tiles_n;
+  __shared__ float target[4];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int row = blockIdx.x * 4 + warp % 4;
+  const int64_t lab = row < T ? labels[row] : ignore_index;
+  const bool has = row < T && lab >= vstart && lab < vstart + V;
+  if (warp >= 4 && has) {
+    const uint4* a = reinterpret_cast<const uint4*>(h + row * ldh);
+    const uint4* b = reinterpret_cast<const uint4*>(w + (lab - vstart) * ldw);
+    float t0 = 0.f, t1 = 0.f;
+#pragma unroll 8
+    for (int i = lane; i < H / 8; i += 32) {
+      const uint4 x = a[i], y = b[i];
+      float2 f = unpack_bf16x2(x.x), g = unpack_bf16x2(y.x);
+      t0 = fmaf(f.x, g.x, t0); t1 = fmaf(f.y, g.y, t1);
+      f = unpack_bf16x2(x.y); g = unpack_bf16x2(y.y);
+      t0 = fmaf(f.x, g.x, t0); t1 = fmaf(f.y, g.y, t1);
+      f = unpack_bf16x2(x.z); g = unpack_bf16x2(y.z);
+      t0 = fmaf(f.x, g.x, t0); t1 = fmaf(f.y, g.y, t1);
+      f = unpack_bf16x2(x.w); g = unpack_bf16x2(y.w);
+      t0 = fmaf(f.x, g.x, t0); t1 = fmaf(f.y, g.y, t1);
+    }
+    t0 = warp_sum(t0 + t1);
+    if (lane == 0) target[warp - 4] = t0;
+  }
   float m = -INFINITY, s = 0.f;
-  for (int i = lane; i < tiles_n; i += 32) {
-    const float2 v = p[i];
+  for (int i = lane; i < (warp < 4 && row < T ? tiles_n : 0); i += 32) {
+    const float2 v = part[(int64_t)row * tiles_n + i];
     const float nm = fmaxf(m, v.x);
     const float base = nm == -INFINITY ? 0.f : nm * kLog2e;
     s = s * exp2f(fmaf(m, kLog2e, -base)) + v.y * exp2f(fmaf(v.x, kLog2e, -base));
@@ -386,10 +395,9 @@ __global__ void __launch_bounds__(256) xent_join_kernel(const float2* __restrict
     s = s * exp2f(fmaf(m, kLog2e, -base)) + os * exp2f(fmaf(om, kLog2e, -base));
     m = nm;
   }
-  if (lane == 0) {
-    const int64_t lab = labels[row];
-    const bool has = lab >= vstart && lab < vstart + V;
-    const float tgt = has ? target[row] : 0.f;
+  __syncthreads();
+  if (warp < 4 && lane == 0 && row < T) {
+    const float tgt = has ? target[warp] : 0.f;
     const float l = m + logf(s);
     stats[row] = make_float4(m, s, tgt, has ? 1.f : 0.f);
     lse[row] = l;
@@ -581,10 +589,8 @@ std::vector<torch::Tensor> linear_xent_fwd(const torch::Tensor& h, const torch::
   const int bn = logits_bn(T, V);
   const int tiles_n = few ? std::min((V + 15) / 16, 2 * num_sms()) : (V + bn - 1) / bn;
   const auto f32 = h.options().dtype(at::kFloat);
-  // one buffer: tiles' partials, target logits, then the results
-  torch::Tensor part = torch::empty({(int64_t)T * tiles_n * 2 + T}, f32);
+  torch::Tensor part = torch::empty({T, tiles_n, 2}, f32);
   torch::Tensor stats = torch::empty({T, 4}, f32), lse_t = torch::empty({T}, f32), losses = torch::empty({T}, f32);
-  float* target = part.data_ptr<float>() + (int64_t)T * tiles_n * 2;
   if (few) {
     const bool wide = H % 16 == 0 && w.stride(0) % 16 == 0 && reinterpret_cast<uintptr_t>(w.data_ptr()) % 32 == 0;
     auto kern = tok == 1 ? (wide ? xent_few_kernel<1, 16> : xent_few_kernel<1, 8>)
@@ -593,17 +599,17 @@ std::vector<torch::Tensor> linear_xent_fwd(const torch::Tensor& h, const torch::
     smem_attr_once(kern, 96 * 1024, done[2 * (tok - 1) + wide]);
     kern<<<tiles_n, kFewThreads, few_bytes, st>>>(
         reinterpret_cast<const __nv_bfloat16*>(h.data_ptr()), h.stride(0),
-        reinterpret_cast<const __nv_bfloat16*>(w.data_ptr()), w.stride(0), labels.data_ptr<int64_t>(),
-        reinterpret_cast<float2*>(part.data_ptr<float>()), target, T, V, H, vstart);
+        reinterpret_cast<const __nv_bfloat16*>(w.data_ptr()), w.stride(0),
+        reinterpret_cast<float2*>(part.data_ptr<float>()), T, V, H);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
   } else {
     Params p = base_params(T, V, H, err);
-    XentStatsEpi::Args e{labels.data_ptr<int64_t>(), reinterpret_cast<float2*>(part.data_ptr<float>()), target, vstart,
-                         tiles_n};
+    XentStatsEpi::Args e{reinterpret_cast<float2*>(part.data_ptr<float>()), tiles_n};
     logits_gemm<XentStatsEpi>(h, w, 0, V, p, e, bn, st);
   }
-  xent_join_kernel<<<(T + 7) / 8, 256, 0, st>>>(
-      reinterpret_cast<const float2*>(part.data_ptr<float>()), target, labels.data_ptr<int64_t>(),
+  xent_join_kernel<<<(T + 3) / 4, 256, 0, st>>>(
+      reinterpret_cast<const float2*>(part.data_ptr<float>()), reinterpret_cast<const __nv_bfloat16*>(h.data_ptr()),
+      h.stride(0), reinterpret_cast<const __nv_bfloat16*>(w.data_ptr()), w.stride(0), H, labels.data_ptr<int64_t>(),
       reinterpret_cast<float4*>(stats.data_ptr<float>()), lse_t.data_ptr<float>(), losses.data_ptr<float>(), T, tiles_n,
       vstart, V, ignore_index);
   C10_CUDA_KERNEL_LAUNCH_CHECK();

@@ -43,7 +43,39 @@ struct XentStatsEpi {
   struct Args {
     float2* part;   // [T, tiles_n]
     int tiles_n;
+    const __nv_bfloat16 *h, *w;
+    int64_t ldh, ldw;
+    const int64_t* labels;
+    float* target;  // [T]
+    int64_t vstart;
   };
+  // The label's logit is summed here in fp32, a row at a time, while the tiles go on: the loss is a
+  // difference of two numbers, and what the tensor cores' truncation leaves of an error in one
+  // logit does not average out of this one (at a hidden size of 8192 it was most of 1.1e-6 of the
+  // loss).
+  __device__ __forceinline__ static void side(const Params& p, const Args& e, int cta, int ctas, int lane) {
+    for (int row = cta; row < p.M; row += ctas) {
+      const int64_t local = e.labels[row] - e.vstart;
+      if (local < 0 || local >= p.N) continue;
+      const uint4* a = reinterpret_cast<const uint4*>(e.h + row * e.ldh);
+      const uint4* b = reinterpret_cast<const uint4*>(e.w + local * e.ldw);
+      float t0 = 0.f, t1 = 0.f;
+#pragma unroll 4
+      for (int i = lane; i < p.K / 8; i += 32) {
+        const uint4 x = a[i], y = b[i];
+        float2 f = unpack_bf16x2(x.x), g = unpack_bf16x2(y.x);
+        t0 = fmaf(f.x, g.x, t0); t1 = fmaf(f.y, g.y, t1);
+        f = unpack_bf16x2(x.y); g = unpack_bf16x2(y.y);
+        t0 = fmaf(f.x, g.x, t0); t1 = fmaf(f.y, g.y, t1);
+        f = unpack_bf16x2(x.z); g = unpack_bf16x2(y.z);
+        t0 = fmaf(f.x, g.x, t0); t1 = fmaf(f.y, g.y, t1);
+        f = unpack_bf16x2(x.w); g = unpack_bf16x2(y.w);
+        t0 = fmaf(f.x, g.x, t0); t1 = fmaf(f.y, g.y, t1);
+      }
+      t0 = warp_sum(t0 + t1);
+      if (lane == 0) e.target[row] = t0;
+    }
+  }
   static constexpr bool kSplitK = false;
   static constexpr bool kScales = false;
   static constexpr bool kBf16Tma = false;
@@ -107,6 +139,8 @@ struct XentGradEpi {
   static constexpr bool kScales = false;
   static constexpr bool kBf16Tma = true;
   __device__ __forceinline__ static float f32_scale(const Args&) { return 1.f; }
+
+  __device__ __forceinline__ static void side(const Params&, const Args&, int, int, int) {}
 
   // What turns the logits of a row into its d: p = 2^(x unit - base), less 1 at column `at`, times g.
   struct Row {
@@ -176,6 +210,7 @@ struct XentProductEpi {
   static constexpr bool kSplitK = true;
   static constexpr bool kScales = true;
   static constexpr bool kBf16Tma = true;  // split K is for fp32 outputs only
+  __device__ __forceinline__ static void side(const Params&, const Args&, int, int, int) {}
   template <int BN>
   __device__ __forceinline__ static void tile_bf16_tma(const Params& p, const Args& e, const CUtensorMap* tma_d,
                                                        float (*box)[32 * 32], uint32_t tmem_acc, int q, int lane,
@@ -248,7 +283,8 @@ constexpr int kFewThreads = 256;
 template <int TOK, int E>  // E: 16 values per pack where rows lie on 32-byte boundaries, else 8
 __global__ void __launch_bounds__(kFewThreads, 2)
     xent_few_kernel(const __nv_bfloat16* __restrict__ h, int64_t ldh, const __nv_bfloat16* __restrict__ w, int64_t ldw,
-                    float2* __restrict__ part, int T, int V, int H) {
+                    const int64_t* __restrict__ labels, float2* __restrict__ part, float* __restrict__ target, int T,
+                    int V, int H, int64_t vstart) {
   extern __shared__ __align__(16) float hs[];  // [TOK][E / 4][packs][4]
   __shared__ float2 red[kFewThreads / 32][TOK];
   constexpr int U = 4;
@@ -321,6 +357,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
         const float base = nm == -INFINITY ? 0.f : nm * kLog2e;
         s[t] = s[t] * ex2_approx(fmaf(m[t], kLog2e, -base)) + ex2_approx(fmaf(x, kLog2e, -base));
         m[t] = nm;
+        if (lane == 0 && t < T && labels[t] == vstart + row + j) target[t] = x;
       }
     }
   }
@@ -343,45 +380,19 @@ __global__ void __launch_bounds__(kFewThreads, 2)
 }
 
 // ------------------------------------------------------------------ small kernels
-// Per row one warp joins the tiles' (max, sum) and another takes the label's logit, side by side;
-// stats[row] = (max, sum, target, has target).
-// The label's logit is summed again here in fp32: the loss is a difference of two numbers, and what
-// the tensor cores' truncation leaves of an error in one logit does not average out of this one
-// (at a hidden size of 8192 it was most of 1.1e-6 of the loss).
+// One warp per row joins the tiles' (max, sum); stats[row] = (max, sum, target, has target).
 __global__ void __launch_bounds__(256) xent_join_kernel(const float2* __restrict__ part,
-                                                        const __nv_bfloat16* __restrict__ h, int64_t ldh,
-                                                        const __nv_bfloat16* __restrict__ w, int64_t ldw, int H,
+                                                        const float* __restrict__ target,
                                                         const int64_t* __restrict__ labels,
                                                         float4* __restrict__ stats, float* __restrict__ lse,
                                                         float* __restrict__ losses, int T, int tiles_n,
                                                         int64_t vstart, int64_t V, int64_t ignore_index) {
-  __shared__ float target[4];
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int row = blockIdx.x * 4 + warp % 4;
-  const int64_t lab = row < T ? labels[row] : ignore_index;
-  const bool has = row < T && lab >= vstart && lab < vstart + V;
-  if (warp >= 4 && has) {
-    const uint4* a = reinterpret_cast<const uint4*>(h + row * ldh);
-    const uint4* b = reinterpret_cast<const uint4*>(w + (lab - vstart) * ldw);
-    float t0 = 0.f, t1 = 0.f;
-#pragma unroll 8
-    for (int i = lane; i < H / 8; i += 32) {
-      const uint4 x = a[i], y = b[i];
-      float2 f = unpack_bf16x2(x.x), g = unpack_bf16x2(y.x);
-      t0 = fmaf(f.x, g.x, t0); t1 = fmaf(f.y, g.y, t1);
-      f = unpack_bf16x2(x.y); g = unpack_bf16x2(y.y);
-      t0 = fmaf(f.x, g.x, t0); t1 = fmaf(f.y, g.y, t1);
-      f = unpack_bf16x2(x.z); g = unpack_bf16x2(y.z);
-      t0 = fmaf(f.x, g.x, t0); t1 = fmaf(f.y, g.y, t1);
-      f = unpack_bf16x2(x.w); g = unpack_bf16x2(y.w);
-      t0 = fmaf(f.x, g.x, t0); t1 = fmaf(f.y, g.y, t1);
-    }
-    t0 = warp_sum(t0 + t1);
-    if (lane == 0) target[warp - 4] = t0;
-  }
+  const int row = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (row >= T) return;
+  const float2* p = part + (int64_t)row * tiles_n;
   float m = -INFINITY, s = 0.f;
-  for (int i = lane; i < (warp < 4 && row < T ? tiles_n : 0); i += 32) {
-    const float2 v = part[(int64_t)row * tiles_n + i];
+  for (int i = lane; i < tiles_n; i += 32) {
+    const float2 v = p[i];
     const float nm = fmaxf(m, v.x);
     const float base = nm == -INFINITY ? 0.f : nm * kLog2e;
     s = s * exp2f(fmaf(m, kLog2e, -base)) + v.y * exp2f(fmaf(v.x, kLog2e, -base));
@@ -395,9 +406,10 @@ __global__ void __launch_bounds__(256) xent_join_kernel(const float2* __restrict
     s = s * exp2f(fmaf(m, kLog2e, -base)) + os * exp2f(fmaf(om, kLog2e, -base));
     m = nm;
   }
-  __syncthreads();
-  if (warp < 4 && lane == 0 && row < T) {
-    const float tgt = has ? target[warp] : 0.f;
+  if (lane == 0) {
+    const int64_t lab = labels[row];
+    const bool has = lab >= vstart && lab < vstart + V;
+    const float tgt = has ? target[row] : 0.f;
     const float l = m + logf(s);
     stats[row] = make_float4(m, s, tgt, has ? 1.f : 0.f);
     lse[row] = l;
@@ -589,7 +601,9 @@ std::vector<torch::Tensor> linear_xent_fwd(const torch::Tensor& h, const torch::
   const int bn = logits_bn(T, V);
   const int tiles_n = few ? std::min((V + 15) / 16, 2 * num_sms()) : (V + bn - 1) / bn;
   const auto f32 = h.options().dtype(at::kFloat);
-  torch::Tensor part = torch::empty({T, tiles_n, 2}, f32);
+  // one buffer: the tiles' pairs, then the labels' logits
+  torch::Tensor part = torch::empty({(int64_t)T * tiles_n * 2 + T}, f32);
+  float* target = part.data_ptr<float>() + (int64_t)T * tiles_n * 2;
   torch::Tensor stats = torch::empty({T, 4}, f32), lse_t = torch::empty({T}, f32), losses = torch::empty({T}, f32);
   if (few) {
     const bool wide = H % 16 == 0 && w.stride(0) % 16 == 0 && reinterpret_cast<uintptr_t>(w.data_ptr()) % 32 == 0;
@@ -599,17 +613,19 @@ std::vector<torch::Tensor> linear_xent_fwd(const torch::Tensor& h, const torch::
     smem_attr_once(kern, 96 * 1024, done[2 * (tok - 1) + wide]);
     kern<<<tiles_n, kFewThreads, few_bytes, st>>>(
         reinterpret_cast<const __nv_bfloat16*>(h.data_ptr()), h.stride(0),
-        reinterpret_cast<const __nv_bfloat16*>(w.data_ptr()), w.stride(0),
-        reinterpret_cast<float2*>(part.data_ptr<float>()), T, V, H);
+        reinterpret_cast<const __nv_bfloat16*>(w.data_ptr()), w.stride(0), labels.data_ptr<int64_t>(),
+        reinterpret_cast<float2*>(part.data_ptr<float>()), target, T, V, H, vstart);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
   } else {
     Params p = base_params(T, V, H, err);
-    XentStatsEpi::Args e{reinterpret_cast<float2*>(part.data_ptr<float>()), tiles_n};
+    XentStatsEpi::Args e{reinterpret_cast<float2*>(part.data_ptr<float>()), tiles_n,
+                         reinterpret_cast<const __nv_bfloat16*>(h.data_ptr()),
+                         reinterpret_cast<const __nv_bfloat16*>(w.data_ptr()), h.stride(0), w.stride(0),
+                         labels.data_ptr<int64_t>(), target, vstart};
     logits_gemm<XentStatsEpi>(h, w, 0, V, p, e, bn, st);
   }
-  xent_join_kernel<<<(T + 3) / 4, 256, 0, st>>>(
-      reinterpret_cast<const float2*>(part.data_ptr<float>()), reinterpret_cast<const __nv_bfloat16*>(h.data_ptr()),
-      h.stride(0), reinterpret_cast<const __nv_bfloat16*>(w.data_ptr()), w.stride(0), H, labels.data_ptr<int64_t>(),
+  xent_join_kernel<<<(T + 7) / 8, 256, 0, st>>>(
+      reinterpret_cast<const float2*>(part.data_ptr<float>()), target, labels.data_ptr<int64_t>(),
       reinterpret_cast<float4*>(stats.data_ptr<float>()), lse_t.data_ptr<float>(), losses.data_ptr<float>(), T, tiles_n,
       vstart, V, ignore_index);
   C10_CUDA_KERNEL_LAUNCH_CHECK();

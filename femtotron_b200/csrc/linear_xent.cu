@@ -12,8 +12,8 @@
 // keeping the logits.
 //
 // Bound by the tensor cores for batches of a thousand tokens and more (81 to 87 % active in each
-// product, 0.94 of the sustained cuBLAS rate for 4096 tokens, 128256 words, hidden 4096: 12.9 ms for
-// the loss and both gradients), by the reads of w and the write of dw below that.
+// product, 0.94 of the sustained cuBLAS rate for 4096 tokens, 128256 words, hidden 4096: 12.7 to
+// 13.2 ms for the loss and both gradients), by the reads of w and the write of dw below that.
 //
 // d is rounded to bf16 because the tensor cores take it as an operand.  It is stored
 // without the upstream gradient's common factor, which is applied in fp32 to the products: the

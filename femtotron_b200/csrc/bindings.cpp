@@ -97,7 +97,7 @@ std::tuple<torch::Tensor, torch::Tensor> rotary_qk(const torch::Tensor& q, const
                                                    bool inverse, bool inplace, torch::Tensor& err);
 std::vector<torch::Tensor> linear_xent_fwd(const torch::Tensor& h, const torch::Tensor& w,
                                            const torch::Tensor& labels, int64_t vstart, int64_t ignore_index,
-                                           int64_t reduce, torch::Tensor& err);
+                                           int64_t reduce, bool graded, torch::Tensor& err);
 int64_t linear_xent_bwd(const torch::Tensor& h, const torch::Tensor& w, const torch::Tensor& labels,
                         const torch::Tensor& lse, const torch::Tensor& grad, const torch::Tensor& factor,
                         const c10::optional<torch::Tensor>& dh, const c10::optional<torch::Tensor>& dw,

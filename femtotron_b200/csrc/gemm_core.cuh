@@ -276,7 +276,6 @@ __device__ __forceinline__ void epilogue_tile(const Params& p, uint32_t tmem_acc
 //   kSplitK         whether the k-blocks of a tile are spread over Args::ksplit partial outputs
 //   tile<BN>()      consumes one accumulator tile, one output row per thread
 //   f32_scale()     factor of an fp32 output (1 unless the epilogue scales)
-//   side()          work of the otherwise idle warp 3 of CTA `cta` of `ctas`
 //   kBf16Tma        whether the pair kernel may store bf16 tiles with tile_bf16_tma<BN>()
 struct StdEpi {
   struct Args {};
@@ -289,7 +288,6 @@ struct StdEpi {
   static constexpr bool kScales = false;
   static constexpr bool kBf16Tma = false;
   __device__ __forceinline__ static float f32_scale(const Args&) { return 1.f; }
-  __device__ __forceinline__ static void side(const Params&, const Args&, int, int, int) {}
 };
 
 // Tile t of a launch -> its output tile and, with split K, its share of the k-blocks.  The
@@ -439,8 +437,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         if (acc == 0) acc_phase ^= 1;
       }
     }
-  } else if (warp == 3) {
-    Epi::side(p, e, blockIdx.x, gridDim.x, lane);
   } else if (warp >= EPI_WARP0) {
     // ---------------- Epilogue ----------------
     const int q = warp - EPI_WARP0;  // TMEM lane quadrant owned by this warp
@@ -725,8 +721,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(128 + 32 * EW, 1)
         if (acc == 0) acc_phase ^= 1;
       }
     }
-  } else if (warp == 3) {
-    Epi::side(p, e, blockIdx.x, gridDim.x, lane);
   } else if (warp >= EPI_WARP0) {
     // ---------------- Epilogue (both CTAs) ----------------
     const int q = (warp - EPI_WARP0) & 3;

@@ -34,48 +34,31 @@ constexpr float kLog2e = 1.4426950408889634f;
 // that a n / 2 of the result.  Measured against 64-bit products, a / 2 = 1.2e-8 (H = 64) to 1.54e-8
 // (H = 8192), 1.49e-8 = 2^-26 at H = 4096, where the loss was 2.0e-6 too small.  The logits of
 // both passes are therefore multiplied by 1 + 2^-26 n, folded into constants of the epilogues.
-__device__ __forceinline__ float untruncate(int K) {
+// A row whose sums do not grow evenly (a dominating channel) is not mended by this, and the loss is a
+// difference of logits.  So the label's logit is left out of the tiles' sums and the loss is
+//   log(1 + sum over j != label of exp(x_j - t)),
+// with t an fp32 sum of the label's products: it cannot be negative, a small loss keeps its digits, and
+// an error of one logit, which the sum of many averages out, does not stand alone in it.  The lse of the
+// backward is that of the accumulator's logits throughout, the label's too, times the one factor that both
+// passes use, so that p - 1 of a certain word vanishes there as well.
+__host__ __device__ __forceinline__ float untruncate(int K) {
   return 1.f + 1.4901161e-8f * static_cast<float>((K + 15) / 16);
 }
 
-// (max, sum exp(x - max)) of a row's logits in this tile.
+// What the exponentials of a row with the maximum m are taken from: m, or 0 for a row of nothing but
+// -inf, whose sum then stays 0.  The difference x - m is taken before the multiplication by log2 e: m
+// log2 e, rounded, would be off by 4e-6 for a logit of 64, and the sum with it.
+__device__ __forceinline__ float finite_base(float m) { return m == -INFINITY ? 0.f : m; }
+
+// (max, sum exp(x - max)) of a row's logits in this tile without the label's, and the label's.
 struct XentStatsEpi {
   struct Args {
-    float2* part;   // [T, tiles_n]
+    float2* part;   // [T, tiles_n]: before `untruncate`
     int tiles_n;
-    const __nv_bfloat16 *h, *w;
-    int64_t ldh, ldw;
     const int64_t* labels;
-    float* target;  // [T]
+    float* target;  // [T] the label's logit, before `untruncate`; it is not in `part`
     int64_t vstart;
   };
-  // The label's logit is summed here in fp32, a row at a time, while the tiles go on: the loss is a
-  // difference of two numbers, and what the tensor cores' truncation leaves of an error in one
-  // logit does not average out of this one (at a hidden size of 8192 it was most of 1.1e-6 of the
-  // loss).
-  __device__ __forceinline__ static void side(const Params& p, const Args& e, int cta, int ctas, int lane) {
-    for (int row = cta; row < p.M; row += ctas) {
-      const int64_t local = e.labels[row] - e.vstart;
-      if (local < 0 || local >= p.N) continue;
-      const uint4* a = reinterpret_cast<const uint4*>(e.h + row * e.ldh);
-      const uint4* b = reinterpret_cast<const uint4*>(e.w + local * e.ldw);
-      float t0 = 0.f, t1 = 0.f;
-#pragma unroll 4
-      for (int i = lane; i < p.K / 8; i += 32) {
-        const uint4 x = a[i], y = b[i];
-        float2 f = unpack_bf16x2(x.x), g = unpack_bf16x2(y.x);
-        t0 = fmaf(f.x, g.x, t0); t1 = fmaf(f.y, g.y, t1);
-        f = unpack_bf16x2(x.y); g = unpack_bf16x2(y.y);
-        t0 = fmaf(f.x, g.x, t0); t1 = fmaf(f.y, g.y, t1);
-        f = unpack_bf16x2(x.z); g = unpack_bf16x2(y.z);
-        t0 = fmaf(f.x, g.x, t0); t1 = fmaf(f.y, g.y, t1);
-        f = unpack_bf16x2(x.w); g = unpack_bf16x2(y.w);
-        t0 = fmaf(f.x, g.x, t0); t1 = fmaf(f.y, g.y, t1);
-      }
-      t0 = warp_sum(t0 + t1);
-      if (lane == 0) e.target[row] = t0;
-    }
-  }
   static constexpr bool kSplitK = false;
   static constexpr bool kScales = false;
   static constexpr bool kBf16Tma = false;
@@ -86,7 +69,8 @@ struct XentStatsEpi {
     const bool row_ok = row < p.M;
     const uint32_t tbase = tmem_acc + (static_cast<uint32_t>(q * 32) << 16);
     float m = -INFINITY, s = 0.f;
-    const float fix = untruncate(p.K), unit = kLog2e * fix;
+    const float unit = kLog2e * untruncate(p.K);
+    const int64_t at = row_ok ? e.labels[row] - e.vstart - n0 : -1;
 #pragma unroll 1
     for (int c = 0; c < BN / 32; ++c) {
       const int valid = p.N - n0 - c * 32;
@@ -102,6 +86,18 @@ struct XentStatsEpi {
         for (int i = 0; i < 32; ++i)
           if (i >= valid) v[i] = -INFINITY;
       }
+      const int64_t off = at - c * 32;
+      const bool hit = off >= 0 && off < 32;
+      if (__any_sync(0xffffffffu, hit)) {
+        float t = 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (off == i) {
+            t = v[i];
+            v[i] = -INFINITY;
+          }
+        if (hit) e.target[row] = t;
+      }
       float m0 = v[0], m1 = v[1], m2 = v[2], m3 = v[3];
 #pragma unroll
       for (int i = 4; i < 32; i += 4) {
@@ -109,20 +105,19 @@ struct XentStatsEpi {
         m2 = fmaxf(m2, v[i + 2]); m3 = fmaxf(m3, v[i + 3]);
       }
       const float nm = fmaxf(m, fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)));
-      // a row of nothing but -inf keeps its sum at 0; NaN makes the sum NaN
-      const float base = nm == -INFINITY ? 0.f : nm * unit;
+      const float from = finite_base(nm);  // NaN makes the sum NaN
       float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
 #pragma unroll
       for (int i = 0; i < 32; i += 4) {
-        s0 += ex2_approx(fmaf(v[i], unit, -base));
-        s1 += ex2_approx(fmaf(v[i + 1], unit, -base));
-        s2 += ex2_approx(fmaf(v[i + 2], unit, -base));
-        s3 += ex2_approx(fmaf(v[i + 3], unit, -base));
+        s0 += ex2_approx((v[i] - from) * unit);
+        s1 += ex2_approx((v[i + 1] - from) * unit);
+        s2 += ex2_approx((v[i + 2] - from) * unit);
+        s3 += ex2_approx((v[i + 3] - from) * unit);
       }
-      s = s * ex2_approx(fmaf(m, unit, -base)) + ((s0 + s1) + (s2 + s3));
+      s = s * ex2_approx((m - from) * unit) + ((s0 + s1) + (s2 + s3));
       m = nm;
     }
-    if (row_ok) e.part[(int64_t)row * e.tiles_n + tn] = make_float2(m * fix, s);
+    if (row_ok) e.part[(int64_t)row * e.tiles_n + tn] = make_float2(m, s);
   }
 };
 
@@ -139,8 +134,6 @@ struct XentGradEpi {
   static constexpr bool kScales = false;
   static constexpr bool kBf16Tma = true;
   __device__ __forceinline__ static float f32_scale(const Args&) { return 1.f; }
-
-  __device__ __forceinline__ static void side(const Params&, const Args&, int, int, int) {}
 
   // What turns the logits of a row into its d: p = 2^(x unit - base), less 1 at column `at`, times g.
   struct Row {
@@ -210,7 +203,6 @@ struct XentProductEpi {
   static constexpr bool kSplitK = true;
   static constexpr bool kScales = true;
   static constexpr bool kBf16Tma = true;  // split K is for fp32 outputs only
-  __device__ __forceinline__ static void side(const Params&, const Args&, int, int, int) {}
   template <int BN>
   __device__ __forceinline__ static void tile_bf16_tma(const Params& p, const Args& e, const CUtensorMap* tma_d,
                                                        float (*box)[32 * 32], uint32_t tmem_acc, int q, int lane,
@@ -353,11 +345,14 @@ __global__ void __launch_bounds__(kFewThreads, 2)
 #pragma unroll
       for (int t = 0; t < TOK; ++t) {
         const float x = warp_sum(acc[j][t]);
+        if (t < T && labels[t] == vstart + row + j) {  // the same for the whole warp
+          if (lane == 0) target[t] = x;
+          continue;
+        }
         const float nm = fmaxf(m[t], x);
-        const float base = nm == -INFINITY ? 0.f : nm * kLog2e;
-        s[t] = s[t] * ex2_approx(fmaf(m[t], kLog2e, -base)) + ex2_approx(fmaf(x, kLog2e, -base));
+        const float from = finite_base(nm);
+        s[t] = s[t] * ex2_approx((m[t] - from) * kLog2e) + ex2_approx((x - from) * kLog2e);
         m[t] = nm;
-        if (lane == 0 && t < T && labels[t] == vstart + row + j) target[t] = x;
       }
     }
   }
@@ -371,8 +366,8 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     for (int i = 1; i < kFewThreads / 32; ++i) {
       const float2 o = red[i][threadIdx.x];
       const float nm = fmaxf(v.x, o.x);
-      const float base = nm == -INFINITY ? 0.f : nm * kLog2e;
-      v.y = v.y * ex2_approx(fmaf(v.x, kLog2e, -base)) + o.y * ex2_approx(fmaf(o.x, kLog2e, -base));
+      const float from = finite_base(nm);
+      v.y = v.y * ex2_approx((v.x - from) * kLog2e) + o.y * ex2_approx((o.x - from) * kLog2e);
       v.x = nm;
     }
     part[threadIdx.x * gridDim.x + blockIdx.x] = v;
@@ -380,41 +375,72 @@ __global__ void __launch_bounds__(kFewThreads, 2)
 }
 
 // ------------------------------------------------------------------ small kernels
-// One warp per row joins the tiles' (max, sum); stats[row] = (max, sum, target, has target).
+// One warp per row joins the tiles' (max, sum), logits times `fix`, and sums the label's products in
+// fp32 (no h: `target` holds that sum already).  stats[row] = (max, sum, t, label's logit of the
+// accumulator), the first two without the label, the last two 0 and -inf where the label is not here.
 __global__ void __launch_bounds__(256) xent_join_kernel(const float2* __restrict__ part,
                                                         const float* __restrict__ target,
                                                         const int64_t* __restrict__ labels,
+                                                        const __nv_bfloat16* __restrict__ h, int64_t ldh,
+                                                        const __nv_bfloat16* __restrict__ w, int64_t ldw, int H,
                                                         float4* __restrict__ stats, float* __restrict__ lse,
                                                         float* __restrict__ losses, int T, int tiles_n,
-                                                        int64_t vstart, int64_t V, int64_t ignore_index) {
+                                                        int64_t vstart, int64_t V, int64_t ignore_index,
+                                                        float fix) {
   const int row = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
   if (row >= T) return;
   const float2* p = part + (int64_t)row * tiles_n;
+  const int64_t lab = labels[row], local = lab - vstart;
+  const bool has = local >= 0 && local < V;
+  float t = 0.f;
+  if (has && h) {
+    const uint4* a = reinterpret_cast<const uint4*>(h + row * ldh);
+    const uint4* b = reinterpret_cast<const uint4*>(w + local * ldw);
+    float t0 = 0.f, t1 = 0.f;
+#pragma unroll 8
+    for (int i = lane; i < H / 8; i += 32) {
+      const uint4 x = a[i], y = b[i];
+      float2 f = unpack_bf16x2(x.x), g = unpack_bf16x2(y.x);
+      t0 = fmaf(f.x, g.x, t0); t1 = fmaf(f.y, g.y, t1);
+      f = unpack_bf16x2(x.y); g = unpack_bf16x2(y.y);
+      t0 = fmaf(f.x, g.x, t0); t1 = fmaf(f.y, g.y, t1);
+      f = unpack_bf16x2(x.z); g = unpack_bf16x2(y.z);
+      t0 = fmaf(f.x, g.x, t0); t1 = fmaf(f.y, g.y, t1);
+      f = unpack_bf16x2(x.w); g = unpack_bf16x2(y.w);
+      t0 = fmaf(f.x, g.x, t0); t1 = fmaf(f.y, g.y, t1);
+    }
+    t = warp_sum(t0 + t1);
+  }
+  const float unit = kLog2e * fix;
   float m = -INFINITY, s = 0.f;
   for (int i = lane; i < tiles_n; i += 32) {
     const float2 v = p[i];
     const float nm = fmaxf(m, v.x);
-    const float base = nm == -INFINITY ? 0.f : nm * kLog2e;
-    s = s * exp2f(fmaf(m, kLog2e, -base)) + v.y * exp2f(fmaf(v.x, kLog2e, -base));
+    const float from = finite_base(nm);
+    s = s * exp2f((m - from) * unit) + v.y * exp2f((v.x - from) * unit);
     m = nm;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const float om = __shfl_xor_sync(0xffffffffu, m, o), os = __shfl_xor_sync(0xffffffffu, s, o);
     const float nm = fmaxf(m, om);
-    const float base = nm == -INFINITY ? 0.f : nm * kLog2e;
-    s = s * exp2f(fmaf(m, kLog2e, -base)) + os * exp2f(fmaf(om, kLog2e, -base));
+    const float from = finite_base(nm);
+    s = s * exp2f((m - from) * unit) + os * exp2f((om - from) * unit);
     m = nm;
   }
   if (lane == 0) {
-    const int64_t lab = labels[row];
-    const bool has = lab >= vstart && lab < vstart + V;
-    const float tgt = has ? target[row] : 0.f;
-    const float l = m + logf(s);
-    stats[row] = make_float4(m, s, tgt, has ? 1.f : 0.f);
-    lse[row] = l;
-    // a label that no column answers to has no probability: its loss is not a number
-    losses[row] = lab == ignore_index ? 0.f : has ? l - tgt : __int_as_float(0x7fffffff);
+    const float top = m * fix, log_s = logf(s);
+    const float at = has ? target[row] * fix : -INFINITY;
+    if (has && !h) t = target[row];
+    stats[row] = make_float4(top, s, t, at);
+    // lse = log(exp(others) + exp(at))
+    const float others = top + log_s;
+    lse[row] = fmaxf(others, at) + log1pf(expf(-fabsf(others - at)));
+    const float z = (top - t) + log_s;
+    const float loss = fmaxf(z, 0.f) + log1pf(expf(-fabsf(z)));
+    // a label that no column answers to has no probability: its loss is not a number (nor is an
+    // infinite logit's)
+    losses[row] = lab == ignore_index ? 0.f : has && t < INFINITY ? loss : __int_as_float(0x7fffffff);
   }
 }
 
@@ -583,21 +609,22 @@ static void check_operands(const torch::Tensor& h, const torch::Tensor& w, const
 
 }  // namespace gemm
 
-// {stats [T, 4] = (max, sum of exponentials, label's logit, whether the label lies in this
-// shard), lse [T], losses [T]} and, for reduce 1 (sum) or 2 (mean), {the loss, the factor of
-// its gradient (1, or 1 / rows that count)} as 0-d tensors.
+// {stats [T, 4] (see xent_join_kernel), lse [T], losses [T]} and, for reduce 1 (sum) or 2 (mean), {the
+// loss, the factor of its gradient (1, or 1 / rows that count)} as 0-d tensors.  `graded`: a
+// backward will use lse.
 std::vector<torch::Tensor> linear_xent_fwd(const torch::Tensor& h, const torch::Tensor& w,
                                            const torch::Tensor& labels, int64_t vstart, int64_t ignore_index,
-                                           int64_t reduce, torch::Tensor& err) {
+                                           int64_t reduce, bool graded, torch::Tensor& err) {
   using namespace gemm;
   check_operands(h, w, labels, err);
   const c10::cuda::CUDAGuard guard(h.device());
   auto st = at::cuda::getCurrentCUDAStream();
   const int T = h.size(0), V = w.size(0), H = h.size(1);
-  // few tokens: a read of w by plain loads (see xent_few_kernel), while h fits beside two blocks
+  // few tokens: a read of w by plain loads (see xent_few_kernel), while h fits beside two blocks.  Its
+  // logits are fp32 sums; a backward needs lse from the accumulators that it will see itself
   const int tok = T <= 1 ? 1 : 2;
   const int few_bytes = tok * H * 4;
-  const bool few = T <= kFewTokens && few_bytes <= 96 * 1024;
+  const bool few = !graded && T <= kFewTokens && few_bytes <= 96 * 1024;
   const int bn = logits_bn(T, V);
   const int tiles_n = few ? std::min((V + 15) / 16, 2 * num_sms()) : (V + bn - 1) / bn;
   const auto f32 = h.options().dtype(at::kFloat);
@@ -618,16 +645,16 @@ std::vector<torch::Tensor> linear_xent_fwd(const torch::Tensor& h, const torch::
     C10_CUDA_KERNEL_LAUNCH_CHECK();
   } else {
     Params p = base_params(T, V, H, err);
-    XentStatsEpi::Args e{reinterpret_cast<float2*>(part.data_ptr<float>()), tiles_n,
-                         reinterpret_cast<const __nv_bfloat16*>(h.data_ptr()),
-                         reinterpret_cast<const __nv_bfloat16*>(w.data_ptr()), h.stride(0), w.stride(0),
-                         labels.data_ptr<int64_t>(), target, vstart};
+    XentStatsEpi::Args e{reinterpret_cast<float2*>(part.data_ptr<float>()), tiles_n, labels.data_ptr<int64_t>(), target,
+                         vstart};
     logits_gemm<XentStatsEpi>(h, w, 0, V, p, e, bn, st);
   }
   xent_join_kernel<<<(T + 7) / 8, 256, 0, st>>>(
       reinterpret_cast<const float2*>(part.data_ptr<float>()), target, labels.data_ptr<int64_t>(),
+      few ? nullptr : reinterpret_cast<const __nv_bfloat16*>(h.data_ptr()), h.stride(0),
+      reinterpret_cast<const __nv_bfloat16*>(w.data_ptr()), w.stride(0), H,
       reinterpret_cast<float4*>(stats.data_ptr<float>()), lse_t.data_ptr<float>(), losses.data_ptr<float>(), T, tiles_n,
-      vstart, V, ignore_index);
+      vstart, V, ignore_index, few ? 1.f : untruncate(H));
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   if (reduce == 0) return {stats, lse_t, losses};
   torch::Tensor total = torch::empty({2}, f32);

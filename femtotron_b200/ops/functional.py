@@ -431,12 +431,12 @@ class LinearCrossEntropyFn(Function):
     number per row, the backward computes the product again (``ops/linear_xent.py``)."""
 
     @staticmethod
-    def forward(ctx, h, w, labels, vstart, tp_group, ignore_index, reduction, workspace_bytes):
+    def forward(ctx, h, w, labels, vstart, tp_group, ignore_index, reduction, workspace_bytes, graded):
         h2 = _as2d(h)
         lab = labels.reshape(-1).contiguous()
         sharded = tp_group is not None and dist.get_world_size(tp_group) > 1
         stats, lse, losses, loss, factor = X.forward(h2, w, lab, vstart, ignore_index,
-                                                     "none" if sharded else reduction, workspace_bytes)
+                                                     "none" if sharded else reduction, workspace_bytes, graded)
         if sharded:  # only [T, 4] numbers cross the group
             ws = dist.get_world_size(tp_group)
             allst = torch.empty(ws * stats.shape[0], 4, dtype=stats.dtype, device=stats.device)
@@ -462,7 +462,7 @@ class LinearCrossEntropyFn(Function):
             write_weight_grad([ctx.param], compute)
         else:
             compute(None, False)
-        return dh.view(ctx.hshape) if dh is not None else None, None, None, None, None, None, None, None
+        return dh.view(ctx.hshape) if dh is not None else None, None, None, None, None, None, None, None, None
 
 
 def linear_cross_entropy(h: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, *, vstart: int = 0, tp_group=None,
@@ -489,7 +489,8 @@ def linear_cross_entropy(h: torch.Tensor, w: torch.Tensor, labels: torch.Tensor,
     if labels.numel() == 0:
         rows = h.reshape(0, h.shape[-1]).float().sum(-1)
         return rows if reduction == "none" else rows.sum() if reduction == "sum" else rows.sum() / 0
-    return LinearCrossEntropyFn.apply(h, w, labels, vstart, tp_group, ignore_index, reduction, workspace_bytes)
+    graded = torch.is_grad_enabled() and (h.requires_grad or w.requires_grad)
+    return LinearCrossEntropyFn.apply(h, w, labels, vstart, tp_group, ignore_index, reduction, workspace_bytes, graded)
 
 
 def shift_labels(labels: torch.Tensor, ignore_index: int = -100) -> torch.Tensor:

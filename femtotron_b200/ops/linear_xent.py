@@ -28,12 +28,15 @@ def _pieces(T: int, V: int, workspace_bytes: int):
 
 
 def forward(h: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, vstart: int, ignore_index: int,
-            reduction: str, workspace_bytes: int = WORKSPACE_BYTES):
-    """(stats [T, 4] = (max, sum of exponentials, label's logit, whether this shard has the
-    label), lse [T], losses [T], loss, gradient factor); the last two are None for "none"."""
+            reduction: str, workspace_bytes: int = WORKSPACE_BYTES, graded: bool = True):
+    """(stats [T, 4], lse [T], losses [T], loss, gradient factor); the last two are None for "none".
+    Stats: the largest logit and the sum of exponentials over this shard without the label, the
+    label's logit in fp32 and as the kernels' accumulator has it (0 and -inf where the label is
+    not in this shard).
+    ``graded=False``: no backward will use lse, so one or two rows may be computed another way."""
     reduce = REDUCTIONS[reduction]
     if h.is_cuda:
-        out = native().linear_xent_fwd(h, w, labels, vstart, ignore_index, reduce, error_flag(h.device))
+        out = native().linear_xent_fwd(h, w, labels, vstart, ignore_index, reduce, graded, error_flag(h.device))
         LAUNCHES[0] += 2 if reduce else 1  # the proxy counted one
         return (*out, None, None) if reduce == 0 else tuple(out)
     T, V = h.shape[0], w.shape[0]
@@ -42,22 +45,30 @@ def forward(h: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, vstart: int,
     local = labels - vstart
     for a, b in _pieces(T, V, workspace_bytes):
         x = h.float() @ w[a:b].float().t()
-        nm = torch.maximum(m, x.max(-1).values)
-        s = s * torch.exp(m - nm) + torch.exp(x - nm[:, None]).sum(-1)
-        m = nm
         rows = torch.nonzero((local >= a) & (local < b))[:, 0]
         tgt[rows] = x[rows, local[rows] - a]
-    has = ((local >= 0) & (local < V)).float()
-    stats = torch.stack([m, s, tgt, has], 1)
+        x[rows, local[rows] - a] = float("-inf")
+        nm = torch.maximum(m, x.max(-1).values)
+        base = torch.where(nm == float("-inf"), torch.zeros_like(nm), nm)
+        s = s * torch.exp(m - base) + torch.exp(x - base[:, None]).sum(-1)
+        m = nm
+    has = (local >= 0) & (local < V)
+    stats = torch.stack([m, s, tgt, torch.where(has, tgt, torch.full_like(tgt, float("-inf")))], 1)
     return stats, *combine(stats, labels, ignore_index, reduction)
 
 
 def combine(stats: torch.Tensor, labels: torch.Tensor, ignore_index: int, reduction: str):
-    """(lse, losses, loss, gradient factor) of whole-vocabulary stats."""
-    lse = stats[:, 0] + torch.log(stats[:, 1])
+    """(lse, losses, loss, gradient factor) of whole-vocabulary stats.  A loss is
+    log(1 + sum over the other words of exp(x_j - label's logit)), never below 0."""
+    top, sums, tgt, at = stats.unbind(1)
+    log_s = torch.log(sums)
+    lse = torch.logaddexp(top + log_s, at)
     valid = labels != ignore_index
-    # a label that no column answers to has no probability: its loss is not a number
-    losses = torch.where(stats[:, 3] > 0, lse - stats[:, 2], torch.full_like(lse, float("nan")))
+    # a label that no column answers to has no probability: its loss is not a number (nor is an
+    # infinite logit's)
+    has = ((at != float("-inf")) | (tgt != 0)) & (tgt != float("inf"))
+    losses = torch.logaddexp((top - tgt) + log_s, torch.zeros_like(tgt))
+    losses = torch.where(has, losses, torch.full_like(lse, float("nan")))
     losses = torch.where(valid, losses, torch.zeros_like(lse))
     if reduction == "none":
         return lse, losses, None, None
@@ -70,8 +81,9 @@ def combine(stats: torch.Tensor, labels: torch.Tensor, ignore_index: int, reduct
 def merge_shards(stats: torch.Tensor) -> torch.Tensor:
     """Stats of the vocabulary shards [world, T, 4] as those of the whole vocabulary."""
     m = stats[..., 0].max(0).values
-    s = (stats[..., 1] * torch.exp(stats[..., 0] - m)).sum(0)
-    return torch.stack([m, s, stats[..., 2].sum(0), stats[..., 3].sum(0)], 1)
+    base = torch.where(m == float("-inf"), torch.zeros_like(m), m)
+    s = (stats[..., 1] * torch.exp(stats[..., 0] - base)).sum(0)
+    return torch.stack([m, s, stats[..., 2].sum(0), stats[..., 3].max(0).values], 1)
 
 
 def backward(h: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, lse: torch.Tensor, grad: torch.Tensor,

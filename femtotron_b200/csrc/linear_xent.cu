@@ -476,16 +476,19 @@ __global__ void __launch_bounds__(1024) xent_total_kernel(const float* __restric
 }
 
 // Row gradients -> their largest magnitude (the common factor) and weights relative to it.
+// Magnitudes are compared as bit patterns, so that NaN wins.  Where the largest is NaN or infinite
+// the factor is 1 and the weights are the gradients themselves: what is not finite stays in its own row.
 __global__ void __launch_bounds__(1024) xent_weights_kernel(const float* __restrict__ g, float* __restrict__ weight,
                                                             float* __restrict__ factor, int T) {
-  __shared__ float red[32];
-  float m = 0.f;
-  for (int i = threadIdx.x; i < T; i += 1024) m = fmaxf(m, fabsf(g[i]));
-  m = warp_max(m);
-  if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = m;
+  __shared__ uint32_t red[32];
+  uint32_t top = 0;
+  for (int i = threadIdx.x; i < T; i += 1024) top = max(top, __float_as_uint(g[i]) & 0x7fffffffu);
+  top = __reduce_max_sync(0xffffffffu, top);
+  if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = top;
   __syncthreads();
-  m = warp_max(red[threadIdx.x % 32]);
-  for (int i = threadIdx.x; i < T; i += 1024) weight[i] = m > 0.f ? g[i] / m : 0.f;
+  top = __reduce_max_sync(0xffffffffu, red[threadIdx.x % 32]);
+  const float m = top > 0 && top < 0x7f800000u ? __uint_as_float(top) : 1.f;
+  for (int i = threadIdx.x; i < T; i += 1024) weight[i] = g[i] / m;
   if (threadIdx.x == 0) { factor[0] = m; factor[1] = 1.f; }
 }
 

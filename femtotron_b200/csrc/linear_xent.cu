@@ -475,20 +475,24 @@ __global__ void __launch_bounds__(1024) xent_total_kernel(const float* __restric
   }
 }
 
-// Row gradients -> their largest magnitude (the common factor) and weights relative to it.
+// Row gradients -> their largest magnitude (the common factor) and weights relative to it.  An ignored
+// row's gradient counts as 0, whatever it holds.
 // Magnitudes are compared as bit patterns, so that NaN wins.  Where the largest is NaN or infinite
 // the factor is 1 and the weights are the gradients themselves: what is not finite stays in its own row.
-__global__ void __launch_bounds__(1024) xent_weights_kernel(const float* __restrict__ g, float* __restrict__ weight,
-                                                            float* __restrict__ factor, int T) {
+__global__ void __launch_bounds__(1024) xent_weights_kernel(const float* __restrict__ g,
+                                                            const int64_t* __restrict__ labels,
+                                                            float* __restrict__ weight, float* __restrict__ factor,
+                                                            int T, int64_t ignore_index) {
   __shared__ uint32_t red[32];
   uint32_t top = 0;
-  for (int i = threadIdx.x; i < T; i += 1024) top = max(top, __float_as_uint(g[i]) & 0x7fffffffu);
+  for (int i = threadIdx.x; i < T; i += 1024)
+    if (labels[i] != ignore_index) top = max(top, __float_as_uint(g[i]) & 0x7fffffffu);
   top = __reduce_max_sync(0xffffffffu, top);
   if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = top;
   __syncthreads();
   top = __reduce_max_sync(0xffffffffu, red[threadIdx.x % 32]);
   const float m = top > 0 && top < 0x7f800000u ? __uint_as_float(top) : 1.f;
-  for (int i = threadIdx.x; i < T; i += 1024) weight[i] = g[i] / m;
+  for (int i = threadIdx.x; i < T; i += 1024) weight[i] = labels[i] != ignore_index ? g[i] / m : 0.f;
   if (threadIdx.x == 0) { factor[0] = m; factor[1] = 1.f; }
 }
 
@@ -706,7 +710,8 @@ int64_t linear_xent_bwd(const torch::Tensor& h, const torch::Tensor& w, const to
   torch::Tensor weights;
   if (grad.dim() > 0) {
     weights = torch::empty({T + 2}, f32);
-    xent_weights_kernel<<<1, 1024, 0, st>>>(fa, weights.data_ptr<float>() + 2, weights.data_ptr<float>(), T);
+    xent_weights_kernel<<<1, 1024, 0, st>>>(fa, labels.data_ptr<int64_t>(), weights.data_ptr<float>() + 2,
+                                            weights.data_ptr<float>(), T, ignore_index);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
     fa = weights.data_ptr<float>();
     fb = fa + 1;

@@ -673,6 +673,8 @@ std::vector<torch::Tensor> linear_xent_fwd(const torch::Tensor& h, const torch::
 
 // grad: fp32, one value (times factor: the gradient of a sum or mean) or one per row.
 // dh: bf16 [T, H] or none; dw: [V, H] bf16 or fp32 or none, stored or accumulated.
+// Holds d and all shares of the hidden gradient but one within workspace_bytes (or 256 columns of d,
+// where that is more), and one fp32 [T, H] sum beside them (T rounded up to 256 above 128).
 // Returns the number of kernels launched.
 int64_t linear_xent_bwd(const torch::Tensor& h, const torch::Tensor& w, const torch::Tensor& labels,
                         const torch::Tensor& lse, const torch::Tensor& grad, const torch::Tensor& factor,
@@ -730,20 +732,25 @@ int64_t linear_xent_bwd(const torch::Tensor& h, const torch::Tensor& w, const to
   // TFLOP/s per unit (a pair of SMs, or half of it), and the last kernel's read of the partial
   // outputs at 6.5 TB/s.  1021 tokens of 5120, 32003 words: 80 tiles for 74 pairs, so unsplit
   // the second wave is nearly empty: 422 us by the model, 262 us in 7 shares (measured: 264 in 12).
+  // All shares but the first, which the sum over the pieces needs anyway, come out of what d leaves
+  // of the workspace.
   const bool pair = T > 128 && H > 128;
   const long units = pair ? num_sms() / 2 : num_sms();
   const long tiles = (T + (pair ? 255 : 127)) / (pair ? 256 : 128) * ((H + 255) / 256);
   const long kblocks = (std::min<int64_t>(piece, V) + BK - 1) / BK;
+  // the pair kernel stores whole tiles of 256 rows into a share
+  const int64_t split_rows = pair ? (T + 255) / 256 * 256 : T;
   long ksplit = 1;
   if (dh.has_value()) {
+    const int64_t left = std::max<int64_t>(0, workspace_bytes - 2 * T * ldd);
+    const long most_shares = std::min<int64_t>({32, std::max<long>(1, kblocks / 8), 1 + left / (4 * split_rows * H)});
     const double tile_s = (pair ? 2.0 : 1.0) * 2 * 128 * 256 * double(V) / (pair ? 20e12 : 10e12);
     double best = 1e30;
-    for (long k = 1; k <= std::min<long>(32, std::max<long>(1, kblocks / 8)); ++k) {
+    for (long k = 1; k <= most_shares; ++k) {
       const double cost = double((tiles * k + units - 1) / units) / k * tile_s + k * (4.0 * T * H) / 6.5e12;
       if (cost < best * 0.98) { best = cost; ksplit = k; }
     }
   }
-  const int64_t split_rows = (T + 255) / 256 * 256;
   torch::Tensor acc;
   if (dh.has_value()) acc = torch::empty({ksplit * split_rows, H}, f32);
 

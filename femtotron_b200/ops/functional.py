@@ -472,8 +472,10 @@ def linear_cross_entropy(h: torch.Tensor, w: torch.Tensor, labels: torch.Tensor,
     h) without its logits in memory: the loss ("mean" over the labels that are not
     ``ignore_index``, or "sum"), or one fp32 loss per row ("none", flat).  With ``tp_group``, w is
     the vocabulary shard that starts at ``vstart``.  The weight gradient goes to w's gradient
-    sink; ``workspace_bytes`` bounds the part of d (the gradient of the logits) that the backward
-    has at a time, down to 256 columns of it; beside it stand fp32 sums of the hidden gradient.
+    sink.  ``workspace_bytes`` bounds what the backward holds of d (the gradient of the logits), down
+    to 256 columns of it, together with the partial sums of the hidden gradient that it splits for
+    speed; one fp32 sum of the size of h stands beside them.  The forward keeps 8 bytes per row and
+    256 columns until it returns.
 
     The mean over no labels is NaN and its gradients are zero.  A label outside the vocabulary
     makes its loss NaN.  On CUDA h and w are bf16 with a hidden size that is a multiple of 8."""

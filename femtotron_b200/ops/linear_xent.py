@@ -4,9 +4,11 @@
     d_tj  = g_t (exp(x_tj - lse_t) - [j = label_t]),   dh = d w,   dw = d^T h
 
 The forward keeps one fp32 number per row (``lse``); the backward computes the product again
-and works through the vocabulary in pieces, so no more than ``workspace_bytes`` of ``d`` exist
-at a time.  CUDA tensors (bf16) run ``csrc/linear_xent.cu``, which keeps the logits in fp32
-(the head that stores them rounds them to bf16); CPU tensors run the same pieces in PyTorch.
+and works through the vocabulary in pieces, so that ``d`` and the partial sums of dh stay within
+``workspace_bytes`` beside one fp32 sum of dh.  CUDA tensors (bf16) run
+``csrc/linear_xent.cu``, which keeps the logits in fp32 (the head that stores them rounds them
+to bf16); CPU tensors run the same pieces in PyTorch.  Where the bf16 logits of a batch are
+smaller than the workspace, a smaller ``workspace_bytes`` keeps the backward below them.
 The autograd entry point is ``functional.linear_cross_entropy``.
 
 The reference computes ``F.cross_entropy`` on full-vocab logits gathered over TP

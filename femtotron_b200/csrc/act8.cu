@@ -595,7 +595,7 @@ __global__ void __launch_bounds__(256, 5) swiglu8_kernel(const __nv_bfloat16* __
     scale[(2 * row + 1) * groups + (slot >> lanes_log2)] = su;
   }
 #pragma unroll
-  for (int i = 0; i < 16; ++i) g[i] = g[i] * u[i] * sigmoid(g[i]);
+  for (int i = 0; i < 16; ++i) g[i] = g[i] * sigmoid(g[i]) * u[i];  // g u may leave fp32's range
   store16<__nv_bfloat16, R>(h + row * ldh + c, left, g);
 }
 
@@ -624,7 +624,7 @@ __global__ void __launch_bounds__(256) swiglu8_bwd_kernel(const __nv_bfloat16* _
     const float s = sigmoid(g[i]);
     const float gs = g[i] * s;
     hv[i] = gs * u[i];
-    u[i] = d[i] * u[i] * s * (1.f + g[i] * (1.f - s));  // dg
+    u[i] = s * (1.f + g[i] * (1.f - s)) * u[i] * d[i];  // dg: s first, d u may leave fp32's range
     g[i] = d[i] * gs;                                   // du
   }
   store16<__nv_bfloat16, R>(dgu + row * lddgu + c, F - c, u);

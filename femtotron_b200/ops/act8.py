@@ -172,5 +172,5 @@ def swiglu_bwd(dh: torch.Tensor, a: Act8):
     v = _decode(a.codes, a.scales, F, a.group).view(-1, 2, F)
     g, u = v[:, 0], v[:, 1]
     s = torch.sigmoid(g)
-    dgu = torch.cat([d * u * s * (1 + g * (1 - s)), d * g * s], 1).to(a.dtype)
+    dgu = torch.cat([s * (1 + g * (1 - s)) * u * d, g * s * d], 1).to(a.dtype)
     return dgu.view(a.shape), (g * s * u).to(a.dtype).view(dh.shape)

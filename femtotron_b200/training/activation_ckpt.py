@@ -7,12 +7,13 @@ and re-add the wrapper prefix, so checkpoints keep the unwrapped parameter names
 wrapped module object itself is reused, so hooks installed on it (e.g. ZeRO-3 unit hooks)
 stay inside the checkpointed region and fire again during the recomputation.
 
-``bits=8`` keeps the wrapped module's first argument (the hidden states) in 8 bits
-(``ops/act8.py``) instead of its own dtype between forward and backward: half the memory of bf16
-checkpoints.  The forward runs on the exact values; the recomputation, and so the gradients,
-on the kept ones."""
+``bits=8`` keeps the wrapped module's first argument (the hidden states, by position or keyword)
+in 8 bits (``ops/act8.py``) instead of its own dtype between forward and backward: half the
+memory of bf16 checkpoints.  The forward runs on the exact values; the recomputation, and so the
+gradients, on the kept ones.  It is a non-reentrant checkpoint like the 16-bit one."""
 from __future__ import annotations
 
+import inspect
 from typing import Any
 
 import torch
@@ -24,39 +25,22 @@ from femtotron_b200.ops import act8
 _PREFIX = "_checkpoint_wrapped_module"
 
 
-class _Checkpoint8Fn(torch.autograd.Function):
-    """Runs ``fn(x)`` without a graph, keeps x in 8 bits, and runs fn again in the backward."""
+def _checkpoint8(x: torch.Tensor, call, preserve_rng_state: bool):
+    """Non-reentrant checkpoint of ``call(x)`` that holds x in 8 bits: the first run takes x itself
+    (in the graph, so its gradient flows on), every recomputation the kept values."""
+    kept, exact, wants = act8.quantize(x), [x], x.requires_grad
 
-    @staticmethod
-    def forward(ctx, x, fn, preserve_rng_state):
-        ctx.fn = fn
-        ctx.devices = [x.device.index] if x.is_cuda else []
-        ctx.rng = None
-        if preserve_rng_state:
-            ctx.rng = (torch.get_rng_state(), [torch.cuda.get_rng_state(d) for d in ctx.devices])
-        ctx.autocast = (torch.is_autocast_enabled(x.device.type), torch.get_autocast_dtype(x.device.type))
-        a = act8.quantize(x)
-        ctx.save_for_backward(a.codes, a.scales)
-        ctx.kept = (a.n, a.shape, a.dtype, a.group)
-        with torch.no_grad():
-            return fn(x)
+    def run(_):
+        return call(exact.pop() if exact else kept.dequantize().requires_grad_(wants))
+    # the empty tensor tells checkpoint whose device's generator to keep
+    return checkpoint(run, x.new_empty(0), use_reentrant=False, preserve_rng_state=preserve_rng_state)
 
-    @staticmethod
-    def backward(ctx, *grads):
-        x = act8.Act8(*ctx.saved_tensors, *ctx.kept).dequantize().requires_grad_()
-        on, dtype = ctx.autocast
-        with torch.random.fork_rng(ctx.devices, enabled=ctx.rng is not None), torch.enable_grad(), \
-                torch.autocast(x.device.type, dtype=dtype, enabled=on):
-            if ctx.rng is not None:
-                torch.set_rng_state(ctx.rng[0])
-                for d, state in zip(ctx.devices, ctx.rng[1]):
-                    torch.cuda.set_rng_state(state, d)
-            out = ctx.fn(x)
-        outs = out if isinstance(out, tuple) else (out,)
-        pairs = [(o, g) for o, g in zip(outs, grads) if torch.is_tensor(o) and o.requires_grad and g is not None]
-        torch.autograd.backward([o for o, _ in pairs], [g for _, g in pairs])
-        ctx.fn = None
-        return x.grad, None, None
+
+def _first_parameter(module: nn.Module) -> str | None:
+    try:
+        return next(iter(inspect.signature(module.forward).parameters), None)
+    except (TypeError, ValueError):
+        return None
 
 
 class ActivationCheckpointWrapper(nn.Module):
@@ -65,6 +49,8 @@ class ActivationCheckpointWrapper(nn.Module):
         super().__init__()
         if bits not in (8, 16):
             raise ValueError(f"activation checkpoints are kept in 8 bits or as they are (16), got {bits}")
+        if bits == 8 and use_reentrant:
+            raise ValueError("activation checkpoints in 8 bits are non-reentrant: use_reentrant must be False")
         self._checkpoint_wrapped_module = module
         self.use_reentrant = use_reentrant
         self.preserve_rng_state = preserve_rng_state
@@ -80,10 +66,14 @@ class ActivationCheckpointWrapper(nn.Module):
     def forward(self, *args: Any, **kwargs: Any) -> Any:
         if not torch.is_grad_enabled():
             return self._checkpoint_wrapped_module(*args, **kwargs)
-        if self.bits == 8 and args and torch.is_tensor(args[0]) and args[0].is_floating_point() and \
-                args[0].requires_grad:
-            module, rest = self._checkpoint_wrapped_module, args[1:]
-            return _Checkpoint8Fn.apply(args[0], lambda x: module(x, *rest, **kwargs), self.preserve_rng_state)
+        if self.bits == 8:
+            module = self._checkpoint_wrapped_module
+            name = _first_parameter(module) if not args else None
+            x = args[0] if args else kwargs.get(name)
+            if torch.is_tensor(x) and x.is_floating_point():
+                rest, others = args[1:], {k: v for k, v in kwargs.items() if k != name}
+                call = (lambda h: module(h, *rest, **others)) if args else (lambda h: module(**{name: h}, **others))
+                return _checkpoint8(x, call, self.preserve_rng_state)
         return checkpoint(self._checkpoint_wrapped_module, *args, use_reentrant=self.use_reentrant,
                           preserve_rng_state=self.preserve_rng_state, **kwargs)
 

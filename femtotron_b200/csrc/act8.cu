@@ -22,6 +22,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_fp16.h>
 
+#include "checks.h"
 #include "common.cuh"
 
 namespace ft {
@@ -746,6 +747,7 @@ std::tuple<torch::Tensor, torch::Tensor> act8_quantize(const torch::Tensor& x, i
 // The kept values as a contiguous tensor of `sizes` (rows of n values).
 torch::Tensor act8_dequantize(const torch::Tensor& q, const torch::Tensor& scale, const std::vector<int64_t>& sizes,
                               int64_t n, torch::ScalarType dtype, int64_t group) {
+  check_one_device("act8.dequantize", q, scale);
   check_code(q, scale, q.size(0), n, group);
   TORCH_CHECK(dtype == at::kBFloat16 || dtype == at::kHalf || dtype == at::kFloat,
               "act8.dequantize: bf16, fp16 or fp32 expected, got ", dtype);
@@ -780,6 +782,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> act8_rms_
                                                                                      const torch::Tensor& weight,
                                                                                      double eps, int64_t group) {
   check_group(group);
+  check_one_device("act8.rms_norm", x, weight);
   const c10::cuda::CUDAGuard guard(x.device());
   const torch::Tensor r = as_rows(x, "x", true);
   const int64_t rows = r.size(0);
@@ -811,6 +814,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> act8_rms_
 std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> act8_rms_norm_bwd(
     const torch::Tensor& dy, const torch::Tensor& q, const torch::Tensor& scale, const torch::Tensor& weight,
     const torch::Tensor& rstd, int64_t group, torch::Tensor& err) {
+  check_one_device("act8.rms_norm_bwd", dy, q, scale, weight, rstd, err);
   const c10::cuda::CUDAGuard guard(dy.device());
   const torch::Tensor g = as_rows(dy, "dy", true);
   const int64_t rows = g.size(0);
@@ -884,6 +888,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> act8_swiglu(const torch:
 // (dgu, h8)
 std::tuple<torch::Tensor, torch::Tensor> act8_swiglu_bwd(const torch::Tensor& dh, const torch::Tensor& q,
                                                          const torch::Tensor& scale, int64_t group) {
+  check_one_device("act8.swiglu_bwd", dh, q, scale);
   const c10::cuda::CUDAGuard guard(dh.device());
   const torch::Tensor r = as_rows(dh, "dh", true);
   const int64_t rows = r.size(0);

@@ -21,6 +21,7 @@
 // dh is summed over the pieces in fp32.  A product with too few tiles for the GPU (dh of a short
 // batch, whose sum runs over the vocabulary) is split over the sum into partial outputs that a
 // last kernel adds in a fixed order: no atomics, the same bits on every run.
+#include "checks.h"
 #include "gemm_core.cuh"
 
 namespace ft {
@@ -598,6 +599,7 @@ static void product(const void* A, int64_t lda, const void* B, int64_t ldb, int 
 
 static void check_operands(const torch::Tensor& h, const torch::Tensor& w, const torch::Tensor& labels,
                            const torch::Tensor& err) {
+  check_one_device("linear_xent", h, w, labels, err);
   TORCH_CHECK(h.dim() == 2 && w.dim() == 2, "linear_xent: h and w must be matrices");
   TORCH_CHECK(h.size(1) == w.size(1) && h.size(1) >= 8 && h.size(1) % 8 == 0,
               "linear_xent: h and w must agree in a hidden size that is a multiple of 8, got ", h.size(1), " and ",
@@ -682,6 +684,9 @@ int64_t linear_xent_bwd(const torch::Tensor& h, const torch::Tensor& w, const to
                         bool accumulate, int64_t vstart, int64_t ignore_index, int64_t workspace_bytes,
                         torch::Tensor& err) {
   using namespace gemm;
+  check_one_device("linear_xent_bwd", h, lse, grad, factor);
+  if (dh.has_value()) check_one_device("linear_xent_bwd", h, *dh);
+  if (dw.has_value()) check_one_device("linear_xent_bwd", h, *dw);
   check_operands(h, w, labels, err);
   const int T = h.size(0), H = h.size(1), V = w.size(0);
   TORCH_CHECK(lse.is_cuda() && lse.scalar_type() == at::kFloat && lse.is_contiguous() && lse.numel() == T);

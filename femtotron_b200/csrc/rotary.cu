@@ -22,6 +22,7 @@
 
 #include <type_traits>
 
+#include "checks.h"
 #include "common.cuh"
 
 namespace ft {
@@ -190,6 +191,8 @@ std::tuple<torch::Tensor, torch::Tensor> rotary_qk(const torch::Tensor& q_, cons
   TORCH_CHECK_VALUE(k.size(0) == B && k.size(1) == S && k.size(3) == d && k.scalar_type() == type &&
                         k.device() == q.device(),
                     "rotary_qk: q and k must agree in batch, tokens, d, dtype and device");
+  check_one_device("rotary_qk", q, cos_t, sin_t, err);
+  if (pos_.has_value()) check_one_device("rotary_qk", q, *pos_);
   TORCH_CHECK(q.is_cuda() && (type == at::kBFloat16 || type == at::kHalf || type == at::kFloat),
               "rotary_qk: bf16, fp16 or fp32 CUDA tensors expected, got ", type);
   TORCH_CHECK_VALUE(cos_t.dim() == 2 && cos_t.sizes() == sin_t.sizes() && cos_t.scalar_type() == at::kFloat &&

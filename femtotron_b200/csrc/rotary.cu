@@ -20,7 +20,10 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
+#include <cstdlib>
 #include <type_traits>
+#include <utility>
 
 #include "checks.h"
 #include "common.cuh"
@@ -174,6 +177,55 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
   }
 }
 
+// Elements from the first to the last one of x, or -1 where, going up the strides, a step does not
+// clear what lies below it: then elements share memory.
+int64_t reach_of(const torch::Tensor& x) {
+  std::pair<int64_t, int64_t> dims[4];
+  int n = 0;
+  for (int i = 0; i < 4; ++i)
+    if (x.size(i) > 1) dims[n++] = {x.stride(i), x.size(i)};
+  std::sort(dims, dims + n);
+  int64_t reach = 0;
+  for (int i = 0; i < n; ++i) {
+    if (dims[i].first <= reach) return -1;
+    reach += dims[i].first * (dims[i].second - 1);
+  }
+  return reach;
+}
+
+struct Steps { int64_t stride, up, down; };  // and the most steps along it in q and in k
+
+// Whether steps of q less steps of k can come to `rest`.
+bool meet(const Steps* dims, int n, int64_t rest) {
+  if (n == 0) return rest == 0;
+  int64_t below = 0;
+  for (int i = 1; i < n; ++i) below += dims[i].stride * std::max(dims[i].up, dims[i].down);
+  // below spans a few strides at most: q and k do not overlap themselves
+  const int64_t st = dims[0].stride;
+  for (int64_t c = std::max(-dims[0].down, (rest - below) / st - 1); c <= dims[0].up && c * st - rest <= below; ++c)
+    if (std::abs(c * st - rest) <= below && meet(dims + 1, n - 1, rest - c * st)) return true;
+  return false;
+}
+
+// Whether q or k overlaps itself, or q and k, laid out alike, have an element in common.
+bool written_twice(const torch::Tensor& q, const torch::Tensor& k) {
+  const int64_t rq = q.numel() ? reach_of(q) : 0, rk = k.numel() ? reach_of(k) : 0;
+  if (rq < 0 || rk < 0) return true;
+  if (q.numel() == 0 || k.numel() == 0) return false;
+  const int64_t bytes = reinterpret_cast<intptr_t>(k.data_ptr()) - reinterpret_cast<intptr_t>(q.data_ptr());
+  const int64_t es = q.element_size(), apart = bytes / es;
+  if (apart > rq || apart < -rk || bytes % es) return false;
+  Steps dims[4];
+  int n = 0;
+  for (int i = 0; i < 4; ++i) {
+    if (q.size(i) > 1 && k.size(i) > 1 && q.stride(i) != k.stride(i)) return false;  // not laid out alike
+    if (q.size(i) > 1 || k.size(i) > 1)
+      dims[n++] = {q.size(i) > 1 ? q.stride(i) : k.stride(i), q.size(i) - 1, k.size(i) - 1};
+  }
+  std::sort(dims, dims + n, [](const Steps& a, const Steps& b) { return a.stride > b.stride; });
+  return meet(dims, n, apart);
+}
+
 }  // namespace
 
 // q [B, S, nq, d] and k [B, S, nkv, d] (any strides with a unit inner one) -> turned copies, or
@@ -208,6 +260,8 @@ std::tuple<torch::Tensor, torch::Tensor> rotary_qk(const torch::Tensor& q_, cons
     q = q.contiguous();
     k = k.contiguous();
   }
+  // threads would race on an element with two names
+  TORCH_CHECK(!inplace || !written_twice(q, k), "rotary_qk: in place on q and k that name an element more than once");
   RotaryParams p;
   p.pos = nullptr;
   p.pb = p.ps = 0;

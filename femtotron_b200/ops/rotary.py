@@ -126,6 +126,46 @@ def _check(q, k, cos, sin, pos):
     return pos
 
 
+def _reach(x: torch.Tensor) -> int:
+    """Elements from the first to the last one of x, or -1 where, going up the strides, a step does
+    not clear what lies below it: then elements share memory."""
+    reach = 0
+    for st, n in sorted((st, n) for st, n in zip(x.stride(), x.shape) if n > 1):
+        if st <= reach:
+            return -1
+        reach += st * (n - 1)
+    return reach
+
+
+def _written_twice(q: torch.Tensor, k: torch.Tensor) -> bool:
+    """Whether q or k overlaps itself, or q and k, laid out alike, have an element in common (as
+    written_twice of csrc/rotary.cu)."""
+    if q.numel() == 0 or k.numel() == 0:
+        return any(x.numel() and _reach(x) < 0 for x in (q, k))
+    reach = [_reach(x) for x in (q, k)]
+    if min(reach) < 0:
+        return True
+    apart, part = divmod(k.data_ptr() - q.data_ptr(), q.element_size())
+    if apart > reach[0] or apart < -reach[1] or part:
+        return False
+    dims = []  # (stride, most steps of q, of k)
+    for sq, sk, nq, nk in zip(q.stride(), k.stride(), q.shape, k.shape):
+        if nq > 1 and nk > 1 and sq != sk:
+            return False  # not laid out alike
+        if nq > 1 or nk > 1:
+            dims.append((sq if nq > 1 else sk, nq - 1, nk - 1))
+    dims.sort(reverse=True)
+
+    def meet(i: int, rest: int) -> bool:  # steps of q less steps of k that come to `rest`
+        if i == len(dims):
+            return rest == 0
+        st, up, down = dims[i]
+        below = sum(t * max(a, b) for t, a, b in dims[i + 1:])
+        return any(meet(i + 1, rest - c * st)
+                   for c in range(max(-down, -((below - rest) // st)), min(up, (rest + below) // st) + 1))
+    return meet(0, apart)
+
+
 def rotary_qk(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
               pos: torch.Tensor | None = None, *, interleaved: bool = False, inverse: bool = False,
               inplace: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
@@ -135,12 +175,14 @@ def rotary_qk(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Te
 
     On CUDA a position outside the tables gives NaN and is reported by
     ``check_kernel_errors`` (code 301); on the CPU it raises.  No autograd: ``rotary`` is the
-    differentiable form."""
+    differentiable form.  In place, every element of q and k has to be one of its own."""
     if inplace and torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
         raise ValueError("rotary_qk: in place on a tensor that autograd follows; use rotary()")
     if q.is_cuda:
         return native().rotary_qk(q, k, cos, sin, pos, interleaved, inverse, inplace, error_flag(q.device))
     pos = _check(q, k, cos, sin, pos)
+    if inplace and _written_twice(q, k):
+        raise RuntimeError("rotary_qk: in place on q and k that name an element more than once")
     if pos is None:
         pos = torch.arange(q.shape[1], device=q.device)[None]
     if pos.numel() and (int(pos.min()) < 0 or int(pos.max()) >= cos.shape[0]):

@@ -444,7 +444,8 @@ class LinearCrossEntropyFn(Function):
             lse, losses, loss, factor = X.combine(X.merge_shards(allst.view(ws, -1, 4)), lab, ignore_index,
                                                   reduction)
         ctx.save_for_backward(h2, w.detach(), lab, lse, lse if factor is None else factor)
-        ctx.param = w
+        # a weight that was itself computed has no sink: its gradient flows on
+        ctx.sink = w if w.is_leaf or getattr(w, "main_grad", None) is not None else None
         ctx.meta = (vstart, ignore_index, workspace_bytes, reduction)
         ctx.hshape = h.shape
         return losses if reduction == "none" else loss
@@ -458,11 +459,15 @@ class LinearCrossEntropyFn(Function):
 
         def compute(dw, acc):
             X.backward(h2, w, lab, lse, grad, factor, dh, dw, acc, vstart, ignore_index, workspace_bytes)
-        if ctx.needs_input_grad[1]:
-            write_weight_grad([ctx.param], compute)
-        else:
+        dw = None
+        if not ctx.needs_input_grad[1]:
             compute(None, False)
-        return dh.view(ctx.hshape) if dh is not None else None, None, None, None, None, None, None, None, None
+        elif ctx.sink is not None:
+            write_weight_grad([ctx.sink], compute)
+        else:
+            dw = torch.empty_like(w, memory_format=torch.contiguous_format)
+            compute(dw, False)
+        return dh.view(ctx.hshape) if dh is not None else None, dw, None, None, None, None, None, None, None
 
 
 def linear_cross_entropy(h: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, *, vstart: int = 0, tp_group=None,
@@ -471,8 +476,10 @@ def linear_cross_entropy(h: torch.Tensor, w: torch.Tensor, labels: torch.Tensor,
     """Cross entropy of the head ``h [..., H] @ w [V, H]^T`` against ``labels`` (one per row of
     h) without its logits in memory: the loss ("mean" over the labels that are not
     ``ignore_index``, or "sum"), or one fp32 loss per row ("none", flat).  With ``tp_group``, w is
-    the vocabulary shard that starts at ``vstart``.  The weight gradient goes to w's gradient
-    sink.  ``workspace_bytes`` bounds what the backward holds of d (the gradient of the logits), down
+    the vocabulary shard that starts at ``vstart``, and the hidden gradient is that shard's part of the
+    sum over the group.  The gradient of a parameter w goes to its gradient sink (see the top of this
+    file: ``torch.autograd.grad`` does not see it), that of a w which was itself computed flows on.
+    ``workspace_bytes`` bounds what the backward holds of d (the gradient of the logits), down
     to 256 columns of it, together with the partial sums of the hidden gradient that it splits for
     speed; one fp32 sum of the size of h stands beside them.  The forward keeps 8 bytes per row and
     256 columns until it returns.

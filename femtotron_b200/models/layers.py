@@ -21,7 +21,8 @@ Attributes that a user may set on the model config:
                   "scaling" (a Hugging Face style rope_scaling dict, or None), "partial" (the
                   share of a head that is rotated, 1.0), "interleaved" (False)
     mlp_act8      True: the MLP block keeps what its backward needs in 8 bits
-                  (``functional.NormMLP8Fn``); without tensor parallelism
+                  (``functional.NormMLP8Fn``); without tensor parallelism, and where neither
+                  the MLP nor its norm is wrapped or has hooks of its own
     loss_keep_logits  False: the loss without the logits in memory
 """
 from __future__ import annotations
@@ -162,6 +163,10 @@ def _sp_comm(x: torch.Tensor, group, sp: bool, world: int):
     from femtotron_b200.parallel.tensor_parallel.fused import tp_fused_comm
     rows = x.reshape(-1, x.shape[-1]).shape[0]
     return tp_fused_comm(group, rows, x.shape[-1], x.device)
+
+
+def _hooked(m: nn.Module) -> bool:
+    return bool(m._forward_pre_hooks or m._forward_hooks or m._backward_pre_hooks or m._backward_hooks)
 
 
 def _enter(x: torch.Tensor, group, sp: bool) -> torch.Tensor:
@@ -309,10 +314,12 @@ class LlamaDecoderLayer(nn.Module):
         self.post_attention_layernorm = LlamaRMSNorm(config.hidden_size, eps, device=device, dtype=dtype)
 
     def _mlp8_applies(self, h: torch.Tensor) -> bool:
-        """The 8-bit block needs the fused projections without tensor parallelism, and a backward."""
-        return torch.is_grad_enabled() and self.mlp._fusable() and _tp_info(self.mlp.gate_proj)[0] is None and \
-            type(self.post_attention_layernorm) is LlamaRMSNorm and \
-            (not h.is_cuda or h.dtype == self.post_attention_layernorm.weight.dtype == torch.bfloat16)
+        """The 8-bit block needs the fused projections without tensor parallelism, a backward, and
+        nothing that hangs on the calls of the two modules it replaces."""
+        mlp, norm = self.mlp, self.post_attention_layernorm
+        return torch.is_grad_enabled() and type(mlp) is LlamaMLP and type(norm) is LlamaRMSNorm and \
+            mlp._fusable() and _tp_info(mlp.gate_proj)[0] is None and not (_hooked(mlp) or _hooked(norm)) and \
+            (not h.is_cuda or h.dtype == norm.weight.dtype == torch.bfloat16)
 
     def forward(self, hidden_states: torch.Tensor, attention_mask=None, position_ids=None,
                 past_key_values=None, use_cache=False, position_embeddings=None,

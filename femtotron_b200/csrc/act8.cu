@@ -420,7 +420,8 @@ __device__ __forceinline__ uint64_t clock_ns() {
 // Long rows: a block per walker.  The rows' codes and dy come through a ring of kStages bulk
 // copies into shared memory, so the next rows are on their way during this one's reduction.
 // One barrier per row: the sums of the warps alternate between two buffers, and the stage that the
-// previous row used is refilled after this row's barrier.
+// previous row used is refilled after this row's barrier.  After a wait that ran out nothing more is
+// fetched, and the block stays (for a bounded time) until what is on its way has landed.
 constexpr int kStages = 3;
 constexpr int kErrNormWait = 302;  // a bulk copy did not arrive
 
@@ -440,6 +441,13 @@ __global__ void __launch_bounds__(NT, 512 / NT)
   const int count = static_cast<int>(min(rows - r0, (int64_t)rows_per_walker));
   const uint32_t code_bytes = static_cast<uint32_t>(pitch), dy_bytes = 2u * H;
   const uint32_t stage_bytes = code_bytes + dy_bytes;
+  auto arrived = [&](int k) {  // waits for row k, about two seconds at most
+    if (mbar_try_wait(&full[k % kStages], (k / kStages) & 1)) return true;
+    const uint64_t start = clock_ns();
+    while (!mbar_try_wait(&full[k % kStages], (k / kStages) & 1))
+      if (clock_ns() - start > 2000000000ull) return false;
+    return true;
+  };
   auto fetch = [&](int k) {  // one thread
     uint8_t* s = ring + (k % kStages) * stage_bytes;
     mbar_arrive_expect_tx(&full[k % kStages], stage_bytes);
@@ -471,7 +479,7 @@ __global__ void __launch_bounds__(NT, 512 / NT)
   }
   float r = rstd[r0];
   __syncthreads();  // barriers are initialised
-  bool late = false;
+  int late = count;  // the first row that did not arrive: the results are marked by err
   for (int k = 0; k < count; ++k) {
     const int64_t row = r0 + k;
     const uint8_t* s = ring + (k % kStages) * stage_bytes;
@@ -483,15 +491,9 @@ __global__ void __launch_bounds__(NT, 512 / NT)
       sc_next[i] = (k + 1 < count && slot * kChunk < H) ? scale[(row + 1) * groups + (slot >> lanes_log2)] : 0.f;
     }
     if (k + 1 < count) r_next = rstd[row + 1];
-    if (!late && !mbar_try_wait(&full[k % kStages], (k / kStages) & 1)) {
-      const uint64_t start = clock_ns();
-      while (!mbar_try_wait(&full[k % kStages], (k / kStages) & 1)) {
-        if (clock_ns() - start > 2000000000ull) {  // give up waiting; the results are marked by err
-          atomicCAS(err, 0, kErrNormWait);
-          late = true;
-          break;
-        }
-      }
+    if (late == count && !arrived(k)) {
+      atomicCAS(err, 0, kErrNormWait);
+      late = k;
     }
     // n and dy w of a chunk; kept in registers over the barrier where one chunk is a thread's share
     auto chunk = [&](int i, float (&n)[16], float (&g)[16]) {
@@ -521,7 +523,7 @@ __global__ void __launch_bounds__(NT, 512 / NT)
     dot = warp_sum(dot);
     if (t % 32 == 0) red[k & 1][t / 32] = dot;
     __syncthreads();
-    if (t == 0 && k + kStages - 1 < count) fetch(k + kStages - 1);
+    if (t == 0 && late == count && k + kStages - 1 < count) fetch(k + kStages - 1);
     dot = 0.f;
 #pragma unroll
     for (int i = 0; i < NT / 32; ++i) dot += red[k & 1][i];
@@ -546,6 +548,8 @@ __global__ void __launch_bounds__(NT, 512 / NT)
     }
     r = r_next;
   }
+  if (t == 0)  // the rows that had been fetched when it gave up
+    for (int k = late; k < min(count, late + kStages - 1); ++k) arrived(k);
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int c = (t + i * NT) * kChunk;

@@ -55,7 +55,10 @@ def inv_frequencies(rot: int, theta: float, scaling: dict | None = None, *, trai
     f = theta ** (-i / rot) if rot else i
     if kind == "default" or rot == 0:
         return f, 1.0
-    factor = float(sc.get("factor", 1.0))
+    for key in ("factor", "low_freq_factor", "high_freq_factor") if kind == "llama3" else ("factor",):
+        if sc.get(key) is None:
+            raise ValueError(f"rotary: {kind} scaling needs {key}, got {sc}")
+    factor = float(sc["factor"])
     if factor < 1:
         raise ValueError(f"rotary: factor must be at least 1, got {factor}")
     if kind == "linear":

@@ -726,36 +726,44 @@ int64_t linear_xent_bwd(const torch::Tensor& h, const torch::Tensor& w, const to
     ++launches;
   }
 
-  // pieces of the vocabulary: whole 256-column tiles, as even as they go
-  const int64_t most = std::max<int64_t>(256, workspace_bytes / (2 * (int64_t)T) / 256 * 256);
-  const int64_t pieces = (V + most - 1) / most;
-  const int64_t piece = ((V + pieces - 1) / pieces + 255) / 256 * 256;
-  const int64_t ldd = std::min<int64_t>(piece, (V + 31) / 32 * 32);
-  torch::Tensor d = torch::empty({T, ldd}, h.options());
-
-  // split of the dh product, by the time that a model of it takes: whole waves of tiles at 20
-  // TFLOP/s per unit (a pair of SMs, or half of it), and the last kernel's read of the partial
-  // outputs at 6.5 TB/s.  1021 tokens of 5120, 32003 words: 80 tiles for 74 pairs, so unsplit
-  // the second wave is nearly empty: 422 us by the model, 262 us in 7 shares (measured: 264 in 12).
-  // All shares but the first, which the sum over the pieces needs anyway, come out of what d leaves
-  // of the workspace.
+  // Pieces of the vocabulary, whole 256-column tiles and as even as they go, and shares of the dh
+  // product, by the time that a model of them takes: whole waves of tiles at 20 TFLOP/s per unit (a pair
+  // of SMs, or half of it), the sums of the pieces and the last kernel's read of the shares at 6.5
+  // TB/s.  All shares but the first, which the sum over the pieces needs anyway, come out of what d
+  // leaves of the workspace, so up to twice the fewest pieces are looked at.
+  // 1021 tokens of 5120, 32003 words: 80 tiles for 74 pairs, so unsplit the second wave is nearly empty:
+  // 422 us by the model, 262 us in 7 shares (measured: 264 in 12).
   const bool pair = T > 128 && H > 128;
-  const long units = pair ? num_sms() / 2 : num_sms();
-  const long tiles = (T + (pair ? 255 : 127)) / (pair ? 256 : 128) * ((H + 255) / 256);
-  const long kblocks = (std::min<int64_t>(piece, V) + BK - 1) / BK;
+  const int64_t units = pair ? num_sms() / 2 : num_sms(), tile_m = pair ? 256 : 128;
+  const auto ceil_div = [](int64_t n, int64_t by) { return (n + by - 1) / by; };
+  const auto tile_s = [&](double K) { return 2 * tile_m * 256 * K / (pair ? 20e12 : 10e12); };
+  const int64_t tm = ceil_div(T, tile_m), th = ceil_div(H, 256);
   // the pair kernel stores whole tiles of 256 rows into a share
-  const int64_t split_rows = pair ? (T + 255) / 256 * 256 : T;
-  long ksplit = 1;
-  if (dh.has_value()) {
-    const int64_t left = std::max<int64_t>(0, workspace_bytes - 2 * T * ldd);
-    const long most_shares = std::min<int64_t>({32, std::max<long>(1, kblocks / 8), 1 + left / (4 * split_rows * H)});
-    const double tile_s = (pair ? 2.0 : 1.0) * 2 * 128 * 256 * double(V) / (pair ? 20e12 : 10e12);
-    double best = 1e30;
-    for (long k = 1; k <= most_shares; ++k) {
-      const double cost = double((tiles * k + units - 1) / units) / k * tile_s + k * (4.0 * T * H) / 6.5e12;
-      if (cost < best * 0.98) { best = cost; ksplit = k; }
+  const int64_t split_rows = pair ? ceil_div(T, 256) * 256 : T;
+  const int64_t fewest = ceil_div(V, std::max<int64_t>(256, workspace_bytes / (2 * (int64_t)T) / 256 * 256));
+  int64_t piece = 0, ldd = 0, ksplit = 1;
+  double best = 1e30;
+  for (int64_t pieces = fewest; pieces <= (pair && dh.has_value() ? 2 * fewest : fewest); ++pieces) {
+    const int64_t cols = ceil_div(ceil_div(V, pieces), 256) * 256, count = ceil_div(V, cols);
+    const int64_t pitch = std::min<int64_t>(cols, (V + 31) / 32 * 32);
+    const int64_t n_tiles = ceil_div(std::min<int64_t>(cols, V), 256);
+    double cost = count * (ceil_div(tm * n_tiles, units) * tile_s(H) + 6e-6);
+    if (dw.has_value()) cost += count * ceil_div(n_tiles * th, units) * tile_s(T);
+    int64_t shares = 1;
+    if (dh.has_value()) {
+      const int64_t left = std::max<int64_t>(0, workspace_bytes - 2 * T * pitch);
+      const int64_t most = std::min<int64_t>({32, std::max<int64_t>(1, ceil_div(std::min<int64_t>(cols, V), BK) / 8),
+                                              1 + left / (4 * split_rows * H)});
+      double least = 1e30;
+      for (int64_t k = 1; k <= most; ++k) {
+        const double c = double(ceil_div(tm * th * k, units)) / k * tile_s(V) + k * (8.0 * count - 4) * T * H / 6.5e12;
+        if (c < least * 0.98) { least = c; shares = k; }
+      }
+      cost += least;
     }
+    if (cost < best * 0.98) { best = cost; piece = cols; ldd = pitch; ksplit = shares; }
   }
+  torch::Tensor d = torch::empty({T, ldd}, h.options());
   torch::Tensor acc;
   if (dh.has_value()) acc = torch::empty({ksplit * split_rows, H}, f32);
 

@@ -398,17 +398,27 @@ __global__ void __launch_bounds__(256) xent_join_kernel(const float2* __restrict
     const uint4* a = reinterpret_cast<const uint4*>(h + row * ldh);
     const uint4* b = reinterpret_cast<const uint4*>(w + local * ldw);
     float t0 = 0.f, t1 = 0.f;
-#pragma unroll 8
-    for (int i = lane; i < H / 8; i += 32) {
-      const uint4 x = a[i], y = b[i];
-      float2 f = unpack_bf16x2(x.x), g = unpack_bf16x2(y.x);
-      t0 = fmaf(f.x, g.x, t0); t1 = fmaf(f.y, g.y, t1);
-      f = unpack_bf16x2(x.y); g = unpack_bf16x2(y.y);
-      t0 = fmaf(f.x, g.x, t0); t1 = fmaf(f.y, g.y, t1);
-      f = unpack_bf16x2(x.z); g = unpack_bf16x2(y.z);
-      t0 = fmaf(f.x, g.x, t0); t1 = fmaf(f.y, g.y, t1);
-      f = unpack_bf16x2(x.w); g = unpack_bf16x2(y.w);
-      t0 = fmaf(f.x, g.x, t0); t1 = fmaf(f.y, g.y, t1);
+    constexpr int U = 4;  // reads of each row in flight: the wait for them is most of this kernel
+    for (int i0 = lane; i0 < H / 8; i0 += 32 * U) {
+      uint4 x[U], y[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = min(i0 + 32 * u, H / 8 - 1);
+        x[u] = a[i];
+        y[u] = b[i];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const uint32_t p4[4] = {x[u].x, x[u].y, x[u].z, x[u].w}, q4[4] = {y[u].x, y[u].y, y[u].z, y[u].w};
+        if (i0 + 32 * u < H / 8) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 f = unpack_bf16x2(p4[j]), g = unpack_bf16x2(q4[j]);
+            t0 = fmaf(f.x, g.x, t0);
+            t1 = fmaf(f.y, g.y, t1);
+          }
+        }
+      }
     }
     t = warp_sum(t0 + t1);
   }

@@ -28,7 +28,10 @@ test:
 test-unit:
 	timeout $(TIMEOUT) $(PYTHON) -m pytest tests/test_units.py tests/test_model_vs_hf.py \
 		tests/test_bench_config.py tests/test_clocks.py tests/test_linear_xent.py tests/test_act8.py \
-		tests/test_rotary.py -q -m "not gpu"
+		tests/test_rotary.py tests/test_linear_xent_rows.py tests/test_linear_xent_row_gradients.py \
+		tests/test_linear_xent_ignored_rows.py tests/test_linear_xent_paths.py tests/test_linear_xent_weight_graph.py \
+		tests/test_act8_strided_rows.py tests/test_swiglu8_range.py tests/test_checkpoint8.py tests/test_mlp8_modules.py \
+		tests/test_rotary_inplace.py tests/test_rope_scaling_keys.py tests/test_one_device.py -q -m "not gpu"
 
 test-race:
 	timeout $(TIMEOUT) $(PYTHON) -m pytest tests/test_protocol_model.py -q

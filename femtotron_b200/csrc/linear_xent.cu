@@ -5,15 +5,16 @@
 //
 // Forward: the tcgen05 GEMM of gemm_core.cuh whose epilogue reduces each 256-column tile of
 // fp32 logits to (max, sum of exponentials) per row; a second kernel joins the tiles of a row.
-// The logits leave TMEM only as those two numbers.
+// The logits leave TMEM only as those two numbers and the label's.
 // Backward, in pieces of the vocabulary so that the workspace stays bounded: the product again,
 // with an epilogue that turns the fp32 logits into d (bf16, [T, piece]), then dW of the
-// piece's rows and the piece's share of dh from it.  The fourth product is the price of not
-// keeping the logits.
+// piece's rows and the piece's share of dh from it.  The fourth product is the price of never
+// storing the logits, whether or not they would fit the workspace.
 //
-// Bound by the tensor cores for batches of a thousand tokens and more (81 to 87 % active in each
-// product, 0.94 of the sustained cuBLAS rate for 4096 tokens, 128256 words, hidden 4096: 12.7 to
-// 13.2 ms for the loss and both gradients), by the reads of w and the write of dw below that.
+// Bound by the tensor cores for batches of a thousand tokens and more (82 to 88 % active in each
+// product) and by the power limit: the four products of 4096 tokens, 128256 words, hidden 4096 run at
+// 0.89 to 0.95 of the sustained cuBLAS rate (12.8 to 13.7 ms for the loss and both gradients); by the
+// reads of w and the write of dw below that.
 //
 // d is rounded to bf16 because the tensor cores take it as an operand.  It is stored
 // without the upstream gradient's common factor, which is applied in fp32 to the products: the
@@ -264,8 +265,8 @@ struct XentProductEpi {
 };
 
 // ------------------------------------------------------------------ few tokens
-// The forward for one or two tokens: one read of w, and nothing for the tensor cores to win (a
-// 128-row tile would be nearly empty).  Over 32000 words of 4096: 44.9 us for one token (5.8 TB/s)
+// The forward for one or two tokens that no backward follows: one read of w, and nothing for the tensor
+// cores to win (a 128-row tile would be nearly empty).  Over 32000 words of 4096: 44.9 us for one token (5.8 TB/s)
 // and 51.5 us for two, where the GEMM takes 51 to 58 us up to 128 tokens; three took 71 us here.  A warp takes two vocabulary rows at a time, 2 x 4
 // packs of E values in flight per lane; h lies in shared memory in fp32, one plane per 4 of a
 // pack's E values, so that the lanes of a 16-byte read touch neighbouring words.  Every warp keeps a

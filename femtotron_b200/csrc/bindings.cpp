@@ -103,6 +103,18 @@ int64_t linear_xent_bwd(const torch::Tensor& h, const torch::Tensor& w, const to
                         const c10::optional<torch::Tensor>& dh, const c10::optional<torch::Tensor>& dw,
                         bool accumulate, int64_t vstart, int64_t ignore_index, int64_t workspace_bytes,
                         torch::Tensor& err);
+std::tuple<torch::Tensor, torch::Tensor> attn_mask(int64_t B, int64_t S, bool causal, int64_t window,
+                                                   const c10::optional<torch::Tensor>& docs,
+                                                   const c10::optional<torch::Tensor>& marks, torch::Device device);
+std::tuple<torch::Tensor, c10::optional<torch::Tensor>> masked_attn_fwd(
+    const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& rows,
+    const torch::Tensor& tiles, double scale, double softcap, const c10::optional<torch::Tensor>& slopes, bool graded,
+    torch::Tensor& err);
+void masked_attn_bwd(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& o,
+                     const torch::Tensor& dout, const torch::Tensor& lse, const torch::Tensor& rows,
+                     const torch::Tensor& tiles, double scale, double softcap,
+                     const c10::optional<torch::Tensor>& slopes, torch::Tensor& dq, torch::Tensor& dk, torch::Tensor& dv,
+                     torch::Tensor& err);
 }  // namespace ft
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -153,5 +165,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("act8_swiglu_bwd", &ft::act8_swiglu_bwd, "SwiGLU backward from 8-bit gate and up");
   m.def("linear_xent_fwd", &ft::linear_xent_fwd, "cross entropy of a linear head without its logits");
   m.def("linear_xent_bwd", &ft::linear_xent_bwd, "its gradients, in pieces of the vocabulary");
+  m.def("attn_mask", &ft::attn_mask, "keys that each row sees: one interval per row");
+  m.def("masked_attn_fwd", &ft::masked_attn_fwd, "attention over a mask of intervals, capped or biased scores");
+  m.def("masked_attn_bwd", &ft::masked_attn_bwd, "its gradients, without atomics");
   m.def("rotary_qk", &ft::rotary_qk, "rotary positions of q and k, half or interleaved");
 }

@@ -1,0 +1,101 @@
+// Attention over whole sequences whose rows each see one interval of keys, with capped scores or a bias
+// of distance, forward and backward, on tcgen05 (sm_100a).
+//
+//     x_ij = scale q_i k_j,   capped: x = c tanh(x / c),   with slopes: x -= slope_h |i - j|
+//     p_ij = exp(x_ij - lse_i) for lo_i <= j < hi_i, else 0;      o_i = sum_j p_ij v_j
+//     dv = p^T do,  dp = do v^T,  ds = p (dp - rowsum(do o)) (1 - tanh^2),  dq = scale ds k,  dk = scale ds^T q
+//
+// Every mask that is served here (documents packed in a row, padding, a sliding window, a prefix that is
+// seen from both sides, causal or not) leaves a row i one interval [lo_i, hi_i) that holds i itself, or
+// nothing.  A mask is two integers per row, made by one kernel, and four per tile of 128 rows (least and
+// largest lo and hi): which tiles meet, and which of those need no test of single elements, is read off them.
+//
+// Layout: q, k, v [batch, tokens, heads, d] with any strides that TMA takes, d a multiple of 8 up to 128.
+// TMA maps have d, heads, tokens and batch as dimensions of their own, so odd lengths and head sizes end
+// in zeros instead of in a neighbour.  Row statistics are padded to whole tiles.
+//
+// No sum depends on the order of atomics: dq comes from a kernel of its own (7 products instead of the
+// 5 of one that adds dq up in memory), and the query heads of a group are added up inside the tile of their
+// keys.  The results of a call are the same bits every time.
+//
+// Padding (rows that see nothing) may hold anything, NaN included: where a tile holds such rows, they are
+// zeroed in shared memory before a product sums over them.
+//
+// masked_attn_host.cpp: the entry points; masked_attn.cu: the mask and the forward pass; masked_attn_dq.cu and
+// masked_attn_dkv.cu: the backward pass; masked_attn.cuh: what the kernels share.  Only the entry points see
+// torch (its headers take nvcc minutes), the kernels are launched through the functions below.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace ft {
+namespace ma {
+
+constexpr int TILE = 128;
+constexpr int HEAD = 128;  // values of a head that a tile has room for
+constexpr int NTHREADS = 320;  // 8 compute warps, 1 TMA warp, 1 MMA warp
+constexpr int PRODUCER_WARP = 8, MMA_WARP = 9;
+constexpr int MAX_TILES = 2048;  // 262144 tokens: the tiles that meet a tile are listed in shared memory
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kNever = 0x7fffffff;  // lo of a row that sees nothing; its hi is 0
+
+// ------------------------------------------------------------------------------ arguments
+struct MaskArgs {
+  const void* docs;        // [B, S] int32 or int64, or null
+  const bool* marks;       // [B, S], or null
+  int64_t docs_stride, marks_stride;
+  int2* rows;              // [B, padded] (lo, hi)
+  int4* tiles;             // [B, ntiles] (least lo, largest lo, least hi, largest hi)
+  int S, padded, window;   // window: 0x40000000 for none
+  bool causal, docs64;
+};
+
+struct Common {
+  int B, S, padded, ntiles, nq, nkv, group, ksteps, d;
+  const int2* rows;       // mask, and 0 or padded (ntiles) per batch
+  const int4* tiles;
+  int64_t rows_stride, tiles_stride;
+  const float* slopes;
+  float scale, scale_log2;
+  float cap_in, cap_out;  // exp2(s cap_in) = exp(2 scale s / c); c log2(e)
+  float* lse2;            // [B, nq, padded], log2 units, +inf where a row sees nothing
+  int* err;
+};
+
+struct Out {  // a [batch, tokens, heads, d] tensor of bf16, strides in elements
+  void* p;
+  int64_t batch, token, head;
+};
+
+struct FwdParams : Common {
+  Out o;
+  bool pair_heads;
+};
+
+struct BwdParams : Common {
+  const float* delta;
+  Out dq, dk, dv;
+};
+
+struct DeltaArgs {  // rowsum(do o) of every row and head
+  Out o, dout;
+  float* delta;            // [B, nq, padded]
+  const int2* rows;
+  int64_t rows_stride;
+  int B, S, padded, nq, d;
+};
+
+// Each returns what cudaGetLastError() says.
+cudaError_t launch_mask(const MaskArgs& a, int batch, cudaStream_t st);
+cudaError_t launch_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const FwdParams& p, bool cap,
+                       bool bias, cudaStream_t st);
+cudaError_t launch_delta(const DeltaArgs& a, cudaStream_t st);
+cudaError_t launch_dq(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& td,
+                      const BwdParams& p, bool cap, bool bias, cudaStream_t st);
+cudaError_t launch_dkv(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& td,
+                       const BwdParams& p, bool cap, bool bias, cudaStream_t st);
+
+}  // namespace ma
+}  // namespace ft

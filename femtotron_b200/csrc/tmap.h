@@ -62,4 +62,35 @@ inline CUtensorMap make_tmap_2d(const void* base, CUtensorMapDataType dtype, int
   return m;
 }
 
+// Tensor [batch, tokens, heads, d] with a unit inner stride (the other strides in elements): a box is
+// 64 values of `box_tokens` tokens of one head, in the 128-byte swizzle.  Values past d and tokens past
+// the last one read as zero, so no size has to be a multiple of the box.
+inline CUtensorMap make_tmap_heads(const void* base, uint64_t d, uint64_t heads, uint64_t tokens, uint64_t batch,
+                                   uint64_t stride_head, uint64_t stride_token, uint64_t stride_batch,
+                                   uint32_t box_tokens) {
+  CUtensorMap m;
+  cuuint64_t dims[4] = {d, heads, tokens, batch};
+  cuuint64_t strides[3] = {stride_head * 2, stride_token * 2, stride_batch * 2};
+  cuuint32_t box[4] = {64, 1, box_tokens, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  if (reinterpret_cast<uintptr_t>(base) % 16 != 0)
+    throw std::runtime_error("femtotron_b200: TMA base address must be 16-byte aligned");
+  for (cuuint64_t st : strides)
+    if (st % 16 != 0) throw std::runtime_error("femtotron_b200: TMA strides must be multiples of 16 bytes");
+  auto encode = [&] {
+    return encode_tiled_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
+                             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {  // as in make_tmap_2d
+    int dev = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = encode();
+  }
+  if (r != CUDA_SUCCESS)
+    throw std::runtime_error("femtotron_b200: cuTensorMapEncodeTiled failed with code " +
+                             std::to_string(static_cast<int>(r)));
+  return m;
+}
+
 }  // namespace ft

@@ -115,6 +115,12 @@ void masked_attn_bwd(const torch::Tensor& q, const torch::Tensor& k, const torch
                      const torch::Tensor& tiles, double scale, double softcap,
                      const c10::optional<torch::Tensor>& slopes, torch::Tensor& dq, torch::Tensor& dk, torch::Tensor& dv,
                      torch::Tensor& err);
+torch::Tensor grad_sumsq(const std::vector<torch::Tensor>& xs, const std::vector<int64_t>& slots, int64_t n_slots);
+void grad_scale(const std::vector<torch::Tensor>& xs, const torch::Tensor& coef, const std::vector<torch::Tensor>& outs);
+torch::Tensor grad_clip(const std::vector<torch::Tensor>& xs, double max_norm, const std::vector<torch::Tensor>& outs);
+torch::Tensor embed_lookup(const torch::Tensor& ids, const torch::Tensor& table, int64_t vstart, double scale);
+int64_t embed_sorted_grad(const torch::Tensor& ids, const torch::Tensor& dout, torch::Tensor& dst, bool accumulate,
+                          int64_t vstart, double scale);
 }  // namespace ft
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -168,5 +174,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("attn_mask", &ft::attn_mask, "keys that each row sees: one interval per row");
   m.def("masked_attn_fwd", &ft::masked_attn_fwd, "attention over a mask of intervals, capped or biased scores");
   m.def("masked_attn_bwd", &ft::masked_attn_bwd, "its gradients, without atomics");
+  m.def("grad_sumsq", &ft::grad_sumsq, "sums of squares of many tensors, in a fixed order");
+  m.def("grad_scale", &ft::grad_scale, "many tensors times one factor on the device");
+  m.def("grad_clip", &ft::grad_clip, "global norm of many tensors, and the tensors clipped by it");
+  m.def("embed_lookup", &ft::embed_lookup, "embedding rows times a factor");
+  m.def("embed_sorted_grad", &ft::embed_sorted_grad, "embedding gradient by sorted tokens, without atomics");
   m.def("rotary_qk", &ft::rotary_qk, "rotary positions of q and k, half or interleaved");
 }

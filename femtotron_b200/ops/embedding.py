@@ -1,0 +1,50 @@
+"""Embedding lookup with a factor, and its gradient by sorted tokens.
+
+    out_t = scale w[id_t - vstart]  (0 where the id is in another shard),
+    dw[v] = scale sum over id_t = vstart + v of dout_t
+
+The gradient's sums run over the tokens in the order of the batch, in fp32, cut where the sorted list
+of tokens is cut into pieces of 32: no atomics, the same bits every time, and a frequent word takes no
+longer than rare ones.  CUDA tensors run ``csrc/embedding.cu`` (fp32, bf16 or fp16; ids int32 or int64),
+CPU tensors PyTorch.  The autograd entry point is ``functional.embedding``.
+
+The reference looks rows up with ``F.embedding`` and masks the ids of other shards
+(femtotron/parallel/tensor_parallel/embedding.py:57-77).
+"""
+from __future__ import annotations
+
+import torch
+
+from .ext import LAUNCHES, native
+
+
+def _local(ids: torch.Tensor, words: int, vstart: int):
+    local = ids.reshape(-1).long() - vstart
+    has = (local >= 0) & (local < words)
+    return local, has
+
+
+def lookup(ids: torch.Tensor, table: torch.Tensor, vstart: int = 0, scale: float = 1.0) -> torch.Tensor:
+    """Rows of ``table`` [words, values] times ``scale``, in its type."""
+    if table.is_cuda:
+        return native().embed_lookup(ids, table, int(vstart), float(scale))
+    local, has = _local(ids, table.shape[0], vstart)
+    out = torch.zeros(local.numel(), table.shape[1], dtype=table.dtype)
+    rows = table[local[has]]
+    out[has] = rows if scale == 1.0 else (rows.float() * scale).to(table.dtype)
+    return out.view(*ids.shape, table.shape[1])
+
+
+def sorted_grad(ids: torch.Tensor, dout: torch.Tensor, dst: torch.Tensor, accumulate: bool, vstart: int = 0,
+                scale: float = 1.0) -> None:
+    """Store the table's gradient in ``dst`` [words, values], or add it (fp32, bf16 or fp16, rounded once)."""
+    dout = dout.reshape(ids.numel(), dst.shape[1])
+    if dst.is_cuda:
+        n = native().embed_sorted_grad(ids, dout, dst, accumulate, int(vstart), float(scale))
+        LAUNCHES[0] += n - 1
+        return
+    local, has = _local(ids, dst.shape[0], vstart)
+    g = torch.zeros(dst.shape, dtype=torch.float32)
+    g.index_add_(0, local[has], dout[has].float())
+    g = g if scale == 1.0 else g * scale
+    dst.copy_(dst.float() + g if accumulate else g)

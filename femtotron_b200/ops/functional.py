@@ -28,6 +28,7 @@ import torch.distributed as dist
 from torch.autograd import Function
 
 from . import act8 as A8
+from . import embedding as E
 from . import kernels as K
 from . import linear_xent as X
 from . import rotary as R
@@ -345,35 +346,47 @@ def rms_norm(x, w, eps, sp_group=None):
 # ------------------------------------------------------------------------------ embedding
 class EmbeddingFn(Function):
     """Vocab-parallel lookup: rows outside [vstart, vstart+V_local) give zeros (the TP
-    reduction that completes them is applied by the caller)."""
+    reduction that completes them is applied by the caller).  The gradient is summed by sorted
+    tokens, in a fixed order (``ops/embedding.py``), straight into the weight's sink; that of a
+    weight which was itself computed flows on."""
 
     @staticmethod
-    def forward(ctx, ids, weight, vstart):
-        out = K.embed_fwd(ids, weight, vstart)
+    def forward(ctx, ids, weight, vstart, scale=1.0):
+        out = E.lookup(ids, weight, vstart, scale)
         ctx.save_for_backward(ids)
-        ctx.param = weight
-        ctx.vstart = vstart
+        ctx.param = weight if weight.is_leaf or getattr(weight, "main_grad", None) is not None else None
+        ctx.meta = (vstart, scale, weight.shape, weight.dtype)
         return out
 
     @staticmethod
     def backward(ctx, dout):
         (ids,) = ctx.saved_tensors
-        weight = ctx.param
-        ctx.param = None
-        if ctx.needs_input_grad[1]:
-            mg = getattr(weight, "main_grad", None)
-            if mg is not None and mg.dtype == torch.float32 and ids.is_cuda:
-                if getattr(weight, "grad_overwrite", False):
-                    mg.zero_()
-                    weight.grad_overwrite = False
-                from .ext import native
-                native().embed_bwd(ids.reshape(-1).contiguous(),
-                                   dout.reshape(-1, dout.shape[-1]).contiguous(),
-                                   mg.view(weight.shape), int(ctx.vstart))
-                grad_ready(weight)
-            else:
-                write_vector_grad(weight, K.embed_bwd(ids, dout, weight.shape[0], ctx.vstart))
-        return None, None, None
+        vstart, scale, shape, dtype = ctx.meta
+        weight, ctx.param = ctx.param, None
+        if not ctx.needs_input_grad[1]:
+            return None, None, None, None
+        if weight is None:
+            dw = torch.empty(shape, dtype=dtype, device=dout.device)
+            E.sorted_grad(ids, dout, dw, False, vstart, scale)
+            return None, dw, None, None
+        write_weight_grad([weight], lambda dst, acc: E.sorted_grad(ids, dout, dst, acc, vstart, scale))
+        return None, None, None, None
+
+
+def embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0, vstart: int = 0) -> torch.Tensor:
+    """``scale * weight[ids - vstart]`` [..., values], rounded once to the weight's type; zeros where an id
+    is outside this shard of the vocabulary (so an id below 0 stands for no word).  The gradient of a
+    parameter goes to its gradient sink (see the top of this file: ``torch.autograd.grad`` does not see it),
+    that of a weight which was itself computed flows on.  Ids are int32 or int64; on CUDA the weight is a
+    contiguous fp32, bf16 or fp16 tensor."""
+    if weight.dim() != 2 or not weight.is_contiguous() or not weight.is_floating_point():
+        raise ValueError(f"embedding: the weight must be a contiguous floating [words, values] tensor, got {weight.dtype} "
+                         f"{tuple(weight.shape)} with strides {weight.stride()}")
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"embedding: ids must be int32 or int64, got {ids.dtype}")
+    if ids.device != weight.device:
+        raise ValueError(f"embedding: ids are on {ids.device}, the weight is on {weight.device}")
+    return EmbeddingFn.apply(ids, weight, int(vstart), float(scale))
 
 
 # ------------------------------------------------------------------------------ LM head + CE

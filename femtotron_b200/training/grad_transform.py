@@ -7,8 +7,9 @@ gradients (ZeRO-1/2 master shards, ZeRO-3 cluster shards), over PP always (each 
 different layers; the reference omits PP).  Gradients replicated across a group are counted
 once: the reference all-reduces the whole total over DP whenever the strategy shards, which
 counts ZeRO-3's unsharded free parameters (embedding, LM head, final norm) dp times.  The sums of squares come
-from one multi-tensor kernel launch, and the clip coefficient stays on the device (no host
-synchronisation); it is exported as ``last_norm`` / ``coef``.
+in fp64 and in a fixed order from ``ops/grad_norm.py``, whose second kernel scales the gradients (or
+leaves them alone where the norm needs no clipping); norm and clip coefficient stay on the device
+(no host synchronisation) and are exported as ``last_norm`` / ``coef``.
 """
 from __future__ import annotations
 
@@ -17,7 +18,7 @@ from typing import Protocol
 import torch
 import torch.distributed as dist
 
-from femtotron_b200.ops.kernels import sumsq_multi
+from femtotron_b200.ops.grad_norm import scale_grads, sum_of_squares
 
 
 class GradTransform(Protocol):
@@ -45,10 +46,9 @@ class ClipGradNorm:
         dev = grads[0].device if grads else torch.device("cpu")
         # slots: 0 tp-sharded & dp-sharded, 1 tp-replicated & dp-sharded,
         #        2 tp-sharded & dp-replicated, 3 tp-replicated & dp-replicated
-        sq = torch.zeros(4, dtype=torch.float32, device=dev)
         slots = [(0 if g_.is_tp_sharded else 1) + (0 if self.dp_sharded and self._dp_sharded(g_) else 2)
                  for g_ in param_groups]
-        sumsq_multi(list(grads), slots, sq)
+        sq = sum_of_squares(grads, slots, 4) if grads else torch.zeros(4, dtype=torch.float64, device=dev)
         ctx = self.parallel_ctx
         if ctx.tp_size > 1 and ctx.tp_group is not None:   # TP shards: sum over the TP group
             t = sq[0::2].clone()
@@ -63,9 +63,9 @@ class ClipGradNorm:
         total = sq.sum().reshape(1)
         if self.reduce_pp and ctx.pp_size > 1 and ctx.pp_group is not None:
             dist.all_reduce(total, group=ctx.pp_group)
-        norm = total.sqrt()[0]
+        norm = total.sqrt()[0].float()
         coef = (self.max_norm / (norm + 1e-6)).clamp(max=1.0)
         if grads:
-            torch._foreach_mul_(list(grads), coef)
+            scale_grads(grads, coef)
         self.last_norm, self.coef = norm, coef
         return norm

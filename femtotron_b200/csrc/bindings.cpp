@@ -106,12 +106,12 @@ int64_t linear_xent_bwd(const torch::Tensor& h, const torch::Tensor& w, const to
 std::tuple<torch::Tensor, torch::Tensor> attn_mask(int64_t B, int64_t S, bool causal, int64_t window,
                                                    const c10::optional<torch::Tensor>& docs,
                                                    const c10::optional<torch::Tensor>& marks, torch::Device device);
-std::tuple<torch::Tensor, c10::optional<torch::Tensor>> masked_attn_fwd(
+std::tuple<torch::Tensor, c10::optional<torch::Tensor>, c10::optional<torch::Tensor>> masked_attn_fwd(
     const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& rows,
     const torch::Tensor& tiles, double scale, double softcap, const c10::optional<torch::Tensor>& slopes, bool graded,
     torch::Tensor& err);
-void masked_attn_bwd(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& o,
-                     const torch::Tensor& dout, const torch::Tensor& lse, const torch::Tensor& rows,
+int64_t masked_attn_bwd(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& o,
+                     const torch::Tensor& low, const torch::Tensor& dout, const torch::Tensor& lse, const torch::Tensor& rows,
                      const torch::Tensor& tiles, double scale, double softcap,
                      const c10::optional<torch::Tensor>& slopes, torch::Tensor& dq, torch::Tensor& dk, torch::Tensor& dv,
                      torch::Tensor& err);

@@ -1,4 +1,4 @@
-// Attention over a mask of intervals: the mask, the forward pass and the row sums of the backward (masked_attn.h).
+// Attention over a mask of intervals: the mask and the forward pass (masked_attn.h).
 #include "masked_attn.cuh"
 
 namespace ft {
@@ -114,8 +114,8 @@ __global__ void __launch_bounds__(1024) mask_kernel(const MaskArgs a) {
 // ------------------------------------------------------------------------------ forward
 // Two query tiles per block share the key and value tiles of a ring: two heads of a group at the same
 // 128 rows where the group has an even number of heads, else 256 rows of one head.  Warps 0-3 and 4-7 each
-// run the softmax of one tile, a row per thread; warp 9 issues the products of one tile while the other's
-// softmax runs.  TMEM: S0, S1, O0, O1; the probabilities go over the first half of S as bf16 pairs.
+// run the softmax of one tile, a row per thread that is read once and kept in registers; warp 9 issues the
+// products of one tile while the other's softmax runs.  TMEM: S0, S1, O0, O1; the probabilities go over the first half of S as bf16 pairs.
 constexpr int KV_STAGES = 4;
 // Growth of a row's running maximum (log2 units) below which the sums stay relative to the old one: the
 // probabilities stay under 2^8, which bf16 and the fp32 sums hold as well as values under 1.
@@ -130,65 +130,42 @@ struct FwdSmem {
   uint32_t tmem_base;
 };
 
-// The largest score of this thread's row among 128 keys.  Without a bias the score grows with the product,
-// so the transform is taken once, of the largest product.  TEST: element e is seen when off + e is in
-// [0, width).
-template <bool CAP, bool ALIBI, bool TEST>
-__device__ __forceinline__ float row_max(uint32_t ts, const Common& p, float slope2, float far, int off, int width) {
-  float mx = -INFINITY;
+// Probabilities of 32 keys relative to 2^m from their scores (times `mul`, log2 units), as bf16 pairs; their fp32
+// sums in `sums` (of the unrounded values: only p v sees the rounding).  A score of -inf gives 0.
+template <bool TEST>
+__device__ __forceinline__ void probs32(const uint32_t* sv, float mul, float m, uint64_t& sums, uint32_t (&pk)[16]) {
+  const uint64_t mul2_ = pair(mul, mul), m2 = pair(-m, -m);
 #pragma unroll
-  for (int h2 = 0; h2 < 2; ++h2) {
-    uint32_t sv[64];
-    tmem_ld_32x32b_x32(ts + h2 * 64, *reinterpret_cast<uint32_t(*)[32]>(sv));
-    tmem_ld_32x32b_x32(ts + h2 * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(sv + 32));
-    tmem_wait_ld();
-    float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-    for (int e = 0; e < 64; ++e) {
-      float keep, y = __uint_as_float(sv[e]);
-      if (ALIBI) y = score<CAP, true>(y, p, slope2, far - (h2 * 64 + e), keep);
-      if (TEST && static_cast<uint32_t>(off + h2 * 64 + e) >= static_cast<uint32_t>(width)) y = -INFINITY;
-      m4[e & 3] = fmaxf(m4[e & 3], y);
-    }
-    mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+  for (int e = 0; e < 16; ++e) {
+    const uint64_t x = fma2(pair(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), mul2_, m2);
+    const float2 y0 = apart(x);
+    float2 y = exp2_of(y0, e);
+    if (TEST && on_fma_pipe(e)) y = make_float2(y0.x == -INFINITY ? 0.f : y.x, y0.y == -INFINITY ? 0.f : y.y);
+    sums = add2(sums, pair(y.x, y.y));
+    pk[e] = pack_bf16x2(y.x, y.y);
   }
-  if (!ALIBI && mx > -INFINITY) {
-    float keep;
-    mx = score<CAP, false>(mx, p, 0.f, 0.f, keep);
-  }
-  return mx;
 }
 
-// Probabilities of 64 keys (half h2) relative to 2^m, as bf16 pairs over the scores; their fp32 sums
-// in sum4 (of the unrounded values: the sum is the exact softmax's, only p v sees the rounding).
+// The scores of 128 keys from their raw products: transformed (capped, biased), and -inf where they are not
+// seen.  TEST: element e is seen when off + e is in [0, width).  Returns the largest.
 template <bool CAP, bool ALIBI, bool TEST>
-__device__ __forceinline__ void row_probs(uint32_t ts, int h2, const Common& p, float slope2, float far, int off,
-                                          int width, float m, float (&sum4)[4]) {
-  uint32_t sv[64];
-  tmem_ld_32x32b_x32(ts + h2 * 64, *reinterpret_cast<uint32_t(*)[32]>(sv));
-  tmem_ld_32x32b_x32(ts + h2 * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(sv + 32));
-  tmem_wait_ld();
+__device__ __forceinline__ float scores128(uint32_t (&sv)[128], const Common& p, float slope2, float far, int off,
+                                           int width) {
+  float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    uint32_t pk[16];
-#pragma unroll
-    for (int e = 0; e < 32; e += 2) {
-      float pr[2];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int col = h2 * 64 + q * 32 + e + u;
-        const float raw = __uint_as_float(sv[q * 32 + e + u]);
-        float keep, y;
-        if (!CAP && !ALIBI) y = fmaf(raw, p.scale_log2, -m);
-        else y = score<CAP, ALIBI>(raw, p, slope2, far - col, keep) - m;
-        pr[u] = ex2_approx(y);
-        if (TEST && static_cast<uint32_t>(off + col) >= static_cast<uint32_t>(width)) pr[u] = 0.f;
-      }
-      sum4[(e >> 1) & 3] += pr[0] + pr[1];
-      pk[e >> 1] = pack_bf16x2(pr[0], pr[1]);
+  for (int e = 0; e < 128; ++e) {
+    if (CAP || ALIBI) {
+      float keep;
+      sv[e] = __float_as_uint(score<CAP, ALIBI>(__uint_as_float(sv[e]), p, slope2, far - e, keep));
     }
-    tmem_st_32x32b_x16(ts + h2 * 32 + q * 16, pk);
+    if (TEST && static_cast<uint32_t>(off + e) >= static_cast<uint32_t>(width)) sv[e] = __float_as_uint(-INFINITY);
   }
+#pragma unroll
+  for (int e = 0; e < 128; e += 2)
+    asm("max.f32 %0, %0, %1, %2;"
+        : "+f"(m4[(e >> 1) & 3])
+        : "f"(__uint_as_float(sv[e])), "f"(__uint_as_float(sv[e + 1])));
+  return fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
 }
 
 template <bool CAP, bool ALIBI>
@@ -247,121 +224,21 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = s.tmem_base;
-  auto tS = [tmem](int t) -> uint32_t { return tmem + static_cast<uint32_t>(t) * 128u; };
-  auto tO = [tmem](int t) -> uint32_t { return tmem + 256u + static_cast<uint32_t>(t) * 128u; };
+  constexpr uint32_t tmem = 0;  // where an allocation of all 512 columns begins
+  auto tS = [](int t) -> uint32_t { return tmem + static_cast<uint32_t>(t) * 128u; };
+  auto tO = [](int t) -> uint32_t { return tmem + 256u + static_cast<uint32_t>(t) * 128u; };
 
-  if (warp == PRODUCER_WARP) {
-    // ------------------------------------------------------------ TMA producer
-    if (j0 < j1) {
-      if (lane == 0) {
-        const bool two = qt[1] < p.ntiles;
-        mbar_arrive_expect_tx(&s.q_full, two ? 2 * tile_bytes : tile_bytes);
-        for (int t = 0; t < (two ? 2 : 1); ++t)
-          for (int c = 0; c < chunks; ++c)
-            tma_load_4d(s.q[t] + c * 128 * 64, &tm_q, &s.q_full, c * 64, head[t], qt[t] * TILE, b);
-      }
-      int item = 0;
-      bool ok = true;
-      for (int j = j0; j < j1 && ok; ++j) {
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv, ++item) {
-          const int st = item % KV_STAGES;
-          ok = ok && wait_warp(&s.kv_empty[st], ((item / KV_STAGES) & 1) ^ 1, p.err, 311);
-          if (!ok) break;
-          if (lane == 0) {
-            mbar_arrive_expect_tx(&s.kv_full[st], tile_bytes);
-            for (int c = 0; c < chunks; ++c)
-              tma_load_4d(s.kv[st] + c * 128 * 64, kv ? &tm_v : &tm_k, &s.kv_full[st], c * 64, kvh, j * TILE, b);
-          }
-          __syncwarp();
-          if (kv && is_dead(s.dead, j)) {
-            ok = wait_warp(&s.kv_full[st], (item / KV_STAGES) & 1, p.err, 312);
-            zero_dead_rows(s.kv[st], chunks, rows + j * TILE, lane);
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&s.clean);
-          }
-        }
-      }
-      // the copies have landed before the block may leave, also after a wait that ran out
-      wait_phase(&s.q_full, 0, p.err, 313);
-      for (int i = max(0, item - KV_STAGES); i < item; ++i)
-        wait_phase(&s.kv_full[i % KV_STAGES], (i / KV_STAGES) & 1, p.err, 313);
-    }
-  } else if (warp == MMA_WARP) {
-    // ------------------------------------------------------------ MMA issuer
-    if (j0 < j1 && elect_one()) {
-      const uint32_t idS = make_idesc_bf16(128, TILE, false, false);           // Q (K-major) x K (K-major)
-      const uint32_t idO = make_idesc_bf16(128, p.ksteps * 16, false, true);   // P (TMEM) x V (MN-major)
-      int cleaned = j0 - 1, n_clean = 0;
-      auto kv_wait = [&](int item) -> bool {
-        return wait_phase(&s.kv_full[item % KV_STAGES], (item / KV_STAGES) & 1, p.err, 314);
-      };
-      // S_t may go over P_t of the block before: that product was issued earlier by this thread
-      auto issue_s = [&](int t, int j) {
-        tc_fence_after();
-        const uint32_t qa = smem_u32(s.q[t]), ka = smem_u32(s.kv[(2 * (j - j0)) % KV_STAGES]);
-        for (int kk = 0; kk < p.ksteps; ++kk) {
-          const uint32_t off = (kk >> 2) * 128 * 128 + (kk & 3) * 32;
-          mma_bf16(tS(t), make_sw128_desc(qa + off, 16, 1024), make_sw128_desc(ka + off, 16, 1024), idS,
-                   kk > 0 ? 1u : 0u);
-        }
-        mma_commit(&s.s_full[t]);
-      };
-      auto issue_pv = [&](int t, int j) -> bool {
-        const int item = 2 * (j - j0) + 1;
-        if (!kv_wait(item)) return false;
-        if (is_dead(s.dead, j) && cleaned < j) {
-          if (!wait_phase(&s.clean, n_clean++ & 1, p.err, 315)) return false;
-          cleaned = j;
-        }
-        const uint32_t va = smem_u32(s.kv[item % KV_STAGES]);
-        const int c = j - first[t];
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          if (!wait_phase(half ? &s.p_full[t] : &s.p_half[t], c & 1, p.err, 316)) return false;
-          tc_fence_after();
-#pragma unroll
-          for (int kk = half * 4; kk < half * 4 + 4; ++kk)
-            mma_bf16_ts(tO(t), tS(t) + kk * 8, make_sw128_desc(va + kk * 2048, 128 * 128, 1024), idO,
-                        (c > 0 || kk > 0) ? 1u : 0u);
-        }
-        mma_commit(&s.o_done[t]);
-        return true;
-      };
-      bool ok = wait_phase(&s.q_full, 0, p.err, 317) && kv_wait(0);
-      if (ok) {
-        for (int t = 0; t < 2; ++t)
-          if (first[t] == j0 && j0 < end[t]) issue_s(t, j0);
-        mma_commit(&s.kv_empty[0]);
-      }
-      for (int j = j0; ok && j < j1; ++j) {
-        const int iv = 2 * (j - j0) + 1, ik = iv + 1;
-        for (int t = 0; ok && t < 2; ++t) {
-          if (first[t] <= j && j < end[t]) ok = issue_pv(t, j);
-          if (ok && first[t] <= j + 1 && j + 1 < end[t]) {
-            ok = kv_wait(ik);
-            if (ok) issue_s(t, j + 1);
-          }
-        }
-        if (!ok) break;
-        mma_commit(&s.kv_empty[iv % KV_STAGES]);
-        if (j + 1 < j1) mma_commit(&s.kv_empty[ik % KV_STAGES]);
-      }
-      if (!ok) {
-        mma_commit(&s.drained);
-        wait_phase(&s.drained, 0, p.err, 318);
-      }
-    }
-  } else {
+  if (warp < COMPUTE_WARPS) {
+    more_registers<FwdRegisters::compute>();
     // ------------------------------------------------------------ softmax warps 0..7
     const int t = warp >> 2, quad = warp & 3;
     const int r = quad * 32 + lane;
-    const bool real = qt[t] < p.ntiles;
-    const int row = qt[t] * TILE + r;
+    // (chosen, not indexed: an array that is indexed at run time lies in local memory)
+    const int tile = t ? qt[1] : qt[0], h = t ? head[1] : head[0], begin = t ? first[1] : first[0];
+    const bool real = tile < p.ntiles;
+    const int row = tile * TILE + r;
     const uint32_t lane_off = static_cast<uint32_t>(quad * 32) << 16;
-    const int n = end[t] - first[t];
+    const int n = (t ? end[1] : end[0]) - begin;
     float m_used = -INFINITY, l_run = 0.f;
     bool ok = true;
     int lo = 0, width = 0;
@@ -370,47 +247,52 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     if (n > 0) {
       const int2 lh = rows[row];
       if (lh.y > lh.x) lo = lh.x, width = lh.y - lh.x;
-      sum = tiles[qt[t]];
-      if (ALIBI) slope2 = p.slopes[head[t]] * kLog2e;
+      sum = tiles[tile];
+      if (ALIBI) slope2 = p.slopes[h] * kLog2e;
     }
     for (int c = 0; c < n && ok; ++c) {
-      const int k0 = (first[t] + c) * TILE;
+      const int k0 = (begin + c) * TILE;
       ok = wait_warp(&s.s_full[t], c & 1, p.err, 319);
       if (!ok) break;
       tc_fence_after();
       const bool test = k0 < sum.y || k0 + TILE > sum.z;
       const int off = k0 - lo;                 // element e is seen when off + e is in [0, width)
       const float far = static_cast<float>(row - k0);
-      float mx = test ? row_max<CAP, ALIBI, true>(tS(t) + lane_off, p, slope2, far, off, width)
-                      : row_max<CAP, ALIBI, false>(tS(t) + lane_off, p, slope2, far, off, width);
-      const bool need = (m_used == -INFINITY) || (mx - m_used > kRescale);
-      const float m_new = need ? fmaxf(m_used, mx) : m_used;
-      const float alpha = (m_used == -INFINITY) ? 0.f : exp2f(m_used - m_new);
-      if (c > 0) {
-        ok = wait_warp(&s.o_done[t], (c - 1) & 1, p.err, 320);
-        if (!ok) break;
-        tc_fence_after();
-        if (__any_sync(0xffffffffu, need)) {
-          for (int cc = 0; cc < p.ksteps; ++cc) {
-            uint32_t ov[16];
-            const uint32_t ta = tO(t) + lane_off + cc * 16;
-            tmem_ld_32x32b_x16(ta, ov);
-            tmem_wait_ld();
+      uint32_t sv[128];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha);
-            tmem_st_32x32b_x16(ta, ov);
-          }
-          tmem_wait_st();
+      for (int q = 0; q < 4; ++q)
+        tmem_ld_32x32b_x32(tS(t) + lane_off + q * 32, *reinterpret_cast<uint32_t(*)[32]>(sv + q * 32));
+      tmem_wait_ld();
+      constexpr bool RAW = !CAP && !ALIBI;  // scores without the scale, which then goes into the exponent's FMA
+      const float mul = RAW ? p.scale_log2 : 1.f;
+      const float mx = mul * (test ? scores128<CAP, ALIBI, true>(sv, p, slope2, far, off, width)
+                                   : scores128<CAP, ALIBI, false>(sv, p, slope2, far, off, width));
+      const bool need = mx - m_used > kRescale || m_used == -INFINITY;
+      const float m_new = need ? fmaxf(m_used, mx) : m_used;
+      // S of this block was committed behind the last product into O, which is complete by now
+      if (c > 0 && __any_sync(0xffffffffu, need)) {
+        const float alpha = m_used == -INFINITY ? 0.f : ex2_approx(m_used - m_new);
+        l_run *= alpha;
+        for (int cc = 0; cc < p.ksteps; ++cc) {
+          uint32_t ov[16];
+          const uint32_t ta = tO(t) + lane_off + cc * 16;
+          tmem_ld_32x32b_x16(ta, ov);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha);
+          tmem_st_32x32b_x16(ta, ov);
         }
       }
-      l_run *= alpha;
       m_used = m_new;
-      float sum4[4] = {0.f, 0.f, 0.f, 0.f};
+      const float m = m_used == -INFINITY ? 0.f : m_used;  // a row that has seen nothing yet
+      uint64_t sums = 0;
 #pragma unroll
-      for (int h2 = 0; h2 < 2; ++h2) {
-        if (test) row_probs<CAP, ALIBI, true>(tS(t) + lane_off, h2, p, slope2, far, off, width, m_used, sum4);
-        else row_probs<CAP, ALIBI, false>(tS(t) + lane_off, h2, p, slope2, far, off, width, m_used, sum4);
-        if (h2 == 0) {  // keys 0..63 are stored: their half of the product may start
+      for (int q = 0; q < 4; ++q) {
+        uint32_t pk[16];
+        if (test) probs32<true>(sv + q * 32, mul, m, sums, pk);
+        else probs32<false>(sv + q * 32, mul, m, sums, pk);
+        tmem_st_32x32b_x16(tS(t) + lane_off + q * 16, pk);
+        if (q == 1) {  // keys 0..63 are stored: their half of the product may start
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
@@ -418,16 +300,17 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         }
       }
       tmem_wait_st();
-      l_run += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
+      const float2 two = apart(sums);
+      l_run += two.x + two.y;
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.p_full[t]);
     }
-    if (n > 0 && ok) ok = wait_warp(&s.o_done[t], (n - 1) & 1, p.err, 321);
+    if (n > 0 && ok) ok = wait_warp(&s.o_done[t], 0, p.err, 321);
     if (real && ok) {
       tc_fence_after();
       const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
-      __nv_bfloat16* out = at(p.o, b, row, head[t]);
+      __nv_bfloat16* out = at(p.o, b, row, h);
       for (int c = 0; c < p.ksteps; ++c) {
         uint32_t ov[16];
         if (n > 0) {
@@ -438,11 +321,131 @@ __global__ void __launch_bounds__(NTHREADS, 1)
           // a sum of NaN stays one (l is NaN then, not 0)
           if (n == 0 || l_run == 0.f) zero16(out + c * 16, p.d - c * 16);
           else store16(out + c * 16, ov, l_run == l_run ? inv : l_run, p.d - c * 16);
+          if (p.low) {
+            __nv_bfloat16* low = static_cast<__nv_bfloat16*>(p.low) + (out - static_cast<__nv_bfloat16*>(p.o.p)) + c * 16;
+            if (n == 0 || l_run == 0.f) {
+              zero16(low, p.d - c * 16);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const float v = __uint_as_float(ov[i]) * inv;
+                ov[i] = __float_as_uint(v - __bfloat162float(__float2bfloat16_rn(v)));
+              }
+              store16(low, ov, 1.f, p.d - c * 16);
+            }
+          }
         }
       }
-      if (p.lse2)
-        p.lse2[(static_cast<int64_t>(b) * p.nq + head[t]) * p.padded + row] =
-            l_run == 0.f ? INFINITY : m_used + log2f(l_run);
+      if (p.neg_lse2)
+        p.neg_lse2[(static_cast<int64_t>(b) * p.nq + h) * p.padded + row] =
+            l_run == 0.f ? -INFINITY : -(m_used + log2f(l_run));
+    }
+  } else {
+    fewer_registers<FwdRegisters::other>();
+    if (warp == PRODUCER_WARP) {
+      // ------------------------------------------------------------ TMA producer
+      if (j0 < j1) {
+        if (lane == 0) {
+          const bool two = qt[1] < p.ntiles;
+          mbar_arrive_expect_tx(&s.q_full, two ? 2 * tile_bytes : tile_bytes);
+          for (int t = 0; t < (two ? 2 : 1); ++t)
+            for (int c = 0; c < chunks; ++c)
+              tma_load_4d(s.q[t] + c * 128 * 64, &tm_q, &s.q_full, c * 64, head[t], qt[t] * TILE, b);
+        }
+        int item = 0;
+        bool ok = true;
+        for (int j = j0; j < j1 && ok; ++j) {
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv, ++item) {
+            const int st = item % KV_STAGES;
+            ok = ok && wait_warp(&s.kv_empty[st], ((item / KV_STAGES) & 1) ^ 1, p.err, 311);
+            if (!ok) break;
+            if (lane == 0) {
+              mbar_arrive_expect_tx(&s.kv_full[st], tile_bytes);
+              for (int c = 0; c < chunks; ++c)
+                tma_load_4d(s.kv[st] + c * 128 * 64, kv ? &tm_v : &tm_k, &s.kv_full[st], c * 64, kvh, j * TILE, b);
+            }
+            __syncwarp();
+            if (kv && is_dead(s.dead, j)) {
+              ok = wait_warp(&s.kv_full[st], (item / KV_STAGES) & 1, p.err, 312);
+              zero_dead_rows(s.kv[st], chunks, rows + j * TILE, lane);
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&s.clean);
+            }
+          }
+        }
+        // the copies have landed before the block may leave, also after a wait that ran out
+        wait_phase(&s.q_full, 0, p.err, 313);
+        for (int i = max(0, item - KV_STAGES); i < item; ++i)
+          wait_phase(&s.kv_full[i % KV_STAGES], (i / KV_STAGES) & 1, p.err, 313);
+      }
+    } else if (warp == MMA_WARP) {
+      // ------------------------------------------------------------ MMA issuer
+      if (j0 < j1) {
+        // The whole warp goes through the loop, so that descriptors are made in uniform registers; one lane issues.
+        const uint32_t leader = elect_one();
+        const uint32_t idS = make_idesc_bf16(128, TILE, false, false);           // Q (K-major) x K (K-major)
+        const uint32_t idO = make_idesc_bf16(128, p.ksteps * 16, false, true);   // P (TMEM) x V (MN-major)
+        int cleaned = j0 - 1, n_clean = 0;
+        auto kv_wait = [&](int item) -> bool {
+          return wait_warp(&s.kv_full[item % KV_STAGES], (item / KV_STAGES) & 1, p.err, 314);
+        };
+        // S_t may go over P_t of the block before: that product was issued earlier by this thread
+        auto issue_s = [&](int t, int j) {
+          tc_fence_after();
+          const uint32_t qa = smem_u32(s.q[t]), ka = smem_u32(s.kv[(2 * (j - j0)) % KV_STAGES]);
+          mma_tiles(tS(t), qa, ka, idS, p.ksteps, leader);
+          commit(&s.s_full[t], leader);
+        };
+        auto issue_pv = [&](int t, int j) -> bool {
+          const int item = 2 * (j - j0) + 1;
+          if (!kv_wait(item)) return false;
+          if (is_dead(s.dead, j) && cleaned < j) {
+            if (!wait_warp(&s.clean, n_clean++ & 1, p.err, 315)) return false;
+            cleaned = j;
+          }
+          const uint32_t va = smem_u32(s.kv[item % KV_STAGES]);
+          const int c = j - first[t];
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            if (!wait_warp(half ? &s.p_full[t] : &s.p_half[t], c & 1, p.err, 316)) return false;
+            tc_fence_after();
+#pragma unroll
+            for (int kk = half * 4; kk < half * 4 + 4; ++kk)
+              mma_ts(tO(t), tS(t) + kk * 8, make_sw128_desc(va + kk * 2048, 128 * 128, 1024), idO,
+                          (c > 0 || kk > 0) ? 1u : 0u, leader);
+          }
+          commit(&s.o_done[t], j + 1 == end[t] ? leader : 0u);
+          return true;
+        };
+        bool ok = wait_warp(&s.q_full, 0, p.err, 317) && kv_wait(0);
+        if (ok) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            if (first[t] == j0 && j0 < end[t]) issue_s(t, j0);
+          commit(&s.kv_empty[0], leader);
+        }
+        for (int j = j0; ok && j < j1; ++j) {
+          const int iv = 2 * (j - j0) + 1, ik = iv + 1;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (!ok) break;
+            if (first[t] <= j && j < end[t]) ok = issue_pv(t, j);
+            if (ok && first[t] <= j + 1 && j + 1 < end[t]) {
+              ok = kv_wait(ik);
+              if (ok) issue_s(t, j + 1);
+            }
+          }
+          if (!ok) break;
+          commit(&s.kv_empty[iv % KV_STAGES], leader);
+          if (j + 1 < j1) commit(&s.kv_empty[ik % KV_STAGES], leader);
+        }
+        if (!ok) {
+          commit(&s.drained, leader);
+          wait_warp(&s.drained, 0, p.err, 318);
+        }
+      }
     }
   }
 
@@ -450,45 +453,12 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   __syncthreads();
   if (warp == MMA_WARP) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(s.tmem_base, 512);
   }
-}
-
-// ------------------------------------------------------------------------------ backward: rowsum(do o)
-// 16 lanes per (row, head), 8 values each; 0 for rows that see nothing and behind the last token.
-__global__ void delta_kernel(const DeltaArgs a) {
-  const int64_t unit = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 4;
-  const int part = threadIdx.x & 15;
-  const int64_t total = static_cast<int64_t>(a.B) * a.padded * a.nq;
-  const bool in = unit < total;
-  const int h = static_cast<int>(unit % a.nq);
-  const int64_t tok = unit / a.nq;
-  const int b = static_cast<int>(tok / a.padded), i = static_cast<int>(tok % a.padded);
-  float acc = 0.f;
-  const bool live = in && i < a.S && a.rows[b * a.rows_stride + i].y > 0;
-  if (live && part * 8 < a.d) {
-    const uint4 x = *reinterpret_cast<const uint4*>(at(a.o, b, i, h) + part * 8);
-    const uint4 y = *reinterpret_cast<const uint4*>(at(a.dout, b, i, h) + part * 8);
-    const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 u = unpack_bf16x2(xs[e]), v = unpack_bf16x2(ys[e]);
-      acc = fmaf(u.x, v.x, fmaf(u.y, v.y, acc));
-    }
-  }
-#pragma unroll
-  for (int w = 8; w > 0; w >>= 1) acc += __shfl_xor_sync(0xffffffff, acc, w);
-  if (in && part == 0) a.delta[(static_cast<int64_t>(b) * a.nq + h) * a.padded + i] = acc;
 }
 
 cudaError_t launch_mask(const MaskArgs& a, int batch, cudaStream_t st) {
   mask_kernel<<<batch, 1024, 0, st>>>(a);
-  return cudaGetLastError();
-}
-
-cudaError_t launch_delta(const DeltaArgs& a, cudaStream_t st) {
-  const int64_t units = static_cast<int64_t>(a.B) * a.padded * a.nq;
-  delta_kernel<<<static_cast<unsigned>((units * 16 + 255) / 256), 256, 0, st>>>(a);
   return cudaGetLastError();
 }
 

@@ -36,10 +36,109 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, int* e
   return __all_sync(0xffffffffu, wait_phase(bar, parity, err, code));
 }
 
+// tcgen05.mma by the lanes where `on` is not 0 (one of the warp).  The predicate is the instruction's own: with a branch
+// around each, issuing took 115 clocks per 128 x 128 x 16 product instead of the 64 that the product takes.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add, uint32_t on) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(add), "r"(on)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add, uint32_t on) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(add), "r"(on)
+      : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t* bar, uint32_t on) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+      "r"(on)
+      : "memory");
+}
+
+// dst = A B^T of two K-major tiles, 16 values of d at a time (those past ksteps are not there)
+__device__ __forceinline__ void mma_tiles(uint32_t dst, uint32_t a, uint32_t b, uint32_t idesc, int ksteps, uint32_t on) {
+#pragma unroll
+  for (int kk = 0; kk < HEAD / 16; ++kk) {
+    const uint32_t off = (kk >> 2) * 128 * 128 + (kk & 3) * 32;
+    mma_ss(dst, make_sw128_desc(a + off, 16, 1024), make_sw128_desc(b + off, 16, 1024), idesc, kk > 0, kk < ksteps ? on : 0u);
+  }
+}
+
+template <int N>
+__device__ __forceinline__ void more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewer_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+// Two fp32 operations in one instruction
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 apart(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+// 2^x of two values on the FMA pipe, for x below 127.  Cody and Waite's reduction x = n + f: adding 1.5 2^23 rounds
+// to the integer n, which is left in the low bits, and f is in [-1/2, 1/2]; 2^f by the cubic that minimises the largest
+// relative error there (7.5e-5, found by linear programming over 4001 points; bf16 rounds by 2e-3), n goes into the exponent.
+// Below -125 the result is 2^-125.
+__device__ __forceinline__ float2 exp2_pair(float a, float b) {
+  const uint64_t shift = pair(12582912.f, 12582912.f);
+  const uint64_t x = pair(fmaxf(a, -125.f), fmaxf(b, -125.f));
+  const uint64_t t = add2(x, shift);
+  const uint64_t f = add2(x, fma2(t, pair(-1.f, -1.f), shift));
+  uint64_t q = fma2(pair(0.0551716685f, 0.0551716685f), f, pair(0.2426111251f, 0.2426111251f));
+  q = fma2(q, f, pair(0.6932609677f, 0.6932609677f));
+  q = fma2(q, f, pair(0.9999280572f, 0.9999280572f));
+  const float2 qs = apart(q), ts = apart(t);
+  // 1.5 2^23 + n has n in its low bits and nothing else in the low nine
+  return make_float2(__uint_as_float(__float_as_uint(qs.x) + (__float_as_uint(ts.x) << 23)),
+                     __uint_as_float(__float_as_uint(qs.y) + (__float_as_uint(ts.y) << 23)));
+}
+
 __device__ __forceinline__ float rcp_approx(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// 2^x of the e-th pair of a row.  Every fourth pair runs on the FMA pipe: the special-function unit takes 8 clocks for
+// one exponential of a warp and would set the pace alone.
+__device__ __forceinline__ constexpr bool on_fma_pipe(int e) { return e % 4 == 3; }
+__device__ __forceinline__ float2 exp2_of(float2 x, int e) {
+  return on_fma_pipe(e) ? exp2_pair(x.x, x.y) : make_float2(ex2_approx(x.x), ex2_approx(x.y));
 }
 
 // A raw product s as a score in log2 units.  tanh(x) = 1 - 2 / (1 + exp(2x)): two special-function

@@ -35,8 +35,18 @@ namespace ma {
 
 constexpr int TILE = 128;
 constexpr int HEAD = 128;  // values of a head that a tile has room for
-constexpr int NTHREADS = 320;  // 8 compute warps, 1 TMA warp, 1 MMA warp
-constexpr int PRODUCER_WARP = 8, MMA_WARP = 9;
+// Three groups of four warps: 8 compute warps, a TMA warp, an MMA warp and two that only hand their registers
+// over.  Launched with 168 registers a thread (64512 in all), of which the kernels move some from the last group
+// to the compute warps: a row of scores stays in registers.
+constexpr int NTHREADS = 384;
+constexpr int PRODUCER_WARP = 8, MMA_WARP = 9, COMPUTE_WARPS = 8;
+template <int COMPUTE, int OTHER>
+struct Registers {
+  static constexpr int compute = COMPUTE, other = OTHER;
+  static_assert(256 * COMPUTE + 128 * OTHER <= NTHREADS * 168, "more registers than the launch has");
+};
+using FwdRegisters = Registers<224, 56>;
+using BwdRegisters = Registers<216, 72>;
 constexpr int MAX_TILES = 2048;  // 262144 tokens: the tiles that meet a tile are listed in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kNever = 0x7fffffff;  // lo of a row that sees nothing; its hi is 0
@@ -60,7 +70,7 @@ struct Common {
   const float* slopes;
   float scale, scale_log2;
   float cap_in, cap_out;  // exp2(s cap_in) = exp(2 scale s / c); c log2(e)
-  float* lse2;            // [B, nq, padded], log2 units, +inf where a row sees nothing
+  float* neg_lse2;        // [B, nq, padded], minus the log-sum-exp in log2 units; -inf where a row sees nothing
   int* err;
 };
 
@@ -71,27 +81,25 @@ struct Out {  // a [batch, tokens, heads, d] tensor of bf16, strides in elements
 
 struct FwdParams : Common {
   Out o;
+  void* low;               // what o's rounding to bf16 left out, in bf16 and laid out like o; or null
   bool pair_heads;
 };
 
 struct BwdParams : Common {
-  const float* delta;
+  Out o;
+  const void* low;
+  float* neg_delta;        // [B, nq, padded], -rowsum(do o)
   Out dq, dk, dv;
+  int split;               // blocks that share the query heads of a group, and with more than one
+  float* part;             // [split][2 (dv, dk)][B, nkv, padded][d]: their sums, joined in order
 };
 
-struct DeltaArgs {  // rowsum(do o) of every row and head
-  Out o, dout;
-  float* delta;            // [B, nq, padded]
-  const int2* rows;
-  int64_t rows_stride;
-  int B, S, padded, nq, d;
-};
-
-// Each returns what cudaGetLastError() says.
+// Each returns what cudaGetLastError() says.  launch_delta comes before the other two of the
+// backward pass.
 cudaError_t launch_mask(const MaskArgs& a, int batch, cudaStream_t st);
 cudaError_t launch_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const FwdParams& p, bool cap,
                        bool bias, cudaStream_t st);
-cudaError_t launch_delta(const DeltaArgs& a, cudaStream_t st);
+cudaError_t launch_delta(const BwdParams& p, const Out& dout, cudaStream_t st);
 cudaError_t launch_dq(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& td,
                       const BwdParams& p, bool cap, bool bias, cudaStream_t st);
 cudaError_t launch_dkv(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& td,

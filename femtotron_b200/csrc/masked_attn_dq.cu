@@ -1,8 +1,56 @@
-// Attention over a mask of intervals: the gradient of the queries (masked_attn.h).
+// Attention over a mask of intervals: the gradient of the queries and the row sums before it (masked_attn.h).
 #include "masked_attn.cuh"
 
 namespace ft {
 namespace ma {
+
+// ------------------------------------------------------------------------------ backward: rowsum(do o)
+// 16 lanes per (row, head), 8 values each, four rows in flight; 0 for rows that see nothing and behind the last
+// token.  o comes with what its rounding left out: where a row sees few keys, that rounding is as large as the
+// one of ds and dq and dk would be off by 1.7 roundings instead of 1.4.  Bound by HBM.
+constexpr int DELTA_UNITS = 4;
+
+__global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ BwdParams p, const Out dout) {
+  const int part = threadIdx.x & 15;
+  const int64_t total = static_cast<int64_t>(p.B) * p.padded * p.nq;
+  const int64_t u0 = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / 16;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * 16;
+  uint4 x[DELTA_UNITS], l[DELTA_UNITS], y[DELTA_UNITS];
+  int64_t stat[DELTA_UNITS];
+  bool live[DELTA_UNITS];
+#pragma unroll
+  for (int k = 0; k < DELTA_UNITS; ++k) {
+    const int64_t unit = u0 + k * step;
+    const int h = static_cast<int>(unit % p.nq);
+    const int64_t tok = unit / p.nq;
+    const int b = static_cast<int>(tok / p.padded), i = static_cast<int>(tok % p.padded);
+    stat[k] = unit < total ? (static_cast<int64_t>(b) * p.nq + h) * p.padded + i : -1;
+    live[k] = unit < total && i < p.S && part * 8 < p.d && p.rows[b * p.rows_stride + i].y > 0;
+    if (live[k]) {
+      const __nv_bfloat16* o = at(p.o, b, i, h) + part * 8;
+      x[k] = __ldg(reinterpret_cast<const uint4*>(o));
+      l[k] = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.low) +
+                                                  (o - static_cast<const __nv_bfloat16*>(p.o.p))));
+      y[k] = __ldg(reinterpret_cast<const uint4*>(at(dout, b, i, h) + part * 8));
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < DELTA_UNITS; ++k) {
+    float acc = 0.f;
+    if (live[k]) {
+      const uint32_t xs[4] = {x[k].x, x[k].y, x[k].z, x[k].w}, ls[4] = {l[k].x, l[k].y, l[k].z, l[k].w},
+                     ys[4] = {y[k].x, y[k].y, y[k].z, y[k].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 u = unpack_bf16x2(xs[e]), w = unpack_bf16x2(ls[e]), v = unpack_bf16x2(ys[e]);
+        acc = fmaf(u.x + w.x, v.x, fmaf(u.y + w.y, v.y, acc));
+      }
+    }
+#pragma unroll
+    for (int w = 8; w > 0; w >>= 1) acc += __shfl_xor_sync(0xffffffff, acc, w);
+    if (part == 0 && stat[k] >= 0) p.neg_delta[stat[k]] = -acc;
+  }
+}
 
 // ------------------------------------------------------------------------------ backward: dq
 // One block per 128 queries of a head; the keys go past.  S = Q K^T and dP = dO V^T come from shared
@@ -59,97 +107,12 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = s.tmem_base;
-  auto tS = [tmem](int st) -> uint32_t { return tmem + static_cast<uint32_t>(st) * 128u; };
+  constexpr uint32_t tmem = 0;  // where an allocation of all 512 columns begins
+  auto tS = [](int st) -> uint32_t { return tmem + static_cast<uint32_t>(st) * 128u; };
   const uint32_t tdP = tmem + 256, tdQ = tmem + 384;
 
-  if (warp == PRODUCER_WARP) {
-    if (n > 0) {
-      auto load = [&](__nv_bfloat16* dst, const CUtensorMap* tm, uint64_t* bar, int head, int tile) {
-        for (int c = 0; c < chunks; ++c) tma_load_4d(dst + c * 128 * 64, tm, bar, c * 64, head, tile * TILE, b);
-      };
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&s.q_full, 2 * tile_bytes);
-        load(s.q, &tm_q, &s.q_full, h, qt);
-        load(s.dout, &tm_do, &s.q_full, h, qt);
-      }
-      bool ok = true;
-      int nk = 0, nv = 0;
-      for (int it = 0; it < n && ok; ++it) {
-        const int ks = it % 3, vs = it & 1;
-        ok = wait_warp(&s.k_empty[ks], ((it / 3) & 1) ^ 1, p.err, 331);
-        if (!ok) break;
-        if (lane == 0) {
-          mbar_arrive_expect_tx(&s.k_full[ks], tile_bytes);
-          load(s.k[ks], &tm_k, &s.k_full[ks], kvh, j0 + it);
-        }
-        ++nk;
-        __syncwarp();
-        if (is_dead(s.dead, j0 + it)) {
-          ok = wait_warp(&s.k_full[ks], (it / 3) & 1, p.err, 332);
-          zero_dead_rows(s.k[ks], chunks, rows + (j0 + it) * TILE, lane);
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&s.clean);
-        }
-        ok = ok && wait_warp(&s.v_empty[vs], ((it >> 1) & 1) ^ 1, p.err, 333);
-        if (!ok) break;
-        if (lane == 0) {
-          mbar_arrive_expect_tx(&s.v_full[vs], tile_bytes);
-          load(s.v[vs], &tm_v, &s.v_full[vs], kvh, j0 + it);
-        }
-        ++nv;
-        __syncwarp();
-      }
-      // the copies have landed before the block may leave, also after a wait that ran out
-      wait_phase(&s.q_full, 0, p.err, 334);
-      for (int i = max(0, nk - 3); i < nk; ++i) wait_phase(&s.k_full[i % 3], (i / 3) & 1, p.err, 334);
-      for (int i = max(0, nv - 2); i < nv; ++i) wait_phase(&s.v_full[i & 1], (i >> 1) & 1, p.err, 334);
-    }
-  } else if (warp == MMA_WARP) {
-    if (n > 0 && elect_one()) {
-      const uint32_t idS = make_idesc_bf16(128, TILE, false, false);
-      const uint32_t idQ = make_idesc_bf16(128, p.ksteps * 16, false, true);
-      int n_clean = 0;
-      auto product = [&](uint32_t dst, uint32_t a, uint32_t bb) {
-        for (int kk = 0; kk < p.ksteps; ++kk) {
-          const uint32_t off = (kk >> 2) * 128 * 128 + (kk & 3) * 32;
-          mma_bf16(dst, make_sw128_desc(a + off, 16, 1024), make_sw128_desc(bb + off, 16, 1024), idS, kk > 0 ? 1u : 0u);
-        }
-      };
-      auto issue_s = [&](int it) -> bool {
-        if (!wait_phase(&s.k_full[it % 3], (it / 3) & 1, p.err, 335)) return false;
-        if (is_dead(s.dead, j0 + it) && !wait_phase(&s.clean, n_clean++ & 1, p.err, 336)) return false;
-        tc_fence_after();
-        product(tS(it & 1), smem_u32(s.q), smem_u32(s.k[it % 3]));
-        mma_commit(&s.s_full[it & 1]);
-        return true;
-      };
-      auto issue_dp = [&](int it) -> bool {
-        if (!wait_phase(&s.v_full[it & 1], (it >> 1) & 1, p.err, 337)) return false;
-        tc_fence_after();
-        product(tdP, smem_u32(s.dout), smem_u32(s.v[it & 1]));
-        mma_commit(&s.dp_full);
-        mma_commit(&s.v_empty[it & 1]);
-        return true;
-      };
-      bool ok = wait_phase(&s.q_full, 0, p.err, 338) && issue_s(0) && issue_dp(0) && (n < 2 || issue_s(1));
-      for (int it = 0; ok && it < n; ++it) {
-        ok = wait_phase(&s.ds_full, it & 1, p.err, 339);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t ka = smem_u32(s.k[it % 3]);
-#pragma unroll
-        for (int kk = 0; kk < TILE / 16; ++kk)  // ds: keys 0..63 in columns 0..31, 64..127 in 64..95
-          mma_bf16_ts(tdQ, tS(it & 1) + (kk >> 2) * 64 + (kk & 3) * 8, make_sw128_desc(ka + kk * 2048, 128 * 128, 1024),
-                      idQ, (it > 0 || kk > 0) ? 1u : 0u);
-        mma_commit(&s.k_empty[it % 3]);
-        ok = (it + 1 >= n || issue_dp(it + 1)) && (it + 2 >= n || issue_s(it + 2));
-      }
-      mma_commit(ok ? &s.done : &s.drained);
-      if (!ok) wait_phase(&s.drained, 0, p.err, 340);
-    }
-  } else {
+  if (warp < COMPUTE_WARPS) {
+    more_registers<BwdRegisters::compute>();
     // two warps per TMEM lane quadrant (32 queries), 64 of the 128 keys each
     const int quad = warp & 3, half = warp >> 2;
     const int row = qt * TILE + quad * 32 + lane;
@@ -158,7 +121,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     int lo = 0, width = 0;
     const int2 lh = rows[row];
     if (lh.y > lh.x) lo = lh.x, width = lh.y - lh.x;
-    const float lse2 = p.lse2[stat], delta = p.delta[stat];
+    const float neg_lse2 = p.neg_lse2[stat], neg_delta = p.neg_delta[stat];
     const float slope2 = ALIBI ? p.slopes[h] * kLog2e : 0.f;
     bool ok = true;
     for (int it = 0; it < n && ok; ++it) {
@@ -176,33 +139,45 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         tmem_ld_32x32b_x32(ts, *reinterpret_cast<uint32_t(*)[32]>(sv));
         tmem_ld_32x32b_x32(ts + 32, *reinterpret_cast<uint32_t(*)[32]>(sv + 32));
         tmem_wait_ld();
+        const uint64_t mul = pair(p.scale_log2, p.scale_log2), m = pair(neg_lse2, neg_lse2);
 #pragma unroll
-        for (int e = 0; e < 64; ++e) {
-          float keep;
-          if (!CAP && !ALIBI) pv[e] = ex2_approx(fmaf(__uint_as_float(sv[e]), p.scale_log2, -lse2));
-          else {
-            pv[e] = ex2_approx(score<CAP, ALIBI>(__uint_as_float(sv[e]), p, slope2, far - e, keep) - lse2);
-            if (CAP) pv[e] *= keep;
+        for (int e = 0; e < 64; e += 2) {
+          float2 y, keep = make_float2(1.f, 1.f);
+          if (!CAP && !ALIBI) {
+            y = apart(fma2(pair(__uint_as_float(sv[e]), __uint_as_float(sv[e + 1])), mul, m));
+          } else {
+            y.x = score<CAP, ALIBI>(__uint_as_float(sv[e]), p, slope2, far - e, keep.x) + neg_lse2;
+            y.y = score<CAP, ALIBI>(__uint_as_float(sv[e + 1]), p, slope2, far - (e + 1), keep.y) + neg_lse2;
           }
+          y = exp2_of(y, e / 2);
+          pv[e] = CAP ? y.x * keep.x : y.x;
+          pv[e + 1] = CAP ? y.y * keep.y : y.y;
         }
       }
       ok = wait_warp(&s.dp_full, it & 1, p.err, 342);
       if (!ok) break;
       tc_fence_after();
+      uint32_t dv[64];
+      tmem_ld_32x32b_x32(tdP + lane_off + half * 64, *reinterpret_cast<uint32_t(*)[32]>(dv));
+      tmem_ld_32x32b_x32(tdP + lane_off + half * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(dv + 32));
+      tmem_wait_ld();
+      const uint64_t nd = pair(neg_delta, neg_delta);
+#pragma unroll
+      for (int e = 0; e < 64; e += 2) {
+        const float2 g = apart(mul2(pair(pv[e], pv[e + 1]), add2(pair(__uint_as_float(dv[e]), __uint_as_float(dv[e + 1])), nd)));
+        pv[e] = g.x;
+        pv[e + 1] = g.y;
+      }
+      if (test) {  // replaced, not multiplied: the product may be NaN in a masked place
+#pragma unroll
+        for (int e = 0; e < 64; ++e)
+          if (static_cast<uint32_t>(off + e) >= static_cast<uint32_t>(width)) pv[e] = 0.f;
+      }
 #pragma unroll
       for (int h32 = 0; h32 < 2; ++h32) {
-        uint32_t dv[32], pk[16];
-        tmem_ld_32x32b_x32(tdP + lane_off + half * 64 + h32 * 32, dv);
-        tmem_wait_ld();
+        uint32_t pk[16];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) pv[h32 * 32 + e] *= __uint_as_float(dv[e]) - delta;
-        if (test) {  // replaced, not multiplied: the product may be NaN in a masked place
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (static_cast<uint32_t>(off + h32 * 32 + e) >= static_cast<uint32_t>(width)) pv[h32 * 32 + e] = 0.f;
-        }
-#pragma unroll
-        for (int e = 0; e < 16; ++e) pk[e] = pack_bf16x2(pv[h32 * 32 + 2 * e], pv[h32 * 32 + 2 * e + 1]);
+        for (int i = 0; i < 16; ++i) pk[i] = pack_bf16x2(pv[h32 * 32 + 2 * i], pv[h32 * 32 + 2 * i + 1]);
         tmem_st_32x32b_x16(ts + h32 * 16, pk);
       }
       tmem_wait_st();
@@ -226,14 +201,105 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         }
       }
     }
+  } else {
+    fewer_registers<BwdRegisters::other>();
+    if (warp == PRODUCER_WARP) {
+      if (n > 0) {
+        auto load = [&](__nv_bfloat16* dst, const CUtensorMap* tm, uint64_t* bar, int head, int tile) {
+          for (int c = 0; c < chunks; ++c) tma_load_4d(dst + c * 128 * 64, tm, bar, c * 64, head, tile * TILE, b);
+        };
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&s.q_full, 2 * tile_bytes);
+          load(s.q, &tm_q, &s.q_full, h, qt);
+          load(s.dout, &tm_do, &s.q_full, h, qt);
+        }
+        bool ok = true;
+        int nk = 0, nv = 0;
+        for (int it = 0; it < n && ok; ++it) {
+          const int ks = it % 3, vs = it & 1;
+          ok = wait_warp(&s.k_empty[ks], ((it / 3) & 1) ^ 1, p.err, 331);
+          if (!ok) break;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&s.k_full[ks], tile_bytes);
+            load(s.k[ks], &tm_k, &s.k_full[ks], kvh, j0 + it);
+          }
+          ++nk;
+          __syncwarp();
+          if (is_dead(s.dead, j0 + it)) {
+            ok = wait_warp(&s.k_full[ks], (it / 3) & 1, p.err, 332);
+            zero_dead_rows(s.k[ks], chunks, rows + (j0 + it) * TILE, lane);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s.clean);
+          }
+          ok = ok && wait_warp(&s.v_empty[vs], ((it >> 1) & 1) ^ 1, p.err, 333);
+          if (!ok) break;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&s.v_full[vs], tile_bytes);
+            load(s.v[vs], &tm_v, &s.v_full[vs], kvh, j0 + it);
+          }
+          ++nv;
+          __syncwarp();
+        }
+        // the copies have landed before the block may leave, also after a wait that ran out
+        wait_phase(&s.q_full, 0, p.err, 334);
+        for (int i = max(0, nk - 3); i < nk; ++i) wait_phase(&s.k_full[i % 3], (i / 3) & 1, p.err, 334);
+        for (int i = max(0, nv - 2); i < nv; ++i) wait_phase(&s.v_full[i & 1], (i >> 1) & 1, p.err, 334);
+      }
+    } else if (warp == MMA_WARP) {
+      if (n > 0) {
+        // The whole warp goes through the loop, so that descriptors are made in uniform registers; one lane issues.
+        const uint32_t leader = elect_one();
+        const uint32_t idS = make_idesc_bf16(128, TILE, false, false);
+        const uint32_t idQ = make_idesc_bf16(128, p.ksteps * 16, false, true);
+        int n_clean = 0;
+        auto issue_s = [&](int it) -> bool {
+          if (!wait_warp(&s.k_full[it % 3], (it / 3) & 1, p.err, 335)) return false;
+          if (is_dead(s.dead, j0 + it) && !wait_warp(&s.clean, n_clean++ & 1, p.err, 336)) return false;
+          tc_fence_after();
+          mma_tiles(tS(it & 1), smem_u32(s.q), smem_u32(s.k[it % 3]), idS, p.ksteps, leader);
+          commit(&s.s_full[it & 1], leader);
+          return true;
+        };
+        auto issue_dp = [&](int it) -> bool {
+          if (!wait_warp(&s.v_full[it & 1], (it >> 1) & 1, p.err, 337)) return false;
+          tc_fence_after();
+          mma_tiles(tdP, smem_u32(s.dout), smem_u32(s.v[it & 1]), idS, p.ksteps, leader);
+          commit(&s.dp_full, leader);
+          commit(&s.v_empty[it & 1], leader);
+          return true;
+        };
+        bool ok = wait_warp(&s.q_full, 0, p.err, 338) && issue_s(0) && issue_dp(0) && (n < 2 || issue_s(1));
+        for (int it = 0; ok && it < n; ++it) {
+          ok = wait_warp(&s.ds_full, it & 1, p.err, 339);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t ka = smem_u32(s.k[it % 3]);
+#pragma unroll
+          for (int kk = 0; kk < TILE / 16; ++kk)  // ds: keys 0..63 in columns 0..31, 64..127 in 64..95
+            mma_ts(tdQ, tS(it & 1) + (kk >> 2) * 64 + (kk & 3) * 8, make_sw128_desc(ka + kk * 2048, 128 * 128, 1024),
+                        idQ, (it > 0 || kk > 0) ? 1u : 0u, leader);
+          commit(&s.k_empty[it % 3], leader);
+          ok = (it + 1 >= n || issue_dp(it + 1)) && (it + 2 >= n || issue_s(it + 2));
+        }
+        commit(ok ? &s.done : &s.drained, leader);
+        if (!ok) wait_warp(&s.drained, 0, p.err, 340);
+      }
+    }
   }
 
   tc_fence_before();
   __syncthreads();
   if (warp == MMA_WARP) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(s.tmem_base, 512);
   }
+}
+
+cudaError_t launch_delta(const BwdParams& p, const Out& dout, cudaStream_t st) {
+  const int64_t per = 16 * DELTA_UNITS, total = static_cast<int64_t>(p.B) * p.padded * p.nq;
+  delta_kernel<<<static_cast<unsigned>((total + per - 1) / per), 256, 0, st>>>(p, dout);
+  return cudaGetLastError();
 }
 
 cudaError_t launch_dq(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& td,

@@ -69,7 +69,7 @@ Shape check(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const
 }
 
 void fill(Common& p, const Shape& n, const at::Tensor& rows, const at::Tensor& tiles, double scale, double softcap,
-          const c10::optional<at::Tensor>& slopes, float* lse2, at::Tensor& err) {
+          const c10::optional<at::Tensor>& slopes, float* neg_lse2, at::Tensor& err) {
   p.B = n.B; p.S = n.S; p.nq = n.nq; p.nkv = n.nkv; p.d = n.d;
   p.ntiles = (n.S + TILE - 1) / TILE;
   p.padded = p.ntiles * TILE;
@@ -84,7 +84,7 @@ void fill(Common& p, const Shape& n, const at::Tensor& rows, const at::Tensor& t
   p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
   p.cap_in = softcap > 0 ? static_cast<float>(2 * scale * 1.4426950408889634 / softcap) : 0.f;
   p.cap_out = static_cast<float>(softcap * 1.4426950408889634);
-  p.lse2 = lse2;
+  p.neg_lse2 = neg_lse2;
   p.err = err.data_ptr<int>();
 }
 
@@ -140,8 +140,8 @@ std::tuple<at::Tensor, at::Tensor> attn_mask(int64_t B, int64_t S, bool causal, 
   return {rows, tiles};
 }
 
-// o [B, S, nq, d] and, where `graded`, the statistics [B, nq, padded] that the backward reads
-std::tuple<at::Tensor, c10::optional<at::Tensor>> masked_attn_fwd(
+// o [B, S, nq, d] and, where `graded`, the statistics [B, nq, padded] and the rest of o that the backward reads
+std::tuple<at::Tensor, c10::optional<at::Tensor>, c10::optional<at::Tensor>> masked_attn_fwd(
     const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_, const at::Tensor& rows,
     const at::Tensor& tiles, double scale, double softcap, const c10::optional<at::Tensor>& slopes, bool graded,
     at::Tensor& err) {
@@ -149,53 +149,73 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> masked_attn_fwd(
   const Shape n = check(q_, k_, v_, rows, tiles, slopes, err);
   const c10::cuda::CUDAGuard g(q_.device());
   at::Tensor o = at::empty({n.B, n.S, n.nq, n.d}, q_.options().memory_format(c10::MemoryFormat::Contiguous));
-  c10::optional<at::Tensor> lse;
+  c10::optional<at::Tensor> lse, low;
   const int64_t nt = (n.S + TILE - 1) / TILE;
+  if (graded) low = at::empty_like(o);
   if (graded) lse = at::empty({n.B, n.nq, nt * TILE}, q_.options().dtype(at::kFloat));
-  if (n.B == 0 || n.S == 0 || n.nq == 0) return {o, lse};
+  if (n.B == 0 || n.S == 0 || n.nq == 0) return {o, lse, low};
   const at::Tensor q = usable(q_), k = usable(k_), v = usable(v_);
   FwdParams p;
   fill(p, n, rows, tiles, scale, softcap, slopes, graded ? lse->data_ptr<float>() : nullptr, err);
   p.o = out_of(o);
+  p.low = graded ? low->data_ptr() : nullptr;
   p.pair_heads = p.group % 2 == 0;
   C10_CUDA_CHECK(launch_fwd(heads_map(q), heads_map(k), heads_map(v), p, softcap > 0, slopes.has_value(),
                             at::cuda::getCurrentCUDAStream()));
-  return {o, lse};
+  return {o, lse, low};
 }
 
-void masked_attn_bwd(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_, const at::Tensor& o,
-                     const at::Tensor& do_, const at::Tensor& lse, const at::Tensor& rows,
+// returns the number of kernels launched
+int64_t masked_attn_bwd(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_, const at::Tensor& o,
+                     const at::Tensor& low, const at::Tensor& do_, const at::Tensor& lse, const at::Tensor& rows,
                      const at::Tensor& tiles, double scale, double softcap,
                      const c10::optional<at::Tensor>& slopes, at::Tensor& dq, at::Tensor& dk, at::Tensor& dv,
                      at::Tensor& err) {
   using namespace ma;
   const Shape n = check(q_, k_, v_, rows, tiles, slopes, err);
-  one_device(q_, o, do_, lse);
+  one_device(q_, o, low, do_, lse);
   const int64_t nt = (n.S + TILE - 1) / TILE;
   TORCH_CHECK(o.sizes() == q_.sizes() && do_.sizes() == q_.sizes() && o.scalar_type() == at::kBFloat16 &&
-                  do_.scalar_type() == at::kBFloat16 && o.is_contiguous(),
+                  do_.scalar_type() == at::kBFloat16 && o.is_contiguous() && low.sizes() == o.sizes() &&
+                  low.scalar_type() == at::kBFloat16 && low.is_contiguous(),
               "masked_attention: the output and its gradient must have the queries' shape and type");
   TORCH_CHECK(lse.is_contiguous() && lse.scalar_type() == at::kFloat && lse.numel() == n.B * n.nq * nt * TILE,
               "masked_attention: statistics of another call");
   check_out(dq, q_, "dq");
   check_out(dk, k_, "dk");
   check_out(dv, v_, "dv");
-  if (n.B == 0 || n.S == 0 || n.nq == 0) return;
+  if (n.B == 0 || n.S == 0 || n.nq == 0) return 0;
   const c10::cuda::CUDAGuard g(q_.device());
   auto st = at::cuda::getCurrentCUDAStream();
   const at::Tensor q = usable(q_), k = usable(k_), v = usable(v_), dout = usable(do_);
   at::Tensor delta = at::empty_like(lse);
   BwdParams p;
   fill(p, n, rows, tiles, scale, softcap, slopes, lse.data_ptr<float>(), err);
-  p.delta = delta.data_ptr<float>();
+  p.neg_delta = delta.data_ptr<float>();
+  p.o = out_of(o);
+  p.low = low.data_ptr();
   p.dq = out_of(dq);
   p.dk = out_of(dk);
   p.dv = out_of(dv);
-  const DeltaArgs a{out_of(o), out_of(dout), delta.data_ptr<float>(), p.rows, p.rows_stride, p.B, p.S, p.padded, p.nq, p.d};
-  C10_CUDA_CHECK(launch_delta(a, st));
+  // Few key tiles leave SMs idle and one block with the whole group's work: then the group is split, as far as
+  // two blocks per SM, where a block keeps 16 tiles to work through.  (16384 tokens, 8 heads over 1: 128 blocks
+  // take 2.19 ms; the partial sums in memory cost 40 us per 4 blocks and 16384 x 128 values.)
+  p.split = 1;
+  while (n.B * n.nkv * nt * p.split < 2 * 148 && p.group / p.split >= 2 && nt * p.group / p.split >= 32) {
+    int next = p.split + 1;
+    while (p.group % next) ++next;
+    p.split = next;
+  }
+  at::Tensor part;
+  if (p.split > 1) {
+    part = at::empty({p.split, 2, n.B * n.nkv, p.padded, n.d}, lse.options());
+    p.part = part.data_ptr<float>();
+  }
   const CUtensorMap tq = heads_map(q), tk = heads_map(k), tv = heads_map(v), td = heads_map(dout);
-  C10_CUDA_CHECK(launch_dkv(tq, tk, tv, td, p, softcap > 0, slopes.has_value(), st));
+  C10_CUDA_CHECK(launch_delta(p, out_of(dout), st));
   C10_CUDA_CHECK(launch_dq(tq, tk, tv, td, p, softcap > 0, slopes.has_value(), st));
+  C10_CUDA_CHECK(launch_dkv(tq, tk, tv, td, p, softcap > 0, slopes.has_value(), st));
+  return p.split > 1 ? 4 : 3;
 }
 
 }  // namespace ft

@@ -158,30 +158,30 @@ class MaskedAttnFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, mask, scale, softcap, slopes, graded):
         if q.is_cuda:
-            o, lse = native().masked_attn_fwd(q, k, v, mask.rows, mask.tiles, scale, softcap, slopes, graded,
-                                              error_flag(q.device))
+            o, lse, low = native().masked_attn_fwd(q, k, v, mask.rows, mask.tiles, scale, softcap, slopes, graded,
+                                                   error_flag(q.device))
         else:
             *_, vf, _, lse, p = _forward_cpu(q, k, v, mask, scale, softcap, slopes)
-            o = (p @ vf).transpose(1, 2).to(q.dtype).contiguous()
+            o, low = (p @ vf).transpose(1, 2).to(q.dtype).contiguous(), None
         if graded:
-            ctx.save_for_backward(q, k, v, o, lse, mask.rows, mask.tiles, slopes)
+            ctx.save_for_backward(q, k, v, o, low, lse, mask.rows, mask.tiles, slopes)
             ctx.meta = (mask.seq_len, scale, softcap)
         return o
 
     @staticmethod
     def backward(ctx, do):
-        q, k, v, o, lse, rows, tiles, slopes = ctx.saved_tensors
+        q, k, v, o, low, lse, rows, tiles, slopes = ctx.saved_tensors
         dq, dk, dv = (torch.empty_like(x, memory_format=torch.contiguous_format) for x in (q, k, v))
-        _backward(q, k, v, o, do, lse, rows, tiles, slopes, ctx.meta, dq, dk, dv)
+        _backward(q, k, v, o, low, do, lse, rows, tiles, slopes, ctx.meta, dq, dk, dv)
         return dq, dk, dv, None, None, None, None, None
 
 
-def _backward(q, k, v, o, do, lse, rows, tiles, slopes, meta, dq, dk, dv):
+def _backward(q, k, v, o, low, do, lse, rows, tiles, slopes, meta, dq, dk, dv):
     seq_len, scale, softcap = meta
     if q.is_cuda:
-        native().masked_attn_bwd(q, k, v, o, do, lse, rows, tiles, scale, softcap, slopes, dq, dk, dv,
-                                 error_flag(q.device))
-        LAUNCHES[0] += 2  # the proxy counted one
+        n = native().masked_attn_bwd(q, k, v, o, low, do, lse, rows, tiles, scale, softcap, slopes, dq, dk, dv,
+                                     error_flag(q.device))
+        LAUNCHES[0] += n - 1  # the proxy counted one
         return
     mask = AttentionMask(rows, tiles, seq_len)
     B, S, nq, d = q.shape

@@ -256,6 +256,13 @@ def test_gpu_long():
 
 
 @gpu
+@pytest.mark.parametrize("S,nq,nkv,d", [(2100, 8, 1, 64), (1500, 6, 1, 40), (700, 12, 2, 128)])
+@pytest.mark.parametrize("kind", ["causal", "padded"])
+def test_gpu_many_heads_on_few_keys(S, nq, nkv, d, kind):
+    check_gpu(1, S, nq, nkv, d, kind)
+
+
+@gpu
 def test_gpu_padding_may_hold_nan():
     B, S, nq, nkv, d = 2, 700, 4, 2, 64
     q, k, v, do = make(B, S, nq, nkv, d, 2, "cuda", torch.bfloat16)

@@ -24,16 +24,23 @@ Attributes that a user may set on the model config:
                   (``functional.NormMLP8Fn``); without tensor parallelism, and where neither
                   the MLP nor its norm is wrapped or has hooks of its own
     loss_keep_logits  False: the loss without the logits in memory
+    attn_spec     dict of what attention does beside the causal mask (``ops/masked_attention.py``):
+                  "softcap" (scores capped by a tanh, 0 for none), "window" (tokens that a row reaches
+                  back, None), "alibi" (a bias of distance beside the rotation, False), "separator" (the
+                  token that ends a document; rows see their own document only, None)
+    embed_scale   factor of the embedding rows (1.0)
 """
 from __future__ import annotations
 
 import math
+from dataclasses import dataclass
 
 import torch
 import torch.nn.functional as F
 from torch import nn
 
 from femtotron_b200.ops import functional as FN
+from femtotron_b200.ops import masked_attention as MA
 from femtotron_b200.ops import rotary
 from femtotron_b200.ops.kernels import rope_tables
 from femtotron_b200.parallel.tensor_parallel import comm_ops as C
@@ -64,6 +71,39 @@ def rotary_spec_of(config) -> dict | None:
         raise ValueError(f"rotary_spec: partial must be in (0, 1], got {partial}")
     rot = int(head_dim_of(config) * partial) // 2 * 2
     return {"scaling": spec.get("scaling"), "interleaved": bool(spec.get("interleaved", False)), "rot": rot}
+
+
+def attn_spec_of(config) -> dict | None:
+    """The config's ``attn_spec`` with its defaults, or None where attention is plainly causal."""
+    spec = _cfg(config, "attn_spec", None)
+    if spec is None:
+        return None
+    unknown = set(spec) - {"softcap", "window", "alibi", "separator"}
+    if unknown:
+        raise ValueError(f"attn_spec: unknown keys {sorted(unknown)}")
+    softcap, window = float(spec.get("softcap") or 0.0), spec.get("window")
+    if not (softcap >= 0 and math.isfinite(softcap)):
+        raise ValueError(f"attn_spec: softcap must be 0 (none) or positive, got {softcap}")
+    if window is not None and window < 1:
+        raise ValueError(f"attn_spec: window must be at least 1, got {window}")
+    return {"softcap": softcap, "window": window, "alibi": bool(spec.get("alibi", False)),
+            "separator": spec.get("separator")}
+
+
+@dataclass
+class Attention:
+    """What the layers of one forward pass share: the mask of the batch, the cap, and the slopes of
+    all heads of the model."""
+    mask: MA.AttentionMask
+    softcap: float = 0.0
+    slopes: torch.Tensor | None = None
+
+    def __call__(self, qkv: torch.Tensor, B: int, S: int, nq: int, nkv: int, d: int, rank: int) -> torch.Tensor:
+        """[B*S, nq*d] of a packed [B*S, (nq+2nkv)*d] projection of the heads of one tensor-parallel rank."""
+        slopes = self.slopes[rank * nq:(rank + 1) * nq] if self.slopes is not None else None
+        o = MA.masked_attention_packed(qkv.view(B, S, nq + 2 * nkv, d), nq, nkv, self.mask, softcap=self.softcap,
+                                       slopes=slopes)
+        return o.reshape(B * S, nq * d)
 
 
 class LlamaRMSNorm(nn.Module):
@@ -202,8 +242,14 @@ class LlamaAttention(nn.Module):
     def _fusable(self) -> bool:
         return all(_plain_col(m) for m in (self.q_proj, self.k_proj, self.v_proj)) and _plain_row(self.o_proj)
 
-    def forward(self, x: torch.Tensor, position_embeddings, batch_shape, residual=None):
-        """x: [T_local, H] tokens (T_local = B*S, or B*S/tp under sequence parallelism)."""
+    def _attend(self, qkv, B, S, nq, nkv, d, attention):
+        if attention is None:
+            return causal_attention(qkv, B, S, nq, nkv, d)
+        return attention(qkv, B, S, nq, nkv, d, getattr(self.q_proj, "rank", 0))
+
+    def forward(self, x: torch.Tensor, position_embeddings, batch_shape, residual=None, attention=None):
+        """x: [T_local, H] tokens (T_local = B*S, or B*S/tp under sequence parallelism);
+        ``attention``: an ``Attention`` in place of the plainly causal one."""
         B, S = batch_shape
         cos, sin, pos = position_embeddings
         d = self.head_dim
@@ -215,7 +261,7 @@ class LlamaAttention(nn.Module):
             from femtotron_b200.parallel.tensor_parallel.fused import SPColumnFn, SPRowFn
             qkv = SPColumnFn.apply(x, comm, "qkv_rope", (cos, sin, pos, nq + nkv, d, S),
                                    self.q_proj.weight, self.k_proj.weight, self.v_proj.weight)
-            o = causal_attention(qkv, B, S, nq, nkv, d)
+            o = self._attend(qkv, B, S, nq, nkv, d, attention)
             return SPRowFn.apply(o, residual, comm, self.o_proj.weight)
         if self._fusable():
             xin = _enter(x, group, sp)
@@ -225,7 +271,7 @@ class LlamaAttention(nn.Module):
             else:
                 qkv = FN.QKVRopeFn.apply(xin, cos, sin, pos, nq + nkv, d, S,
                                          self.q_proj.weight, self.k_proj.weight, self.v_proj.weight)
-            o = causal_attention(qkv, B, S, nq, nkv, d)
+            o = self._attend(qkv, B, S, nq, nkv, d, attention)
             if group is None:
                 return FN.linear(o, self.o_proj.weight, residual=residual) if residual is not None \
                     else FN.linear(o, self.o_proj.weight)
@@ -243,7 +289,7 @@ class LlamaAttention(nn.Module):
         else:
             qk = _RopeFn.apply(torch.cat([q2, k2], -1), cos, sin, pos, nq + nkv, d, S)
         qkv = torch.cat([qk, v2], -1).contiguous()
-        o = causal_attention(qkv, B, S, nq, nkv, d)
+        o = self._attend(qkv, B, S, nq, nkv, d, attention)
         y = self.o_proj(o)
         return y + residual if residual is not None else y
 
@@ -323,7 +369,7 @@ class LlamaDecoderLayer(nn.Module):
 
     def forward(self, hidden_states: torch.Tensor, attention_mask=None, position_ids=None,
                 past_key_values=None, use_cache=False, position_embeddings=None,
-                batch_shape=None, **kwargs) -> torch.Tensor:
+                batch_shape=None, attention=None, **kwargs) -> torch.Tensor:
         shape = hidden_states.shape
         x = hidden_states.reshape(-1, shape[-1])
         if batch_shape is None:
@@ -334,7 +380,8 @@ class LlamaDecoderLayer(nn.Module):
             position_embeddings = (position_embeddings[0], position_embeddings[1], None)
         with nvtx_range(f"layer{self.layer_idx}"):
             n = self.input_layernorm(x)
-            h = self.self_attn(n, position_embeddings, batch_shape, residual=x)
+            h = self.self_attn(n, position_embeddings, batch_shape, residual=x,
+                               **({"attention": attention} if attention is not None else {}))
             if self.mlp_act8 and self._mlp8_applies(h):
                 m, norm = self.mlp, self.post_attention_layernorm
                 out = FN.NormMLP8Fn.apply(h, norm.weight, norm.variance_epsilon, 128, m.gate_proj.weight,

@@ -35,8 +35,10 @@ class LlamaForTraining(nn.Module):
         self.lm_head.weight = self.model.embed_tokens.weight
 
     def forward(self, input_ids: torch.Tensor, labels: torch.Tensor | None = None,
-                materialize_logits: bool | None = None) -> dict:
-        hidden = self.model(input_ids)
+                materialize_logits: bool | None = None, docs: torch.Tensor | None = None,
+                prefix: torch.Tensor | None = None) -> dict:
+        """``docs`` and ``prefix``: see ``LlamaPartialModel.forward``."""
+        hidden = self.model(input_ids, docs=docs, prefix=prefix)
         out: dict = {}
         if labels is not None:
             out["loss"] = lm_head_loss(self.lm_head, hidden, labels,

@@ -15,7 +15,9 @@ from __future__ import annotations
 import torch
 from torch import nn
 
-from .layers import LlamaDecoderLayer, LlamaRMSNorm, LlamaRotaryEmbedding
+from femtotron_b200.ops import masked_attention as MA
+
+from .layers import Attention, LlamaDecoderLayer, LlamaRMSNorm, LlamaRotaryEmbedding, attn_spec_of
 
 
 class LlamaPartialModel(nn.Module):
@@ -36,10 +38,14 @@ class LlamaPartialModel(nn.Module):
         self.layer_range = layer_range
         self.is_first = (layer_range.start == 0) if is_first is None else is_first
         self.is_last = (layer_range.stop == n_layers) if is_last is None else is_last
+        self.attn_spec = attn_spec_of(model_config)
+        scale = getattr(model_config, "embed_scale", None)
+        self.embed_scale = 1.0 if scale is None else float(scale)
         if self.is_first:
             self.embed_tokens = nn.Embedding(model_config.vocab_size, model_config.hidden_size,
                                              padding_idx=getattr(model_config, "pad_token_id", None),
                                              device=device, dtype=dtype)
+            self.embed_tokens.scale = self.embed_scale  # a vocabulary-parallel replacement takes it over
         self.layers = nn.ModuleDict({str(i): LlamaDecoderLayer(model_config, i, device=device, dtype=dtype)
                                      for i in layer_range})
         self.rotary_emb = LlamaRotaryEmbedding(model_config, device=device)
@@ -56,14 +62,33 @@ class LlamaPartialModel(nn.Module):
             return sp and ws > 1, ws
         return False, 1
 
+    def _attention(self, x: torch.Tensor, B: int, S: int, docs, prefix) -> Attention | None:
+        """What attention does beyond the causal mask in this batch, or None."""
+        spec = self.attn_spec or {"softcap": 0.0, "window": None, "alibi": False, "separator": None}
+        if docs is None and spec["separator"] is not None:
+            if not self.is_first:
+                raise NotImplementedError("documents are read off the input ids, which only the first pipeline stage has")
+            docs = MA.document_ids(x, spec["separator"])
+        if self.attn_spec is None and docs is None and prefix is None:
+            return None
+        mask = MA.attention_mask(B if docs is not None or prefix is not None else 1, S, window=spec["window"], docs=docs,
+                                 prefix=prefix, device=x.device)
+        slopes = MA.alibi_slopes(self.config.num_attention_heads, x.device) if spec["alibi"] else None
+        return Attention(mask, spec["softcap"], slopes)
+
     def forward(self, x: torch.Tensor, attention_mask: torch.Tensor | None = None,
-                position_ids: torch.Tensor | None = None, batch_shape=None) -> torch.Tensor:
+                position_ids: torch.Tensor | None = None, batch_shape=None, docs: torch.Tensor | None = None,
+                prefix: torch.Tensor | None = None) -> torch.Tensor:
+        """``docs`` and ``prefix`` [B, S]: documents, padding and prompts of the batch
+        (``ops/masked_attention.py``); without ``docs`` they follow from the config's separator."""
         if attention_mask is not None:
-            raise NotImplementedError("only causal attention without padding masks is supported")
+            raise NotImplementedError("attention_mask is not supported: documents and padding are given as docs")
         sp, tp = self._sequence_parallel()
         if self.is_first:
             B, S = x.shape
             h = self.embed_tokens(x)
+            if self.embed_scale != 1.0 and isinstance(self.embed_tokens, nn.Embedding):
+                h = h * self.embed_scale
         else:
             h = x
             if batch_shape is not None:
@@ -76,13 +101,15 @@ class LlamaPartialModel(nn.Module):
             # a plain embedding (not vocab-parallel) was used: shard tokens here
             from femtotron_b200.parallel.tensor_parallel.comm_ops import scatter_to_tp
             h = scatter_to_tp(h.reshape(-1, h.shape[-1]), self.layers[next(iter(self.layers))].self_attn.q_proj.group, 0)
+        attention = self._attention(x, B, S, docs, prefix)
+        extra = {} if attention is None else {"attention": attention}
         cos, sin = self.rotary_emb(h, position_ids=position_ids, seq_len=S)
         pos = None
         if position_ids is not None:
             pos = position_ids.expand(B, S).reshape(-1).to(torch.int32).contiguous()
         pe = (cos, sin, pos)
         for layer in self.layers.values():
-            h = layer(h, position_embeddings=pe, position_ids=position_ids, batch_shape=(B, S))
+            h = layer(h, position_embeddings=pe, position_ids=position_ids, batch_shape=(B, S), **extra)
         if self.is_last:
             h = self.norm(h)
         return h

@@ -14,7 +14,8 @@
              nothing
   window     keys less than ``window`` tokens away
 
-``masked_attention`` is differentiable in q, k and v.  On CUDA it runs ``csrc/masked_attn*.cu`` on bf16
+``masked_attention`` is differentiable in q, k and v (``masked_attention_packed`` in one projection that holds
+all three).  On CUDA it runs ``csrc/masked_attn*.cu`` on bf16
 tensors of any strides with a head size that is a multiple of 8 up to 128 (one that TMA does not
 take is copied first); its results and gradients are the same bits every time.  Beside the rows
 that see it, a NaN or an infinity of a token that is no padding may reach the rows of the 128-row tiles
@@ -154,19 +155,23 @@ def _forward_cpu(q, k, v, mask, scale, softcap, slopes):
     return qf, kf, vf, keep, lse, p
 
 
+def _forward(ctx, q, k, v, mask, scale, softcap, slopes, graded, *kept):
+    if q.is_cuda:
+        o, lse, low = native().masked_attn_fwd(q, k, v, mask.rows, mask.tiles, scale, softcap, slopes, graded,
+                                               error_flag(q.device))
+    else:
+        *_, vf, _, lse, p = _forward_cpu(q, k, v, mask, scale, softcap, slopes)
+        o, low = (p @ vf).transpose(1, 2).to(q.dtype).contiguous(), None
+    if graded:
+        ctx.save_for_backward(*kept, o, low, lse, mask.rows, mask.tiles, slopes)
+        ctx.meta = (mask.seq_len, scale, softcap)
+    return o
+
+
 class MaskedAttnFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, mask, scale, softcap, slopes, graded):
-        if q.is_cuda:
-            o, lse, low = native().masked_attn_fwd(q, k, v, mask.rows, mask.tiles, scale, softcap, slopes, graded,
-                                                   error_flag(q.device))
-        else:
-            *_, vf, _, lse, p = _forward_cpu(q, k, v, mask, scale, softcap, slopes)
-            o, low = (p @ vf).transpose(1, 2).to(q.dtype).contiguous(), None
-        if graded:
-            ctx.save_for_backward(q, k, v, o, low, lse, mask.rows, mask.tiles, slopes)
-            ctx.meta = (mask.seq_len, scale, softcap)
-        return o
+        return _forward(ctx, q, k, v, mask, scale, softcap, slopes, graded, q, k, v)
 
     @staticmethod
     def backward(ctx, do):
@@ -174,6 +179,27 @@ class MaskedAttnFn(torch.autograd.Function):
         dq, dk, dv = (torch.empty_like(x, memory_format=torch.contiguous_format) for x in (q, k, v))
         _backward(q, k, v, o, low, do, lse, rows, tiles, slopes, ctx.meta, dq, dk, dv)
         return dq, dk, dv, None, None, None, None, None
+
+
+def _heads(qkv, nq, nkv):
+    return qkv[:, :, :nq], qkv[:, :, nq:nq + nkv], qkv[:, :, nq + nkv:nq + 2 * nkv]
+
+
+class MaskedAttnPackedFn(torch.autograd.Function):
+    """MaskedAttnFn of one packed projection [batch, tokens, q heads | k heads | v heads, d], whose gradient
+    comes back in one piece too."""
+
+    @staticmethod
+    def forward(ctx, qkv, nq, nkv, mask, scale, softcap, slopes, graded):
+        ctx.heads = (nq, nkv)
+        return _forward(ctx, *_heads(qkv, nq, nkv), mask, scale, softcap, slopes, graded, qkv)
+
+    @staticmethod
+    def backward(ctx, do):
+        qkv, o, low, lse, rows, tiles, slopes = ctx.saved_tensors
+        d = torch.empty_like(qkv, memory_format=torch.contiguous_format)
+        _backward(*_heads(qkv, *ctx.heads), o, low, do, lse, rows, tiles, slopes, ctx.meta, *_heads(d, *ctx.heads))
+        return d, None, None, None, None, None, None, None
 
 
 def _backward(q, k, v, o, low, do, lse, rows, tiles, slopes, meta, dq, dk, dv):
@@ -241,3 +267,19 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: At
     graded = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
     slopes = slopes.detach().contiguous() if slopes is not None else None
     return MaskedAttnFn.apply(q, k, v, mask, scale, softcap, slopes, graded)
+
+
+def masked_attention_packed(qkv: torch.Tensor, heads: int, key_heads: int, mask: AttentionMask, *,
+                            scale: float | None = None, softcap: float = 0.0,
+                            slopes: torch.Tensor | None = None) -> torch.Tensor:
+    """``masked_attention`` of a packed projection [batch, tokens, heads + 2 key_heads, d]."""
+    if qkv.dim() != 4 or heads < 1 or key_heads < 1 or qkv.shape[2] != heads + 2 * key_heads:
+        raise ValueError(f"masked_attention_packed: {tuple(qkv.shape)} does not hold {heads} + 2 x {key_heads} heads")
+    scale = 1.0 / math.sqrt(qkv.shape[-1]) if scale is None else float(scale)
+    softcap = float(softcap)
+    _check(*_heads(qkv, heads, key_heads), mask, scale, softcap, slopes)
+    if qkv.numel() == 0:
+        return torch.zeros_like(qkv[:, :, :heads]) + 0 * qkv.sum()
+    graded = torch.is_grad_enabled() and qkv.requires_grad
+    slopes = slopes.detach().contiguous() if slopes is not None else None
+    return MaskedAttnPackedFn.apply(qkv, heads, key_heads, mask, scale, softcap, slopes, graded)

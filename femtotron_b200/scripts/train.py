@@ -16,7 +16,9 @@ synthetic_data (uniform random tokens instead of a tokenised dataset), seed, met
 for long sequences loss_keep_logits (false: the loss without its logits in memory), ac_bits (8:
 activation checkpoints in 8 bits), mlp_act8 (true: the MLP blocks keep 8-bit activations) and
 rope_scaling (a dict such as {rope_type: linear, factor: 4}, or "config" for the one of
-model_name's configuration), rope_partial, rope_interleaved.
+model_name's configuration), rope_partial, rope_interleaved; for packed documents doc_separator (the token
+id that ends a document: attention stays within documents), attn_window, attn_softcap, attn_alibi and
+embed_scale.
 
 Unlike the reference script, pipeline parallelism (pp > 1) builds a PipelineRunner, gradient
 clipping and gradient accumulation are applied, and the vocabulary comes from the config
@@ -57,15 +59,16 @@ def parse_args(argv=None):
               "num_attention_heads", "num_key_value_heads", "vocab_size", "max_position_embeddings",
               "train_steps", "micro_batch_size",
               "seq_len", "warmup_steps", "num_samples", "log_interval", "checkpoint_interval",
-              "grad_accum_steps", "num_microbatches", "seed", "ac_bits"):
+              "grad_accum_steps", "num_microbatches", "seed", "ac_bits", "doc_separator", "attn_window"):
         p.add_argument(f"--{k}", type=int, default=None)
     for k in ("lr", "grad_clip", "weight_decay", "min_lr_ratio", "init_std", "rope_theta", "rms_norm_eps",
-              "rope_partial"):
+              "rope_partial", "attn_softcap", "embed_scale"):
         p.add_argument(f"--{k}", type=float, default=None)
     for k in ("zero_wrap_policy", "ac_policy", "model_name", "dataset", "checkpoint_dir", "resume",
               "schedule", "metrics_path", "data_dir", "tokenizer"):
         p.add_argument(f"--{k}", type=str, default=None)
-    for k in ("ac_enabled", "sequence_parallel", "synthetic_data", "loss_keep_logits", "mlp_act8", "rope_interleaved"):
+    for k in ("ac_enabled", "sequence_parallel", "synthetic_data", "loss_keep_logits", "mlp_act8", "rope_interleaved",
+              "attn_alibi"):
         # `--ac_enabled true|false` as in the reference's CLI, or the bare flag for true
         p.add_argument(f"--{k}", type=_bool, nargs="?", const=True, default=None)
     return p.parse_args(argv)
@@ -83,7 +86,8 @@ DEFAULTS = dict(tp=1, pp=1, zero_stage=0, zero_wrap_policy="llama_decoder_layer"
                 schedule="1f1b", sequence_parallel=False, rope_theta=10000.0, rms_norm_eps=1e-5,
                 synthetic_data=True, seed=1234, metrics_path=None, data_dir="./data", dataset=None,
                 tokenizer=None, loss_keep_logits=True, ac_bits=16, mlp_act8=False, rope_scaling=None,
-                rope_partial=1.0, rope_interleaved=False)
+                rope_partial=1.0, rope_interleaved=False,
+                doc_separator=None, attn_window=None, attn_softcap=0.0, attn_alibi=False, embed_scale=1.0)
 
 
 def load_config(args) -> dict:
@@ -120,6 +124,14 @@ def model_config_from(cfg: dict):
     partial, interleaved = cfg.get("rope_partial", 1.0), cfg.get("rope_interleaved", False)
     if scaling is not None or partial != 1.0 or interleaved:
         mc.rotary_spec = {"scaling": scaling, "partial": partial, "interleaved": interleaved}
+    spec = {"softcap": cfg.get("attn_softcap", 0.0), "window": cfg.get("attn_window"),
+            "alibi": cfg.get("attn_alibi", False), "separator": cfg.get("doc_separator")}
+    if spec["softcap"] or spec["window"] is not None or spec["alibi"] or spec["separator"] is not None:
+        if spec["separator"] is not None and cfg.get("pp", 1) > 1:
+            raise ValueError("doc_separator: the stages of a pipeline behind the first one do not see the documents")
+        mc.attn_spec = spec
+    if cfg.get("embed_scale", 1.0) != 1.0:
+        mc.embed_scale = cfg["embed_scale"]
     return mc
 
 

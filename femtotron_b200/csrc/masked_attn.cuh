@@ -10,6 +10,11 @@ namespace ft {
 namespace ma {
 
 // ------------------------------------------------------------------------------ shared device parts
+// A value that all lanes of the warp share, in a form that the compiler knows to be so: what branches and descriptors are
+// made of then stays in uniform registers (without it every product of the MMA warp waited for six moves into them: 110
+// clocks where the product takes 32 to 64).
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+
 __device__ __forceinline__ uint64_t clock_ns() {
   uint64_t t;
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
@@ -36,24 +41,33 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, int* e
   return __all_sync(0xffffffffu, wait_phase(bar, parity, err, code));
 }
 
-// tcgen05.mma by the lanes where `on` is not 0 (one of the warp).  The predicate is the instruction's own: with a branch
-// around each, issuing took 115 clocks per 128 x 128 x 16 product instead of the 64 that the product takes.
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add, uint32_t on) {
+// tcgen05.mma by the lanes where `on` is not 0 (one of the warp).  Operands in shared memory come as the low word of their
+// descriptor (address and leading offset), which grows by a constant from product to product; the high word is the
+// same for all tiles here (128-byte swizzle, 1024 bytes between groups of 8 rows).  The predicate is the
+// instruction's own.  What stands between two products counts: one of 64 columns takes 32 to 48 clocks.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_low(uint32_t addr, uint32_t leading) {
+  return ((addr >> 4) & 0x3FFFu) | ((leading >> 4) << 16);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t add, uint32_t on) {
   asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 x, y;\n\t"
+      "mov.b64 x, {%1, %6};\n\t"
+      "mov.b64 y, {%2, %6};\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
       "setp.ne.b32 q, %5, 0;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(add), "r"(on)
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(add), "r"(on), "n"(kDescHigh)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add, uint32_t on) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t add, uint32_t on) {
   asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 y;\n\t"
+      "mov.b64 y, {%2, %6};\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
       "setp.ne.b32 q, %5, 0;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(add), "r"(on)
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(add), "r"(on), "n"(kDescHigh)
       : "memory");
 }
 __device__ __forceinline__ void commit(uint64_t* bar, uint32_t on) {
@@ -65,22 +79,27 @@ __device__ __forceinline__ void commit(uint64_t* bar, uint32_t on) {
       : "memory");
 }
 
-// dst = A B^T of two K-major tiles, 16 values of d at a time (those past ksteps are not there)
-__device__ __forceinline__ void mma_tiles(uint32_t dst, uint32_t a, uint32_t b, uint32_t idesc, int ksteps, uint32_t on) {
+// Bytes between the two 64-value pieces of a tile of 128 and of STEP rows
+constexpr uint32_t PIECE = TILE * 128, STEP_PIECE = STEP * 128;
+
+// dst = A B^T of a tile of 128 rows and one of STEP rows, 16 values of d at a time; a, b: desc_low(tile, 16)
+__device__ __forceinline__ void mma_scores(uint32_t dst, uint32_t a, uint32_t b, int ksteps, uint32_t on) {
+  constexpr uint32_t idesc = make_idesc_bf16(TILE, STEP, false, false);
 #pragma unroll
   for (int kk = 0; kk < HEAD / 16; ++kk) {
-    const uint32_t off = (kk >> 2) * 128 * 128 + (kk & 3) * 32;
-    mma_ss(dst, make_sw128_desc(a + off, 16, 1024), make_sw128_desc(b + off, 16, 1024), idesc, kk > 0, kk < ksteps ? on : 0u);
+    if (kk >= ksteps) break;
+    mma_ss(dst, a + (((kk >> 2) * PIECE + (kk & 3) * 32) >> 4), b + (((kk >> 2) * STEP_PIECE + (kk & 3) * 32) >> 4), idesc,
+           kk > 0, on);
   }
 }
 
-template <int N>
-__device__ __forceinline__ void more_registers() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void fewer_registers() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+// dst (+)= A B with A in TMEM (bf16 pairs: 16 values in 8 columns, and `jump` columns from one 32 to the next) and the STEP
+// rows of B; b: desc_low(tile, STEP_PIECE)
+__device__ __forceinline__ void mma_values(uint32_t dst, uint32_t a, int jump, uint32_t b, uint32_t idesc, bool add,
+                                           uint32_t on) {
+#pragma unroll
+  for (int kk = 0; kk < STEP / 16; ++kk)
+    mma_ts(dst, a + (kk >> 1) * jump + (kk & 1) * 8, b + (kk * 2048 >> 4), idesc, (add || kk > 0) ? 1u : 0u, on);
 }
 
 // Two fp32 operations in one instruction
@@ -158,15 +177,15 @@ __device__ __forceinline__ float score(float s, const Common& p, float slope2, f
   return ALIBI ? fmaf(-slope2, fabsf(dist), y) : y;
 }
 
-// Zero the rows of a tile (`chunks` pieces of [128 rows][128 bytes]) that see nothing; one warp.  The
-// swizzle permutes within a row's 128 bytes only.
+// Zero the rows that see nothing of a tile of STEP rows (`chunks` pieces of 128 bytes a row); one warp.  The swizzle
+// permutes within a row's 128 bytes only.
 __device__ __forceinline__ void zero_dead_rows(void* tile, int chunks, const int2* rows, int lane) {
-  for (int r = lane; r < TILE; r += 32)
+  for (int r = lane; r < STEP; r += 32)
     if (rows[r].y == 0)
       for (int c = 0; c < chunks; ++c) {
-        uint4* at = reinterpret_cast<uint4*>(static_cast<uint8_t*>(tile) + c * 16384 + r * 128);
+        uint4* to = reinterpret_cast<uint4*>(static_cast<uint8_t*>(tile) + c * STEP_PIECE + r * 128);
 #pragma unroll
-        for (int u = 0; u < 8; ++u) at[u] = make_uint4(0, 0, 0, 0);
+        for (int u = 0; u < 8; ++u) to[u] = make_uint4(0, 0, 0, 0);
       }
 }
 

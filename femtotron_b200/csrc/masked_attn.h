@@ -35,18 +35,9 @@ namespace ma {
 
 constexpr int TILE = 128;
 constexpr int HEAD = 128;  // values of a head that a tile has room for
-// Three groups of four warps: 8 compute warps, a TMA warp, an MMA warp and two that only hand their registers
-// over.  Launched with 168 registers a thread (64512 in all), of which the kernels move some from the last group
-// to the compute warps: a row of scores stays in registers.
-constexpr int NTHREADS = 384;
+constexpr int STEP = 64;   // keys (or, for dk and dv, queries) that a step of a kernel takes
+constexpr int NTHREADS = 320;  // 8 compute warps, 1 TMA warp, 1 MMA warp
 constexpr int PRODUCER_WARP = 8, MMA_WARP = 9, COMPUTE_WARPS = 8;
-template <int COMPUTE, int OTHER>
-struct Registers {
-  static constexpr int compute = COMPUTE, other = OTHER;
-  static_assert(256 * COMPUTE + 128 * OTHER <= NTHREADS * 168, "more registers than the launch has");
-};
-using FwdRegisters = Registers<224, 56>;
-using BwdRegisters = Registers<216, 72>;
 constexpr int MAX_TILES = 2048;  // 262144 tokens: the tiles that meet a tile are listed in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kNever = 0x7fffffff;  // lo of a row that sees nothing; its hi is 0

@@ -5,18 +5,19 @@ namespace ft {
 namespace ma {
 
 // ------------------------------------------------------------------------------ backward: dk, dv
-// One block per 128 keys of a key head; the query tiles that see any of them go past, for every query head
-// of the group, so dk and dv are complete in TMEM.  S^T = K Q^T and dP^T = V dO^T (rows are keys); P^T and
-// dS^T go over them as bf16 pairs and are the left operands of dv += P^T dO and dk += dS^T Q.  The order
-// dv_i, S_i+1, dk_i, dP_i+1 lets the exponentials of one tile run under the products of its neighbours.
-constexpr int Q_STAGES = 2;
+// One block per 128 keys of a key head; the query tiles that see any of them go past, 64 queries at a time, for every
+// query head of the group (or the block's share of them), so dk and dv are complete in TMEM.  S^T = K Q^T and
+// dP^T = V dO^T (rows are keys); P^T and dS^T go over them as bf16 pairs and are the left operands of dv += P^T dO and
+// dk += dS^T Q.  S and dP have two buffers each, so the products of one step run under the exponentials of another:
+// with one buffer of 128 queries the two took turns (3320 clocks per 128 x 128 block).
+constexpr int Q_STAGES = 4;
 
 struct DkvSmem {
-  __nv_bfloat16 k[TILE * HEAD], v[TILE * HEAD], q[Q_STAGES][TILE * HEAD], dout[Q_STAGES][TILE * HEAD];
-  int2 rows[Q_STAGES][TILE];
-  float neg_lse2[Q_STAGES][TILE], neg_delta[Q_STAGES][TILE];
-  uint64_t kv_full, q_full[Q_STAGES], q_empty[Q_STAGES], do_full[Q_STAGES], do_empty[Q_STAGES], clean;
-  uint64_t s_full, dp_full, p_full, ds_full, done, drained;
+  __nv_bfloat16 k[TILE * HEAD], v[TILE * HEAD], q[Q_STAGES][STEP * HEAD], dout[Q_STAGES][STEP * HEAD];
+  int2 rows[Q_STAGES][STEP];
+  float neg_lse2[Q_STAGES][STEP], neg_delta[Q_STAGES][STEP];
+  uint64_t kv_full, full[Q_STAGES], empty[Q_STAGES], landed;
+  uint64_t sp_full[2], pd_full[2], done, drained;
   uint16_t list[MAX_TILES];  // query tiles that see a key of this block; bit 14: elements need a test, 15: dead rows
   int count;
   uint32_t tmem_base;
@@ -30,9 +31,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   using Sm = DkvSmem;
   extern __shared__ uint8_t smem_raw[];
   Sm& s = *reinterpret_cast<Sm*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int chunks = p.d > 64 ? 2 : 1;  // pieces of 64 values that a head has
-  const uint32_t tile_bytes = chunks * TILE * 64 * 2;
   // early key tiles (seen by the most rows of a causal mask) first
   const int bk = blockIdx.x / p.split, sp = blockIdx.x % p.split, jt = blockIdx.y;
   const int b = bk / p.nkv, kvh = bk % p.nkv, heads = p.group / p.split, head0 = kvh * p.group + sp * heads;
@@ -42,17 +42,9 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 
   if (threadIdx.x == 0) {
     mbar_init(&s.kv_full, 1);
-    for (int i = 0; i < Q_STAGES; ++i) {
-      mbar_init(&s.q_full[i], 1);
-      mbar_init(&s.q_empty[i], 1);
-      mbar_init(&s.do_full[i], 1);
-      mbar_init(&s.do_empty[i], 1);
-    }
-    mbar_init(&s.clean, 1);
-    mbar_init(&s.s_full, 1);
-    mbar_init(&s.dp_full, 1);
-    mbar_init(&s.p_full, 8);
-    mbar_init(&s.ds_full, 8);
+    for (int i = 0; i < Q_STAGES; ++i) mbar_init(&s.full[i], 1), mbar_init(&s.empty[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&s.sp_full[i], 1), mbar_init(&s.pd_full[i], COMPUTE_WARPS);
+    mbar_init(&s.landed, 1);
     mbar_init(&s.done, 1);
     mbar_init(&s.drained, 1);
     fence_barrier_init();
@@ -80,113 +72,83 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   __syncthreads();
   tc_fence_after();
   constexpr uint32_t tmem = 0;  // where an allocation of all 512 columns begins
-  const uint32_t tS = tmem, tdP = tmem + 128, tdV = tmem + 256, tdK = tmem + 384;
-  const int count = s.count, n = count * heads;
+  auto tS = [](int buf) -> uint32_t { return tmem + static_cast<uint32_t>(buf) * 64u; };
+  auto tdP = [](int buf) -> uint32_t { return tmem + 128u + static_cast<uint32_t>(buf) * 64u; };
+  constexpr uint32_t tdV = tmem + 256, tdK = tmem + 384;
+  const int count = uniform(s.count), n = count * heads * (TILE / STEP);  // steps: the halves of the tiles, head by head
 
   if (warp < COMPUTE_WARPS) {
-    more_registers<BwdRegisters::compute>();
-    // two warps per TMEM lane quadrant (32 keys), 64 of the 128 queries each
+    // two warps per TMEM lane quadrant (32 keys), 32 of the 64 queries each
     const int quad = warp & 3, half = warp >> 2;
     const int key = k0 + quad * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quad * 32) << 16;
-    const uint32_t ts = tS + lane_off + half * 64, td = tdP + lane_off + half * 64;
+    const uint64_t mul = pair(p.scale_log2, p.scale_log2);
     bool ok = true;
-    for (int it = 0; it < n && ok; ++it) {
-      const int st = it % Q_STAGES, entry = s.list[it % count], i = entry & 0x3fff;
+    for (int it = 0; it < n; ++it) {
+      const int st = it % Q_STAGES, buf = it & 1, tile = it / 2, entry = s.list[tile % count];
+      const int q0 = (entry & 0x3fff) * TILE + (it & 1) * STEP + half * 32;
       const bool test = entry & 0x4000;
-      const float slope2 = ALIBI ? p.slopes[head0 + it / count] * kLog2e : 0.f;
-      const float far = static_cast<float>(key - i * TILE - half * 64);
+      const float slope2 = ALIBI ? p.slopes[head0 + tile / count] * kLog2e : 0.f;
+      const float far = static_cast<float>(key - q0);
+      const uint32_t ts = tS(buf) + lane_off + half * 32, td = tdP(buf) + lane_off + half * 32;
       // the statistics of the queries come into registers while S is still in work: between the products'
       // operand reads, shared memory answers late
-      ok = wait_warp(&s.q_full[st], (it / Q_STAGES) & 1, p.err, 365);
+      ok = wait_warp(&s.full[st], (it / Q_STAGES) & 1, p.err, 365);
       if (!ok) break;
-      float4 L[16], Dl[16];
+      float4 L[8], Dl[8];
 #pragma unroll
-      for (int c4 = 0; c4 < 16; ++c4) L[c4] = reinterpret_cast<const float4*>(s.neg_lse2[st] + half * 64)[c4];
+      for (int i = 0; i < 8; ++i) L[i] = reinterpret_cast<const float4*>(s.neg_lse2[st] + half * 32)[i];
 #pragma unroll
-      for (int c4 = 0; c4 < 16; ++c4) Dl[c4] = reinterpret_cast<const float4*>(s.neg_delta[st] + half * 64)[c4];
-      ok = wait_warp(&s.s_full, it & 1, p.err, 362);
-      if (!ok) break;
-      tc_fence_after();
-      float pv[64];
-      {
-        uint32_t sv[64];
-        tmem_ld_32x32b_x32(ts, *reinterpret_cast<uint32_t(*)[32]>(sv));
-        tmem_ld_32x32b_x32(ts + 32, *reinterpret_cast<uint32_t(*)[32]>(sv + 32));
-        tmem_wait_ld();
-        const int4* R = reinterpret_cast<const int4*>(s.rows[st] + half * 64);
-        const uint64_t mul = pair(p.scale_log2, p.scale_log2);
-        float kp[CAP ? 64 : 1];
-#pragma unroll
-        for (int e = 0; e < 64; e += 2) {
-          const float2 l = e & 2 ? make_float2(L[e / 4].z, L[e / 4].w) : make_float2(L[e / 4].x, L[e / 4].y);
-          float2 y, keep = make_float2(1.f, 1.f);
-          if (!CAP && !ALIBI) {
-            y = apart(fma2(pair(__uint_as_float(sv[e]), __uint_as_float(sv[e + 1])), mul, pair(l.x, l.y)));
-          } else {
-            y.x = score<CAP, ALIBI>(__uint_as_float(sv[e]), p, slope2, far - e, keep.x) + l.x;
-            y.y = score<CAP, ALIBI>(__uint_as_float(sv[e + 1]), p, slope2, far - (e + 1), keep.y) + l.y;
-          }
-          y = exp2_of(y, e / 2);
-          pv[e] = y.x;
-          pv[e + 1] = y.y;
-          if (CAP) kp[e] = keep.x, kp[e + 1] = keep.y;
-        }
-        if (test) {
-#pragma unroll
-          for (int e = 0; e < 64; e += 2) {
-            const int4 two = R[e / 2];  // rows e and e + 1: (lo, hi, lo, hi)
-            if (key < two.x || key >= two.y) pv[e] = 0.f;
-            if (key < two.z || key >= two.w) pv[e + 1] = 0.f;
-          }
-        }
-#pragma unroll
-        for (int h32 = 0; h32 < 2; ++h32) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) pk[i] = pack_bf16x2(pv[h32 * 32 + 2 * i], pv[h32 * 32 + 2 * i + 1]);
-          tmem_st_32x32b_x16(ts + h32 * 16, pk);
-        }
-        if (CAP) {
-#pragma unroll
-          for (int e = 0; e < 64; ++e) pv[e] *= kp[CAP ? e : 0];
-        }
-      }
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&s.p_full);
-      ok = wait_warp(&s.dp_full, it & 1, p.err, 363);
+      for (int i = 0; i < 8; ++i) Dl[i] = reinterpret_cast<const float4*>(s.neg_delta[st] + half * 32)[i];
+      ok = wait_warp(&s.sp_full[buf], (it >> 1) & 1, p.err, 362);
       if (!ok) break;
       tc_fence_after();
-      uint32_t dv[64];
-      tmem_ld_32x32b_x32(td, *reinterpret_cast<uint32_t(*)[32]>(dv));
-      tmem_ld_32x32b_x32(td + 32, *reinterpret_cast<uint32_t(*)[32]>(dv + 32));
+      uint32_t sv[32], dv[32], pk[16];
+      tmem_ld_32x32b_x32(ts, sv);
+      tmem_ld_32x32b_x32(td, dv);
       tmem_wait_ld();
+      float keeps[CAP ? 32 : 1];
 #pragma unroll
-      for (int e = 0; e < 64; e += 2) {
+      for (int e = 0; e < 32; e += 2) {
+        const float2 l = e & 2 ? make_float2(L[e / 4].z, L[e / 4].w) : make_float2(L[e / 4].x, L[e / 4].y);
+        float2 y, keep = make_float2(1.f, 1.f);
+        if (!CAP && !ALIBI) {
+          y = apart(fma2(pair(__uint_as_float(sv[e]), __uint_as_float(sv[e + 1])), mul, pair(l.x, l.y)));
+        } else {
+          y.x = score<CAP, ALIBI>(__uint_as_float(sv[e]), p, slope2, far - e, keep.x) + l.x;
+          y.y = score<CAP, ALIBI>(__uint_as_float(sv[e + 1]), p, slope2, far - (e + 1), keep.y) + l.y;
+        }
+        y = exp2_of(y, e / 2);
+        sv[e] = __float_as_uint(y.x);
+        sv[e + 1] = __float_as_uint(y.y);
+        if (CAP) keeps[e] = keep.x, keeps[e + 1] = keep.y;
+      }
+      if (test) {
+        const int4* R = reinterpret_cast<const int4*>(s.rows[st] + half * 32);
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          const int4 two = R[e / 2];  // rows e and e + 1: (lo, hi, lo, hi)
+          // a masked place may hold NaN in dP too
+          if (key < two.x || key >= two.y) sv[e] = 0u, dv[e] = 0u;
+          if (key < two.z || key >= two.w) sv[e + 1] = 0u, dv[e + 1] = 0u;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) pk[i] = pack_bf16x2(__uint_as_float(sv[2 * i]), __uint_as_float(sv[2 * i + 1]));
+      tmem_st_32x32b_x16(ts, pk);
+#pragma unroll
+      for (int e = 0; e < 32; e += 2) {
         const uint64_t nd = e & 2 ? pair(Dl[e / 4].z, Dl[e / 4].w) : pair(Dl[e / 4].x, Dl[e / 4].y);
-        const float2 g = apart(mul2(pair(pv[e], pv[e + 1]), add2(pair(__uint_as_float(dv[e]), __uint_as_float(dv[e + 1])), nd)));
-        dv[e] = __float_as_uint(g.x);
-        dv[e + 1] = __float_as_uint(g.y);
+        uint64_t w = pair(__uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
+        if (CAP) w = mul2(w, pair(keeps[CAP ? e : 0], keeps[CAP ? e + 1 : 0]));
+        const float2 g = apart(mul2(w, add2(pair(__uint_as_float(dv[e]), __uint_as_float(dv[e + 1])), nd)));
+        pk[e / 2] = pack_bf16x2(g.x, g.y);
       }
-      if (test) {  // a masked place may hold NaN
-#pragma unroll
-        for (int e = 0; e < 64; ++e)
-          if (pv[e] == 0.f) dv[e] = 0u;
-      }
-#pragma unroll
-      for (int h32 = 0; h32 < 2; ++h32) {
-        uint32_t pk[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          pk[i] = pack_bf16x2(__uint_as_float(dv[h32 * 32 + 2 * i]), __uint_as_float(dv[h32 * 32 + 2 * i + 1]));
-        tmem_st_32x32b_x16(td + h32 * 16, pk);
-      }
+      tmem_st_32x32b_x16(td, pk);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&s.ds_full);
+      if (lane == 0) mbar_arrive(&s.pd_full[buf]);
     }
     if (n > 0 && ok) ok = wait_warp(&s.done, 0, p.err, 364);
     if (ok) {
@@ -218,110 +180,82 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         }
       }
     }
-  } else {
-    fewer_registers<BwdRegisters::other>();
-    if (warp == PRODUCER_WARP) {
-      if (n > 0) {
-        auto load = [&](__nv_bfloat16* dst, const CUtensorMap* tm, uint64_t* bar, int head, int tile) {
-          for (int c = 0; c < chunks; ++c) tma_load_4d(dst + c * 128 * 64, tm, bar, c * 64, head, tile * TILE, b);
-        };
+  } else if (warp == PRODUCER_WARP) {
+    if (n > 0) {
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&s.kv_full, 2 * chunks * PIECE);
+        for (int c = 0; c < chunks; ++c) {
+          tma_load_4d(s.k + c * TILE * 64, &tm_k, &s.kv_full, c * 64, kvh, k0, b);
+          tma_load_4d(s.v + c * TILE * 64, &tm_v, &s.kv_full, c * 64, kvh, k0, b);
+        }
+      }
+      bool ok = true;
+      int got = 0, n_dead = 0;
+      for (int it = 0; it < n && ok; ++it) {
+        const int st = it % Q_STAGES, ph = (it / Q_STAGES) & 1, tile = it / 2, entry = s.list[tile % count];
+        const int h = head0 + tile / count, q0 = (entry & 0x3fff) * TILE + (it & 1) * STEP;
+        ok = wait_warp(&s.empty[st], ph ^ 1, p.err, 351);
+        if (!ok) break;
+        // rows that see nothing are zeroed before the products sum over them
+        const bool dead = entry & 0x8000;
+        uint64_t* bar = dead ? &s.landed : &s.full[st];
         if (lane == 0) {
-          mbar_arrive_expect_tx(&s.kv_full, 2 * tile_bytes);
-          load(s.k, &tm_k, &s.kv_full, kvh, jt);
-          load(s.v, &tm_v, &s.kv_full, kvh, jt);
-        }
-        bool ok = true;
-        int nq = 0, nd = 0;
-        for (int it = 0; it < n && ok; ++it) {
-          const int st = it % Q_STAGES, ph = (it / Q_STAGES) & 1;
-          const int h = head0 + it / count, entry = s.list[it % count], i = entry & 0x3fff;
-          ok = wait_warp(&s.q_empty[st], ph ^ 1, p.err, 351);
-          if (!ok) break;
-          if (lane == 0) {
-            const int64_t stat = (static_cast<int64_t>(b) * p.nq + h) * p.padded + i * TILE;
-            mbar_arrive_expect_tx(&s.q_full[st], tile_bytes + TILE * 16);
-            load(s.q[st], &tm_q, &s.q_full[st], h, i);
-            bulk_load(s.rows[st], rows + i * TILE, TILE * 8, &s.q_full[st]);
-            bulk_load(s.neg_lse2[st], p.neg_lse2 + stat, TILE * 4, &s.q_full[st]);
-            bulk_load(s.neg_delta[st], p.neg_delta + stat, TILE * 4, &s.q_full[st]);
+          const int64_t stat = (static_cast<int64_t>(b) * p.nq + h) * p.padded + q0;
+          mbar_arrive_expect_tx(bar, 2 * chunks * STEP_PIECE + STEP * 16);
+          for (int c = 0; c < chunks; ++c) {
+            tma_load_4d(s.q[st] + c * STEP * 64, &tm_q, bar, c * 64, h, q0, b);
+            tma_load_4d(s.dout[st] + c * STEP * 64, &tm_do, bar, c * 64, h, q0, b);
           }
-          ++nq;
+          bulk_load(s.rows[st], rows + q0, STEP * 8, bar);
+          bulk_load(s.neg_lse2[st], p.neg_lse2 + stat, STEP * 4, bar);
+          bulk_load(s.neg_delta[st], p.neg_delta + stat, STEP * 4, bar);
+        }
+        ++got;
+        __syncwarp();
+        if (dead) {
+          ok = wait_warp(&s.landed, n_dead++ & 1, p.err, 353);
+          zero_dead_rows(s.q[st], chunks, rows + q0, lane);
+          zero_dead_rows(s.dout[st], chunks, rows + q0, lane);
+          fence_proxy_async_smem();
           __syncwarp();
-          ok = wait_warp(&s.do_empty[st], ph ^ 1, p.err, 352);
-          if (!ok) break;
-          if (lane == 0) {
-            mbar_arrive_expect_tx(&s.do_full[st], tile_bytes);
-            load(s.dout[st], &tm_do, &s.do_full[st], h, i);
-          }
-          ++nd;
-          __syncwarp();
-          if (entry & 0x8000) {
-            ok = wait_warp(&s.q_full[st], ph, p.err, 353) && wait_warp(&s.do_full[st], ph, p.err, 353);
-            zero_dead_rows(s.q[st], chunks, rows + i * TILE, lane);
-            zero_dead_rows(s.dout[st], chunks, rows + i * TILE, lane);
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&s.clean);
-          }
+          if (lane == 0) mbar_arrive(&s.full[st]);
         }
-        // the copies have landed before the block may leave, also after a wait that ran out
-        wait_phase(&s.kv_full, 0, p.err, 354);
-        for (int i = max(0, nq - Q_STAGES); i < nq; ++i)
-          wait_phase(&s.q_full[i % Q_STAGES], (i / Q_STAGES) & 1, p.err, 354);
-        for (int i = max(0, nd - Q_STAGES); i < nd; ++i)
-          wait_phase(&s.do_full[i % Q_STAGES], (i / Q_STAGES) & 1, p.err, 354);
       }
-    } else if (warp == MMA_WARP) {
-      if (n > 0) {
-        // The whole warp goes through the loop, so that descriptors are made in uniform registers; one lane issues.
-        const uint32_t leader = elect_one();
-        const uint32_t idS = make_idesc_bf16(128, TILE, false, false);
-        const uint32_t idKV = make_idesc_bf16(128, p.ksteps * 16, false, true);
-        int n_clean = 0;
-        auto gather = [&](uint32_t dst, uint32_t a, uint32_t bb, bool more) {
-          // queries 0..63 in columns 0..31, 64..127 in 64..95
-#pragma unroll
-          for (int kk = 0; kk < TILE / 16; ++kk)
-            mma_ts(dst, a + (kk >> 2) * 64 + (kk & 3) * 8, make_sw128_desc(bb + kk * 2048, 128 * 128, 1024), idKV,
-                        (more || kk > 0) ? 1u : 0u, leader);
-        };
-        auto issue_s = [&](int it) -> bool {
-          const int st = it % Q_STAGES;
-          if (!wait_warp(&s.q_full[st], (it / Q_STAGES) & 1, p.err, 355)) return false;
-          if ((s.list[it % count] & 0x8000) && !wait_warp(&s.clean, n_clean++ & 1, p.err, 356)) return false;
-          tc_fence_after();
-          mma_tiles(tS, smem_u32(s.k), smem_u32(s.q[st]), idS, p.ksteps, leader);
-          commit(&s.s_full, leader);
-          return true;
-        };
-        auto issue_dp = [&](int it) -> bool {
-          const int st = it % Q_STAGES;
-          if (!wait_warp(&s.do_full[st], (it / Q_STAGES) & 1, p.err, 357)) return false;
-          tc_fence_after();
-          mma_tiles(tdP, smem_u32(s.v), smem_u32(s.dout[st]), idS, p.ksteps, leader);
-          commit(&s.dp_full, leader);
-          return true;
-        };
-        bool ok = wait_warp(&s.kv_full, 0, p.err, 358) && issue_s(0) && issue_dp(0);
-        for (int it = 0; ok && it < n; ++it) {
-          const int st = it % Q_STAGES;
-          ok = wait_warp(&s.p_full, it & 1, p.err, 359);
-          if (!ok) break;
-          tc_fence_after();
-          gather(tdV, tS, smem_u32(s.dout[st]), it > 0);
-          commit(&s.do_empty[st], leader);
-          if (it + 1 < n) ok = issue_s(it + 1);
-          ok = ok && wait_warp(&s.ds_full, it & 1, p.err, 360);
-          if (!ok) break;
-          tc_fence_after();
-          gather(tdK, tdP, smem_u32(s.q[st]), it > 0);
-          commit(&s.q_empty[st], leader);
-          if (it + 1 < n) ok = issue_dp(it + 1);
-        }
-        commit(ok ? &s.done : &s.drained, leader);
-        if (!ok) wait_warp(&s.drained, 0, p.err, 361);
-      }
+      // the copies have landed before the block may leave, also after a wait that ran out
+      wait_phase(&s.kv_full, 0, p.err, 354);
+      for (int i = max(0, got - Q_STAGES); i < got; ++i) wait_phase(&s.full[i % Q_STAGES], (i / Q_STAGES) & 1, p.err, 354);
     }
+  } else if (n > 0) {
+    // The whole warp goes through the loop, so that descriptors are made in uniform registers; one lane issues.
+    const uint32_t leader = elect_one();
+    const uint32_t idKV = make_idesc_bf16(TILE, p.ksteps * 16, false, true);
+    const uint32_t ka = desc_low(smem_u32(s.k), 16), va = desc_low(smem_u32(s.v), 16);
+    const uint32_t qa = desc_low(smem_u32(s.q[0]), 16), da = desc_low(smem_u32(s.dout[0]), 16);
+    const uint32_t qt = desc_low(smem_u32(s.q[0]), STEP_PIECE), dt = desc_low(smem_u32(s.dout[0]), STEP_PIECE);
+    constexpr uint32_t stage = STEP * HEAD * 2 >> 4;
+    auto issue = [&](int it) -> bool {
+      const int st = it % Q_STAGES, buf = it & 1;
+      if (!wait_warp(&s.full[st], (it / Q_STAGES) & 1, p.err, 355)) return false;
+      tc_fence_after();
+      mma_scores(tS(buf), ka, qa + st * stage, p.ksteps, leader);
+      mma_scores(tdP(buf), va, da + st * stage, p.ksteps, leader);
+      commit(&s.sp_full[buf], leader);
+      return true;
+    };
+    bool ok = wait_warp(&s.kv_full, 0, p.err, 358) && issue(0) && issue(1);
+    for (int it = 0; ok && it < n; ++it) {
+      const int st = it % Q_STAGES, buf = it & 1;
+      ok = wait_warp(&s.pd_full[buf], (it >> 1) & 1, p.err, 359);
+      if (!ok) break;
+      tc_fence_after();
+      // queries 0..31 in columns 0..15 of the buffer, 32..63 in 32..47
+      mma_values(tdV, tS(buf), 32, dt + st * stage, idKV, it > 0, leader);
+      mma_values(tdK, tdP(buf), 32, qt + st * stage, idKV, it > 0, leader);
+      commit(&s.empty[st], leader);
+      if (it + 2 < n) ok = issue(it + 2);
+    }
+    commit(ok ? &s.done : &s.drained, leader);
+    if (!ok) wait_warp(&s.drained, 0, p.err, 361);
   }
 
   tc_fence_before();

@@ -22,9 +22,10 @@ void one_device(const at::Tensor& first, const Tensors&... rest) {
                 " and ", t->device());
 }
 
-CUtensorMap heads_map(const at::Tensor& x) {
+// tiles of 128 rows that stay, of STEP rows that go past
+CUtensorMap heads_map(const at::Tensor& x, int rows) {
   auto stride = [&](int i) { return x.size(i) == 1 ? x.size(3) : x.stride(i); };  // of one element: never taken
-  return make_tmap_heads(x.data_ptr(), x.size(3), x.size(2), x.size(1), x.size(0), stride(2), stride(1), stride(0), TILE);
+  return make_tmap_heads(x.data_ptr(), x.size(3), x.size(2), x.size(1), x.size(0), stride(2), stride(1), stride(0), rows);
 }
 
 // x itself where TMA and 16-byte accesses take it, else a contiguous copy
@@ -64,7 +65,8 @@ Shape check(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const
                     slopes->size(0) == n.nq,
                 "masked_attention: slopes must be one fp32 number per query head");
   }
-  TORCH_CHECK(n.B * std::max<int64_t>(n.nq, 1) < (int64_t(1) << 31), "masked_attention: too many heads in the batch");
+  TORCH_CHECK(n.B <= 65535 && n.nq <= 8192 && n.B * n.nq < (int64_t(1) << 31), "masked_attention: at most 65535 sequences of ",
+              "8192 heads, got ", n.B, " of ", n.nq);
   return n;
 }
 
@@ -160,7 +162,7 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>, c10::optional<at::Tensor>> mas
   p.o = out_of(o);
   p.low = graded ? low->data_ptr() : nullptr;
   p.pair_heads = p.group % 2 == 0;
-  C10_CUDA_CHECK(launch_fwd(heads_map(q), heads_map(k), heads_map(v), p, softcap > 0, slopes.has_value(),
+  C10_CUDA_CHECK(launch_fwd(heads_map(q, TILE), heads_map(k, STEP), heads_map(v, STEP), p, softcap > 0, slopes.has_value(),
                             at::cuda::getCurrentCUDAStream()));
   return {o, lse, low};
 }
@@ -211,10 +213,11 @@ int64_t masked_attn_bwd(const at::Tensor& q_, const at::Tensor& k_, const at::Te
     part = at::empty({p.split, 2, n.B * n.nkv, p.padded, n.d}, lse.options());
     p.part = part.data_ptr<float>();
   }
-  const CUtensorMap tq = heads_map(q), tk = heads_map(k), tv = heads_map(v), td = heads_map(dout);
   C10_CUDA_CHECK(launch_delta(p, out_of(dout), st));
-  C10_CUDA_CHECK(launch_dq(tq, tk, tv, td, p, softcap > 0, slopes.has_value(), st));
-  C10_CUDA_CHECK(launch_dkv(tq, tk, tv, td, p, softcap > 0, slopes.has_value(), st));
+  C10_CUDA_CHECK(launch_dq(heads_map(q, TILE), heads_map(k, STEP), heads_map(v, STEP), heads_map(dout, TILE), p, softcap > 0,
+                           slopes.has_value(), st));
+  C10_CUDA_CHECK(launch_dkv(heads_map(q, STEP), heads_map(k, TILE), heads_map(v, TILE), heads_map(dout, STEP), p,
+                            softcap > 0, slopes.has_value(), st));
   return p.split > 1 ? 4 : 3;
 }
 

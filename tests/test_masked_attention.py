@@ -280,6 +280,25 @@ def test_gpu_padding_may_hold_nan():
 
 
 @gpu
+@pytest.mark.parametrize("d", [64, 128])
+def test_gpu_padding_over_many_tiles(d):
+    # padding inside and behind documents in every one of nine tiles, and whole tiles of it
+    B, S, nq, nkv = 2, 1100, 4, 2
+    q, k, v, do = make(B, S, nq, nkv, d, 7, "cuda", torch.bfloat16)
+    i = torch.arange(S, device="cuda")
+    docs = torch.where(i % 61 < 7, -1, 0).int().repeat(B, 1)
+    docs[1] = torch.where((i > 200) & (i < 900), -1, i // 500).int()
+    mask = MA.attention_mask(B, S, causal=False, docs=torch.where(docs < 0, docs, 3 * (i // 61).int()))
+    clean = run(q, k, v, do, mask)
+    dead = docs < 0
+    for x in (q, k, v, do):
+        x[dead] = float("nan")
+    for x, y in zip(run(q, k, v, do, mask), clean):
+        assert torch.equal(x, y) and not x[dead].any()
+    check_kernel_errors(q.device)
+
+
+@gpu
 def test_gpu_strides_and_packed_views():
     B, S, nq, nkv, d = 2, 257, 4, 2, 64
     q, k, v, do = make(B, S, nq, nkv, d, 4, "cuda", torch.bfloat16)

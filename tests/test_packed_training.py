@@ -200,5 +200,5 @@ def test_gpu_model_on_packed_rows():
         out["loss"].backward()
         # some thirty roundings of 2^-9 of two layers and the head
         assert abs(float(out["loss"].detach()) - loss) < 0.02 * loss
-        assert float((out["logits"].float().cpu() - logits).norm() / logits.norm()) < 30 ** 0.5 * 2 ** -8
+        assert float((out["logits"].detach().float().cpu() - logits).norm() / logits.norm()) < 30 ** 0.5 * 2 ** -8
     assert all(torch.isfinite(p.grad).all() for p in model.parameters())

@@ -32,18 +32,27 @@ __device__ __forceinline__ int64_t id_at(const void* ids, bool wide, int64_t t) 
 }
 
 // ------------------------------------------------------------------------------ lookup
-// One block per (token, piece of the row); VEC values per access.
+// One block per (token, piece of the row) with 16 bytes per thread; one per token, eight loads in flight, where rows are not
+// on 16-byte boundaries.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(128) fwd_kernel(const FwdArgs a) {
   const int64_t t = blockIdx.x;
-  const int c = (blockIdx.y * 128 + threadIdx.x) * VEC;
+  const int c = VEC == 1 ? threadIdx.x : (blockIdx.y * 128 + threadIdx.x) * VEC;
   if (c >= a.H) return;
   const int64_t id = id_at(a.ids, a.ids64, t) - a.vstart;
   const bool has = id >= 0 && id < a.V;
   const T* w = static_cast<const T*>(a.table) + id * a.H + c;
   T* o = static_cast<T*>(a.out) + t * a.H + c;
   if constexpr (VEC == 1) {
-    *o = has ? from_f<T>(to_f(*w) * a.scale) : from_f<T>(0.f);
+    const int n = (a.H - c + 127) / 128;
+    for (int i0 = 0; i0 < n; i0 += 8) {
+      T v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = has && i0 + i < n ? w[(i0 + i) * 128] : from_f<T>(0.f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i0 + i < n) o[(i0 + i) * 128] = from_f<T>(to_f(v[i]) * a.scale);
+    }
   } else {
     uint4 q = make_uint4(0, 0, 0, 0);
     if (has) {
@@ -59,8 +68,7 @@ __global__ void __launch_bounds__(128) fwd_kernel(const FwdArgs a) {
 template <typename T>
 void fwd_of(const FwdArgs& a, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
-  const int per = 128 * (a.vec ? V : 1);
-  const dim3 grid(static_cast<unsigned>(a.T), (a.H + per - 1) / per);
+  const dim3 grid(static_cast<unsigned>(a.T), a.vec ? (a.H + 128 * V - 1) / (128 * V) : 1);
   if (a.vec) fwd_kernel<T, V><<<grid, 128, 0, st>>>(a);
   else fwd_kernel<T, 1><<<grid, 128, 0, st>>>(a);
 }
@@ -168,6 +176,92 @@ __global__ void __launch_bounds__(SORT_NT) move_kernel(const SortArgs a, const P
       p.key_out[to] = key;
       p.pos_out[to] = p.first ? t : p.pos[t];
     }
+  }
+}
+
+// The same passes for up to SMALL_SORT tokens, in the shared memory of one block; a warp's tokens are neighbours, so equal
+// digits keep their order.
+constexpr int SMALL_NT = 1024, SMALL_WARPS = SMALL_NT / 32, SMALL_BINS = 1 << SMALL_BITS, ROUNDS = SMALL_SORT / SMALL_NT;
+struct SmallSort {
+  uint32_t key[2][SMALL_SORT];
+  uint16_t pos[2][SMALL_SORT];
+  uint16_t at[SMALL_WARPS][SMALL_BINS];  // counts, then where a warp's next token of a digit goes
+  uint32_t warps[SMALL_WARPS];
+};
+
+__global__ void __launch_bounds__(SMALL_NT) small_sort_kernel(const SortArgs a) {
+  extern __shared__ uint8_t raw[];
+  SmallSort& s = *reinterpret_cast<SmallSort*>(raw);
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  for (int t = threadIdx.x; t < a.T; t += SMALL_NT) {
+    const int64_t id = id_at(a.ids, a.ids64, t) - a.vstart;
+    s.key[0][t] = static_cast<uint32_t>(id >= 0 && id < a.V ? id : a.V);
+    s.pos[0][t] = static_cast<uint16_t>(t);
+  }
+  const int rounds = (a.T + SMALL_NT - 1) / SMALL_NT, t0 = w * rounds * 32;
+  int shift = 0;
+  for (int pass = 0; pass < a.passes; ++pass) {
+    const int bins = 1 << a.bits[pass], from = pass & 1;
+    for (int i = threadIdx.x; i < SMALL_WARPS * bins / 2; i += SMALL_NT)
+      reinterpret_cast<uint32_t*>(s.at)[i / (bins / 2) * (SMALL_BINS / 2) + i % (bins / 2)] = 0;
+    __syncthreads();
+    // a token's place among its warp's equal digits, kept for the move (matching is what takes the time)
+    uint16_t place[ROUNDS];
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+      if (r >= rounds) break;
+      const int t = t0 + r * 32 + lane;
+      const bool in = t < a.T;
+      const uint32_t digit = in ? (s.key[from][t] >> shift) & (bins - 1) : bins;
+      const uint32_t same = __match_any_sync(0xffffffff, digit), rank = __popc(same & ((1u << lane) - 1));
+      const uint32_t before = in ? s.at[w][digit] : 0;
+      place[r] = static_cast<uint16_t>(before + rank);
+      __syncwarp();
+      if (in && rank == 0) s.at[w][digit] = static_cast<uint16_t>(before + __popc(same));
+      __syncwarp();
+    }
+    __syncthreads();
+    // exclusive scan, digit by digit over the warps
+    uint32_t sum = 0;
+    if (static_cast<int>(threadIdx.x) < bins)
+      for (int k = 0; k < SMALL_WARPS; ++k) sum += s.at[k][threadIdx.x];
+    uint32_t inc = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t u = __shfl_up_sync(0xffffffff, inc, o);
+      if (lane >= o) inc += u;
+    }
+    if (lane == 31) s.warps[w] = inc;
+    __syncthreads();
+    uint32_t base = inc - sum;
+    for (int k = 0; k < w; ++k) base += s.warps[k];
+    if (static_cast<int>(threadIdx.x) < bins)
+      for (int k = 0; k < SMALL_WARPS; ++k) {
+        const uint32_t c = s.at[k][threadIdx.x];
+        s.at[k][threadIdx.x] = static_cast<uint16_t>(base);
+        base += c;
+      }
+    __syncthreads();
+    const bool last = pass + 1 == a.passes;
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+      if (r >= rounds) break;
+      const int t = t0 + r * 32 + lane;
+      const bool in = t < a.T;
+      const uint32_t key = in ? s.key[from][t] : 0;
+      const uint32_t to = in ? s.at[w][(key >> shift) & (bins - 1)] + place[r] : 0;
+      if (in) {
+        if (last) {
+          a.key[0][to] = key;
+          a.pos[0][to] = s.pos[from][t];
+        } else {
+          s.key[from ^ 1][to] = key;
+          s.pos[from ^ 1][to] = s.pos[from][t];
+        }
+      }
+    }
+    __syncthreads();
+    shift += a.bits[pass];
   }
 }
 
@@ -318,6 +412,34 @@ cudaError_t launch_fwd(const FwdArgs& a, cudaStream_t st) {
   if (a.type == F32) fwd_of<float>(a, st);
   else if (a.type == BF16) fwd_of<__nv_bfloat16>(a, st);
   else fwd_of<__half>(a, st);
+  return cudaGetLastError();
+}
+
+// 16 bytes per store, four per thread, in many small blocks: 2.1 GB in 280 us.  (A block of 1024 threads per SM, beside the
+// block that sorts, took 350 us; the runtime's memset 337.)
+__global__ void __launch_bounds__(256) clear_kernel(uint4* __restrict__ x, int64_t words) {
+  const int64_t i0 = static_cast<int64_t>(blockIdx.x) * 1024 + threadIdx.x;
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    if (i0 + u * 256 < words) x[i0 + u * 256] = make_uint4(0, 0, 0, 0);
+}
+
+cudaError_t launch_clear(void* x, int64_t bytes, cudaStream_t st) {
+  const int64_t words = bytes / 16, blocks = (words + 1023) / 1024;
+  if (reinterpret_cast<uintptr_t>(x) % 16 || bytes % 16 || blocks >= (int64_t(1) << 31)) return cudaMemsetAsync(x, 0, bytes, st);
+  clear_kernel<<<static_cast<unsigned>(blocks), 256, 0, st>>>(static_cast<uint4*>(x), words);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_small_sort(const SortArgs& a, cudaStream_t st) {
+  int dev = 0;
+  static unsigned long long done = 0;  // one bit per device
+  cudaGetDevice(&dev);
+  if (!(done >> (dev & 63) & 1)) {
+    cudaFuncSetAttribute(small_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(SmallSort));
+    done |= 1ull << (dev & 63);
+  }
+  small_sort_kernel<<<1, SMALL_NT, sizeof(SmallSort), st>>>(a);
   return cudaGetLastError();
 }
 

@@ -72,8 +72,9 @@ int64_t embed_sorted_grad(const at::Tensor& ids_, const at::Tensor& dout_, at::T
   auto st = at::cuda::getCurrentCUDAStream();
   if (dst.numel() == 0) return 0;
   TORCH_CHECK(H <= 65535 * 128, "embedding: rows of up to ", 65535 * 128, " values");
-  if (!accumulate) C10_CUDA_CHECK(cudaMemsetAsync(dst.data_ptr(), 0, dst.nbytes(), st));
-  if (T == 0) return 0;
+  const bool small = T > 0 && T <= SMALL_SORT;
+  if (!accumulate) C10_CUDA_CHECK(launch_clear(dst.data_ptr(), dst.nbytes(), st));
+  if (T == 0) return accumulate ? 0 : 1;
   const at::Tensor ids = ids_.contiguous(), dout = dout_.contiguous();
   SortArgs s{};
   s.ids = ids.data_ptr();
@@ -84,26 +85,29 @@ int64_t embed_sorted_grad(const at::Tensor& ids_, const at::Tensor& dout_, at::T
   s.blocks = static_cast<int>((T + SORT_CHUNK - 1) / SORT_CHUNK);
   int bits = 1;
   while ((int64_t(1) << bits) <= V) ++bits;  // keys 0 ... V
-  s.passes = (bits + 9) / 10;
+  const int digit = small ? SMALL_BITS : 10;
+  s.passes = (bits + digit - 1) / digit;
+  TORCH_CHECK(s.passes <= 4, "embedding: too many words");
   int most = 0;
   for (int i = 0; i < s.passes; ++i) {
     s.bits[i] = (bits - i + s.passes - 1) / s.passes;
     most = std::max(most, s.bits[i]);
   }
   const int64_t pieces = (T + PIECE - 1) / PIECE;
-  const int64_t words = 4 * T + (int64_t(1) << most) * s.blocks;
+  const int64_t words = small ? 2 * T : 4 * T + (int64_t(1) << most) * s.blocks;
   at::Tensor work = at::empty({words}, dst.options().dtype(at::kInt));
   uint32_t* w = reinterpret_cast<uint32_t*>(work.data_ptr<int>());
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < (small ? 1 : 2); ++i) {
     s.key[i] = w + 2 * i * T;
     s.pos[i] = w + (2 * i + 1) * T;
   }
   s.counts = w + 4 * T;
-  C10_CUDA_CHECK(launch_sort(s, st));
+  if (small) C10_CUDA_CHECK(launch_small_sort(s, st));
+  else C10_CUDA_CHECK(launch_sort(s, st));
   at::Tensor partial = at::empty({pieces, 2, H}, dst.options().dtype(at::kFloat));
   GradArgs a{};
-  a.key = s.key[s.passes & 1];
-  a.pos = s.pos[s.passes & 1];
+  a.key = s.key[small ? 0 : s.passes & 1];
+  a.pos = s.pos[small ? 0 : s.passes & 1];
   a.dout = dout.data_ptr();
   a.dw = dst.data_ptr();
   a.partial = partial.data_ptr<float>();
@@ -119,7 +123,7 @@ int64_t embed_sorted_grad(const at::Tensor& ids_, const at::Tensor& dout_, at::T
           (dst.element_size() >= dout.element_size() || H % 8 == 0);
   a.scale = static_cast<float>(scale);
   C10_CUDA_CHECK(launch_grad(a, st));
-  return 3 * s.passes + (pieces > 1 ? 2 : 1);
+  return (accumulate ? 0 : 1) + (small ? 1 : 3 * s.passes) + (pieces > 1 ? 2 : 1);
 }
 
 }  // namespace ft

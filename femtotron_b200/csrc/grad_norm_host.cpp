@@ -26,22 +26,43 @@ uint8_t type_of(const char* op, const at::Tensor& x) {
     case at::kFloat: return F32;
     case at::kBFloat16: return BF16;
     case at::kHalf: return F16;
-    default: TORCH_CHECK(false, op, ": fp32, bf16 or fp16 tensors are required, got ", x.scalar_type());
+    default: TORCH_CHECK_TYPE(false, op, ": fp32, bf16 or fp16 tensors are required, got ", x.scalar_type());
   }
 }
 
 void check(const char* op, const std::vector<at::Tensor>& xs) {
   for (const at::Tensor& x : xs) {
-    TORCH_CHECK(x.is_cuda() && x.device() == xs[0].device(), op, ": all tensors must be on one CUDA device, got ",
+    TORCH_CHECK_VALUE(x.is_cuda() && x.device() == xs[0].device(), op, ": all tensors must be on one CUDA device, got ",
                 xs[0].device(), " and ", x.device());
     type_of(op, x);
   }
 }
 
-// The tables of a list, one after the other, each as small as it may be.
-template <class F>
-void each_table(const std::vector<Item>& items, F&& go) {
-  auto fill = [&](auto& t, size_t from, size_t to) {
+// The tables of a list: one of up to 64 tensors, or as many large ones as it takes.
+struct Tables {
+  std::unique_ptr<Table<64>> small;
+  std::vector<std::unique_ptr<Table<MAX_TENSORS>>> large;
+
+  explicit Tables(const std::vector<Item>& items) {
+    if (items.size() <= 64) {
+      small = std::make_unique<Table<64>>();
+      fill(*small, items, 0, items.size());
+      return;
+    }
+    for (size_t from = 0; from < items.size(); from += MAX_TENSORS) {
+      large.push_back(std::make_unique<Table<MAX_TENSORS>>());
+      fill(*large.back(), items, from, std::min(items.size(), from + MAX_TENSORS));
+    }
+  }
+  template <class F>
+  void each(F&& go) const {
+    if (small) go(*small);
+    for (const auto& t : large) go(*t);
+  }
+
+ private:
+  template <int N>
+  static void fill(Table<N>& t, const std::vector<Item>& items, size_t from, size_t to) {
     t.count = static_cast<int>(to - from);
     int64_t chunks = 0;
     for (size_t i = from; i < to; ++i) {
@@ -56,19 +77,8 @@ void each_table(const std::vector<Item>& items, F&& go) {
       t.chunk_end[k] = static_cast<int>(chunks);
     }
     t.chunks = static_cast<int>(chunks);
-    go(t);
-  };
-  for (size_t from = 0; from < items.size(); from += MAX_TENSORS) {
-    const size_t to = std::min(items.size(), from + MAX_TENSORS);
-    if (to - from <= 64) {
-      Table<64> t;
-      fill(t, from, to);
-    } else {
-      auto t = std::make_unique<Table<MAX_TENSORS>>();
-      fill(*t, from, to);
-    }
   }
-}
+};
 
 // Memory of one call's outputs: no value may be written by two of them, nor read by another one.
 void check_apart(const char* op, const std::vector<Item>& items, const std::vector<int>& size) {
@@ -81,7 +91,8 @@ void check_apart(const char* op, const std::vector<Item>& items, const std::vect
     const uintptr_t p = reinterpret_cast<uintptr_t>(items[i].y);
     out.push_back({p, p + items[i].n * size[items[i].type], i});
   }
-  std::sort(out.begin(), out.end(), [](const Span& a, const Span& b) { return a.from < b.from; });
+  auto before = [](const Span& a, const Span& b) { return a.from < b.from; };
+  if (!std::is_sorted(out.begin(), out.end(), before)) std::sort(out.begin(), out.end(), before);
   for (size_t i = 1; i < out.size(); ++i)
     TORCH_CHECK(out[i].from >= out[i - 1].to, op, ": two of the tensors written share memory");
   for (size_t i = 0; i < items.size(); ++i) {
@@ -106,11 +117,11 @@ Plan plan_of(const char* op, const std::vector<at::Tensor>& xs, const std::vecto
   check(op, xs);
   Plan p;
   p.in_place = outs.empty();
-  TORCH_CHECK(p.in_place || outs.size() == xs.size(), op, ": ", xs.size(), " tensors and ", outs.size(), " outputs");
+  TORCH_CHECK_VALUE(p.in_place || outs.size() == xs.size(), op, ": ", xs.size(), " tensors and ", outs.size(), " outputs");
   for (size_t i = 0; i < xs.size(); ++i) {
     const at::Tensor& o = p.in_place ? xs[i] : outs[i];
-    TORCH_CHECK(o.sizes() == xs[i].sizes() && o.scalar_type() == xs[i].scalar_type() && o.device() == xs[0].device(), op,
-                ": output ", i, " must have its tensor's shape, type and device");
+    TORCH_CHECK_VALUE(o.sizes() == xs[i].sizes() && o.scalar_type() == xs[i].scalar_type() && o.device() == xs[0].device(), op,
+                      ": an output of ", o.scalar_type(), " ", o.sizes(), " for ", xs[i].scalar_type(), " ", xs[i].sizes());
     if (xs[i].numel() == 0) continue;
     at::Tensor src = dense(xs[i]);
     at::Tensor dst = o.is_non_overlapping_and_dense() && o.strides() == src.strides() ? o : at::Tensor();
@@ -127,12 +138,12 @@ Plan plan_of(const char* op, const std::vector<at::Tensor>& xs, const std::vecto
 }
 
 // Launches the sums of all tables; the partial sums [blocks, n_slots].
-at::Tensor partials(const std::vector<Item>& items, int64_t n_slots, const at::Device& dev, cudaStream_t st) {
+at::Tensor partials(const Tables& tables, int64_t n_slots, const at::Device& dev, cudaStream_t st) {
   int64_t blocks = 0;
-  each_table(items, [&](auto& t) { blocks += sumsq_blocks(t.chunks); });
+  tables.each([&](const auto& t) { blocks += sumsq_blocks(t.chunks); });
   at::Tensor part = at::empty({blocks, n_slots}, at::TensorOptions().dtype(at::kDouble).device(dev));
   double* at_ = part.data_ptr<double>();
-  each_table(items, [&](auto& t) {
+  tables.each([&](const auto& t) {
     C10_CUDA_CHECK(launch_sumsq(t, static_cast<int>(n_slots), at_, st));
     at_ += sumsq_blocks(t.chunks) * n_slots;
   });
@@ -161,7 +172,7 @@ at::Tensor grad_sumsq(const std::vector<at::Tensor>& xs, const std::vector<int64
   }
   at::Tensor sums = at::empty({n_slots}, at::TensorOptions().dtype(at::kDouble).device(xs[0].device()));
   if (items.empty()) return sums.zero_();
-  const at::Tensor part = partials(items, n_slots, xs[0].device(), st);
+  const at::Tensor part = partials(Tables(items), n_slots, xs[0].device(), st);
   C10_CUDA_CHECK(launch_finish(part.data_ptr<double>(), static_cast<int>(part.size(0)), static_cast<int>(n_slots),
                                sums.data_ptr<double>(), st));
   return sums;
@@ -175,8 +186,10 @@ void grad_scale(const std::vector<at::Tensor>& xs, const at::Tensor& coef, const
               "scale_grads: the factor must be one fp32 number on the tensors' device");
   const c10::cuda::CUDAGuard g(xs[0].device());
   auto st = at::cuda::getCurrentCUDAStream();
+  if (p.items.empty()) return;
+  const Tables tables(p.items);
   const Factor f{coef.data_ptr<float>(), nullptr, 0, 0.f, nullptr, p.in_place};
-  each_table(p.items, [&](auto& t) { C10_CUDA_CHECK(launch_scale(t, f, st)); });
+  tables.each([&](const auto& t) { C10_CUDA_CHECK(launch_scale(t, f, st)); });
   for (auto& [to, from] : p.back) to.copy_(from);
 }
 
@@ -188,10 +201,11 @@ at::Tensor grad_clip(const std::vector<at::Tensor>& xs, double max_norm, const s
   auto st = at::cuda::getCurrentCUDAStream();
   at::Tensor norm = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(xs[0].device()));
   if (p.items.empty()) return norm.zero_();
-  const at::Tensor part = partials(p.items, 1, xs[0].device(), st);
+  const Tables tables(p.items);
+  const at::Tensor part = partials(tables, 1, xs[0].device(), st);
   const Factor f{nullptr, part.data_ptr<double>(), static_cast<int>(part.size(0)), static_cast<float>(max_norm),
                  norm.data_ptr<float>(), p.in_place};
-  each_table(p.items, [&](auto& t) { C10_CUDA_CHECK(launch_scale(t, f, st)); });
+  tables.each([&](const auto& t) { C10_CUDA_CHECK(launch_scale(t, f, st)); });
   for (auto& [to, from] : p.back) to.copy_(from);
   return norm;
 }

@@ -147,31 +147,30 @@ struct FwdSmem {
 
 // Probabilities of 32 keys relative to 2^m from their scores (times `mul`, log2 units), as bf16 pairs; their fp32
 // sums in `sums` (of the unrounded values: only p v sees the rounding).  A score of -inf gives 0.
-template <bool TEST>
+template <bool CAP, bool TEST>
 __device__ __forceinline__ void probs32(const uint32_t* sv, float mul, float m, uint64_t& sums, uint32_t (&pk)[16]) {
   const uint64_t mul2_ = pair(mul, mul), m2 = pair(-m, -m);
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
     const uint64_t x = fma2(pair(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), mul2_, m2);
     const float2 y0 = apart(x);
-    float2 y = exp2_of(y0, e);
-    if (TEST && on_fma_pipe(e)) y = make_float2(y0.x == -INFINITY ? 0.f : y.x, y0.y == -INFINITY ? 0.f : y.y);
+    float2 y = exp2_of<CAP>(y0, e);
+    if (TEST && on_fma_pipe<CAP>(e)) y = make_float2(y0.x == -INFINITY ? 0.f : y.x, y0.y == -INFINITY ? 0.f : y.y);
     sums = add2(sums, pair(y.x, y.y));
     pk[e] = pack_bf16x2(y.x, y.y);
   }
 }
 
-// The scores of STEP keys from their raw products: transformed (capped, biased), and -inf where they are not
-// seen.  TEST: element e is seen when off + e is in [0, width).  Returns the largest.
+// What `mul` times makes the scores of STEP keys, from their raw products (capped, biased), and -inf where they are
+// not seen.  TEST: element e is seen when off + e is in [0, width).  Returns the largest.
 template <bool CAP, bool ALIBI, bool TEST>
 __device__ __forceinline__ float scores(uint32_t (&sv)[STEP], const Common& p, float slope2, float far, int off, int width) {
   float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  float none[1];
+  cap_scores<CAP, false>(sv, none, p);
 #pragma unroll
   for (int e = 0; e < STEP; ++e) {
-    if (CAP || ALIBI) {
-      float keep;
-      sv[e] = __float_as_uint(score<CAP, ALIBI>(__uint_as_float(sv[e]), p, slope2, far - e, keep));
-    }
+    if (ALIBI) sv[e] = __float_as_uint(fmaf(-slope2, fabsf(far - e), __uint_as_float(sv[e]) * unit<CAP>(p)));
     if (TEST && static_cast<uint32_t>(off + e) >= static_cast<uint32_t>(width)) sv[e] = __float_as_uint(-INFINITY);
   }
 #pragma unroll
@@ -260,8 +259,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       sum = tiles[tile];
       if (ALIBI) slope2 = p.slopes[h] * kLog2e;
     }
-    constexpr bool RAW = !CAP && !ALIBI;  // scores without the scale, which then goes into the exponent's FMA
-    const float mul = RAW ? p.scale_log2 : 1.f;
+    const float mul = ALIBI ? 1.f : unit<CAP>(p);  // goes into the exponent's FMA
     for (int c = 0; c < n; ++c) {
       const int k0 = (begin + c) * STEP, buf = c & 1;
       const uint32_t ts = tS(t, buf) + lane_off;
@@ -303,8 +301,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 #pragma unroll
       for (int q = 0; q < STEP / 32; ++q) {
         uint32_t pk[16];
-        if (test) probs32<true>(sv + q * 32, mul, m, sums, pk);
-        else probs32<false>(sv + q * 32, mul, m, sums, pk);
+        if (test) probs32<CAP, true>(sv + q * 32, mul, m, sums, pk);
+        else probs32<CAP, false>(sv + q * 32, mul, m, sums, pk);
         tmem_st_32x32b_x16(ts + q * 16, pk);
       }
       tmem_wait_st();

@@ -154,28 +154,53 @@ __device__ __forceinline__ float rcp_approx(float x) {
 }
 
 // 2^x of the e-th pair of a row.  Every fourth pair runs on the FMA pipe: the special-function unit takes 8 clocks for
-// one exponential of a warp and would set the pace alone.
-__device__ __forceinline__ constexpr bool on_fma_pipe(int e) { return e % 4 == 3; }
+// one exponential of a warp and would set the pace alone.  With capped scores the FMA pipe sets it.
+template <bool CAP>
+__device__ __forceinline__ constexpr bool on_fma_pipe(int e) { return !CAP && e % 4 == 3; }
+template <bool CAP>
 __device__ __forceinline__ float2 exp2_of(float2 x, int e) {
-  return on_fma_pipe(e) ? exp2_pair(x.x, x.y) : make_float2(ex2_approx(x.x), ex2_approx(x.y));
+  return on_fma_pipe<CAP>(e) ? exp2_pair(x.x, x.y) : make_float2(ex2_approx(x.x), ex2_approx(x.y));
 }
 
-// A raw product s as a score in log2 units.  tanh(x) = 1 - 2 / (1 + exp(2x)): two special-function
-// instructions, off by 1e-7 in all (tanh.approx would be 5e-4 of the cap: whole percents of p).
-// `keep` is 1 - tanh^2, the slope of the cap.
-template <bool CAP, bool ALIBI>
-__device__ __forceinline__ float score(float s, const Common& p, float slope2, float dist, float& keep) {
-  float y;
-  if (CAP) {
-    const float r = rcp_approx(1.f + ex2_approx(s * p.cap_in));
-    y = fmaf(-2.f * p.cap_out, r, p.cap_out);
-    keep = 4.f * r * (1.f - r);
+// Raw products as what an FMA with `unit(p)` turns into scores in log2 units: with the cap tanh(x) (KEEP: `keep` is
+// 1 - tanh^2, the slope of the cap), without it the products themselves.  tanh(x) = 1 - 2 / (1 + exp(2x)) costs two
+// special-function instructions of 8 clocks each (tanh.approx would be off by 5e-4 of the cap: whole percents of p).
+// Where a warp's products are all within 0.7 of the cap, as nearly all are, a polynomial does it on the FMA pipe, off by
+// 2e-7 (the other form by 1e-7): 288 -> 259 us for the forward pass of two rows of 4096 tokens in windows of 1024.
+template <bool CAP, bool KEEP, int N>
+__device__ __forceinline__ void cap_scores(uint32_t (&sv)[N], float (&keep)[KEEP ? N : 1], const Common& p) {
+  if (!CAP) return;
+  float m[2] = {0.f, 0.f};
+#pragma unroll
+  for (int e = 0; e < N; ++e) m[e & 1] = fmaxf(m[e & 1], fabsf(__uint_as_float(sv[e])));
+  if (__all_sync(0xffffffffu, fmaxf(m[0], m[1]) <= p.cap_small)) {
+    uint64_t c[5];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) c[i] = pair(p.cap_poly[i], p.cap_poly[i]);
+#pragma unroll
+    for (int e = 0; e < N; e += 2) {
+      const uint64_t s = pair(__uint_as_float(sv[e]), __uint_as_float(sv[e + 1])), u = mul2(s, s);
+      const uint64_t t = mul2(fma2(fma2(fma2(fma2(u, c[4], c[3]), u, c[2]), u, c[1]), u, c[0]), s);
+      const float2 y = apart(t);
+      sv[e] = __float_as_uint(y.x);
+      sv[e + 1] = __float_as_uint(y.y);
+      if (KEEP) {
+        const float2 k = apart(fma2(mul2(t, pair(-1.f, -1.f)), t, pair(1.f, 1.f)));
+        keep[KEEP ? e : 0] = k.x;
+        keep[KEEP ? e + 1 : 0] = k.y;
+      }
+    }
   } else {
-    y = s * p.scale_log2;
-    keep = 1.f;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float r = rcp_approx(1.f + ex2_approx(__uint_as_float(sv[e]) * p.cap_in));
+      sv[e] = __float_as_uint(fmaf(-2.f, r, 1.f));
+      if (KEEP) keep[KEEP ? e : 0] = 4.f * r * (1.f - r);
+    }
   }
-  return ALIBI ? fmaf(-slope2, fabsf(dist), y) : y;
 }
+template <bool CAP>
+__device__ __forceinline__ float unit(const Common& p) { return CAP ? p.cap_out : p.scale_log2; }
 
 // Zero the rows that see nothing of a tile of STEP rows (`chunks` pieces of 128 bytes a row); one warp.  The swizzle
 // permutes within a row's 128 bytes only.

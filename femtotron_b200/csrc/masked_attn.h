@@ -61,6 +61,8 @@ struct Common {
   const float* slopes;
   float scale, scale_log2;
   float cap_in, cap_out;  // exp2(s cap_in) = exp(2 scale s / c); c log2(e)
+  float cap_small;        // products up to this take the polynomial
+  float cap_poly[5];      // tanh(scale s / c) = s (cap_poly[0] + cap_poly[1] s^2 + ...)
   float* neg_lse2;        // [B, nq, padded], minus the log-sum-exp in log2 units; -inf where a row sees nothing
   int* err;
 };

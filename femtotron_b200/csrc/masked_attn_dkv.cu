@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     const int quad = warp & 3, half = warp >> 2;
     const int key = k0 + quad * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quad * 32) << 16;
-    const uint64_t mul = pair(p.scale_log2, p.scale_log2);
+    const uint64_t mul = pair(unit<CAP>(p), unit<CAP>(p));
     bool ok = true;
     for (int it = 0; it < n; ++it) {
       const int st = it % Q_STAGES, buf = it & 1, tile = it / 2, entry = s.list[tile % count];
@@ -107,21 +107,17 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       tmem_ld_32x32b_x32(ts, sv);
       tmem_ld_32x32b_x32(td, dv);
       tmem_wait_ld();
-      float keeps[CAP ? 32 : 1];
+      float keep[CAP ? 32 : 1];
+      cap_scores<CAP, CAP>(sv, keep, p);
 #pragma unroll
       for (int e = 0; e < 32; e += 2) {
-        const float2 l = e & 2 ? make_float2(L[e / 4].z, L[e / 4].w) : make_float2(L[e / 4].x, L[e / 4].y);
-        float2 y, keep = make_float2(1.f, 1.f);
-        if (!CAP && !ALIBI) {
-          y = apart(fma2(pair(__uint_as_float(sv[e]), __uint_as_float(sv[e + 1])), mul, pair(l.x, l.y)));
-        } else {
-          y.x = score<CAP, ALIBI>(__uint_as_float(sv[e]), p, slope2, far - e, keep.x) + l.x;
-          y.y = score<CAP, ALIBI>(__uint_as_float(sv[e + 1]), p, slope2, far - (e + 1), keep.y) + l.y;
-        }
-        y = exp2_of(y, e / 2);
+        const uint64_t l = e & 2 ? pair(L[e / 4].z, L[e / 4].w) : pair(L[e / 4].x, L[e / 4].y);
+        const uint64_t x = pair(__uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
+        float2 y = apart(fma2(x, mul, l));
+        if (ALIBI) y.x = fmaf(-slope2, fabsf(far - e), y.x), y.y = fmaf(-slope2, fabsf(far - (e + 1)), y.y);
+        y = exp2_of<CAP>(y, e / 2);
         sv[e] = __float_as_uint(y.x);
         sv[e + 1] = __float_as_uint(y.y);
-        if (CAP) keeps[e] = keep.x, keeps[e + 1] = keep.y;
       }
       if (test) {
         const int4* R = reinterpret_cast<const int4*>(s.rows[st] + half * 32);
@@ -140,7 +136,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       for (int e = 0; e < 32; e += 2) {
         const uint64_t nd = e & 2 ? pair(Dl[e / 4].z, Dl[e / 4].w) : pair(Dl[e / 4].x, Dl[e / 4].y);
         uint64_t w = pair(__uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
-        if (CAP) w = mul2(w, pair(keeps[CAP ? e : 0], keeps[CAP ? e + 1 : 0]));
+        if (CAP) w = mul2(w, pair(keep[CAP ? e : 0], keep[CAP ? e + 1 : 0]));
         const float2 g = apart(mul2(w, add2(pair(__uint_as_float(dv[e]), __uint_as_float(dv[e + 1])), nd)));
         pk[e / 2] = pack_bf16x2(g.x, g.y);
       }

@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     if (lh.y > lh.x) lo = lh.x, width = lh.y - lh.x;
     const float neg_lse2 = p.neg_lse2[stat], neg_delta = p.neg_delta[stat];
     const float slope2 = ALIBI ? p.slopes[h] * kLog2e : 0.f;
-    const uint64_t mul = pair(p.scale_log2, p.scale_log2), m = pair(neg_lse2, neg_lse2), nd = pair(neg_delta, neg_delta);
+    const uint64_t mul = pair(unit<CAP>(p), unit<CAP>(p)), m = pair(neg_lse2, neg_lse2), nd = pair(neg_delta, neg_delta);
     bool ok = true;
     for (int it = 0; it < n; ++it) {
       const int buf = it & 1, k0 = (j0 + it) * STEP;
@@ -130,17 +130,15 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       tmem_ld_32x32b_x32(ts, sv);
       tmem_ld_32x32b_x32(tdP(buf) + lane_off + half * 32, dv);
       tmem_wait_ld();
+      float keep[CAP ? 32 : 1];
+      cap_scores<CAP, CAP>(sv, keep, p);
 #pragma unroll
       for (int e = 0; e < 32; e += 2) {
-        float2 y, keep = make_float2(1.f, 1.f);
-        if (!CAP && !ALIBI) {
-          y = apart(fma2(pair(__uint_as_float(sv[e]), __uint_as_float(sv[e + 1])), mul, m));
-        } else {
-          y.x = score<CAP, ALIBI>(__uint_as_float(sv[e]), p, slope2, far - e, keep.x) + neg_lse2;
-          y.y = score<CAP, ALIBI>(__uint_as_float(sv[e + 1]), p, slope2, far - (e + 1), keep.y) + neg_lse2;
-        }
-        y = exp2_of(y, e / 2);
-        if (CAP) y.x *= keep.x, y.y *= keep.y;
+        const uint64_t x = pair(__uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
+        float2 y = apart(fma2(x, mul, m));
+        if (ALIBI) y.x = fmaf(-slope2, fabsf(far - e), y.x), y.y = fmaf(-slope2, fabsf(far - (e + 1)), y.y);
+        y = exp2_of<CAP>(y, e / 2);
+        if (CAP) y.x *= keep[CAP ? e : 0], y.y *= keep[CAP ? e + 1 : 0];
         const float2 g = apart(mul2(pair(y.x, y.y), add2(pair(__uint_as_float(dv[e]), __uint_as_float(dv[e + 1])), nd)));
         sv[e] = __float_as_uint(g.x);
         sv[e + 1] = __float_as_uint(g.y);

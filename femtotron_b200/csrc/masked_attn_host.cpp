@@ -5,6 +5,7 @@
 #include <c10/cuda/CUDAGuard.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "masked_attn.h"
 #include "tmap.h"
@@ -86,6 +87,11 @@ void fill(Common& p, const Shape& n, const at::Tensor& rows, const at::Tensor& t
   p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
   p.cap_in = softcap > 0 ? static_cast<float>(2 * scale * 1.4426950408889634 / softcap) : 0.f;
   p.cap_out = static_cast<float>(softcap * 1.4426950408889634);
+  // tanh(x) / x at the Chebyshev nodes of x^2 in [0, 0.49] as a polynomial in x^2, with x = scale s / c put in
+  const double poly[5] = {0.999999702, -0.333301812, 0.132807881, -0.0508257188, 0.0137630384};
+  const double r = softcap > 0 ? scale / softcap : 0.0;
+  p.cap_small = softcap > 0 ? static_cast<float>(0.7 / r) : 0.f;
+  for (int i = 0; i < 5; ++i) p.cap_poly[i] = static_cast<float>(poly[i] * std::pow(r, 2 * i + 1));
   p.neg_lse2 = neg_lse2;
   p.err = err.data_ptr<int>();
 }

@@ -26,7 +26,7 @@ MAX_SLOTS = 8
 
 
 def _tables(tensors) -> int:
-    return (sum(t.numel() > 0 for t in tensors) + TABLE - 1) // TABLE
+    return (len(tensors) + TABLE - 1) // TABLE
 
 
 def _check(op: str, tensors) -> None:
@@ -56,10 +56,10 @@ def sum_of_squares(tensors, slots=None, n_slots: int = 1) -> torch.Tensor:
         raise ValueError(f"sum_of_squares: slots must be in [0, {n_slots}), of 1 to {MAX_SLOTS}")
     if not tensors:
         return torch.zeros(n_slots, dtype=torch.float64)
-    _check("sum_of_squares", tensors)
-    if tensors[0].is_cuda:
+    if tensors[0].is_cuda:  # (the entry points check all of this again, so it is not done twice)
         LAUNCHES[0] += _tables(tensors)  # and one that the proxy counts
         return native().grad_sumsq(tensors, slots, n_slots)
+    _check("sum_of_squares", tensors)
     out = torch.zeros(n_slots, dtype=torch.float64)
     for t, s in zip(tensors, slots):
         out[s] += t.detach().double().pow(2).sum()
@@ -78,16 +78,14 @@ def scale_grads(tensors, coef: torch.Tensor, out=None) -> None:
     one that is read)."""
     tensors = list(tensors)
     out = None if out is None else list(out)
-    if out is not None:
-        _check_out("scale_grads", tensors, out)
-    if not tensors:
-        return
-    _check("scale_grads", tensors)
     coef = coef.detach().reshape(())
-    if tensors[0].is_cuda:
-        LAUNCHES[0] += max(_tables(tensors), 1) - 1
+    if tensors and tensors[0].is_cuda and (out is None or out):
+        LAUNCHES[0] += _tables(tensors) - 1
         native().grad_scale(tensors, coef, out or [])
         return
+    if out is not None:
+        _check_out("scale_grads", tensors, out)
+    _check("scale_grads", tensors)
     _scale_cpu(tensors, coef, out)
 
 
@@ -100,14 +98,14 @@ def clip_grads(grads, max_norm: float, out=None) -> torch.Tensor:
     max_norm = float(max_norm)
     if not max_norm >= 0 or math.isinf(max_norm):
         raise ValueError(f"clip_grads: max_norm must be a number from 0 on, got {max_norm}")
+    if grads and grads[0].is_cuda and (out is None or out):
+        LAUNCHES[0] += 2 * _tables(grads) - 1
+        return native().grad_clip(grads, max_norm, out or [])
     if out is not None:
         _check_out("clip_grads", grads, out)
     if not grads:
         return torch.zeros(())
     _check("clip_grads", grads)
-    if grads[0].is_cuda:
-        LAUNCHES[0] += 2 * max(_tables(grads), 1) - 1
-        return native().grad_clip(grads, max_norm, out or [])
     norm = sum_of_squares(grads)[0].sqrt().float()
     _scale_cpu(grads, (max_norm / (norm + 1e-6)).clamp(max=1.0), out)
     return norm

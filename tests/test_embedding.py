@@ -113,7 +113,7 @@ def test_empty_and_refusals(device):
 
 
 @gpu
-@pytest.mark.parametrize("T,V", [(9000, 128257), (40000, 1200000), (5000, 1023), (5000, 1024)])
+@pytest.mark.parametrize("T,V", [(9000, 128257), (40000, 1200000), (5000, 1023), (5000, 1024), (8192, 262143), (8193, 262144), (7000, 1200000)])
 def test_gpu_large_vocabularies(T, V):
     g = torch.Generator().manual_seed(1)
     ids = (torch.exp(torch.rand(T, generator=g) * 12) - 1).long().clamp_(max=V - 1).cuda()

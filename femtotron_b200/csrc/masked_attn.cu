@@ -13,29 +13,31 @@ namespace ma {
 // them (8192 tokens: 25 us with a load per question, see below for what is left).
 constexpr int MASK_THREADS = 1024, PER = 8;
 
-// The largest v of the threads before this one (`none` for the first), and of all in `total`.
+// The largest v of the threads before this one (AFTER: behind it; `none` where there are none), and of all in `total`.
+template <bool AFTER>
 __device__ __forceinline__ int block_scan_max(int v, int none, int* warps, int& total) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  auto from = [](int x, int o) { return AFTER ? __shfl_down_sync(0xffffffff, x, o) : __shfl_up_sync(0xffffffff, x, o); };
+  const int edge = AFTER ? 31 - lane : lane;  // lanes on the side that is looked at
+  auto scan = [&](int x) {
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int u = __shfl_up_sync(0xffffffff, v, o);
-    if (lane >= o) v = max(v, u);
-  }
-  int before = __shfl_up_sync(0xffffffff, v, 1);
-  if (lane == 0) before = none;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = from(x, o);
+      if (edge >= o) x = max(x, u);
+    }
+    return x;
+  };
+  v = scan(v);
+  int beside = from(v, 1);
+  if (edge == 0) beside = none;
   __syncthreads();
-  if (lane == 31) warps[w] = v;
+  if (edge == 31) warps[w] = v;
   __syncthreads();
   // every warp scans the 32 totals by itself
-  int t = warps[lane];
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int u = __shfl_up_sync(0xffffffff, t, o);
-    if (lane >= o) t = max(t, u);
-  }
-  total = __shfl_sync(0xffffffff, t, 31);
-  const int ahead = __shfl_sync(0xffffffff, t, max(w - 1, 0));
-  return w ? max(before, ahead) : before;
+  const int t = scan(warps[lane]);
+  total = __shfl_sync(0xffffffff, t, AFTER ? 0 : 31);
+  const int ahead = __shfl_sync(0xffffffff, t, AFTER ? min(w + 1, 31) : max(w - 1, 0));
+  return (AFTER ? w < 31 : w > 0) ? max(beside, ahead) : beside;
 }
 
 // What the rows i0 ... i0 + 7 are: does a document begin, is there no mark, is it padding (bits of the result)
@@ -61,6 +63,22 @@ struct Tokens {
   }
 };
 
+// Eight rows, two per access; padded is a multiple of eight
+__device__ __forceinline__ void put_rows(int2* rows, int i0, int padded, const int2 (&r)[PER]) {
+  if (i0 >= padded) return;
+#pragma unroll
+  for (int e = 0; e < PER; e += 2)
+    reinterpret_cast<int4*>(rows + i0)[e / 2] = make_int4(r[e].x, r[e].y, r[e + 1].x, r[e + 1].y);
+}
+__device__ __forceinline__ void get_rows(const int2* rows, int i0, int padded, int2 (&r)[PER]) {
+#pragma unroll
+  for (int e = 0; e < PER; e += 2) {
+    const int4 two = i0 < padded ? reinterpret_cast<const int4*>(rows + i0)[e / 2] : make_int4(0, 0, 0, 0);
+    r[e] = make_int2(two.x, two.y);
+    r[e + 1] = make_int2(two.z, two.w);
+  }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(MASK_THREADS) mask_kernel(const MaskArgs a) {
   __shared__ int warps[32];
@@ -75,43 +93,39 @@ __global__ void __launch_bounds__(MASK_THREADS) mask_kernel(const MaskArgs a) {
     const uint32_t in = i0 >= S ? 0u : i0 + PER <= S ? 0xffu : (1u << (S - i0)) - 1;
     const uint32_t bg = k.begins & in, pl = k.plain & in;
     int all_f, all_u;
-    int f = max(block_scan_max(bg ? i0 + 31 - __clz(bg) : -1, -1, warps, all_f), carry_first);
-    int u = max(block_scan_max(pl ? i0 + 31 - __clz(pl) : -1, -1, warps, all_u), carry_plain);
+    int f = max(block_scan_max<false>(bg ? i0 + 31 - __clz(bg) : -1, -1, warps, all_f), carry_first);
+    int u = max(block_scan_max<false>(pl ? i0 + 31 - __clz(pl) : -1, -1, warps, all_u), carry_plain);
+    int2 r[PER];
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
       if (bg >> e & 1) f = i0 + e;
       if (pl >> e & 1) u = i0 + e;
-      if (in >> e & 1) rows[i0 + e] = make_int2(f, u < f);  // .y: does the row lead
+      r[e] = make_int2(f, u < f);  // .y: does the row lead
     }
+    put_rows(rows, i0, a.padded, r);
     carry_first = max(carry_first, all_f);
     carry_plain = max(carry_plain, all_u);
   }
-  __syncthreads();  // the rows go on to other threads
-  // backward, with the order of rows turned so that the same scan serves: -(place) grows
+  // backward: the largest of the negative places of the threads behind; each thread reads the rows that it wrote
   int carry = -S;
-  for (int c = (a.padded + chunk - 1) / chunk - 1; c >= 0; --c) {
-    const int i0 = c * chunk + (MASK_THREADS - 1 - static_cast<int>(threadIdx.x)) * PER;
+  for (int c0 = (a.padded - 1) / chunk * chunk; c0 >= 0; c0 -= chunk) {
+    const int i0 = c0 + threadIdx.x * PER;
     const Tokens<T> k(a, b, i0);
-    int2 got[PER];
-#pragma unroll
-    for (int e = 0; e < PER; ++e) got[e] = i0 + e < S ? rows[i0 + e] : make_int2(0, 0);
+    int2 r[PER];
+    get_rows(rows, i0, a.padded, r);
     const uint32_t in = i0 >= S ? 0u : i0 + PER <= S ? 0xffu : (1u << (S - i0)) - 1;
     const uint32_t stops = (k.begins | (a.causal && a.marks ? k.plain : 0u)) & in;
     int all;
-    int next = max(block_scan_max(stops ? -(i0 + __ffs(stops) - 1) : -kNever, -kNever, warps, all), carry);
+    int next = max(block_scan_max<true>(stops ? -(i0 + __ffs(stops) - 1) : -kNever, -kNever, warps, all), carry);
     int4 t = make_int4(kNever, 0, kNever, 0);
 #pragma unroll
     for (int e = PER - 1; e >= 0; --e) {
-      const int i = i0 + e;
-      int2 r = make_int2(kNever, 0);
-      if (!(k.dead >> e & 1)) {
-        const int hi = !a.causal || (a.marks && got[e].y) ? min(S, -next) : i + 1;
-        r = make_int2(max(got[e].x, i - a.window + 1), min(hi, i + a.window));
-      }
-      if (i < a.padded) rows[i] = r;
-      t = make_int4(min(t.x, r.x), max(t.y, r.x), min(t.z, r.y), max(t.w, r.y));
+      const int i = i0 + e, hi = !a.causal || (a.marks && r[e].y) ? min(S, -next) : i + 1;
+      r[e] = k.dead >> e & 1 ? make_int2(kNever, 0) : make_int2(max(r[e].x, i - a.window + 1), min(hi, i + a.window));
+      t = make_int4(min(t.x, r[e].x), max(t.y, r[e].x), min(t.z, r[e].y), max(t.w, r[e].y));
       if (stops >> e & 1) next = -i;
     }
+    put_rows(rows, i0, a.padded, r);
     // 16 threads of 8 rows each: two tiles per warp
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) {
@@ -120,7 +134,7 @@ __global__ void __launch_bounds__(MASK_THREADS) mask_kernel(const MaskArgs a) {
       t.z = min(t.z, __shfl_xor_sync(0xffffffff, t.z, o));
       t.w = max(t.w, __shfl_xor_sync(0xffffffff, t.w, o));
     }
-    if ((threadIdx.x & 15) == 15 && i0 < a.padded) tiles[i0 / TILE] = t;
+    if ((threadIdx.x & 15) == 0 && i0 < a.padded) tiles[i0 / TILE] = t;
     carry = max(carry, all);
   }
 }

@@ -22,8 +22,11 @@ __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ BwdP
     const uint32_t unit = u0 + k * step, h = unit % p.nq;
     const int i = static_cast<int>(unit / p.nq);
     stat[k] = unit < total ? (static_cast<int64_t>(b) * p.nq + h) * p.padded + i : -1;
-    live[k] = unit < total && i < p.S && part * 8 < p.d && p.rows[b * p.rows_stride + i].y > 0;
-    if (live[k]) {
+    // loaded wherever there is a row, whether it sees anything or not: nothing waits for the mask
+    const bool in = unit < total && i < p.S;
+    live[k] = in && p.rows[b * p.rows_stride + i].y > 0;
+    x[k] = l[k] = y[k] = make_uint4(0, 0, 0, 0);
+    if (in && part * 8 < p.d) {
       const __nv_bfloat16* o = at(p.o, b, i, h) + part * 8;
       x[k] = __ldg(reinterpret_cast<const uint4*>(o));
       l[k] = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.low) +
@@ -34,7 +37,7 @@ __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ BwdP
 #pragma unroll
   for (int k = 0; k < DELTA_UNITS; ++k) {
     float acc = 0.f;
-    if (live[k]) {
+    {
       const uint32_t xs[4] = {x[k].x, x[k].y, x[k].z, x[k].w}, ls[4] = {l[k].x, l[k].y, l[k].z, l[k].w},
                      ys[4] = {y[k].x, y[k].y, y[k].z, y[k].w};
 #pragma unroll
@@ -45,7 +48,7 @@ __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ BwdP
     }
 #pragma unroll
     for (int w = 8; w > 0; w >>= 1) acc += __shfl_xor_sync(0xffffffff, acc, w);
-    if (part == 0 && stat[k] >= 0) p.neg_delta[stat[k]] = -acc;
+    if (part == 0 && stat[k] >= 0) p.neg_delta[stat[k]] = live[k] ? -acc : 0.f;
   }
 }
 

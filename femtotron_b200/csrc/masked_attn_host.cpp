@@ -92,6 +92,7 @@ void fill(Common& p, const Shape& n, const at::Tensor& rows, const at::Tensor& t
   const double r = softcap > 0 ? scale / softcap : 0.0;
   p.cap_small = softcap > 0 ? static_cast<float>(0.7 / r) : 0.f;
   for (int i = 0; i < 5; ++i) p.cap_poly[i] = static_cast<float>(poly[i] * std::pow(r, 2 * i + 1));
+  if (!std::isfinite(p.cap_poly[4])) p.cap_small = -1.f;  // a cap so small that only the other form serves
   p.neg_lse2 = neg_lse2;
   p.err = err.data_ptr<int>();
 }

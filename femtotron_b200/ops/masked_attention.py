@@ -30,6 +30,7 @@ import math
 from dataclasses import dataclass
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .ext import LAUNCHES, error_flag, native
 
@@ -174,6 +175,7 @@ class MaskedAttnFn(torch.autograd.Function):
         return _forward(ctx, q, k, v, mask, scale, softcap, slopes, graded, q, k, v)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, do):
         q, k, v, o, low, lse, rows, tiles, slopes = ctx.saved_tensors
         dq, dk, dv = (torch.empty_like(x, memory_format=torch.contiguous_format) for x in (q, k, v))
@@ -195,6 +197,7 @@ class MaskedAttnPackedFn(torch.autograd.Function):
         return _forward(ctx, *_heads(qkv, nq, nkv), mask, scale, softcap, slopes, graded, qkv)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, do):
         qkv, o, low, lse, rows, tiles, slopes = ctx.saved_tensors
         d = torch.empty_like(qkv, memory_format=torch.contiguous_format)
@@ -246,8 +249,8 @@ def _check(q, k, v, mask, scale, softcap, slopes):
         raise ValueError(f"masked_attention: a mask of {mask.batch} x {mask.seq_len} for {q.shape[0]} x {q.shape[1]} tokens")
     if not (scale > 0 and math.isfinite(scale)):
         raise ValueError(f"masked_attention: scale must be positive, got {scale}")
-    if not (softcap >= 0 and math.isfinite(softcap)):
-        raise ValueError(f"masked_attention: softcap must be 0 (none) or positive, got {softcap}")
+    if not (softcap >= 0 and math.isfinite(softcap)) or (softcap and not 1e-30 < scale / softcap < 1e30):
+        raise ValueError(f"masked_attention: softcap must be 0 (none) or positive, got {softcap} (and scale {scale})")
     if slopes is not None and (slopes.dtype != torch.float32 or tuple(slopes.shape) != (q.shape[2],)):
         raise ValueError(f"masked_attention: slopes must be one fp32 number per query head, got {slopes.dtype} "
                          f"{tuple(slopes.shape)}")

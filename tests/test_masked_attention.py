@@ -152,6 +152,15 @@ def test_padding_may_hold_nan():
         assert torch.equal(x, y) and not x[:, dead].any()
 
 
+def test_second_derivatives_are_refused():
+    q, k, v, do = make(1, 5, 2, 1, 4, 0, "cpu", torch.float32)
+    q.requires_grad_()
+    do.requires_grad_()
+    g, = torch.autograd.grad(MA.masked_attention(q, k, v, MA.attention_mask(1, 5)), q, do, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
+
+
 def test_slopes_and_document_ids():
     assert torch.equal(MA.alibi_slopes(8), torch.tensor([2.0 ** -i for i in range(1, 9)]))
     assert MA.alibi_slopes(12).shape == (12,)
@@ -191,8 +200,12 @@ def test_refusals():
         MA.masked_attention(q, k, v, mask, scale=0.0)
     with pytest.raises(ValueError, match="softcap"):
         MA.masked_attention(q, k, v, mask, softcap=-1.0)
+    with pytest.raises(ValueError, match="softcap"):
+        MA.masked_attention(q, k, v, mask, softcap=1e-40)
     with pytest.raises(ValueError, match="slopes"):
         MA.masked_attention(q, k, v, mask, slopes=torch.ones(nkv))
+    with pytest.raises(ValueError, match="does not hold"):
+        MA.masked_attention_packed(torch.zeros(B, S, 5, d), 4, 2, mask)
 
 
 # ------------------------------------------------------------------------------ GPU
@@ -201,7 +214,7 @@ gpu = pytest.mark.gpu
 
 @gpu
 @pytest.mark.parametrize("kind", KINDS)
-@pytest.mark.parametrize("B,S", [(1, 1), (2, 130), (3, 5000)])
+@pytest.mark.parametrize("B,S", [(1, 1), (2, 130), (3, 5000), (2, 20000)])
 def test_gpu_mask_equals_the_cpu_mask(kind, B, S):
     parts = mask_parts(kind, B, S, 3)
     on_gpu = {n: x.cuda() if torch.is_tensor(x) else x for n, x in parts.items()}
@@ -240,6 +253,21 @@ def test_gpu_masks(kind):
 @pytest.mark.parametrize("kind", ["causal", "all", "docs both ways"])
 def test_gpu_scores(kind, softcap, bias):
     check_gpu(2, 389, 4, 4, 128, kind, softcap=softcap, bias=bias, spread=2.0)
+
+
+@gpu
+@pytest.mark.parametrize("softcap", [1e-7, 1e-3, 0.2, 1e5])
+def test_gpu_caps_of_any_size(softcap):
+    # tiny caps make every score +-cap (and zero scores, q = 0, stay 0), large ones change nothing
+    q, k, v, do = make(1, 150, 2, 1, 64, 3, "cuda", torch.bfloat16)
+    q[:, 10:20] = 0
+    mask = MA.attention_mask(1, 150, device="cuda")
+    got = run(q, k, v, do, mask, softcap=softcap)
+    vis = torch.ones(150, 150, dtype=torch.bool).tril()[None]
+    want, size = reference(q, k, v, do, vis, 1 / 8, softcap, None)
+    for x, y, z in zip(got, want, size):
+        # as check_gpu, and what fp32 loses of 1 - tanh^2 next to 1: 2^-22 of the largest terms
+        assert ((x.double() - y).abs() <= (2 * U16 + 2 ** -14) * z + U16 * y.abs() + 2 ** -22 * z.max() + 1e-30).all()
 
 
 @gpu
@@ -315,6 +343,9 @@ def test_gpu_strides_and_packed_views():
         o = MA.masked_attention(*leaves, mask)
         got = [o.detach(), *torch.autograd.grad(o, leaves, xs[3])]
         assert all(torch.equal(x, y) for x, y in zip(got, want))
+    leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+    MA.masked_attention(*leaves, mask).sum().backward()  # an expanded gradient, all strides 0
+    assert all(torch.equal(x.grad, y) for x, y in zip(leaves, run(q, k, v, torch.ones_like(do), mask)[1:]))
     wide = torch.randn(B, S, nkv, 1, device="cuda", dtype=torch.bfloat16).expand(B, S, nkv, d)
     full = run(q, k, wide.contiguous(), do, mask)
     leaves = [x.detach().requires_grad_() for x in (q, k, wide)]

@@ -198,7 +198,8 @@ __device__ __forceinline__ float scores(uint32_t (&sv)[STEP], const Common& p, f
 template <bool CAP, bool ALIBI>
 __global__ void __launch_bounds__(NTHREADS, 1)
     fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-               const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ FwdParams p) {
+               const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o,
+               const __grid_constant__ CUtensorMap tm_low, const __grid_constant__ FwdParams p) {
   using Sm = FwdSmem;
   extern __shared__ uint8_t smem_raw[];
   Sm& s = *reinterpret_cast<Sm*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -327,36 +328,40 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       if (lane == 0) mbar_arrive(&s.p_full[t][buf]);
     }
     if (n > 0 && ok) ok = wait_warp(&s.done[t], 0, p.err, 321);
-    if (real && ok) {
+    // a tile without keys may still wait for its queries, whose place its output takes
+    if (n == 0 && j0 < j1) ok = wait_warp(&s.q_full, 0, p.err, 322);
+    if (real) {
       tc_fence_after();
-      const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
-      __nv_bfloat16* out = at(p.o, b, row, h);
-      for (int c = 0; c < p.ksteps; ++c) {
-        uint32_t ov[16];
-        if (n > 0) {
-          tmem_ld_32x32b_x16(tO(t) + lane_off + c * 16, ov);
-          tmem_wait_ld();
-        }
-        if (row < p.S) {
-          // a sum of NaN stays one (l is NaN then, not 0)
-          if (n == 0 || l_run == 0.f) zero16(out + c * 16, p.d - c * 16);
-          else store16(out + c * 16, ov, l_run == l_run ? inv : l_run, p.d - c * 16);
-          if (p.low) {
-            __nv_bfloat16* low = static_cast<__nv_bfloat16*>(p.low) + (out - static_cast<__nv_bfloat16*>(p.o.p)) + c * 16;
-            if (n == 0 || l_run == 0.f) {
-              zero16(low, p.d - c * 16);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const float v = __uint_as_float(ov[i]) * inv;
-                ov[i] = __float_as_uint(v - __bfloat162float(__float2bfloat16_rn(v)));
-              }
-              store16(low, ov, 1.f, p.d - c * 16);
-            }
+      const bool none = n == 0 || l_run == 0.f;
+      const float inv = none ? 0.f : 1.f / l_run;
+      // (the barriers are met also after a wait that ran out)
+      auto pass = [&](bool rest) {
+        for (int c = 0; ok && c < p.ksteps; ++c) {
+          uint32_t ov[16] = {};
+          if (n > 0) {
+            tmem_ld_32x32b_x16(tO(t) + lane_off + c * 16, ov);
+            tmem_wait_ld();
           }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float v = none ? 0.f : __uint_as_float(ov[i]) * inv;  // a sum that is NaN stays one
+            ov[i] = __float_as_uint(rest ? v - __bfloat162float(__float2bfloat16_rn(v)) : v);
+          }
+          stage16(s.q[t], r, c, ov, 1.f);
         }
+        fence_proxy_async_smem();
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory");  // the four warps of this tile
+        if (ok && quad == 0 && lane == 0) {
+          tma_store_tile(rest ? &tm_low : &tm_o, s.q[t], chunks, h, tile * TILE, b);
+          tma_store_wait_read();
+        }
+      };
+      pass(false);
+      if (p.rest) {
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory");
+        pass(true);
       }
-      if (p.neg_lse2)
+      if (p.neg_lse2 && ok)
         p.neg_lse2[(static_cast<int64_t>(b) * p.nq + h) * p.padded + row] =
             l_run == 0.f ? -INFINITY : -(m_used + log2f(l_run));
     }
@@ -466,15 +471,15 @@ cudaError_t launch_mask(const MaskArgs& a, int batch, cudaStream_t st) {
   return cudaGetLastError();
 }
 
-cudaError_t launch_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const FwdParams& p, bool cap,
-                       bool bias, cudaStream_t st) {
+cudaError_t launch_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& to,
+                       const CUtensorMap& tlow, const FwdParams& p, bool cap, bool bias, cudaStream_t st) {
   static_assert(sizeof(FwdSmem) + 1024 <= 232448, "shared memory");
   const dim3 grid(p.B * (p.pair_heads ? p.nq / 2 : p.nq), p.pair_heads ? p.ntiles : (p.ntiles + 1) / 2);
   pick(cap, bias, [&](auto CAP, auto BIAS) {
     constexpr auto kernel = fwd_kernel<decltype(CAP)::value, decltype(BIAS)::value>;
     static unsigned long long cfg = 0;
     smem_attr_once(kernel, sizeof(FwdSmem) + 1024, cfg);
-    kernel<<<grid, NTHREADS, sizeof(FwdSmem) + 1024, st>>>(tq, tk, tv, p);
+    kernel<<<grid, NTHREADS, sizeof(FwdSmem) + 1024, st>>>(tq, tk, tv, to, tlow, p);
   });
   return cudaGetLastError();
 }

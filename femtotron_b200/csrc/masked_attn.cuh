@@ -225,15 +225,23 @@ __device__ __forceinline__ void note_dead(uint32_t* words, const int4* tiles, in
 }
 __device__ __forceinline__ bool is_dead(const uint32_t* words, int t) { return (words[t >> 5] >> (t & 31)) & 1; }
 
-// 16 fp32 TMEM columns times f as bf16 to out[0..16), of which the first n are real (n a multiple of 8)
-__device__ __forceinline__ void store16(__nv_bfloat16* out, const uint32_t (&v)[16], float f, int n) {
+// Results leave through shared memory and TMA: a thread has a row of a tile, and 32 rows of 16 bytes each, kilobytes apart, are
+// the slowest way to memory (forward pass of 8192 tokens 180 -> 169 us).  The tile is laid
+// out as it would have been loaded; rows behind the last token and values behind d are not written.
+__device__ __forceinline__ void stage16(void* tile, int r, int c, const uint32_t (&v)[16], float f) {
+  uint8_t* row = static_cast<uint8_t*>(tile) + (c >> 2) * PIECE + r * 128;
   auto p = [&](int i) { return pack_bf16x2(__uint_as_float(v[i]) * f, __uint_as_float(v[i + 1]) * f); };
-  if (n > 0) *reinterpret_cast<uint4*>(out) = make_uint4(p(0), p(2), p(4), p(6));
-  if (n > 8) *reinterpret_cast<uint4*>(out + 8) = make_uint4(p(8), p(10), p(12), p(14));
+  const int u = (c & 3) * 2;
+  *reinterpret_cast<uint4*>(row + ((u ^ (r & 7)) * 16)) = make_uint4(p(0), p(2), p(4), p(6));
+  *reinterpret_cast<uint4*>(row + (((u + 1) ^ (r & 7)) * 16)) = make_uint4(p(8), p(10), p(12), p(14));
 }
-__device__ __forceinline__ void zero16(__nv_bfloat16* out, int n) {
-  if (n > 0) *reinterpret_cast<uint4*>(out) = make_uint4(0, 0, 0, 0);
-  if (n > 8) *reinterpret_cast<uint4*>(out + 8) = make_uint4(0, 0, 0, 0);
+__device__ __forceinline__ void tma_store_tile(const CUtensorMap* map, const void* tile, int chunks, int head, int row, int b) {
+  for (int c = 0; c < chunks; ++c)
+    asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(
+                     reinterpret_cast<uint64_t>(map)),
+                 "r"(smem_u32(static_cast<const uint8_t*>(tile) + c * PIECE)), "r"(c * 64), "r"(head), "r"(row), "r"(b)
+                 : "memory");
+  tma_store_commit();
 }
 
 __device__ __forceinline__ __nv_bfloat16* at(const Out& x, int b, int s, int h) {

@@ -73,16 +73,15 @@ struct Out {  // a [batch, tokens, heads, d] tensor of bf16, strides in elements
 };
 
 struct FwdParams : Common {
-  Out o;
-  void* low;               // what o's rounding to bf16 left out, in bf16 and laid out like o; or null
   bool pair_heads;
+  bool rest;               // write what o's rounding to bf16 left out, in bf16
 };
 
 struct BwdParams : Common {
   Out o;
-  const void* low;
+  const void* low;         // what o's rounding to bf16 left out, in bf16 and laid out like o
   float* neg_delta;        // [B, nq, padded], -rowsum(do o)
-  Out dq, dk, dv;
+  Out dk, dv;
   int split;               // blocks that share the query heads of a group, and with more than one
   float* part;             // [split][2 (dv, dk)][B, nkv, padded][d]: their sums, joined in order
 };
@@ -90,13 +89,13 @@ struct BwdParams : Common {
 // Each returns what cudaGetLastError() says.  launch_delta comes before the other two of the
 // backward pass.
 cudaError_t launch_mask(const MaskArgs& a, int batch, cudaStream_t st);
-cudaError_t launch_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const FwdParams& p, bool cap,
-                       bool bias, cudaStream_t st);
+cudaError_t launch_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& to,
+                       const CUtensorMap& tlow, const FwdParams& p, bool cap, bool bias, cudaStream_t st);
 cudaError_t launch_delta(const BwdParams& p, const Out& dout, cudaStream_t st);
 cudaError_t launch_dq(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& td,
-                      const BwdParams& p, bool cap, bool bias, cudaStream_t st);
+                      const CUtensorMap& tdq, const BwdParams& p, bool cap, bool bias, cudaStream_t st);
 cudaError_t launch_dkv(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& td,
-                       const BwdParams& p, bool cap, bool bias, cudaStream_t st);
+                       const CUtensorMap& tdk, const CUtensorMap& tdv, const BwdParams& p, bool cap, bool bias, cudaStream_t st);
 
 }  // namespace ma
 }  // namespace ft

@@ -27,6 +27,7 @@ template <bool CAP, bool ALIBI>
 __global__ void __launch_bounds__(NTHREADS, 1)
     dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
+               const __grid_constant__ CUtensorMap tm_dk, const __grid_constant__ CUtensorMap tm_dv,
                const __grid_constant__ BwdParams p) {
   using Sm = DkvSmem;
   extern __shared__ uint8_t smem_raw[];
@@ -149,11 +150,11 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     if (n > 0 && ok) ok = wait_warp(&s.done, 0, p.err, 364);
     if (ok) {
       tc_fence_after();
+      // the keys and values are no longer needed: dk and dv take their places on the way out
 #pragma unroll
       for (int which = 0; which < 2; ++which) {
-        __nv_bfloat16* out = at(which ? p.dk : p.dv, b, key, kvh);
         for (int c = half; c < p.ksteps; c += 2) {
-          uint32_t v[16];
+          uint32_t v[16] = {};
           if (n > 0) {
             tmem_ld_32x32b_x16((which ? tdK : tdV) + lane_off + c * 16, v);
             tmem_wait_ld();
@@ -165,16 +166,20 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 #pragma unroll
             for (int i = 0; i < 16; i += 4)
               if (i < m)
-                *reinterpret_cast<float4*>(part + i) =
-                    n == 0 ? make_float4(0.f, 0.f, 0.f, 0.f)
-                           : make_float4(__uint_as_float(v[i]), __uint_as_float(v[i + 1]), __uint_as_float(v[i + 2]),
-                                         __uint_as_float(v[i + 3]));
-          } else if (key < p.S) {
-            if (n == 0) zero16(out + c * 16, p.d - c * 16);
-            else store16(out + c * 16, v, which ? p.scale : 1.f, p.d - c * 16);
+                *reinterpret_cast<float4*>(part + i) = make_float4(__uint_as_float(v[i]), __uint_as_float(v[i + 1]),
+                                                                   __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
+          } else {
+            stage16(which ? s.k : s.v, quad * 32 + lane, c, v, which ? p.scale : 1.f);
           }
         }
       }
+      fence_proxy_async_smem();
+    }
+    asm volatile("bar.sync 1, 256;" ::: "memory");  // the compute warps, also after a wait that ran out
+    if (ok && p.split == 1 && threadIdx.x == 0) {
+      tma_store_tile(&tm_dv, s.v, chunks, kvh, k0, b);
+      tma_store_tile(&tm_dk, s.k, chunks, kvh, k0, b);
+      tma_store_wait_read();
     }
   } else if (warp == PRODUCER_WARP) {
     if (n > 0) {
@@ -274,7 +279,6 @@ __global__ void __launch_bounds__(256) join_kernel(const BwdParams p) {
   const int key = static_cast<int>(row % p.padded);
   if (key >= p.S) return;
   const int bk = static_cast<int>(row / p.padded), c = static_cast<int>(j % units) * 8;
-  uint32_t v[16];
   float acc[8] = {};
   for (int sp = 0; sp < p.split; ++sp) {
     const float4* part = reinterpret_cast<const float4*>(
@@ -283,19 +287,21 @@ __global__ void __launch_bounds__(256) join_kernel(const BwdParams p) {
     acc[0] += x.x, acc[1] += x.y, acc[2] += x.z, acc[3] += x.w;
     acc[4] += y.x, acc[5] += y.y, acc[6] += y.z, acc[7] += y.w;
   }
-#pragma unroll
-  for (int k = 0; k < 16; ++k) v[k] = k < 8 ? __float_as_uint(acc[k]) : 0u;
-  store16(at(which ? p.dk : p.dv, bk / p.nkv, key, bk % p.nkv) + c, v, which ? p.scale : 1.f, 8);
+  const float f = which ? p.scale : 1.f;
+  *reinterpret_cast<uint4*>(at(which ? p.dk : p.dv, bk / p.nkv, key, bk % p.nkv) + c) =
+      make_uint4(pack_bf16x2(acc[0] * f, acc[1] * f), pack_bf16x2(acc[2] * f, acc[3] * f),
+                 pack_bf16x2(acc[4] * f, acc[5] * f), pack_bf16x2(acc[6] * f, acc[7] * f));
 }
 
 cudaError_t launch_dkv(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& td,
-                       const BwdParams& p, bool cap, bool bias, cudaStream_t st) {
+                       const CUtensorMap& tdk, const CUtensorMap& tdv, const BwdParams& p, bool cap, bool bias,
+                       cudaStream_t st) {
   static_assert(sizeof(DkvSmem) + 1024 <= 232448, "shared memory");
   pick(cap, bias, [&](auto CAP, auto BIAS) {
     constexpr auto kernel = dkv_kernel<decltype(CAP)::value, decltype(BIAS)::value>;
     static unsigned long long cfg = 0;
     smem_attr_once(kernel, sizeof(DkvSmem) + 1024, cfg);
-    kernel<<<dim3(p.B * p.nkv * p.split, p.ntiles), NTHREADS, sizeof(DkvSmem) + 1024, st>>>(tq, tk, tv, td, p);
+    kernel<<<dim3(p.B * p.nkv * p.split, p.ntiles), NTHREADS, sizeof(DkvSmem) + 1024, st>>>(tq, tk, tv, td, tdk, tdv, p);
   });
   if (p.split > 1) {
     const int64_t n = static_cast<int64_t>(p.B) * p.nkv * p.padded * (p.d / 8) * 2;

@@ -71,7 +71,7 @@ template <bool CAP, bool ALIBI>
 __global__ void __launch_bounds__(NTHREADS, 1)
     dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
               const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
-              const __grid_constant__ BwdParams p) {
+              const __grid_constant__ CUtensorMap tm_dq, const __grid_constant__ BwdParams p) {
   using Sm = DqSmem;
   extern __shared__ uint8_t smem_raw[];
   Sm& s = *reinterpret_cast<Sm*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -160,19 +160,28 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       if (lane == 0) mbar_arrive(&s.ds_full[buf]);
     }
     if (n > 0 && ok) ok = wait_warp(&s.done, 0, p.err, 343);
-    if (ok) {
+    if (!ok) {
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+    } else {
       tc_fence_after();
-      __nv_bfloat16* out = at(p.dq, b, row, h);
+      // the queries are no longer needed: dq takes their place on the way out
       for (int c = half; c < p.ksteps; c += 2) {
-        uint32_t v[16];
+        uint32_t v[16] = {};
         if (n > 0) {
           tmem_ld_32x32b_x16(tdQ + lane_off + c * 16, v);
           tmem_wait_ld();
         }
-        if (row < p.S) {
-          if (width == 0) zero16(out + c * 16, p.d - c * 16);
-          else store16(out + c * 16, v, p.scale, p.d - c * 16);
+        if (width == 0) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] = 0u;
         }
+        stage16(s.q, quad * 32 + lane, c, v, p.scale);
+      }
+      fence_proxy_async_smem();
+      asm volatile("bar.sync 1, 256;" ::: "memory");  // the compute warps
+      if (threadIdx.x == 0) {
+        tma_store_tile(&tm_dq, s.q, chunks, h, qt * TILE, b);
+        tma_store_wait_read();
       }
     }
   } else if (warp == PRODUCER_WARP) {
@@ -261,13 +270,13 @@ cudaError_t launch_delta(const BwdParams& p, const Out& dout, cudaStream_t st) {
 }
 
 cudaError_t launch_dq(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& td,
-                      const BwdParams& p, bool cap, bool bias, cudaStream_t st) {
+                      const CUtensorMap& tdq, const BwdParams& p, bool cap, bool bias, cudaStream_t st) {
   static_assert(sizeof(DqSmem) + 1024 <= 232448, "shared memory");
   pick(cap, bias, [&](auto CAP, auto BIAS) {
     constexpr auto kernel = dq_kernel<decltype(CAP)::value, decltype(BIAS)::value>;
     static unsigned long long cfg = 0;
     smem_attr_once(kernel, sizeof(DqSmem) + 1024, cfg);
-    kernel<<<dim3(p.B * p.nq, p.ntiles), NTHREADS, sizeof(DqSmem) + 1024, st>>>(tq, tk, tv, td, p);
+    kernel<<<dim3(p.B * p.nq, p.ntiles), NTHREADS, sizeof(DqSmem) + 1024, st>>>(tq, tk, tv, td, tdq, p);
   });
   return cudaGetLastError();
 }

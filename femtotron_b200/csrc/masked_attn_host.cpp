@@ -166,10 +166,10 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>, c10::optional<at::Tensor>> mas
   const at::Tensor q = usable(q_), k = usable(k_), v = usable(v_);
   FwdParams p;
   fill(p, n, rows, tiles, scale, softcap, slopes, graded ? lse->data_ptr<float>() : nullptr, err);
-  p.o = out_of(o);
-  p.low = graded ? low->data_ptr() : nullptr;
+  p.rest = graded;
   p.pair_heads = p.group % 2 == 0;
-  C10_CUDA_CHECK(launch_fwd(heads_map(q, TILE), heads_map(k, STEP), heads_map(v, STEP), p, softcap > 0, slopes.has_value(),
+  C10_CUDA_CHECK(launch_fwd(heads_map(q, TILE), heads_map(k, STEP), heads_map(v, STEP), heads_map(o, TILE),
+                            heads_map(graded ? *low : o, TILE), p, softcap > 0, slopes.has_value(),
                             at::cuda::getCurrentCUDAStream()));
   return {o, lse, low};
 }
@@ -203,7 +203,6 @@ int64_t masked_attn_bwd(const at::Tensor& q_, const at::Tensor& k_, const at::Te
   p.neg_delta = delta.data_ptr<float>();
   p.o = out_of(o);
   p.low = low.data_ptr();
-  p.dq = out_of(dq);
   p.dk = out_of(dk);
   p.dv = out_of(dv);
   // Few key tiles leave SMs idle and one block with the whole group's work: then the group is split, as far as
@@ -221,9 +220,11 @@ int64_t masked_attn_bwd(const at::Tensor& q_, const at::Tensor& k_, const at::Te
     p.part = part.data_ptr<float>();
   }
   C10_CUDA_CHECK(launch_delta(p, out_of(dout), st));
-  C10_CUDA_CHECK(launch_dq(heads_map(q, TILE), heads_map(k, STEP), heads_map(v, STEP), heads_map(dout, TILE), p, softcap > 0,
+  C10_CUDA_CHECK(launch_dq(heads_map(q, TILE), heads_map(k, STEP), heads_map(v, STEP), heads_map(dout, TILE),
+                           heads_map(dq, TILE), p, softcap > 0,
                            slopes.has_value(), st));
-  C10_CUDA_CHECK(launch_dkv(heads_map(q, STEP), heads_map(k, TILE), heads_map(v, TILE), heads_map(dout, STEP), p,
+  C10_CUDA_CHECK(launch_dkv(heads_map(q, STEP), heads_map(k, TILE), heads_map(v, TILE), heads_map(dout, STEP),
+                            heads_map(dk, TILE), heads_map(dv, TILE), p,
                             softcap > 0, slopes.has_value(), st));
   return p.split > 1 ? 4 : 3;
 }

@@ -159,10 +159,14 @@ struct FwdSmem {
   uint32_t tmem_base;
 };
 
-// Probabilities of 32 keys relative to 2^m from their scores (times `mul`, log2 units), as bf16 pairs; their fp32
-// sums in `sums` (of the unrounded values: only p v sees the rounding).  A score of -inf gives 0.
+// Probabilities of 32 keys relative to 2^m from their scores (times `mul`, log2 units), as bf16 pairs; their fp32 sums
+// before and after that rounding in `sums` and `used`.  The first are the softmax's (and the backward's); the values'
+// weighted sum is divided by the second, so that its weights add up to 1: what rounding does to a weight then counts against
+// v_j - o instead of v_j, which where a row has one or two large weights is the difference between an exact and a rounded
+// o, and, by way of rowsum(do o), dq.  A score of -inf gives 0.
 template <bool CAP, bool TEST>
-__device__ __forceinline__ void probs32(const uint32_t* sv, float mul, float m, uint64_t& sums, uint32_t (&pk)[16]) {
+__device__ __forceinline__ void probs32(const uint32_t* sv, float mul, float m, uint64_t& sums, uint64_t& used,
+                                        uint32_t (&pk)[16]) {
   const uint64_t mul2_ = pair(mul, mul), m2 = pair(-m, -m);
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
@@ -172,6 +176,7 @@ __device__ __forceinline__ void probs32(const uint32_t* sv, float mul, float m, 
     if (TEST && on_fma_pipe<CAP>(e)) y = make_float2(y0.x == -INFINITY ? 0.f : y.x, y0.y == -INFINITY ? 0.f : y.y);
     sums = add2(sums, pair(y.x, y.y));
     pk[e] = pack_bf16x2(y.x, y.y);
+    used = add2(used, pair(__uint_as_float(pk[e] << 16), __uint_as_float(pk[e] & 0xffff0000u)));
   }
 }
 
@@ -263,7 +268,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     const int row = tile * TILE + r;
     const uint32_t lane_off = static_cast<uint32_t>(quad * 32) << 16;
     const int n = (t ? end1 : end0) - begin;
-    float m_used = -INFINITY, l_run = 0.f;
+    float m_used = -INFINITY, l_run = 0.f, l_used = 0.f;
     bool ok = true;
     int lo = 0, width = 0;
     int4 sum = make_int4(0, 0, 0, 0);
@@ -300,6 +305,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         tc_fence_after();
         const float alpha = m_used == -INFINITY ? 0.f : ex2_approx(m_used - m_new);
         l_run *= alpha;
+        l_used *= alpha;
         for (int cc = 0; cc < p.ksteps; ++cc) {
           uint32_t ov[16];
           const uint32_t ta = tO(t) + lane_off + cc * 16;
@@ -312,17 +318,18 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       }
       m_used = m_new;
       const float m = m_used == -INFINITY ? 0.f : m_used;  // a row that has seen nothing yet
-      uint64_t sums = 0;
+      uint64_t sums = 0, used = 0;
 #pragma unroll
       for (int q = 0; q < STEP / 32; ++q) {
         uint32_t pk[16];
-        if (test) probs32<CAP, true>(sv + q * 32, mul, m, sums, pk);
-        else probs32<CAP, false>(sv + q * 32, mul, m, sums, pk);
+        if (test) probs32<CAP, true>(sv + q * 32, mul, m, sums, used, pk);
+        else probs32<CAP, false>(sv + q * 32, mul, m, sums, used, pk);
         tmem_st_32x32b_x16(ts + q * 16, pk);
       }
       tmem_wait_st();
-      const float2 two = apart(sums);
+      const float2 two = apart(sums), rounded = apart(used);
       l_run += two.x + two.y;
+      l_used += rounded.x + rounded.y;
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.p_full[t][buf]);
@@ -333,7 +340,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     if (real) {
       tc_fence_after();
       const bool none = n == 0 || l_run == 0.f;
-      const float inv = none ? 0.f : 1.f / l_run;
+      const float inv = none ? 0.f : 1.f / l_used;
       // (the barriers are met also after a wait that ran out)
       auto pass = [&](bool rest) {
         for (int c = 0; ok && c < p.ksteps; ++c) {

@@ -72,8 +72,9 @@ def attention_mask(batch: int, seq_len: int, *, causal: bool = True, window: int
             raise TypeError(f"attention_mask: {name} must be {' or '.join(str(t) for t in types)}, got {x.dtype}")
         if tuple(x.shape) != (batch, seq_len):
             raise ValueError(f"attention_mask: {name} of shape {tuple(x.shape)} for [{batch}, {seq_len}]")
-        if device is not None and x.device.type != torch.device(device).type:
-            raise ValueError(f"attention_mask: {name} is on {x.device}, the mask on {device}")
+        want = torch.device(device) if device is not None else (docs if docs is not None else prefix).device
+        if x.device.type != want.type or (want.index is not None and x.device.index != want.index):
+            raise ValueError(f"attention_mask: {name} is on {x.device}, the mask on {want}")
     given = docs if docs is not None else prefix
     device = given.device if given is not None else torch.device(device if device is not None else "cpu")
     if device.type == "cuda":

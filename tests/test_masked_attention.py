@@ -182,6 +182,11 @@ def test_refusals():
         MA.attention_mask(B, S, docs=torch.zeros(B, S))
     with pytest.raises(TypeError, match="prefix must be"):
         MA.attention_mask(B, S, prefix=torch.zeros(B, S, dtype=torch.int32))
+    with pytest.raises(ValueError, match="the mask on"):
+        MA.attention_mask(B, S, docs=torch.zeros(B, S, dtype=torch.int32), device="cuda")
+    with pytest.raises(ValueError, match="the mask on"):
+        MA.attention_mask(B, S, docs=torch.zeros(B, S, dtype=torch.int32),
+                          prefix=torch.zeros(B, S, dtype=torch.bool, device="meta"))
     with pytest.raises(ValueError, match="tokens"):
         MA.attention_mask(B, 0)
     with pytest.raises(ValueError, match="tokens"):
@@ -281,6 +286,32 @@ def test_gpu_sizes(S, nq, nkv, d):
 def test_gpu_long():
     check_gpu(1, 5003, 2, 1, 64, "padded")
     check_gpu(1, 5003, 2, 2, 128, "window")
+
+
+@gpu
+def test_gpu_longest_sequence_and_offsets_past_32_bits():
+    B, S, nq, nkv, d, w = 1, MA.MAX_TOKENS, 68, 4, 128, 100
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 60e9:
+        pytest.skip("needs 60 GB of free GPU memory")
+    g = torch.Generator(device="cuda").manual_seed(0)
+    q = torch.randn(B, S, nq, d, generator=g, device="cuda", dtype=torch.bfloat16).requires_grad_()
+    k, v = (torch.randn(B, S, nkv, d, generator=g, device="cuda", dtype=torch.bfloat16).requires_grad_() for _ in range(2))
+    assert q.numel() > 2 ** 31
+    o = MA.masked_attention(q, k, v, MA.attention_mask(1, S, window=w, device="cuda"))
+    do = torch.randn(B, S, nq, d, generator=g, device="cuda", dtype=torch.bfloat16)
+    grads = torch.autograd.grad(o, [q, k, v], do)
+    check_kernel_errors(q.device)
+    for end in (S, 130 * 1024 + 77):  # the last 300 rows and some in the middle, with what they see and what sees them
+        a = end - 600
+        part = [x.detach()[:, a:end] for x in (q, k, v, do)]
+        i = torch.arange(end - a)
+        vis = ((i[:, None] >= i) & (i[:, None] - i < w))[None]
+        want, size = reference(*part, vis, 1 / math.sqrt(d), 0.0, None)
+        for n, (x, y, z) in enumerate(zip([o.detach(), *grads], want, size)):
+            rows = slice(300, 600 if end == S or n < 2 else 500)  # later keys are seen from behind the piece
+            x, y, z = x[:, a:end][:, rows].double(), y[:, rows], z[:, rows]
+            assert ((x - y).abs() <= (2 * U16 + 2 ** -14) * z + U16 * y.abs()).all()
 
 
 @gpu

@@ -370,7 +370,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       }
       if (p.neg_lse2 && ok)
         p.neg_lse2[(static_cast<int64_t>(b) * p.nq + h) * p.padded + row] =
-            l_run == 0.f ? -INFINITY : -(m_used + log2f(l_run));
+            l_run == 0.f ? -INFINITY : -(m_used + log2f(l_run)) + 0.f * l_used;  // NaN where a score was
     }
   } else if (warp == PRODUCER_WARP) {
     // ------------------------------------------------------------ TMA producer
@@ -431,10 +431,10 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     auto arrived = [&](int j) {
       if (j < j1) ok = ok && wait_warp(&s.full[(j - j0) % KV_STAGES], ((j - j0) / KV_STAGES) & 1, p.err, 314);
     };
-    auto issue_o = [&](int j, int t, int first, int end) {
+    auto issue_o = [&](int j, int t, int first, int end, bool ready) {
       if (first > j || j >= end) return;
       const int c = j - first, buf = c & 1;
-      ok = ok && wait_warp(&s.p_full[t][buf], (c >> 1) & 1, p.err, 316);
+      ok = ok && (ready || wait_warp(&s.p_full[t][buf], (c >> 1) & 1, p.err, 316));
       if (!ok) return;
       tc_fence_after();
       mma_values(tO(t), tS(t, buf), 16, va + ((j - j0) % KV_STAGES) * stage, idO, c > 0, leader);
@@ -449,11 +449,14 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       issue_s(j, 1, first1, min(end1, j1));
     }
     for (int j = j0; ok && j < j1; ++j) {
-      arrived(j + 2);
-      issue_o(j, 0, first0, end0);
+      const int next = j + 2 - j0, c0 = j - first0, c1 = j - first1;
+      const uint32_t have = over(&s.full[next % KV_STAGES], (next / KV_STAGES) & 1, &s.p_full[0][c0 & 1], (c0 >> 1) & 1,
+                                 &s.p_full[1][c1 & 1], (c1 >> 1) & 1);
+      if (!(have & 1)) arrived(j + 2);
+      issue_o(j, 0, first0, end0, have & 2);
       if (!ok) break;
       issue_s(j + 2, 0, first0, end0);
-      issue_o(j, 1, first1, end1);
+      issue_o(j, 1, first1, end1, have & 4);
       if (!ok) break;
       commit(&s.empty[(j - j0) % KV_STAGES], leader);
       issue_s(j + 2, 1, first1, end1);

@@ -129,13 +129,20 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   return d;
 }
 
+// The larger value, NaN where one is NaN (fmaxf would drop it)
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // 2^x of two values on the FMA pipe, for x below 127.  Cody and Waite's reduction x = n + f: adding 1.5 2^23 rounds
 // to the integer n, which is left in the low bits, and f is in [-1/2, 1/2]; 2^f by the cubic that minimises the largest
 // relative error there (7.5e-5, found by linear programming over 4001 points; bf16 rounds by 2e-3), n goes into the exponent.
-// Below -125 the result is 2^-125.
+// Below -125 the result is 2^-125; a NaN gives the largest number there is, which bf16 rounds to infinity.
 __device__ __forceinline__ float2 exp2_pair(float a, float b) {
   const uint64_t shift = pair(12582912.f, 12582912.f);
-  const uint64_t x = pair(fmaxf(a, -125.f), fmaxf(b, -125.f));
+  const uint64_t x = pair(max_nan(a, -125.f), max_nan(b, -125.f));
   const uint64_t t = add2(x, shift);
   const uint64_t f = add2(x, fma2(t, pair(-1.f, -1.f), shift));
   uint64_t q = fma2(pair(0.0551716685f, 0.0551716685f), f, pair(0.2426111251f, 0.2426111251f));
@@ -145,6 +152,27 @@ __device__ __forceinline__ float2 exp2_pair(float a, float b) {
   // 1.5 2^23 + n has n in its low bits and nothing else in the low nine
   return make_float2(__uint_as_float(__float_as_uint(qs.x) + (__float_as_uint(ts.x) << 23)),
                      __uint_as_float(__float_as_uint(qs.y) + (__float_as_uint(ts.y) << 23)));
+}
+
+// Whether each of three phases is over (bits 0 to 2), for a whole warp, without waiting.  The three answers are under way
+// together: where products read all that shared memory gives, each takes its time, and the MMA warp asks for all that its
+// step needs at once (forward of 16384 tokens, 8 heads: 495 -> 489 us; no gain in the two backward kernels, which ask singly).
+// The phase before the one asked for has to be over already: two phases back has the same parity.
+__device__ __forceinline__ uint32_t over(uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb, uint64_t* c, uint32_t pc) {
+  uint32_t x, y, z;
+  asm volatile(
+      "{\n\t.reg .pred p, q, r;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%3], %4;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 q, [%5], %6;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 r, [%7], %8;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "selp.u32 %1, 1, 0, q;\n\t"
+      "selp.u32 %2, 1, 0, r;\n\t}"
+      : "=r"(x), "=r"(y), "=r"(z)
+      : "r"(smem_u32(a)), "r"(pa), "r"(smem_u32(b)), "r"(pb), "r"(smem_u32(c)), "r"(pc)
+      : "memory");
+  return (__all_sync(0xffffffffu, x) ? 1u : 0u) | (__all_sync(0xffffffffu, y) ? 2u : 0u) |
+         (__all_sync(0xffffffffu, z) ? 4u : 0u);
 }
 
 __device__ __forceinline__ float rcp_approx(float x) {

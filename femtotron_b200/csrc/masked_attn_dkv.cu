@@ -125,9 +125,15 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
           const int4 two = R[e / 2];  // rows e and e + 1: (lo, hi, lo, hi)
-          // a masked place may hold NaN in dP too
-          if (key < two.x || key >= two.y) sv[e] = 0u, dv[e] = 0u;
-          if (key < two.z || key >= two.w) sv[e + 1] = 0u, dv[e + 1] = 0u;
+          // a masked place may hold NaN in dP and in the cap's slope too
+          if (key < two.x || key >= two.y) {
+            sv[e] = 0u, dv[e] = 0u;
+            if (CAP) keep[CAP ? e : 0] = 0.f;
+          }
+          if (key < two.z || key >= two.w) {
+            sv[e + 1] = 0u, dv[e + 1] = 0u;
+            if (CAP) keep[CAP ? e + 1 : 0] = 0.f;
+          }
         }
       }
 #pragma unroll

@@ -339,6 +339,47 @@ def test_gpu_padding_may_hold_nan():
 
 
 @gpu
+@pytest.mark.parametrize("softcap,bias", [(3.0, False), (1e-3, False), (0.0, True), (3.0, True)])
+def test_gpu_padding_may_hold_nan_with_other_scores(softcap, bias):
+    B, S, nq, nkv, d = 1, 400, 4, 2, 64
+    q, k, v, do = make(B, S, nq, nkv, d, 2, "cuda", torch.bfloat16)
+    docs = (torch.arange(S, device="cuda") // 90).int().repeat(B, 1)
+    docs[0, 150:170] = -1
+    docs[0, 390:] = -1
+    mask = MA.attention_mask(B, S, docs=docs)
+    kw = dict(softcap=softcap, slopes=MA.alibi_slopes(nq, "cuda") if bias else None)
+    clean = run(q, k, v, do, mask, **kw)
+    dead = docs < 0
+    for bad in (float("nan"), float("inf")):
+        for x in (q, k, v, do):
+            x[dead] = bad
+        for x, y in zip(run(q, k, v, do, mask, **kw), clean):
+            assert torch.equal(x, y) and not x[dead].any()
+
+
+@gpu
+@pytest.mark.parametrize("softcap,bias", [(0.0, False), (3.0, False), (0.0, True)])
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_gpu_nan_reaches_the_rows_that_see_it(which, softcap, bias):
+    # one key at every place of a run of 64, so that every way an exponential is taken meets it
+    S, nq, nkv, d = 512, 2, 1, 64
+    docs = (torch.arange(S, device="cuda") // 256).int().repeat(64, 1)
+    mask = MA.attention_mask(64, S, docs=docs)
+    q, k, v, do = (x.expand(64, -1, -1, -1).contiguous() for x in make(1, S, nq, nkv, d, 2, "cuda", torch.bfloat16))
+    kw = dict(softcap=softcap, slopes=MA.alibi_slopes(nq, "cuda") if bias else None)
+    clean = run(q, k, v, do, mask, **kw)
+    at = torch.arange(64, device="cuda")
+    {"k": k, "v": v}[which][at, 100 + at] = float("nan")
+    got = run(q, k, v, do, mask, **kw)
+    for name, x, y in zip(("o", "dq", "dk", "dv"), got, clean):
+        assert torch.equal(x[:, 256:], y[:, 256:]), name
+    sees = torch.arange(256, device="cuda") >= 100 + at[:, None]
+    for x in got[:2]:
+        assert not x[:, :256][sees].isfinite().any()
+    assert not got[2][:, :256].isfinite().any()  # each key is seen by a row that is lost
+
+
+@gpu
 @pytest.mark.parametrize("d", [64, 128])
 def test_gpu_padding_over_many_tiles(d):
     # padding inside and behind documents in every one of nine tiles, and whole tiles of it

@@ -103,16 +103,16 @@ int64_t linear_xent_bwd(const torch::Tensor& h, const torch::Tensor& w, const to
                         const c10::optional<torch::Tensor>& dh, const c10::optional<torch::Tensor>& dw,
                         bool accumulate, int64_t vstart, int64_t ignore_index, int64_t workspace_bytes,
                         torch::Tensor& err);
-std::tuple<torch::Tensor, torch::Tensor> attn_mask(int64_t B, int64_t S, bool causal, int64_t window,
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> attn_mask(int64_t B, int64_t S, bool causal, int64_t window,
                                                    const c10::optional<torch::Tensor>& docs,
                                                    const c10::optional<torch::Tensor>& marks, torch::Device device);
 std::tuple<torch::Tensor, c10::optional<torch::Tensor>, c10::optional<torch::Tensor>> masked_attn_fwd(
     const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& rows,
-    const torch::Tensor& tiles, double scale, double softcap, const c10::optional<torch::Tensor>& slopes, bool graded,
-    torch::Tensor& err);
+    const torch::Tensor& tiles, const torch::Tensor& order, double scale, double softcap,
+    const c10::optional<torch::Tensor>& slopes, bool graded, torch::Tensor& err);
 int64_t masked_attn_bwd(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& o,
                      const torch::Tensor& low, const torch::Tensor& dout, const torch::Tensor& lse, const torch::Tensor& rows,
-                     const torch::Tensor& tiles, double scale, double softcap,
+                     const torch::Tensor& tiles, const torch::Tensor& order, double scale, double softcap,
                      const c10::optional<torch::Tensor>& slopes, torch::Tensor& dq, torch::Tensor& dk, torch::Tensor& dv,
                      torch::Tensor& err);
 torch::Tensor grad_sumsq(const std::vector<torch::Tensor>& xs, const std::vector<int64_t>& slots, int64_t n_slots);

@@ -137,6 +137,30 @@ __global__ void __launch_bounds__(MASK_THREADS) mask_kernel(const MaskArgs a) {
     if ((threadIdx.x & 15) == 0 && i0 < a.padded) tiles[i0 / TILE] = t;
     carry = max(carry, all);
   }
+  // The order of the key tiles, by how many query tiles look at them and then by index; 16 threads per tile count, and
+  // count the tiles before it.
+  __shared__ int2 reach[MAX_TILES];
+  __shared__ int work[MAX_TILES];
+  const int n = a.padded / TILE, part = threadIdx.x & 15;
+  auto each = [&](auto&& count, auto&& put) {
+    for (int i0 = 0; i0 < n; i0 += MASK_THREADS / 16) {
+      const int i = i0 + threadIdx.x / 16;
+      int c = 0;
+      if (i < n)
+        for (int j = part; j < n; j += 16) c += count(i, j);
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffff, c, o);
+      if (part == 0 && i < n) put(i, c);
+    }
+    __syncthreads();
+  };
+  __syncthreads();  // the tiles are written
+  for (int i = threadIdx.x; i < n; i += MASK_THREADS) reach[i] = make_int2(tiles[i].x, tiles[i].w);
+  __syncthreads();
+  each([&](int i, int j) { return reach[j].y > i * TILE && reach[j].x < (i + 1) * TILE; },
+       [&](int i, int c) { work[i] = c * MAX_TILES + MAX_TILES - 1 - i; });
+  each([&](int i, int j) { return work[j] > work[i]; },
+       [&](int i, int c) { a.order[static_cast<int64_t>(b) * n + c] = i; });
 }
 
 // ------------------------------------------------------------------------------ forward
@@ -155,7 +179,6 @@ struct FwdSmem {
   __nv_bfloat16 q[2][TILE * HEAD], k[KV_STAGES][STEP * HEAD], v[KV_STAGES][STEP * HEAD];
   uint64_t q_full, full[KV_STAGES], empty[KV_STAGES], landed;
   uint64_t s_full[2][2], p_full[2][2], o_done[2], done[2], drained;
-  uint32_t dead[MAX_TILES / 32];
   uint32_t tmem_base;
 };
 
@@ -217,19 +240,10 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   const int yr = static_cast<int>(gridDim.y) - 1 - static_cast<int>(blockIdx.y);
   const int head0 = p.pair_heads ? 2 * hx : hx, head1 = p.pair_heads ? 2 * hx + 1 : hx;
   const int tile0 = p.pair_heads ? yr : 2 * yr, tile1 = p.pair_heads ? yr : 2 * yr + 1;
+  const int4* tiles = p.tiles + b * p.tiles_stride;
   const int kvh = head0 / p.group;
   const int2* rows = p.rows + b * p.rows_stride;
-  const int4* tiles = p.tiles + b * p.tiles_stride;
-  // the steps of 64 keys that each tile takes: none, or a run that holds the tile's own keys, so the two runs meet
-  int first0 = 0, end0 = 0, first1 = 0, end1 = 0;
-  if (const int4 u = tiles[tile0]; u.w > 0) first0 = u.x / STEP, end0 = (u.w + STEP - 1) / STEP;
-  if (tile1 < p.ntiles)
-    if (const int4 u = tiles[tile1]; u.w > 0) first1 = u.x / STEP, end1 = (u.w + STEP - 1) / STEP;
-  first0 = uniform(first0), end0 = uniform(end0), first1 = uniform(first1), end1 = uniform(end1);
-  const int j0 = first0 == end0 ? first1 : first1 == end1 ? first0 : min(first0, first1);
-  const int j1 = max(end0, end1);  // no keys at all: both 0
-
-  if (threadIdx.x == 0) {
+  if (threadIdx.x == PRODUCER_WARP * 32) {
     mbar_init(&s.q_full, 1);
     for (int i = 0; i < KV_STAGES; ++i) {
       mbar_init(&s.full[i], 1);
@@ -246,12 +260,30 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       mbar_init(&s.done[t], 1);
     }
     fence_barrier_init();
+    // the queries are on their way before it is known whether they see anything
+    const bool two = tile1 < p.ntiles;
+    mbar_arrive_expect_tx(&s.q_full, chunks * PIECE * (two ? 2 : 1));
+    for (int c = 0; c < chunks; ++c) {
+      tma_load_4d(s.q[0] + c * TILE * 64, &tm_q, &s.q_full, c * 64, head0, tile0 * TILE, b);
+      if (two) tma_load_4d(s.q[1] + c * TILE * 64, &tm_q, &s.q_full, c * 64, head1, tile1 * TILE, b);
+    }
+    prefetch(tm_k), prefetch(tm_v), prefetch(tm_o);
+    if (p.rest) prefetch(tm_low);
   }
+  DeadTiles dead_rows(warp == PRODUCER_WARP, tiles, tile1 - 30, p.ntiles);
+  const int4 u0 = tiles[tile0], u1 = tile1 < p.ntiles ? tiles[tile1] : make_int4(kNever, 0, 0, 0);
+  // the steps of 64 keys that each tile takes: none, or a run that holds the tile's own keys, so the two runs meet
+  int first0 = 0, end0 = 0, first1 = 0, end1 = 0;
+  if (u0.w > 0) first0 = u0.x / STEP, end0 = (u0.w + STEP - 1) / STEP;
+  if (u1.w > 0) first1 = u1.x / STEP, end1 = (u1.w + STEP - 1) / STEP;
+  first0 = uniform(first0), end0 = uniform(end0), first1 = uniform(first1), end1 = uniform(end1);
+  const int j0 = first0 == end0 ? first1 : first1 == end1 ? first0 : min(first0, first1);
+  const int j1 = max(end0, end1);  // no keys at all: both 0
+
   if (warp == MMA_WARP) {
     tmem_alloc(&s.tmem_base, 512);
     tmem_relinquish();
   }
-  note_dead(s.dead, tiles, j0 / 2, (j1 + 1) / 2);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -271,12 +303,11 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     float m_used = -INFINITY, l_run = 0.f, l_used = 0.f;
     bool ok = true;
     int lo = 0, width = 0;
-    int4 sum = make_int4(0, 0, 0, 0);
+    const int4 sum = t ? u1 : u0;
     float slope2 = 0.f;
     if (n > 0) {
       const int2 lh = rows[row];
       if (lh.y > lh.x) lo = lh.x, width = lh.y - lh.x;
-      sum = tiles[tile];
       if (ALIBI) slope2 = p.slopes[h] * kLog2e;
     }
     const float mul = ALIBI ? 1.f : unit<CAP>(p);  // goes into the exponent's FMA
@@ -335,54 +366,55 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       if (lane == 0) mbar_arrive(&s.p_full[t][buf]);
     }
     if (n > 0 && ok) ok = wait_warp(&s.done[t], 0, p.err, 321);
-    // a tile without keys may still wait for its queries, whose place its output takes
-    if (n == 0 && j0 < j1) ok = wait_warp(&s.q_full, 0, p.err, 322);
+    // o takes the place of the queries (a tile without keys may still wait for them) and what its rounding leaves out that of
+    // keys, which the other tile has to be done with too.
+    if (n == 0) ok = wait_warp(&s.q_full, 0, p.err, 322);
+    if (p.rest && ok && (t ? end0 > first0 : end1 > first1)) ok = wait_warp(&s.done[t ^ 1], 0, p.err, 323);
     if (real) {
       tc_fence_after();
       const bool none = n == 0 || l_run == 0.f;
       const float inv = none ? 0.f : 1.f / l_used;
-      // (the barriers are met also after a wait that ran out)
-      auto pass = [&](bool rest) {
-        for (int c = 0; ok && c < p.ksteps; ++c) {
-          uint32_t ov[16] = {};
-          if (n > 0) {
-            tmem_ld_32x32b_x16(tO(t) + lane_off + c * 16, ov);
-            tmem_wait_ld();
-          }
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float v = none ? 0.f : __uint_as_float(ov[i]) * inv;  // a sum that is NaN stays one
-            ov[i] = __float_as_uint(rest ? v - __bfloat162float(__float2bfloat16_rn(v)) : v);
-          }
-          stage16(s.q[t], r, c, ov, 1.f);
-        }
-        fence_proxy_async_smem();
-        asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory");  // the four warps of this tile
-        if (ok && quad == 0 && lane == 0) {
-          tma_store_tile(rest ? &tm_low : &tm_o, s.q[t], chunks, h, tile * TILE, b);
-          tma_store_wait_read();
-        }
-      };
-      pass(false);
-      if (p.rest) {
-        asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory");
-        pass(true);
-      }
       if (p.neg_lse2 && ok)
         p.neg_lse2[(static_cast<int64_t>(b) * p.nq + h) * p.padded + row] =
             l_run == 0.f ? -INFINITY : -(m_used + log2f(l_run)) + 0.f * l_used;  // NaN where a score was
+      // (the barrier is met also after a wait that ran out)
+      const int parts = (p.ksteps + 1) / 2;  // of 32 values
+      uint32_t ov[2][32] = {};
+      if (n > 0 && ok) tmem_ld_32x32b_x32(tO(t) + lane_off, ov[0]);
+#pragma unroll
+      for (int c = 0; c < HEAD / 32; ++c) {
+        if (c >= parts || !ok) break;
+        if (n > 0) {
+          tmem_wait_ld();
+          if (c + 1 < parts) tmem_ld_32x32b_x32(tO(t) + lane_off + (c + 1) * 32, ov[(c + 1) & 1]);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          uint32_t w[4], rest[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            // a sum that is NaN stays one
+            const float x = none ? 0.f : __uint_as_float(ov[c & 1][u * 8 + i * 2]) * inv;
+            const float y = none ? 0.f : __uint_as_float(ov[c & 1][u * 8 + i * 2 + 1]) * inv;
+            w[i] = pack_bf16x2(x, y);
+            const float2 r2 = unpack_bf16x2(w[i]);
+            rest[i] = pack_bf16x2(x - r2.x, y - r2.y);
+          }
+          stage8(s.q[t], r, c * 4 + u, make_uint4(w[0], w[1], w[2], w[3]));
+          if (p.rest) stage8(s.k[2 * t], r, c * 4 + u, make_uint4(rest[0], rest[1], rest[2], rest[3]));
+        }
+      }
+      fence_proxy_async_smem();
+      asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory");  // the four warps of this tile
+      if (ok && quad == 0 && lane == 0) {
+        tma_store_tile(&tm_o, s.q[t], chunks, h, tile * TILE, b);
+        if (p.rest) tma_store_tile(&tm_low, s.k[2 * t], chunks, h, tile * TILE, b);
+        tma_store_wait_read();
+      }
     }
   } else if (warp == PRODUCER_WARP) {
     // ------------------------------------------------------------ TMA producer
     if (j0 < j1) {
-      if (lane == 0) {
-        const bool two = tile1 < p.ntiles;
-        mbar_arrive_expect_tx(&s.q_full, chunks * PIECE * (two ? 2 : 1));
-        for (int c = 0; c < chunks; ++c) {
-          tma_load_4d(s.q[0] + c * TILE * 64, &tm_q, &s.q_full, c * 64, head0, tile0 * TILE, b);
-          if (two) tma_load_4d(s.q[1] + c * TILE * 64, &tm_q, &s.q_full, c * 64, head1, tile1 * TILE, b);
-        }
-      }
       bool ok = true;
       int got = 0, n_dead = 0;
       for (int j = j0; j < j1 && ok; ++j) {
@@ -390,7 +422,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         ok = wait_warp(&s.empty[st], ph ^ 1, p.err, 311);
         if (!ok) break;
         // values of rows that see nothing are zeroed before the products may have them
-        const bool dead = is_dead(s.dead, j / 2);
+        const bool dead = dead_rows(tiles, j / 2, p.ntiles);
         uint64_t* bar = dead ? &s.landed : &s.full[st];
         if (lane == 0) {
           mbar_arrive_expect_tx(bar, 2 * chunks * STEP_PIECE);
@@ -409,10 +441,10 @@ __global__ void __launch_bounds__(NTHREADS, 1)
           if (lane == 0) mbar_arrive(&s.full[st]);
         }
       }
-      // the copies have landed before the block may leave, also after a wait that ran out
-      wait_phase(&s.q_full, 0, p.err, 313);
       for (int i = max(0, got - KV_STAGES); i < got; ++i) wait_phase(&s.full[i % KV_STAGES], (i / KV_STAGES) & 1, p.err, 313);
     }
+    // (all copies have landed before the block may leave, also after a wait that ran out)
+    wait_phase(&s.q_full, 0, p.err, 313);
   } else if (j0 < j1) {
     // ------------------------------------------------------------ MMA issuer
     // The whole warp goes through the loop, so that descriptors are made in uniform registers; one lane issues.

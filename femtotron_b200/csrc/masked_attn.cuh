@@ -242,26 +242,38 @@ __device__ __forceinline__ void zero_dead_rows(void* tile, int chunks, const int
       }
 }
 
-// Bits of the tiles in [a, b) that hold rows which see nothing; all warps of the block.
-__device__ __forceinline__ void note_dead(uint32_t* words, const int4* tiles, int a, int b) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int w = (a >> 5) + warp; w <= (b - 1) >> 5 && a < b; w += NTHREADS / 32) {
-    const int t = w * 32 + lane;
-    const uint32_t m = __ballot_sync(0xffffffff, t >= a && t < b && tiles[t].z == 0);
-    if (lane == 0) words[w] = m;
+// Which of 32 tiles hold rows that see nothing, for one warp.  The first 32 are asked for before it is known which of them are
+// needed (one latency instead of two); what lies elsewhere follows when the walk gets there.
+struct DeadTiles {
+  int base;
+  uint32_t bits;
+  __device__ __forceinline__ DeadTiles(bool here, const int4* tiles, int first, int ntiles) : base(0), bits(0) {
+    if (here) look(tiles, max(first, 0), ntiles);
   }
+  __device__ __forceinline__ void look(const int4* tiles, int first, int ntiles) {
+    base = first;
+    const int t = first + (threadIdx.x & 31);
+    bits = __ballot_sync(0xffffffff, t < ntiles && tiles[t].z == 0);
+  }
+  __device__ __forceinline__ bool operator()(const int4* tiles, int t, int ntiles) {
+    if (t < base || t >= base + 32) look(tiles, t, ntiles);
+    return bits >> (t - base) & 1;
+  }
+};
+__device__ __forceinline__ void prefetch(const CUtensorMap& map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map)) : "memory");
 }
-__device__ __forceinline__ bool is_dead(const uint32_t* words, int t) { return (words[t >> 5] >> (t & 31)) & 1; }
 
 // Results leave through shared memory and TMA: a thread has a row of a tile, and 32 rows of 16 bytes each, kilobytes apart, are
 // the slowest way to memory (forward pass of 8192 tokens 180 -> 169 us).  The tile is laid
 // out as it would have been loaded; rows behind the last token and values behind d are not written.
-__device__ __forceinline__ void stage16(void* tile, int r, int c, const uint32_t (&v)[16], float f) {
-  uint8_t* row = static_cast<uint8_t*>(tile) + (c >> 2) * PIECE + r * 128;
+__device__ __forceinline__ void stage8(void* tile, int r, int unit, uint4 v) {  // values 8 unit ... 8 unit + 7 of row r
+  *reinterpret_cast<uint4*>(static_cast<uint8_t*>(tile) + (unit >> 3) * PIECE + r * 128 + (((unit & 7) ^ (r & 7)) * 16)) = v;
+}
+__device__ __forceinline__ void stage16(void* tile, int r, int c, const uint32_t* v, float f) {
   auto p = [&](int i) { return pack_bf16x2(__uint_as_float(v[i]) * f, __uint_as_float(v[i + 1]) * f); };
-  const int u = (c & 3) * 2;
-  *reinterpret_cast<uint4*>(row + ((u ^ (r & 7)) * 16)) = make_uint4(p(0), p(2), p(4), p(6));
-  *reinterpret_cast<uint4*>(row + (((u + 1) ^ (r & 7)) * 16)) = make_uint4(p(8), p(10), p(12), p(14));
+  stage8(tile, r, 2 * c, make_uint4(p(0), p(2), p(4), p(6)));
+  stage8(tile, r, 2 * c + 1, make_uint4(p(8), p(10), p(12), p(14)));
 }
 __device__ __forceinline__ void tma_store_tile(const CUtensorMap* map, const void* tile, int chunks, int head, int row, int b) {
   for (int c = 0; c < chunks; ++c)

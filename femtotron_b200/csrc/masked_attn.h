@@ -49,6 +49,7 @@ struct MaskArgs {
   int64_t docs_stride, marks_stride;
   int2* rows;              // [B, padded] (lo, hi)
   int4* tiles;             // [B, ntiles] (least lo, largest lo, least hi, largest hi)
+  int* order;              // [B, ntiles]: key tiles, the one that the most query tiles look at first
   int S, padded, window;   // window: 0x40000000 for none
   bool causal, docs64;
 };
@@ -58,6 +59,7 @@ struct Common {
   const int2* rows;       // mask, and 0 or padded (ntiles) per batch
   const int4* tiles;
   int64_t rows_stride, tiles_stride;
+  const int* order;       // strides as tiles
   const float* slopes;
   float scale, scale_log2;
   float cap_in, cap_out;  // exp2(s cap_in) = exp(2 scale s / c); c log2(e)

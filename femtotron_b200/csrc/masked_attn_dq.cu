@@ -63,7 +63,6 @@ struct DqSmem {
   __nv_bfloat16 q[TILE * HEAD], dout[TILE * HEAD], k[DQ_STAGES][STEP * HEAD], v[DQ_STAGES][STEP * HEAD];
   uint64_t q_full, full[DQ_STAGES], empty[DQ_STAGES], landed;
   uint64_t sp_full[2], ds_full[2], done, drained;
-  uint32_t dead[MAX_TILES / 32];
   uint32_t tmem_base;
 };
 
@@ -81,11 +80,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   const int qt = static_cast<int>(gridDim.y) - 1 - static_cast<int>(blockIdx.y);
   const int2* rows = p.rows + b * p.rows_stride;
   const int4* tiles = p.tiles + b * p.tiles_stride;
-  const int4 sum = tiles[qt];
-  const int j0 = uniform(sum.w > 0 ? sum.x / STEP : 0);
-  const int n = uniform(sum.w > 0 ? (sum.w + STEP - 1) / STEP - j0 : 0);
-
-  if (threadIdx.x == 0) {
+  if (threadIdx.x == PRODUCER_WARP * 32) {
     mbar_init(&s.q_full, 1);
     for (int i = 0; i < DQ_STAGES; ++i) mbar_init(&s.full[i], 1), mbar_init(&s.empty[i], 1);
     for (int i = 0; i < 2; ++i) mbar_init(&s.sp_full[i], 1), mbar_init(&s.ds_full[i], COMPUTE_WARPS);
@@ -93,12 +88,23 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     mbar_init(&s.done, 1);
     mbar_init(&s.drained, 1);
     fence_barrier_init();
+    // on their way before it is known whether the queries see anything
+    mbar_arrive_expect_tx(&s.q_full, 2 * chunks * PIECE);
+    for (int c = 0; c < chunks; ++c) {
+      tma_load_4d(s.q + c * TILE * 64, &tm_q, &s.q_full, c * 64, h, qt * TILE, b);
+      tma_load_4d(s.dout + c * TILE * 64, &tm_do, &s.q_full, c * 64, h, qt * TILE, b);
+    }
+    prefetch(tm_k), prefetch(tm_v), prefetch(tm_dq);
   }
+  DeadTiles dead_rows(warp == PRODUCER_WARP, tiles, qt - 30, p.ntiles);
+  const int4 sum = tiles[qt];
+  const int j0 = uniform(sum.w > 0 ? sum.x / STEP : 0);
+  const int n = uniform(sum.w > 0 ? (sum.w + STEP - 1) / STEP - j0 : 0);
+
   if (warp == MMA_WARP) {
     tmem_alloc(&s.tmem_base, 512);
     tmem_relinquish();
   }
-  note_dead(s.dead, tiles, j0 / 2, (j0 + n + 1) / 2);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -159,12 +165,12 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.ds_full[buf]);
     }
-    if (n > 0 && ok) ok = wait_warp(&s.done, 0, p.err, 343);
+    // (dq takes the place of the queries on its way out: without keys they may still be arriving)
+    if (ok) ok = n > 0 ? wait_warp(&s.done, 0, p.err, 343) : wait_warp(&s.q_full, 0, p.err, 344);
     if (!ok) {
       asm volatile("bar.sync 1, 256;" ::: "memory");
     } else {
       tc_fence_after();
-      // the queries are no longer needed: dq takes their place on the way out
       for (int c = half; c < p.ksteps; c += 2) {
         uint32_t v[16] = {};
         if (n > 0) {
@@ -186,13 +192,6 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     }
   } else if (warp == PRODUCER_WARP) {
     if (n > 0) {
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&s.q_full, 2 * chunks * PIECE);
-        for (int c = 0; c < chunks; ++c) {
-          tma_load_4d(s.q + c * TILE * 64, &tm_q, &s.q_full, c * 64, h, qt * TILE, b);
-          tma_load_4d(s.dout + c * TILE * 64, &tm_do, &s.q_full, c * 64, h, qt * TILE, b);
-        }
-      }
       bool ok = true;
       int got = 0, n_dead = 0;
       for (int it = 0; it < n && ok; ++it) {
@@ -200,7 +199,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         ok = wait_warp(&s.empty[st], ph ^ 1, p.err, 331);
         if (!ok) break;
         // keys of rows that see nothing are zeroed before the products may have them
-        const bool dead = is_dead(s.dead, (j0 + it) / 2);
+        const bool dead = dead_rows(tiles, (j0 + it) / 2, p.ntiles);
         uint64_t* bar = dead ? &s.landed : &s.full[st];
         if (lane == 0) {
           mbar_arrive_expect_tx(bar, 2 * chunks * STEP_PIECE);
@@ -219,10 +218,10 @@ __global__ void __launch_bounds__(NTHREADS, 1)
           if (lane == 0) mbar_arrive(&s.full[st]);
         }
       }
-      // the copies have landed before the block may leave, also after a wait that ran out
-      wait_phase(&s.q_full, 0, p.err, 334);
       for (int i = max(0, got - DQ_STAGES); i < got; ++i) wait_phase(&s.full[i % DQ_STAGES], (i / DQ_STAGES) & 1, p.err, 334);
     }
+    // (all copies have landed before the block may leave, also after a wait that ran out)
+    wait_phase(&s.q_full, 0, p.err, 334);
   } else if (n > 0) {
     // The whole warp goes through the loop, so that descriptors are made in uniform registers; one lane issues.
     const uint32_t leader = elect_one();

@@ -41,7 +41,8 @@ struct Shape {
 };
 
 Shape check(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& rows,
-            const at::Tensor& tiles, const c10::optional<at::Tensor>& slopes, const at::Tensor& err) {
+            const at::Tensor& tiles, const at::Tensor& order, const c10::optional<at::Tensor>& slopes,
+            const at::Tensor& err) {
   TORCH_CHECK(q.is_cuda(), "masked_attention: q must be a CUDA tensor");
   TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && v.dim() == 4, "masked_attention: q, k, v must be [batch, tokens, heads, d]");
   TORCH_CHECK(q.scalar_type() == at::kBFloat16 && k.scalar_type() == at::kBFloat16 && v.scalar_type() == at::kBFloat16,
@@ -52,11 +53,13 @@ Shape check(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const
   TORCH_CHECK(n.d % 8 == 0 && n.d >= 8 && n.d <= 128, "masked_attention: the head size must be a multiple of 8 up to 128, got ",
               n.d);
   TORCH_CHECK(n.nkv > 0 && n.nq % n.nkv == 0, "masked_attention: ", n.nq, " query heads do not share ", n.nkv, " key heads evenly");
-  one_device(q, k, v, rows, tiles, err);
+  one_device(q, k, v, rows, tiles, order, err);
   const int64_t nt = (n.S + TILE - 1) / TILE;
   TORCH_CHECK(rows.scalar_type() == at::kInt && rows.is_contiguous() && rows.dim() == 3 && rows.size(1) == nt * TILE &&
                   rows.size(2) == 2 && tiles.scalar_type() == at::kInt && tiles.is_contiguous() && tiles.dim() == 3 &&
-                  tiles.size(1) == nt && tiles.size(2) == 4 && tiles.size(0) == rows.size(0),
+                  tiles.size(1) == nt && tiles.size(2) == 4 && tiles.size(0) == rows.size(0) &&
+                  order.scalar_type() == at::kInt && order.is_contiguous() && order.dim() == 2 &&
+                  order.size(0) == rows.size(0) && order.size(1) == nt,
               "masked_attention: the mask was not made for ", n.S, " tokens");
   TORCH_CHECK(rows.size(0) == 1 || rows.size(0) == n.B, "masked_attention: a mask of ", rows.size(0),
               " sequences for a batch of ", n.B);
@@ -71,7 +74,8 @@ Shape check(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const
   return n;
 }
 
-void fill(Common& p, const Shape& n, const at::Tensor& rows, const at::Tensor& tiles, double scale, double softcap,
+void fill(Common& p, const Shape& n, const at::Tensor& rows, const at::Tensor& tiles,
+          const at::Tensor& order, double scale, double softcap,
           const c10::optional<at::Tensor>& slopes, float* neg_lse2, at::Tensor& err) {
   p.B = n.B; p.S = n.S; p.nq = n.nq; p.nkv = n.nkv; p.d = n.d;
   p.ntiles = (n.S + TILE - 1) / TILE;
@@ -82,6 +86,7 @@ void fill(Common& p, const Shape& n, const at::Tensor& rows, const at::Tensor& t
   p.tiles = reinterpret_cast<const int4*>(tiles.data_ptr<int>());
   p.rows_stride = rows.size(0) == 1 ? 0 : p.padded;
   p.tiles_stride = rows.size(0) == 1 ? 0 : p.ntiles;
+  p.order = order.data_ptr<int>();
   p.slopes = slopes.has_value() ? slopes->data_ptr<float>() : nullptr;
   p.scale = static_cast<float>(scale);
   p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
@@ -112,8 +117,8 @@ void check_out(const at::Tensor& x, const at::Tensor& like, const char* name) {
 }  // namespace
 }  // namespace ma
 
-std::tuple<at::Tensor, at::Tensor> attn_mask(int64_t B, int64_t S, bool causal, int64_t window,
-                                                   const c10::optional<at::Tensor>& docs,
+std::tuple<at::Tensor, at::Tensor, at::Tensor> attn_mask(int64_t B, int64_t S, bool causal, int64_t window,
+                                                         const c10::optional<at::Tensor>& docs,
                                                    const c10::optional<at::Tensor>& marks, at::Device device) {
   using namespace ma;
   TORCH_CHECK(B > 0 && S > 0, "attention_mask: needs at least one sequence of one token");
@@ -139,23 +144,25 @@ std::tuple<at::Tensor, at::Tensor> attn_mask(int64_t B, int64_t S, bool causal, 
   const int64_t nt = (S + TILE - 1) / TILE;
   auto opt = at::TensorOptions().dtype(at::kInt).device(device);
   at::Tensor rows = at::empty({B, nt * TILE, 2}, opt), tiles = at::empty({B, nt, 4}, opt);
+  at::Tensor order = at::empty({B, nt}, opt);
   a.rows = reinterpret_cast<int2*>(rows.data_ptr<int>());
   a.tiles = reinterpret_cast<int4*>(tiles.data_ptr<int>());
+  a.order = order.data_ptr<int>();
   a.S = S;
   a.padded = nt * TILE;
   a.window = window > 0 && window < 0x40000000 ? window : 0x40000000;
   a.causal = causal;
   C10_CUDA_CHECK(launch_mask(a, B, at::cuda::getCurrentCUDAStream()));
-  return {rows, tiles};
+  return {rows, tiles, order};
 }
 
 // o [B, S, nq, d] and, where `graded`, the statistics [B, nq, padded] and the rest of o that the backward reads
 std::tuple<at::Tensor, c10::optional<at::Tensor>, c10::optional<at::Tensor>> masked_attn_fwd(
     const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_, const at::Tensor& rows,
-    const at::Tensor& tiles, double scale, double softcap, const c10::optional<at::Tensor>& slopes, bool graded,
-    at::Tensor& err) {
+    const at::Tensor& tiles, const at::Tensor& order, double scale, double softcap,
+    const c10::optional<at::Tensor>& slopes, bool graded, at::Tensor& err) {
   using namespace ma;
-  const Shape n = check(q_, k_, v_, rows, tiles, slopes, err);
+  const Shape n = check(q_, k_, v_, rows, tiles, order, slopes, err);
   const c10::cuda::CUDAGuard g(q_.device());
   at::Tensor o = at::empty({n.B, n.S, n.nq, n.d}, q_.options().memory_format(c10::MemoryFormat::Contiguous));
   c10::optional<at::Tensor> lse, low;
@@ -165,7 +172,7 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>, c10::optional<at::Tensor>> mas
   if (n.B == 0 || n.S == 0 || n.nq == 0) return {o, lse, low};
   const at::Tensor q = usable(q_), k = usable(k_), v = usable(v_);
   FwdParams p;
-  fill(p, n, rows, tiles, scale, softcap, slopes, graded ? lse->data_ptr<float>() : nullptr, err);
+  fill(p, n, rows, tiles, order, scale, softcap, slopes, graded ? lse->data_ptr<float>() : nullptr, err);
   p.rest = graded;
   p.pair_heads = p.group % 2 == 0;
   C10_CUDA_CHECK(launch_fwd(heads_map(q, TILE), heads_map(k, STEP), heads_map(v, STEP), heads_map(o, TILE),
@@ -177,11 +184,11 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>, c10::optional<at::Tensor>> mas
 // returns the number of kernels launched
 int64_t masked_attn_bwd(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_, const at::Tensor& o,
                      const at::Tensor& low, const at::Tensor& do_, const at::Tensor& lse, const at::Tensor& rows,
-                     const at::Tensor& tiles, double scale, double softcap,
+                     const at::Tensor& tiles, const at::Tensor& order, double scale, double softcap,
                      const c10::optional<at::Tensor>& slopes, at::Tensor& dq, at::Tensor& dk, at::Tensor& dv,
                      at::Tensor& err) {
   using namespace ma;
-  const Shape n = check(q_, k_, v_, rows, tiles, slopes, err);
+  const Shape n = check(q_, k_, v_, rows, tiles, order, slopes, err);
   one_device(q_, o, low, do_, lse);
   const int64_t nt = (n.S + TILE - 1) / TILE;
   TORCH_CHECK(o.sizes() == q_.sizes() && do_.sizes() == q_.sizes() && o.scalar_type() == at::kBFloat16 &&
@@ -199,7 +206,7 @@ int64_t masked_attn_bwd(const at::Tensor& q_, const at::Tensor& k_, const at::Te
   const at::Tensor q = usable(q_), k = usable(k_), v = usable(v_), dout = usable(do_);
   at::Tensor delta = at::empty_like(lse);
   BwdParams p;
-  fill(p, n, rows, tiles, scale, softcap, slopes, lse.data_ptr<float>(), err);
+  fill(p, n, rows, tiles, order, scale, softcap, slopes, lse.data_ptr<float>(), err);
   p.neg_delta = delta.data_ptr<float>();
   p.o = out_of(o);
   p.low = low.data_ptr();

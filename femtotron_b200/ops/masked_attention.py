@@ -44,10 +44,12 @@ _NO_WINDOW = 2 ** 30
 class AttentionMask:
     """``rows`` int32 [batch or 1, tokens rounded up to 128, 2]: the interval (lo, hi) of each row,
     (2^31 - 1, 0) where it sees nothing; ``tiles`` int32 [batch or 1, tiles, 4]: least and largest lo,
-    least and largest hi of 128 rows each."""
+    least and largest hi of 128 rows each; ``order`` (CUDA) int32 [batch or 1, tiles]: the tiles as keys, the
+    one that the most tiles look at first."""
     rows: torch.Tensor
     tiles: torch.Tensor
     seq_len: int
+    order: torch.Tensor | None = None
 
     @property
     def batch(self) -> int:
@@ -81,8 +83,8 @@ def attention_mask(batch: int, seq_len: int, *, causal: bool = True, window: int
         if device.index is None:
             device = torch.device("cuda", torch.cuda.current_device())
         docs, prefix = (x if x is None or x.stride(-1) == 1 else x.contiguous() for x in (docs, prefix))
-        rows, tiles = native().attn_mask(batch, seq_len, causal, window or 0, docs, prefix, device)
-        return AttentionMask(rows, tiles, seq_len)
+        rows, tiles, order = native().attn_mask(batch, seq_len, causal, window or 0, docs, prefix, device)
+        return AttentionMask(rows, tiles, seq_len, order)
     S = seq_len
     i = torch.arange(S).expand(batch, S)
     new = i == 0
@@ -159,13 +161,13 @@ def _forward_cpu(q, k, v, mask, scale, softcap, slopes):
 
 def _forward(ctx, q, k, v, mask, scale, softcap, slopes, graded, *kept):
     if q.is_cuda:
-        o, lse, low = native().masked_attn_fwd(q, k, v, mask.rows, mask.tiles, scale, softcap, slopes, graded,
-                                               error_flag(q.device))
+        o, lse, low = native().masked_attn_fwd(q, k, v, mask.rows, mask.tiles, mask.order, scale, softcap, slopes,
+                                               graded, error_flag(q.device))
     else:
         *_, vf, _, lse, p = _forward_cpu(q, k, v, mask, scale, softcap, slopes)
         o, low = (p @ vf).transpose(1, 2).to(q.dtype).contiguous(), None
     if graded:
-        ctx.save_for_backward(*kept, o, low, lse, mask.rows, mask.tiles, slopes)
+        ctx.save_for_backward(*kept, o, low, lse, mask.rows, mask.tiles, mask.order, slopes)
         ctx.meta = (mask.seq_len, scale, softcap)
     return o
 
@@ -178,9 +180,9 @@ class MaskedAttnFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
-        q, k, v, o, low, lse, rows, tiles, slopes = ctx.saved_tensors
+        q, k, v, o, low, lse, rows, tiles, order, slopes = ctx.saved_tensors
         dq, dk, dv = (torch.empty_like(x, memory_format=torch.contiguous_format) for x in (q, k, v))
-        _backward(q, k, v, o, low, do, lse, rows, tiles, slopes, ctx.meta, dq, dk, dv)
+        _backward(q, k, v, o, low, do, lse, rows, tiles, order, slopes, ctx.meta, dq, dk, dv)
         return dq, dk, dv, None, None, None, None, None
 
 
@@ -200,16 +202,16 @@ class MaskedAttnPackedFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
-        qkv, o, low, lse, rows, tiles, slopes = ctx.saved_tensors
+        qkv, o, low, lse, rows, tiles, order, slopes = ctx.saved_tensors
         d = torch.empty_like(qkv, memory_format=torch.contiguous_format)
-        _backward(*_heads(qkv, *ctx.heads), o, low, do, lse, rows, tiles, slopes, ctx.meta, *_heads(d, *ctx.heads))
+        _backward(*_heads(qkv, *ctx.heads), o, low, do, lse, rows, tiles, order, slopes, ctx.meta, *_heads(d, *ctx.heads))
         return d, None, None, None, None, None, None, None
 
 
-def _backward(q, k, v, o, low, do, lse, rows, tiles, slopes, meta, dq, dk, dv):
+def _backward(q, k, v, o, low, do, lse, rows, tiles, order, slopes, meta, dq, dk, dv):
     seq_len, scale, softcap = meta
     if q.is_cuda:
-        n = native().masked_attn_bwd(q, k, v, o, low, do, lse, rows, tiles, scale, softcap, slopes, dq, dk, dv,
+        n = native().masked_attn_bwd(q, k, v, o, low, do, lse, rows, tiles, order, scale, softcap, slopes, dq, dk, dv,
                                      error_flag(q.device))
         LAUNCHES[0] += n - 1  # the proxy counted one
         return
@@ -243,9 +245,11 @@ def _check(q, k, v, mask, scale, softcap, slopes):
         raise TypeError(f"masked_attention: bfloat16 tensors are required on CUDA (floating ones on the CPU), got {q.dtype}")
     if q.is_cuda and (q.shape[3] % 8 or not 8 <= q.shape[3] <= 128):
         raise ValueError(f"masked_attention: the head size must be a multiple of 8 up to 128 on CUDA, got {q.shape[3]}")
-    for x in (k, v, mask.rows, mask.tiles, *([slopes] if slopes is not None else [])):
+    for x in (k, v, mask.rows, mask.tiles, *([mask.order] if mask.order is not None else []), *([slopes] if slopes is not None else [])):
         if x.device != q.device:
             raise ValueError(f"masked_attention: all operands must be on one device, got {q.device} and {x.device}")
+    if q.is_cuda and mask.order is None:
+        raise ValueError("masked_attention: the mask must come from attention_mask, on CUDA")
     if mask.seq_len != q.shape[1] or mask.batch not in (1, q.shape[0]):
         raise ValueError(f"masked_attention: a mask of {mask.batch} x {mask.seq_len} for {q.shape[0]} x {q.shape[1]} tokens")
     if not (scale > 0 and math.isfinite(scale)):

@@ -227,6 +227,22 @@ def test_gpu_mask_equals_the_cpu_mask(kind, B, S):
     assert torch.equal(m.rows.cpu(), w.rows) and torch.equal(m.tiles.cpu(), w.tiles)
 
 
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("B,S", [(1, 1), (2, 130), (3, 5000), (1, 262144)])
+def test_gpu_order_of_the_tiles(kind, B, S):
+    mask = MA.attention_mask(B, S, device="cuda", **{k: v.cuda() if torch.is_tensor(v) else v
+                                                     for k, v in mask_parts(kind, B, S, 3).items()})
+    t = mask.tiles.long()
+    n = t.shape[1]
+    begin = torch.arange(n, device="cuda") * 128
+    seen_by = torch.stack([((u[:, 3, None] > begin) & (u[:, 0, None] < begin + 128)).sum(0) for u in t])
+    at = mask.order.long()
+    assert torch.equal(at.sort(-1).values, torch.arange(n, device="cuda").expand(mask.batch, n))
+    work = seen_by.gather(1, at)
+    assert (work.diff(dim=1) <= 0).all() and (at.diff(dim=1)[work.diff(dim=1) == 0] > 0).all()
+
+
 def check_gpu(B, S, nq, nkv, d, kind, softcap=0.0, bias=False, seed=1, spread=1.0):
     q, k, v, do = make(B, S, nq, nkv, d, seed, "cuda", torch.bfloat16)
     q = q * spread
@@ -451,6 +467,14 @@ def test_gpu_in_a_graph_and_on_another_stream():
         graph.replay()
         fresh = run(q, k, v, do, MA.attention_mask(B, S, docs=docs))
         assert all(torch.equal(x, y) for x, y in zip(kept, fresh))
+
+
+@gpu
+def test_gpu_mask_made_on_the_host_is_refused():
+    q, k, v, _ = make(1, 200, 2, 2, 64, 1, "cuda", torch.bfloat16)
+    m = MA.attention_mask(1, 200)
+    with pytest.raises(ValueError, match="attention_mask"):
+        MA.masked_attention(q, k, v, MA.AttentionMask(m.rows.cuda(), m.tiles.cuda(), 200))
 
 
 @gpu

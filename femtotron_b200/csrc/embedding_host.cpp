@@ -30,7 +30,7 @@ void check_ids(const at::Tensor& ids, const at::Tensor& other) {
               ids.scalar_type());
   TORCH_CHECK(ids.is_cuda() && ids.device() == other.device(), "embedding: all operands must be on one device, got ",
               ids.device(), " and ", other.device());
-  TORCH_CHECK(ids.numel() < (int64_t(1) << 31), "embedding: too many ids");
+  TORCH_CHECK(ids.numel() <= (int64_t(1) << 30), "embedding: at most 2^30 ids, got ", ids.numel());
 }
 
 }  // namespace

@@ -157,3 +157,13 @@ def test_gpu_strides_streams_and_graphs():
     graph.replay()
     E.sorted_grad(ids, dout, want, False)
     assert torch.equal(got, want)
+
+
+@gpu
+def test_more_ids_than_places_are_refused():
+    ids = torch.zeros(1, dtype=torch.int32, device="cuda").expand(2 ** 30 + 1)
+    w = torch.zeros(4, 8, device="cuda")
+    with pytest.raises(RuntimeError, match="at most"):
+        E.lookup(ids, w)
+    with pytest.raises(RuntimeError, match="at most"):
+        E.sorted_grad(ids, torch.zeros(1, 8, device="cuda").expand(2 ** 30 + 1, 8), w, False)

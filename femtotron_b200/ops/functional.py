@@ -26,6 +26,7 @@ from dataclasses import replace
 import torch
 import torch.distributed as dist
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from . import act8 as A8
 from . import embedding as E
@@ -359,10 +360,11 @@ class EmbeddingFn(Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         (ids,) = ctx.saved_tensors
         vstart, scale, shape, dtype = ctx.meta
-        weight, ctx.param = ctx.param, None
+        weight = ctx.param  # kept: a graph that is retained may run again
         if not ctx.needs_input_grad[1]:
             return None, None, None, None
         if weight is None:

@@ -167,3 +167,24 @@ def test_more_ids_than_places_are_refused():
         E.lookup(ids, w)
     with pytest.raises(RuntimeError, match="at most"):
         E.sorted_grad(ids, torch.zeros(1, 8, device="cuda").expand(2 ** 30 + 1, 8), w, False)
+
+
+@pytest.mark.parametrize("sink", [False, True])
+def test_a_retained_graph_runs_again(sink):
+    w = torch.nn.Parameter(torch.arange(12.0).view(4, 3))
+    if sink:
+        w.main_grad = torch.zeros(4, 3)
+    out = FN.embedding(torch.tensor([1, 1, 3]), w, scale=2.0)
+    out.sum().backward(retain_graph=True)
+    out.sum().backward()
+    want = torch.tensor([0.0, 8.0, 0.0, 4.0])[:, None].expand(4, 3)
+    assert torch.equal(w.main_grad if sink else w.grad, want)
+    assert (w.grad is None) == sink
+
+
+def test_second_derivatives_are_refused():
+    base = torch.randn(4, 3, requires_grad=True)
+    out = FN.embedding(torch.tensor([1, 2]), base * 2.0)
+    (g,) = torch.autograd.grad(out.square().sum(), base, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()

@@ -10,7 +10,8 @@ namespace ma {
 // beginnings, and of the places that are not marked as prefix (a row leads when there is none in its document so
 // far).  Backward: the running minimum of the places where a document begins or a mark is missing, which ends the
 // interval of a leading row.  Bound by latency: a thread's tokens are loaded together, before anything depends on
-// them (8192 tokens: 25 us with a load per question, see below for what is left).
+// them (8192 tokens: 25 us with a load per question, 12 us so, and 1 us for the order of the tiles; the sequences of a batch
+// run beside each other).
 constexpr int MASK_THREADS = 1024, PER = 8;
 
 // The largest v of the threads before this one (AFTER: behind it; `none` where there are none), and of all in `total`.
@@ -170,6 +171,14 @@ __global__ void __launch_bounds__(MASK_THREADS) mask_kernel(const MaskArgs a) {
 // go over the first half of their S as bf16 pairs.  S of step j+2 is issued behind the product of step j, so one S
 // waits while the other is worked on: with one S of 128 keys a tile's softmax (2100 clocks) and its products (512
 // each, and 400 until their result is seen) took turns, 3750 clocks for two tiles of 128 keys.
+//
+// Measured (32 heads over 8, d = 128): 8192 tokens in documents 170 us, of which a block of 20 000 clocks in its steps (1600 per
+// step of two tiles) spends another 16 000 on its way in and out: two loads before the first key tile can be asked for (1900),
+// that tile and its S (3600), the last product (1900), results (7500: o and its rest are 128 KB on their way to L2), the
+// next block (1300).  16384 tokens, 8 heads over 1: 490 us, 0.68 of the GEMM rate.  What bounds it there: the products of 64
+// columns, which read 128 bytes of shared memory per clock (48 clocks where the tensor cores need 32).  128 keys per step in
+// two halves (8192: 180 -> 190 us), all waits before the products (180 -> 185), rings of their own for K and V (175 -> 179)
+// and the first key tiles before the block has met (173 -> 176) were slower.
 constexpr int KV_STAGES = 4;
 // Growth of a row's running maximum (log2 units) below which the sums stay relative to the old one: the
 // probabilities stay under 2^8, which bf16 and the fp32 sums hold as well as values under 1.

@@ -194,7 +194,7 @@ __device__ __forceinline__ float2 exp2_of(float2 x, int e) {
 // 1 - tanh^2, the slope of the cap), without it the products themselves.  tanh(x) = 1 - 2 / (1 + exp(2x)) costs two
 // special-function instructions of 8 clocks each (tanh.approx would be off by 5e-4 of the cap: whole percents of p).
 // Where a warp's products are all within 0.7 of the cap, as nearly all are, a polynomial does it on the FMA pipe, off by
-// 2e-7 (the other form by 1e-7): 288 -> 259 us for the forward pass of two rows of 4096 tokens in windows of 1024.
+// 2e-7 (the other form by 1e-7): 288 -> 242 us for the forward pass of two rows of 4096 tokens in windows of 1024.
 template <bool CAP, bool KEEP, int N>
 __device__ __forceinline__ void cap_scores(uint32_t (&sv)[N], float (&keep)[KEEP ? N : 1], const Common& p) {
   if (!CAP) return;

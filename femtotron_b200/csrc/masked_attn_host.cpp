@@ -214,7 +214,7 @@ int64_t masked_attn_bwd(const at::Tensor& q_, const at::Tensor& k_, const at::Te
   p.dv = out_of(dv);
   // Few key tiles leave SMs idle and one block with the whole group's work: then the group is split, as far as
   // two blocks per SM, where a block keeps 16 tiles to work through.  (16384 tokens, 8 heads over 1: 128 blocks
-  // take 2.19 ms; the partial sums in memory cost 40 us per 4 blocks and 16384 x 128 values.)
+  // took 2.19 ms, 512 blocks 1.11; joining their sums takes 14 us.)
   p.split = 1;
   while (n.B * n.nkv * nt * p.split < 2 * 148 && p.group / p.split >= 2 && nt * p.group / p.split >= 32) {
     int next = p.split + 1;

@@ -165,29 +165,25 @@ __global__ void __launch_bounds__(MASK_THREADS) mask_kernel(const MaskArgs a) {
 }
 
 // ------------------------------------------------------------------------------ forward
-// Two query tiles per block share the key and value tiles of a ring: two heads of a group at the same
-// 128 rows where the group has an even number of heads, else 256 rows of one head.  Warps 0-3 and 4-7 each
-// run the softmax of one tile, a row per thread.  TMEM: two S of 64 keys and O for each tile; the probabilities
-// go over the first half of their S as bf16 pairs.  S of step j+2 is issued behind the product of step j, so one S
-// waits while the other is worked on: with one S of 128 keys a tile's softmax (2100 clocks) and its products (512
-// each, and 400 until their result is seen) took turns, 3750 clocks for two tiles of 128 keys.
-//
-// Measured (32 heads over 8, d = 128): 8192 tokens in documents 170 us, of which a block of 20 000 clocks in its steps (1600 per
-// step of two tiles) spends another 16 000 on its way in and out: two loads before the first key tile can be asked for (1900),
-// that tile and its S (3600), the last product (1900), results (7500: o and its rest are 128 KB on their way to L2), the
-// next block (1300).  16384 tokens, 8 heads over 1: 490 us, 0.68 of the GEMM rate.  What bounds it there: the products of 64
-// columns, which read 128 bytes of shared memory per clock (48 clocks where the tensor cores need 32).  128 keys per step in
-// two halves (8192: 180 -> 190 us), all waits before the products (180 -> 185), rings of their own for K and V (175 -> 179)
-// and the first key tiles before the block has met (173 -> 176) were slower.
-constexpr int KV_STAGES = 4;
+// One block per 128 queries of a head, two blocks per SM: half of TMEM and 97 KB of shared memory each.  While one waits for
+// its products, for the softmax, or on its way in or out (where blocks of short documents spend nearly half of their time:
+// 16 000 clocks of 36 000), the other one works.  Warps 0-3 run the softmax, a row per thread.  TMEM: two S of 64 keys, and O;
+// the probabilities go over the first half of their S as bf16 pairs.  S of step j + 2 is issued behind the product of step j,
+// so one S waits while the other is worked on.  Keys leave their place with their S, values with their product: two of each do.
+// Measured (32 heads over 8, d = 128, us; in brackets one block per SM with two query tiles that shared the keys): 8192 tokens
+// in documents 163 (171), 2 x 4096 with windows of 1024 and a cap 226 (241), 16384 tokens with 8 heads over 1 459 (497), 0.73
+// of the GEMM rate.  What bounds it: the softmax's instructions, 900 clocks per step and tile at 642 of products.  There, 128
+// keys per step in halves, all waits before the products and the first keys before the block has met had been slower.
+constexpr int FWD_THREADS = 192, FWD_PRODUCER = 4, FWD_MMA = 5;
+constexpr int KV_STAGES = 2;  // as many as S: a place for keys is free when the S of its buffer is there
 // Growth of a row's running maximum (log2 units) below which the sums stay relative to the old one: the
 // probabilities stay under 2^8, which bf16 and the fp32 sums hold as well as values under 1.
 constexpr float kRescale = 8.0f;
 
 struct FwdSmem {
-  __nv_bfloat16 q[2][TILE * HEAD], k[KV_STAGES][STEP * HEAD], v[KV_STAGES][STEP * HEAD];
-  uint64_t q_full, full[KV_STAGES], empty[KV_STAGES], landed;
-  uint64_t s_full[2][2], p_full[2][2], o_done[2], done[2], drained;
+  __nv_bfloat16 q[TILE * HEAD], k[KV_STAGES][STEP * HEAD], v[KV_STAGES][STEP * HEAD];
+  uint64_t q_full, k_full[KV_STAGES], v_full[KV_STAGES], v_empty[KV_STAGES], landed;
+  uint64_t s_full[2], p_full[2], o_done, done, drained;
   uint32_t tmem_base;
 };
 
@@ -233,7 +229,7 @@ __device__ __forceinline__ float scores(uint32_t (&sv)[STEP], const Common& p, f
 }
 
 template <bool CAP, bool ALIBI>
-__global__ void __launch_bounds__(NTHREADS, 1)
+__global__ void __launch_bounds__(FWD_THREADS, 2)
     fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o,
                const __grid_constant__ CUtensorMap tm_low, const __grid_constant__ FwdParams p) {
@@ -244,86 +240,63 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   const int chunks = p.d > 64 ? 2 : 1;  // pieces of 64 values that a head has
 
   // late query tiles (the longest rows of a causal mask) first
-  const int per = p.pair_heads ? p.nq / 2 : p.nq;
-  const int b = blockIdx.x / per, hx = blockIdx.x % per;
-  const int yr = static_cast<int>(gridDim.y) - 1 - static_cast<int>(blockIdx.y);
-  const int head0 = p.pair_heads ? 2 * hx : hx, head1 = p.pair_heads ? 2 * hx + 1 : hx;
-  const int tile0 = p.pair_heads ? yr : 2 * yr, tile1 = p.pair_heads ? yr : 2 * yr + 1;
-  const int4* tiles = p.tiles + b * p.tiles_stride;
-  const int kvh = head0 / p.group;
+  const int b = blockIdx.x / p.nq, h = blockIdx.x % p.nq, kvh = h / p.group;
+  const int tile = static_cast<int>(gridDim.y) - 1 - static_cast<int>(blockIdx.y);
   const int2* rows = p.rows + b * p.rows_stride;
-  if (threadIdx.x == PRODUCER_WARP * 32) {
+  const int4* tiles = p.tiles + b * p.tiles_stride;
+  if (threadIdx.x == FWD_PRODUCER * 32) {
     mbar_init(&s.q_full, 1);
     for (int i = 0; i < KV_STAGES; ++i) {
-      mbar_init(&s.full[i], 1);
-      mbar_init(&s.empty[i], 1);
+      mbar_init(&s.k_full[i], 1);
+      mbar_init(&s.v_full[i], 1);
+      mbar_init(&s.v_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.s_full[i], 1);
+      mbar_init(&s.p_full[i], 4);
     }
     mbar_init(&s.landed, 1);
+    mbar_init(&s.o_done, 1);
+    mbar_init(&s.done, 1);
     mbar_init(&s.drained, 1);
-    for (int t = 0; t < 2; ++t) {
-      for (int i = 0; i < 2; ++i) {
-        mbar_init(&s.s_full[t][i], 1);
-        mbar_init(&s.p_full[t][i], 4);
-      }
-      mbar_init(&s.o_done[t], 1);
-      mbar_init(&s.done[t], 1);
-    }
     fence_barrier_init();
     // the queries are on their way before it is known whether they see anything
-    const bool two = tile1 < p.ntiles;
-    mbar_arrive_expect_tx(&s.q_full, chunks * PIECE * (two ? 2 : 1));
-    for (int c = 0; c < chunks; ++c) {
-      tma_load_4d(s.q[0] + c * TILE * 64, &tm_q, &s.q_full, c * 64, head0, tile0 * TILE, b);
-      if (two) tma_load_4d(s.q[1] + c * TILE * 64, &tm_q, &s.q_full, c * 64, head1, tile1 * TILE, b);
-    }
+    mbar_arrive_expect_tx(&s.q_full, chunks * PIECE);
+    for (int c = 0; c < chunks; ++c) tma_load_4d(s.q + c * TILE * 64, &tm_q, &s.q_full, c * 64, h, tile * TILE, b);
     prefetch(tm_k), prefetch(tm_v), prefetch(tm_o);
     if (p.rest) prefetch(tm_low);
   }
-  DeadTiles dead_rows(warp == PRODUCER_WARP, tiles, tile1 - 30, p.ntiles);
-  const int4 u0 = tiles[tile0], u1 = tile1 < p.ntiles ? tiles[tile1] : make_int4(kNever, 0, 0, 0);
-  // the steps of 64 keys that each tile takes: none, or a run that holds the tile's own keys, so the two runs meet
-  int first0 = 0, end0 = 0, first1 = 0, end1 = 0;
-  if (u0.w > 0) first0 = u0.x / STEP, end0 = (u0.w + STEP - 1) / STEP;
-  if (u1.w > 0) first1 = u1.x / STEP, end1 = (u1.w + STEP - 1) / STEP;
-  first0 = uniform(first0), end0 = uniform(end0), first1 = uniform(first1), end1 = uniform(end1);
-  const int j0 = first0 == end0 ? first1 : first1 == end1 ? first0 : min(first0, first1);
-  const int j1 = max(end0, end1);  // no keys at all: both 0
+  DeadTiles dead_rows(warp == FWD_PRODUCER, tiles, tile - 30, p.ntiles);
+  const int4 sum = tiles[tile];
+  const int j0 = uniform(sum.w > 0 ? sum.x / STEP : 0);
+  const int n = uniform(sum.w > 0 ? (sum.w + STEP - 1) / STEP - j0 : 0);  // steps of 64 keys
 
-  if (warp == MMA_WARP) {
-    tmem_alloc(&s.tmem_base, 512);
+  if (warp == FWD_MMA) {
+    tmem_alloc(&s.tmem_base, 256);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  constexpr uint32_t tmem = 0;  // where an allocation of all 512 columns begins
-  auto tS = [](int t, int buf) -> uint32_t { return tmem + static_cast<uint32_t>(t) * 128u + static_cast<uint32_t>(buf) * 64u; };
-  auto tO = [](int t) -> uint32_t { return tmem + 256u + static_cast<uint32_t>(t) * 128u; };
+  const uint32_t tmem = uniform(s.tmem_base);
+  auto tS = [&](int buf) -> uint32_t { return tmem + static_cast<uint32_t>(buf) * 64u; };
+  const uint32_t tO = tmem + 128u;
 
-  if (warp < COMPUTE_WARPS) {
-    // ------------------------------------------------------------ softmax warps 0..7
-    const int t = warp >> 2, quad = warp & 3;
-    const int r = quad * 32 + lane;
-    const int tile = t ? tile1 : tile0, h = t ? head1 : head0, begin = t ? first1 : first0;
-    const bool real = tile < p.ntiles;
-    const int row = tile * TILE + r;
-    const uint32_t lane_off = static_cast<uint32_t>(quad * 32) << 16;
-    const int n = (t ? end1 : end0) - begin;
+  if (warp < 4) {
+    // ------------------------------------------------------------ softmax warps
+    const int r = warp * 32 + lane, row = tile * TILE + r;
+    const uint32_t lane_off = static_cast<uint32_t>(warp * 32) << 16;
     float m_used = -INFINITY, l_run = 0.f, l_used = 0.f;
     bool ok = true;
     int lo = 0, width = 0;
-    const int4 sum = t ? u1 : u0;
-    float slope2 = 0.f;
-    if (n > 0) {
-      const int2 lh = rows[row];
-      if (lh.y > lh.x) lo = lh.x, width = lh.y - lh.x;
-      if (ALIBI) slope2 = p.slopes[h] * kLog2e;
-    }
+    const int2 lh = rows[row];
+    if (lh.y > lh.x) lo = lh.x, width = lh.y - lh.x;
+    const float slope2 = ALIBI ? p.slopes[h] * kLog2e : 0.f;
     const float mul = ALIBI ? 1.f : unit<CAP>(p);  // goes into the exponent's FMA
     for (int c = 0; c < n; ++c) {
-      const int k0 = (begin + c) * STEP, buf = c & 1;
-      const uint32_t ts = tS(t, buf) + lane_off;
-      ok = wait_warp(&s.s_full[t][buf], (c >> 1) & 1, p.err, 319);
+      const int k0 = (j0 + c) * STEP, buf = c & 1;
+      const uint32_t ts = tS(buf) + lane_off;
+      ok = wait_warp(&s.s_full[buf], (c >> 1) & 1, p.err, 319);
       if (!ok) break;
       tc_fence_after();
       const bool test = k0 < sum.y || k0 + STEP > sum.z;
@@ -340,7 +313,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       if (c > 0 && __any_sync(0xffffffffu, need)) {
         // O holds still: the product of the step before is done, the next one waits for this warp.  (S of this step was
         // committed behind the product of step c - 2, so the barrier is at most one phase behind.)
-        ok = wait_warp(&s.o_done[t], (c - 1) & 1, p.err, 320);
+        ok = wait_warp(&s.o_done, (c - 1) & 1, p.err, 320);
         if (!ok) break;
         tc_fence_after();
         const float alpha = m_used == -INFINITY ? 0.f : ex2_approx(m_used - m_new);
@@ -348,7 +321,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         l_used *= alpha;
         for (int cc = 0; cc < p.ksteps; ++cc) {
           uint32_t ov[16];
-          const uint32_t ta = tO(t) + lane_off + cc * 16;
+          const uint32_t ta = tO + lane_off + cc * 16;
           tmem_ld_32x32b_x16(ta, ov);
           tmem_wait_ld();
 #pragma unroll
@@ -372,135 +345,121 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       l_used += rounded.x + rounded.y;
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&s.p_full[t][buf]);
+      if (lane == 0) mbar_arrive(&s.p_full[buf]);
     }
-    if (n > 0 && ok) ok = wait_warp(&s.done[t], 0, p.err, 321);
-    // o takes the place of the queries (a tile without keys may still wait for them) and what its rounding leaves out that of
-    // keys, which the other tile has to be done with too.
-    if (n == 0) ok = wait_warp(&s.q_full, 0, p.err, 322);
-    if (p.rest && ok && (t ? end0 > first0 : end1 > first1)) ok = wait_warp(&s.done[t ^ 1], 0, p.err, 323);
-    if (real) {
-      tc_fence_after();
-      const bool none = n == 0 || l_run == 0.f;
-      const float inv = none ? 0.f : 1.f / l_used;
-      if (p.neg_lse2 && ok)
-        p.neg_lse2[(static_cast<int64_t>(b) * p.nq + h) * p.padded + row] =
-            l_run == 0.f ? -INFINITY : -(m_used + log2f(l_run)) + 0.f * l_used;  // NaN where a score was
-      // (the barrier is met also after a wait that ran out)
-      const int parts = (p.ksteps + 1) / 2;  // of 32 values
-      uint32_t ov[2][32] = {};
-      if (n > 0 && ok) tmem_ld_32x32b_x32(tO(t) + lane_off, ov[0]);
+    // o takes the place of the queries (without keys they may still be arriving) and what its rounding leaves out that of
+    // the keys
+    if (ok) ok = n > 0 ? wait_warp(&s.done, 0, p.err, 321) : wait_warp(&s.q_full, 0, p.err, 322);
+    tc_fence_after();
+    const bool none = n == 0 || l_run == 0.f;
+    const float inv = none ? 0.f : 1.f / l_used;
+    if (p.neg_lse2 && ok)
+      p.neg_lse2[(static_cast<int64_t>(b) * p.nq + h) * p.padded + row] =
+          l_run == 0.f ? -INFINITY : -(m_used + log2f(l_run)) + 0.f * l_used;  // NaN where a score was
+    // (the barrier is met also after a wait that ran out)
+    const int parts = (p.ksteps + 1) / 2;  // of 32 values
+    uint32_t ov[2][32] = {};
+    if (n > 0 && ok) tmem_ld_32x32b_x32(tO + lane_off, ov[0]);
 #pragma unroll
-      for (int c = 0; c < HEAD / 32; ++c) {
-        if (c >= parts || !ok) break;
-        if (n > 0) {
-          tmem_wait_ld();
-          if (c + 1 < parts) tmem_ld_32x32b_x32(tO(t) + lane_off + (c + 1) * 32, ov[(c + 1) & 1]);
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          uint32_t w[4], rest[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            // a sum that is NaN stays one
-            const float x = none ? 0.f : __uint_as_float(ov[c & 1][u * 8 + i * 2]) * inv;
-            const float y = none ? 0.f : __uint_as_float(ov[c & 1][u * 8 + i * 2 + 1]) * inv;
-            w[i] = pack_bf16x2(x, y);
-            const float2 r2 = unpack_bf16x2(w[i]);
-            rest[i] = pack_bf16x2(x - r2.x, y - r2.y);
-          }
-          stage8(s.q[t], r, c * 4 + u, make_uint4(w[0], w[1], w[2], w[3]));
-          if (p.rest) stage8(s.k[2 * t], r, c * 4 + u, make_uint4(rest[0], rest[1], rest[2], rest[3]));
-        }
+    for (int c = 0; c < HEAD / 32; ++c) {
+      if (c >= parts || !ok) break;
+      if (n > 0) {
+        tmem_wait_ld();
+        if (c + 1 < parts) tmem_ld_32x32b_x32(tO + lane_off + (c + 1) * 32, ov[(c + 1) & 1]);
       }
-      fence_proxy_async_smem();
-      asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory");  // the four warps of this tile
-      if (ok && quad == 0 && lane == 0) {
-        tma_store_tile(&tm_o, s.q[t], chunks, h, tile * TILE, b);
-        if (p.rest) tma_store_tile(&tm_low, s.k[2 * t], chunks, h, tile * TILE, b);
-        tma_store_wait_read();
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        uint32_t w[4], rest[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          // a sum that is NaN stays one
+          const float x = none ? 0.f : __uint_as_float(ov[c & 1][u * 8 + i * 2]) * inv;
+          const float y = none ? 0.f : __uint_as_float(ov[c & 1][u * 8 + i * 2 + 1]) * inv;
+          w[i] = pack_bf16x2(x, y);
+          const float2 r2 = unpack_bf16x2(w[i]);
+          rest[i] = pack_bf16x2(x - r2.x, y - r2.y);
+        }
+        stage8(s.q, r, c * 4 + u, make_uint4(w[0], w[1], w[2], w[3]));
+        if (p.rest) stage8(s.k[0], r, c * 4 + u, make_uint4(rest[0], rest[1], rest[2], rest[3]));
       }
     }
-  } else if (warp == PRODUCER_WARP) {
+    fence_proxy_async_smem();
+    asm volatile("bar.sync 1, 128;" ::: "memory");  // the four warps
+    if (ok && threadIdx.x == 0) {
+      tma_store_tile(&tm_o, s.q, chunks, h, tile * TILE, b);
+      if (p.rest) tma_store_tile(&tm_low, s.k[0], chunks, h, tile * TILE, b);
+      tma_store_wait_read();
+    }
+  } else if (warp == FWD_PRODUCER) {
     // ------------------------------------------------------------ TMA producer
-    if (j0 < j1) {
-      bool ok = true;
-      int got = 0, n_dead = 0;
-      for (int j = j0; j < j1 && ok; ++j) {
-        const int st = (j - j0) % KV_STAGES, ph = ((j - j0) / KV_STAGES) & 1;
-        ok = wait_warp(&s.empty[st], ph ^ 1, p.err, 311);
-        if (!ok) break;
-        // values of rows that see nothing are zeroed before the products may have them
-        const bool dead = dead_rows(tiles, j / 2, p.ntiles);
-        uint64_t* bar = dead ? &s.landed : &s.full[st];
-        if (lane == 0) {
-          mbar_arrive_expect_tx(bar, 2 * chunks * STEP_PIECE);
-          for (int c = 0; c < chunks; ++c) {
-            tma_load_4d(s.k[st] + c * STEP * 64, &tm_k, bar, c * 64, kvh, j * STEP, b);
-            tma_load_4d(s.v[st] + c * STEP * 64, &tm_v, bar, c * 64, kvh, j * STEP, b);
-          }
-        }
-        ++got;
-        __syncwarp();
-        if (dead) {
-          ok = wait_warp(&s.landed, n_dead++ & 1, p.err, 312);
-          zero_dead_rows(s.v[st], chunks, rows + j * STEP, lane);
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&s.full[st]);
-        }
+    bool ok = true;
+    int got_k = 0, got_v = 0, n_dead = 0;
+    for (int c = 0; c < n && ok; ++c) {
+      const int st = c % KV_STAGES, ph = (c / KV_STAGES) & 1, k0 = (j0 + c) * STEP;
+      // a place for keys is free when their S is done
+      if (c >= KV_STAGES) ok = wait_warp(&s.s_full[st], ph ^ 1, p.err, 310);
+      if (!ok) break;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&s.k_full[st], chunks * STEP_PIECE);
+        for (int i = 0; i < chunks; ++i) tma_load_4d(s.k[st] + i * STEP * 64, &tm_k, &s.k_full[st], i * 64, kvh, k0, b);
       }
-      for (int i = max(0, got - KV_STAGES); i < got; ++i) wait_phase(&s.full[i % KV_STAGES], (i / KV_STAGES) & 1, p.err, 313);
+      ++got_k;
+      __syncwarp();
+      ok = wait_warp(&s.v_empty[st], ph ^ 1, p.err, 311);
+      if (!ok) break;
+      // values of rows that see nothing are zeroed before the products may have them
+      const bool dead = dead_rows(tiles, (j0 + c) / 2, p.ntiles);
+      uint64_t* bar = dead ? &s.landed : &s.v_full[st];
+      if (lane == 0) {
+        mbar_arrive_expect_tx(bar, chunks * STEP_PIECE);
+        for (int i = 0; i < chunks; ++i) tma_load_4d(s.v[st] + i * STEP * 64, &tm_v, bar, i * 64, kvh, k0, b);
+      }
+      ++got_v;
+      __syncwarp();
+      if (dead) {
+        ok = wait_warp(&s.landed, n_dead++ & 1, p.err, 312);
+        zero_dead_rows(s.v[st], chunks, rows + k0, lane);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.v_full[st]);
+      }
     }
-    // (all copies have landed before the block may leave, also after a wait that ran out)
+    // all copies have landed before the block may leave, also after a wait that ran out
+    for (int i = max(0, got_k - KV_STAGES); i < got_k; ++i) wait_phase(&s.k_full[i % KV_STAGES], (i / KV_STAGES) & 1, p.err, 313);
+    for (int i = max(0, got_v - KV_STAGES); i < got_v; ++i) wait_phase(&s.v_full[i % KV_STAGES], (i / KV_STAGES) & 1, p.err, 313);
     wait_phase(&s.q_full, 0, p.err, 313);
-  } else if (j0 < j1) {
+  } else if (n > 0) {
     // ------------------------------------------------------------ MMA issuer
     // The whole warp goes through the loop, so that descriptors are made in uniform registers; one lane issues.
     const uint32_t leader = elect_one();
     const uint32_t idO = make_idesc_bf16(TILE, p.ksteps * 16, false, true);  // P (TMEM) x V (MN-major)
-    const uint32_t qa = desc_low(smem_u32(s.q[0]), 16), ka = desc_low(smem_u32(s.k[0]), 16);
+    const uint32_t qa = desc_low(smem_u32(s.q), 16), ka = desc_low(smem_u32(s.k[0]), 16);
     const uint32_t va = desc_low(smem_u32(s.v[0]), STEP_PIECE);
-    constexpr uint32_t stage = STEP * HEAD * 2 >> 4, tile = TILE * HEAD * 2 >> 4;
+    constexpr uint32_t stage = STEP * HEAD * 2 >> 4;
     bool ok = wait_warp(&s.q_full, 0, p.err, 317);
-    auto issue_s = [&](int j, int t, int first, int end) {
-      if (first > j || j >= end) return;
-      const int buf = (j - first) & 1;
-      mma_scores(tS(t, buf), qa + t * tile, ka + ((j - j0) % KV_STAGES) * stage, p.ksteps, leader);
-      commit(&s.s_full[t][buf], leader);
-    };
-    auto arrived = [&](int j) {
-      if (j < j1) ok = ok && wait_warp(&s.full[(j - j0) % KV_STAGES], ((j - j0) / KV_STAGES) & 1, p.err, 314);
-    };
-    auto issue_o = [&](int j, int t, int first, int end, bool ready) {
-      if (first > j || j >= end) return;
-      const int c = j - first, buf = c & 1;
-      ok = ok && (ready || wait_warp(&s.p_full[t][buf], (c >> 1) & 1, p.err, 316));
+    auto issue_s = [&](int c, bool ready) {
+      if (!ok || c >= n) return;
+      ok = ready || wait_warp(&s.k_full[c % KV_STAGES], (c / KV_STAGES) & 1, p.err, 314);
       if (!ok) return;
       tc_fence_after();
-      mma_values(tO(t), tS(t, buf), 16, va + ((j - j0) % KV_STAGES) * stage, idO, c > 0, leader);
-      commit(&s.o_done[t], leader);
-      if (j + 1 == end) commit(&s.done[t], leader);
+      mma_scores(tS(c & 1), qa, ka + (c % KV_STAGES) * stage, p.ksteps, leader);
+      commit(&s.s_full[c & 1], leader);
     };
-    for (int j = j0; j < j0 + 2; ++j) {
-      arrived(j);
+    issue_s(0, false);
+    issue_s(1, false);
+    for (int c = 0; ok && c < n; ++c) {
+      const int st = c % KV_STAGES, ph = (c / KV_STAGES) & 1, buf = c & 1;
+      const uint32_t have = over(&s.p_full[buf], (c >> 1) & 1, &s.v_full[st], ph, &s.k_full[(c + 2) % KV_STAGES],
+                                 ((c + 2) / KV_STAGES) & 1);
+      ok = (have & 2) || wait_warp(&s.v_full[st], ph, p.err, 315);
+      ok = ok && ((have & 1) || wait_warp(&s.p_full[buf], (c >> 1) & 1, p.err, 316));
       if (!ok) break;
       tc_fence_after();
-      issue_s(j, 0, first0, min(end0, j1));
-      issue_s(j, 1, first1, min(end1, j1));
-    }
-    for (int j = j0; ok && j < j1; ++j) {
-      const int next = j + 2 - j0, c0 = j - first0, c1 = j - first1;
-      const uint32_t have = over(&s.full[next % KV_STAGES], (next / KV_STAGES) & 1, &s.p_full[0][c0 & 1], (c0 >> 1) & 1,
-                                 &s.p_full[1][c1 & 1], (c1 >> 1) & 1);
-      if (!(have & 1)) arrived(j + 2);
-      issue_o(j, 0, first0, end0, have & 2);
-      if (!ok) break;
-      issue_s(j + 2, 0, first0, end0);
-      issue_o(j, 1, first1, end1, have & 4);
-      if (!ok) break;
-      commit(&s.empty[(j - j0) % KV_STAGES], leader);
-      issue_s(j + 2, 1, first1, end1);
+      mma_values(tO, tS(buf), 16, va + st * stage, idO, c > 0, leader);
+      commit(&s.o_done, leader);
+      commit(&s.v_empty[st], leader);
+      if (c + 1 == n) commit(&s.done, leader);
+      issue_s(c + 2, have & 4);
     }
     if (!ok) {
       commit(&s.drained, leader);
@@ -510,9 +469,9 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 
   tc_fence_before();
   __syncthreads();
-  if (warp == MMA_WARP) {
+  if (warp == FWD_MMA) {
     tc_fence_after();
-    tmem_dealloc(s.tmem_base, 512);
+    tmem_dealloc(s.tmem_base, 256);
   }
 }
 
@@ -524,13 +483,12 @@ cudaError_t launch_mask(const MaskArgs& a, int batch, cudaStream_t st) {
 
 cudaError_t launch_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& to,
                        const CUtensorMap& tlow, const FwdParams& p, bool cap, bool bias, cudaStream_t st) {
-  static_assert(sizeof(FwdSmem) + 1024 <= 232448, "shared memory");
-  const dim3 grid(p.B * (p.pair_heads ? p.nq / 2 : p.nq), p.pair_heads ? p.ntiles : (p.ntiles + 1) / 2);
+  static_assert(2 * (sizeof(FwdSmem) + 2048) <= 233472, "shared memory of two blocks");
   pick(cap, bias, [&](auto CAP, auto BIAS) {
     constexpr auto kernel = fwd_kernel<decltype(CAP)::value, decltype(BIAS)::value>;
     static unsigned long long cfg = 0;
     smem_attr_once(kernel, sizeof(FwdSmem) + 1024, cfg);
-    kernel<<<grid, NTHREADS, sizeof(FwdSmem) + 1024, st>>>(tq, tk, tv, to, tlow, p);
+    kernel<<<dim3(p.B * p.nq, p.ntiles), FWD_THREADS, sizeof(FwdSmem) + 1024, st>>>(tq, tk, tv, to, tlow, p);
   });
   return cudaGetLastError();
 }

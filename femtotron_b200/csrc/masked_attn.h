@@ -75,7 +75,6 @@ struct Out {  // a [batch, tokens, heads, d] tensor of bf16, strides in elements
 };
 
 struct FwdParams : Common {
-  bool pair_heads;
   bool rest;               // write what o's rounding to bf16 left out, in bf16
 };
 

@@ -174,7 +174,6 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>, c10::optional<at::Tensor>> mas
   FwdParams p;
   fill(p, n, rows, tiles, order, scale, softcap, slopes, graded ? lse->data_ptr<float>() : nullptr, err);
   p.rest = graded;
-  p.pair_heads = p.group % 2 == 0;
   C10_CUDA_CHECK(launch_fwd(heads_map(q, TILE), heads_map(k, STEP), heads_map(v, STEP), heads_map(o, TILE),
                             heads_map(graded ? *low : o, TILE), p, softcap > 0, slopes.has_value(),
                             at::cuda::getCurrentCUDAStream()));

@@ -156,7 +156,8 @@ __device__ __forceinline__ float2 exp2_pair(float a, float b) {
 
 // Whether each of three phases is over (bits 0 to 2), for a whole warp, without waiting.  The three answers are under way
 // together: where products read all that shared memory gives, each takes its time, and the MMA warp asks for all that its
-// step needs at once (forward of 16384 tokens, 8 heads: 495 -> 489 us; no gain in the two backward kernels, which ask singly).
+// step needs at once (forward of 16384 tokens, 8 heads, when a block had two query tiles: 495 -> 489 us; no gain in the two
+// backward kernels, which ask singly).
 // The phase before the one asked for has to be over already: two phases back has the same parity.
 __device__ __forceinline__ uint32_t over(uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb, uint64_t* c, uint32_t pc) {
   uint32_t x, y, z;
@@ -181,10 +182,12 @@ __device__ __forceinline__ float rcp_approx(float x) {
   return y;
 }
 
-// 2^x of the e-th pair of a row.  Every fourth pair runs on the FMA pipe: the special-function unit takes 8 clocks for
-// one exponential of a warp and would set the pace alone.  With capped scores the FMA pipe sets it.
+// 2^x of the e-th pair of a row.  Every eighth pair runs on the FMA pipe: the special-function unit takes 8 clocks for one
+// exponential of a warp and would set the pace alone, the other form takes nine instructions.  (Forward, and dk and dv, of 16384
+// tokens, 8 heads over 1: none 460 and 817 us, every eighth 448 and 808, fourth 451 and 818, third 470 and 841.)  With capped
+// scores the FMA pipe sets the pace.
 template <bool CAP>
-__device__ __forceinline__ constexpr bool on_fma_pipe(int e) { return !CAP && e % 4 == 3; }
+__device__ __forceinline__ constexpr bool on_fma_pipe(int e) { return !CAP && e % 8 == 7; }
 template <bool CAP>
 __device__ __forceinline__ float2 exp2_of(float2 x, int e) {
   return on_fma_pipe<CAP>(e) ? exp2_pair(x.x, x.y) : make_float2(ex2_approx(x.x), ex2_approx(x.y));

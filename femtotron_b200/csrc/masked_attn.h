@@ -36,7 +36,7 @@ namespace ma {
 constexpr int TILE = 128;
 constexpr int HEAD = 128;  // values of a head that a tile has room for
 constexpr int STEP = 64;   // keys (or, for dk and dv, queries) that a step of a kernel takes
-constexpr int NTHREADS = 320;  // 8 compute warps, 1 TMA warp, 1 MMA warp
+constexpr int NTHREADS = 320;  // of the backward kernels: 8 compute warps, 1 TMA warp, 1 MMA warp
 constexpr int PRODUCER_WARP = 8, MMA_WARP = 9, COMPUTE_WARPS = 8;
 constexpr int MAX_TILES = 2048;  // 262144 tokens: the tiles that meet a tile are listed in shared memory
 constexpr float kLog2e = 1.4426950408889634f;

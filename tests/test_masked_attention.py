@@ -7,6 +7,7 @@ import torch
 
 from femtotron_b200.ops import check_kernel_errors
 from femtotron_b200.ops import masked_attention as MA
+from femtotron_b200.ops.matmul import linear_fwd
 
 U16 = torch.finfo(torch.bfloat16).eps / 2  # one rounding to bf16, relative
 
@@ -467,6 +468,30 @@ def test_gpu_in_a_graph_and_on_another_stream():
         graph.replay()
         fresh = run(q, k, v, do, MA.attention_mask(B, S, docs=docs))
         assert all(torch.equal(x, y) for x, y in zip(kept, fresh))
+
+
+@gpu
+def test_gpu_beside_other_work_on_two_streams():
+    # blocks of two calls and of products share SMs, their tensor memory and their shared memory
+    args = [make(1, 900, 8, 2, 128, seed, "cuda", torch.bfloat16) for seed in (1, 2)]
+    mask = MA.attention_mask(1, 900, device="cuda")
+    want = [run(*a, mask) for a in args]
+    a = torch.randn(2048, 2048, device="cuda", dtype=torch.bfloat16)
+    product = linear_fwd(a, a)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for s, x in zip(streams, args):
+            with torch.cuda.stream(s):
+                got.append(run(*x, mask))
+        with torch.cuda.stream(streams[2]):
+            again = linear_fwd(a, a)
+        torch.cuda.synchronize()
+        for g, w in zip(got, want):
+            assert all(torch.equal(x, y) for x, y in zip(g, w))
+        assert torch.equal(again, product)
+    check_kernel_errors(a.device)
 
 
 @gpu

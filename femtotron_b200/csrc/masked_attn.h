@@ -97,6 +97,7 @@ cudaError_t launch_dq(const CUtensorMap& tq, const CUtensorMap& tk, const CUtens
                       const CUtensorMap& tdq, const BwdParams& p, bool cap, bool bias, cudaStream_t st);
 cudaError_t launch_dkv(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& td,
                        const CUtensorMap& tdk, const CUtensorMap& tdv, const BwdParams& p, bool cap, bool bias, cudaStream_t st);
+cudaError_t launch_join(const BwdParams& p, cudaStream_t st);  // of the shares of dk and dv, where p.split > 1
 
 }  // namespace ma
 }  // namespace ft

@@ -32,6 +32,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
                const __grid_constant__ CUtensorMap tm_dk, const __grid_constant__ CUtensorMap tm_dv,
                const __grid_constant__ BwdParams p) {
+  asm volatile("griddepcontrol.launch_dependents;");  // dq may begin where this kernel leaves SMs idle
   using Sm = DkvSmem;
   extern __shared__ uint8_t smem_raw[];
   Sm& s = *reinterpret_cast<Sm*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -316,10 +317,12 @@ cudaError_t launch_dkv(const CUtensorMap& tq, const CUtensorMap& tk, const CUten
     smem_attr_once(kernel, sizeof(DkvSmem) + 1024, cfg);
     kernel<<<dim3(p.B * p.nkv * p.split, p.ntiles), NTHREADS, sizeof(DkvSmem) + 1024, st>>>(tq, tk, tv, td, tdk, tdv, p);
   });
-  if (p.split > 1) {
-    const int64_t n = static_cast<int64_t>(p.B) * p.nkv * p.padded * (p.d / 8) * 2;
-    join_kernel<<<static_cast<unsigned>((n + 255) / 256), 256, 0, st>>>(p);
-  }
+  return cudaGetLastError();
+}
+
+cudaError_t launch_join(const BwdParams& p, cudaStream_t st) {
+  const int64_t n = static_cast<int64_t>(p.B) * p.nkv * p.padded * (p.d / 8) * 2;
+  join_kernel<<<static_cast<unsigned>((n + 255) / 256), 256, 0, st>>>(p);
   return cudaGetLastError();
 }
 

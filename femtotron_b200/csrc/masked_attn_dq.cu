@@ -265,6 +265,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     tc_fence_after();
     tmem_dealloc(s.tmem_base, 512);
   }
+  // what follows on the stream waits for this kernel, so one of its blocks waits for the one before (launch_dq)
+  if (blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && threadIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 cudaError_t launch_delta(const BwdParams& p, const Out& dout, cudaStream_t st) {
@@ -278,9 +280,22 @@ cudaError_t launch_dq(const CUtensorMap& tq, const CUtensorMap& tk, const CUtens
   static_assert(sizeof(DqSmem) + 1024 <= 232448, "shared memory");
   pick(cap, bias, [&](auto CAP, auto BIAS) {
     constexpr auto kernel = dq_kernel<decltype(CAP)::value, decltype(BIAS)::value>;
-    static unsigned long long cfg = 0;
-    smem_attr_once(kernel, sizeof(DqSmem) + 1024, cfg);
-    kernel<<<dim3(p.B * p.nq, p.ntiles), NTHREADS, sizeof(DqSmem) + 1024, st>>>(tq, tk, tv, td, tdq, p);
+    static unsigned long long set = 0;
+    smem_attr_once(kernel, sizeof(DqSmem) + 1024, set);
+    // Launched behind dk and dv, of which it reads nothing: its blocks may start as soon as all of theirs have, so that they
+    // fill the SMs on which the last of those are through (both passes: 8192 tokens in documents 640 -> 626 us, 2 x 4096 in windows of
+    // 1024 with a cap 826 -> 811).
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(p.B * p.nq, p.ntiles);
+    cfg.blockDim = dim3(NTHREADS);
+    cfg.dynamicSmemBytes = sizeof(DqSmem) + 1024;
+    cfg.stream = st;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, kernel, tq, tk, tv, td, tdq, p);
   });
   return cudaGetLastError();
 }

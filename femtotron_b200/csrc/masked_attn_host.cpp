@@ -226,12 +226,11 @@ int64_t masked_attn_bwd(const at::Tensor& q_, const at::Tensor& k_, const at::Te
     p.part = part.data_ptr<float>();
   }
   C10_CUDA_CHECK(launch_delta(p, out_of(dout), st));
-  C10_CUDA_CHECK(launch_dq(heads_map(q, TILE), heads_map(k, STEP), heads_map(v, STEP), heads_map(dout, TILE),
-                           heads_map(dq, TILE), p, softcap > 0,
-                           slopes.has_value(), st));
   C10_CUDA_CHECK(launch_dkv(heads_map(q, STEP), heads_map(k, TILE), heads_map(v, TILE), heads_map(dout, STEP),
-                            heads_map(dk, TILE), heads_map(dv, TILE), p,
-                            softcap > 0, slopes.has_value(), st));
+                            heads_map(dk, TILE), heads_map(dv, TILE), p, softcap > 0, slopes.has_value(), st));
+  C10_CUDA_CHECK(launch_dq(heads_map(q, TILE), heads_map(k, STEP), heads_map(v, STEP), heads_map(dout, TILE),
+                           heads_map(dq, TILE), p, softcap > 0, slopes.has_value(), st));  // right behind: see there
+  if (p.split > 1) C10_CUDA_CHECK(launch_join(p, st));
   return p.split > 1 ? 4 : 3;
 }
 

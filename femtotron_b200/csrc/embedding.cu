@@ -190,6 +190,7 @@ struct SmallSort {
 };
 
 __global__ void __launch_bounds__(SMALL_NT) small_sort_kernel(const SortArgs a) {
+  asm volatile("griddepcontrol.launch_dependents;");  // clearing may run beside this block
   extern __shared__ uint8_t raw[];
   SmallSort& s = *reinterpret_cast<SmallSort*>(raw);
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
@@ -416,19 +417,29 @@ cudaError_t launch_fwd(const FwdArgs& a, cudaStream_t st) {
 }
 
 // 16 bytes per store, four per thread, in many small blocks: 2.1 GB in 280 us.  (A block of 1024 threads per SM, beside the
-// block that sorts, took 350 us; the runtime's memset 337.)
+// block that sorts, took 350 us; the runtime's memset 337.)  Behind the sort in one block it may start beside it, as it reads
+// nothing of it; what follows on the stream waits for this kernel, so one of its blocks waits for the sort.
 __global__ void __launch_bounds__(256) clear_kernel(uint4* __restrict__ x, int64_t words) {
   const int64_t i0 = static_cast<int64_t>(blockIdx.x) * 1024 + threadIdx.x;
 #pragma unroll
   for (int u = 0; u < 4; ++u)
     if (i0 + u * 256 < words) x[i0 + u * 256] = make_uint4(0, 0, 0, 0);
+  if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-cudaError_t launch_clear(void* x, int64_t bytes, cudaStream_t st) {
+cudaError_t launch_clear(void* x, int64_t bytes, bool beside_sort, cudaStream_t st) {
   const int64_t words = bytes / 16, blocks = (words + 1023) / 1024;
   if (reinterpret_cast<uintptr_t>(x) % 16 || bytes % 16 || blocks >= (int64_t(1) << 31)) return cudaMemsetAsync(x, 0, bytes, st);
-  clear_kernel<<<static_cast<unsigned>(blocks), 256, 0, st>>>(static_cast<uint4*>(x), words);
-  return cudaGetLastError();
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cfg.attrs = &early;
+  cfg.numAttrs = beside_sort ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, clear_kernel, static_cast<uint4*>(x), words);
 }
 
 cudaError_t launch_small_sort(const SortArgs& a, cudaStream_t st) {

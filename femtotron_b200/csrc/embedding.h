@@ -43,7 +43,7 @@ struct SortArgs {
   uint32_t *key[2], *pos[2];       // [T] each, in turn
   uint32_t* counts;                // [bins][blocks]
 };
-cudaError_t launch_clear(void* x, int64_t bytes, cudaStream_t st);
+cudaError_t launch_clear(void* x, int64_t bytes, bool beside_sort, cudaStream_t st);
 // One launch for T <= SMALL_SORT: key[0] and pos[0] get the result.
 cudaError_t launch_small_sort(const SortArgs& a, cudaStream_t st);
 // The sorted keys (V for ids of other shards, last) and their places in the batch are in key[passes & 1].

@@ -73,7 +73,7 @@ int64_t embed_sorted_grad(const at::Tensor& ids_, const at::Tensor& dout_, at::T
   if (dst.numel() == 0) return 0;
   TORCH_CHECK(H <= 65535 * 128, "embedding: rows of up to ", 65535 * 128, " values");
   const bool small = T > 0 && T <= SMALL_SORT;
-  if (!accumulate) C10_CUDA_CHECK(launch_clear(dst.data_ptr(), dst.nbytes(), st));
+  if (!accumulate && !small) C10_CUDA_CHECK(launch_clear(dst.data_ptr(), dst.nbytes(), false, st));
   if (T == 0) return accumulate ? 0 : 1;
   const at::Tensor ids = ids_.contiguous(), dout = dout_.contiguous();
   SortArgs s{};
@@ -102,8 +102,10 @@ int64_t embed_sorted_grad(const at::Tensor& ids_, const at::Tensor& dout_, at::T
     s.pos[i] = w + (2 * i + 1) * T;
   }
   s.counts = w + 4 * T;
-  if (small) C10_CUDA_CHECK(launch_small_sort(s, st));
-  else C10_CUDA_CHECK(launch_sort(s, st));
+  if (small) {
+    C10_CUDA_CHECK(launch_small_sort(s, st));
+    if (!accumulate) C10_CUDA_CHECK(launch_clear(dst.data_ptr(), dst.nbytes(), true, st));
+  } else C10_CUDA_CHECK(launch_sort(s, st));
   at::Tensor partial = at::empty({pieces, 2, H}, dst.options().dtype(at::kFloat));
   GradArgs a{};
   a.key = s.key[small ? 0 : s.passes & 1];

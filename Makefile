@@ -38,7 +38,8 @@ test-race:
 	timeout $(TIMEOUT) $(PYTHON) -m pytest tests/test_protocol_model.py -q
 
 test-integration:
-	timeout $(TIMEOUT) $(PYTHON) -m pytest tests/test_distributed_cpu.py tests/test_cli.py tests/test_long_context.py tests/test_packed_training.py -q -m "not gpu"
+	timeout $(TIMEOUT) $(PYTHON) -m pytest tests/test_distributed_cpu.py tests/test_cli.py tests/test_long_context.py tests/test_packed_training.py \
+		tests/test_packed_models.py -q -m "not gpu"
 
 test-quick:
 	timeout $(TIMEOUT) $(PYTHON) -m pytest tests/test_units.py -q

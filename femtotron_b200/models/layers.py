@@ -28,7 +28,8 @@ Attributes that a user may set on the model config:
                   "softcap" (scores capped by a tanh, 0 for none), "window" (tokens that a row reaches
                   back, None), "alibi" (a bias of distance beside the rotation, False), "separator" (the
                   token that ends a document; rows see their own document only, None)
-    embed_scale   factor of the embedding rows (1.0)
+    embed_scale   factor of the embedding rows (1.0), whatever module gives them; one that multiplies by its
+                  own ``scale`` says so with ``applies_scale = True``
 """
 from __future__ import annotations
 

@@ -45,7 +45,7 @@ class LlamaPartialModel(nn.Module):
             self.embed_tokens = nn.Embedding(model_config.vocab_size, model_config.hidden_size,
                                              padding_idx=getattr(model_config, "pad_token_id", None),
                                              device=device, dtype=dtype)
-            self.embed_tokens.scale = self.embed_scale  # a vocabulary-parallel replacement takes it over
+            self.embed_tokens.scale = self.embed_scale  # a vocabulary-parallel replacement takes it over (_embed)
         self.layers = nn.ModuleDict({str(i): LlamaDecoderLayer(model_config, i, device=device, dtype=dtype)
                                      for i in layer_range})
         self.rotary_emb = LlamaRotaryEmbedding(model_config, device=device)
@@ -61,6 +61,18 @@ class LlamaPartialModel(nn.Module):
             ws = int(getattr(q, "world_size", 1))
             return sp and ws > 1, ws
         return False, 1
+
+    def _embed(self, ids: torch.Tensor) -> torch.Tensor:
+        """The embedding's rows times ``embed_scale``.  The factor is the model's: whatever the embedding is or
+        is wrapped in, its rows are multiplied here, unless it says by ``applies_scale`` that it has done so
+        with its ``scale``."""
+        h = self.embed_tokens(ids)
+        if self.embed_scale == 1.0:
+            return h
+        done = float(self.embed_tokens.scale) if getattr(self.embed_tokens, "applies_scale", False) else 1.0
+        if done not in (1.0, self.embed_scale):
+            raise ValueError(f"embed_scale is {self.embed_scale}, but the embedding multiplies its rows by {done}")
+        return h * self.embed_scale if done == 1.0 else h
 
     def _attention(self, x: torch.Tensor, B: int, S: int, docs, prefix) -> Attention | None:
         """What attention does beyond the causal mask in this batch, or None."""
@@ -86,9 +98,7 @@ class LlamaPartialModel(nn.Module):
         sp, tp = self._sequence_parallel()
         if self.is_first:
             B, S = x.shape
-            h = self.embed_tokens(x)
-            if self.embed_scale != 1.0 and isinstance(self.embed_tokens, nn.Embedding):
-                h = h * self.embed_scale
+            h = self._embed(x)
         else:
             h = x
             if batch_shape is not None:

@@ -18,6 +18,8 @@ from femtotron_b200.parallel.tensor_parallel import comm_ops as C
 
 
 class VocabParallelEmbedding(nn.Module):
+    applies_scale = True  # the rows come out times ``scale``: a model with a factor leaves them as they are
+
     def __init__(self, vocab_size: int, hidden_size: int, parallel_ctx, parallel_dim_name="tp",
                  device=None, dtype=None, sequence_parallel: bool = False):
         super().__init__()
@@ -59,4 +61,5 @@ class VocabParallelEmbedding(nn.Module):
                 dtype=embedding.weight.dtype)
         with torch.no_grad():
             m.weight.copy_(embedding.weight[r * chunk:(r + 1) * chunk])
+        m.scale = getattr(embedding, "scale", 1.0)
         return m

@@ -1,0 +1,77 @@
+"""Models on packed documents: the factor of the embedding wherever the embedding comes from."""
+import pytest
+import torch
+
+from femtotron_b200.models import LlamaForTraining
+from femtotron_b200.models.layer_factory import DefaultLayerFactory
+from femtotron_b200.models.parallel_plan import ParallelRule
+from femtotron_b200.parallel.tensor_parallel import VocabParallelEmbedding
+from femtotron_b200.training import apply_activation_checkpointing
+from test_packed_training import base, config, run, same  # noqa: F401
+
+
+def graded(model, ids):
+    out = model(ids, labels=ids, materialize_logits=True)
+    out["loss"].backward()
+    return float(out["loss"].detach()), out["logits"].detach(), \
+        {k.replace("._checkpoint_wrapped_module", ""): p.grad for k, p in model.named_parameters()}
+
+
+class OneRank:
+    """A parallel context without groups."""
+    tp_size = 1
+
+    def get_group(self, name):
+        return None
+
+    def get_size(self, name):
+        return 1
+
+    def get_rank(self, name):
+        return 0
+
+
+class OwnEmbedding(torch.nn.Module):
+    def __init__(self, plain):
+        super().__init__()
+        self.weight = plain.weight
+
+    def forward(self, ids):
+        return self.weight[ids]
+
+
+@pytest.mark.parametrize("kind", ["checkpointed", "vocabulary", "vocabulary, checkpointed", "vocabulary, temporary", "factory", "own"])
+def test_embed_scale_reaches_every_embedding(base, kind):
+    sd, ids, _ = base
+    want = run(config(embed_scale=4.0), sd, ids)
+    cfg = config(embed_scale=4.0)
+    model = LlamaForTraining(cfg, dtype=torch.float32)
+    plain = model.model.embed_tokens
+    if kind.startswith("vocabulary"):
+        if "temporary" in kind:
+            model.model.embed_tokens = VocabParallelEmbedding.from_embedding_temp(plain, OneRank())
+            assert model.model.embed_tokens.scale == 4.0
+        else:
+            model.model.embed_tokens = VocabParallelEmbedding.from_embedding(plain, OneRank(), ParallelRule("vocab_embed", {}))
+    elif kind == "factory":  # what it makes without tensor parallelism, and with it
+        model.model.embed_tokens = DefaultLayerFactory().make_embedding(cfg, None, dtype=torch.float32, device=None)
+        model.load_state_dict(sd)
+        same(graded(model, ids), want)
+        model.zero_grad(set_to_none=True)
+        model.model.embed_tokens = VocabParallelEmbedding(cfg.vocab_size, cfg.hidden_size, OneRank(), dtype=torch.float32)
+    elif kind == "own":
+        model.model.embed_tokens = OwnEmbedding(plain)
+    model.load_state_dict(sd)
+    if "checkpointed" in kind:
+        assert apply_activation_checkpointing(model, lambda m: isinstance(m, (torch.nn.Embedding, VocabParallelEmbedding))) == 1
+    same(graded(model, ids), want)
+
+
+def test_another_factor_of_the_embedding_is_refused(base):
+    sd, ids, _ = base
+    model = LlamaForTraining(config(embed_scale=4.0), dtype=torch.float32)
+    model.model.embed_tokens = VocabParallelEmbedding.from_embedding(model.model.embed_tokens, OneRank(), ParallelRule("vocab_embed", {}))
+    model.load_state_dict(sd)
+    model.model.embed_tokens.scale = 2.0
+    with pytest.raises(ValueError, match="embed_scale"):
+        model(ids)

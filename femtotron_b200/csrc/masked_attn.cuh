@@ -196,20 +196,24 @@ __device__ __forceinline__ float2 exp2_of(float2 x, int e) {
 // Raw products as what an FMA with `unit(p)` turns into scores in log2 units: with the cap tanh(x) (KEEP: `keep` is
 // 1 - tanh^2, the slope of the cap), without it the products themselves.  tanh(x) = 1 - 2 / (1 + exp(2x)) costs two
 // special-function instructions of 8 clocks each (tanh.approx would be off by 5e-4 of the cap: whole percents of p).
-// Where a warp's products are all within 0.7 of the cap, as nearly all are, a polynomial does it on the FMA pipe, off by
-// 2e-7 (the other form by 1e-7): 288 -> 242 us for the forward pass of two rows of 4096 tokens in windows of 1024.
+// Products within 0.7 of the cap, as nearly all are, take a polynomial, off by 2e-7 (the other form by 1e-7).  Which form a
+// product takes depends on its own value alone, so that a row's bits do not depend on what it cannot see (padding, other
+// documents, later tokens) nor on the rows beside it.  A warp whose products are all small, seen or not, is through with
+// that; else it works out both where one of its next eight products is large.  (Two rows of 4096 tokens in windows of 1024, 32
+// heads over 8, all small: 213, 273, 293 us for forward, dq, and dk and dv, where the other form alone took 288 forward; every
+// fourth product large: 393, 393, 444, where a form chosen by the warp took 288, 337, 357.)
 template <bool CAP, bool KEEP, int N>
 __device__ __forceinline__ void cap_scores(uint32_t (&sv)[N], float (&keep)[KEEP ? N : 1], const Common& p) {
   if (!CAP) return;
   float m[2] = {0.f, 0.f};
 #pragma unroll
   for (int e = 0; e < N; ++e) m[e & 1] = fmaxf(m[e & 1], fabsf(__uint_as_float(sv[e])));
-  if (__all_sync(0xffffffffu, fmaxf(m[0], m[1]) <= p.cap_small)) {
-    uint64_t c[5];
+  uint64_t c[5];
 #pragma unroll
-    for (int i = 0; i < 5; ++i) c[i] = pair(p.cap_poly[i], p.cap_poly[i]);
+  for (int i = 0; i < 5; ++i) c[i] = pair(p.cap_poly[i], p.cap_poly[i]);
+  auto near = [&](int from, int to) {
 #pragma unroll
-    for (int e = 0; e < N; e += 2) {
+    for (int e = from; e < to; e += 2) {
       const uint64_t s = pair(__uint_as_float(sv[e]), __uint_as_float(sv[e + 1])), u = mul2(s, s);
       const uint64_t t = mul2(fma2(fma2(fma2(fma2(u, c[4], c[3]), u, c[2]), u, c[1]), u, c[0]), s);
       const float2 y = apart(t);
@@ -221,12 +225,28 @@ __device__ __forceinline__ void cap_scores(uint32_t (&sv)[N], float (&keep)[KEEP
         keep[KEEP ? e + 1 : 0] = k.y;
       }
     }
-  } else {
+  };
+  if (__all_sync(0xffffffffu, fmaxf(m[0], m[1]) <= p.cap_small)) {
+    near(0, N);
+    return;
+  }
+  constexpr int G = 8;  // (groups of two: 428, 467, 524 us, of four: 408, 401, 457; of 16 spill more)
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const float r = rcp_approx(1.f + ex2_approx(__uint_as_float(sv[e]) * p.cap_in));
-      sv[e] = __float_as_uint(fmaf(-2.f, r, 1.f));
-      if (KEEP) keep[KEEP ? e : 0] = 4.f * r * (1.f - r);
+  for (int g = 0; g < N; g += G) {
+    float far[G];
+    bool any = false;
+#pragma unroll
+    for (int e = 0; e < G; ++e) far[e] = __uint_as_float(sv[g + e]), any = any || !(fabsf(far[e]) <= p.cap_small);
+    near(g, g + G);
+    if (__any_sync(0xffffffffu, any)) {
+#pragma unroll
+      for (int e = 0; e < G; ++e) {
+        const float r = rcp_approx(1.f + ex2_approx(far[e] * p.cap_in));
+        if (!(fabsf(far[e]) <= p.cap_small)) {
+          sv[g + e] = __float_as_uint(fmaf(-2.f, r, 1.f));
+          if (KEEP) keep[KEEP ? g + e : 0] = 4.f * r * (1.f - r);
+        }
+      }
     }
   }
 }

@@ -1,0 +1,61 @@
+"""Masked attention on the GPU: bits of a row that do not depend on what it cannot see, and combinations of heads, scores and
+masks against the formulas in 64 bits."""
+import math
+
+import pytest
+import torch
+
+from femtotron_b200.ops import masked_attention as MA
+from test_masked_attention import make, run
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("softcap", [30.0, 50.0])
+@pytest.mark.parametrize("bad", [1e3, 3e38, math.inf, math.nan])
+def test_capped_scores_do_not_depend_on_padding(bad, softcap, bias):
+    # scores of N(0, 1): all within 0.7 of the cap, those of the padding far beyond it
+    B, S, nq, nkv, d = 1, 400, 4, 2, 64
+    q, k, v, do = make(B, S, nq, nkv, d, 2, "cuda", torch.bfloat16)
+    docs = (torch.arange(S, device="cuda") // 90).int().repeat(B, 1)
+    docs[0, 150:170] = -1
+    docs[0, 390:] = -1
+    mask = MA.attention_mask(B, S, docs=docs)
+    kw = dict(softcap=softcap, slopes=MA.alibi_slopes(nq, "cuda") if bias else None)
+    clean = run(q, k, v, do, mask, **kw)
+    dead = docs < 0
+    for x in (q, k, v, do):
+        x[dead] = bad
+    for name, x, y in zip(("o", "dq", "dk", "dv"), run(q, k, v, do, mask, **kw), clean):
+        assert torch.equal(x, y), name
+
+
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("d", [64, 128])
+def test_capped_scores_do_not_depend_on_other_documents(d, bias):
+    B, S, nq, nkv, cap = 1, 400, 4, 2, 30.0
+    q, k, v, do = make(B, S, nq, nkv, d, 3, "cuda", torch.bfloat16)
+    docs = (torch.arange(S, device="cuda") // 90).int()[None]
+    mask = MA.attention_mask(B, S, docs=docs)
+    kw = dict(softcap=cap, slopes=MA.alibi_slopes(nq, "cuda") if bias else None)
+    clean = run(q, k, v, do, mask, **kw)
+    other = docs[0] == 1
+    q[:, other] *= 16
+    k[:, other] *= 16
+    for name, x, y in zip(("o", "dq", "dk", "dv"), run(q, k, v, do, mask, **kw), clean):
+        assert torch.equal(x[:, ~other], y[:, ~other]), name
+        assert not torch.equal(x[:, other], y[:, other])
+
+
+@pytest.mark.parametrize("cut", [1, 40, 200, 250])
+def test_capped_scores_do_not_depend_on_later_tokens(cut):
+    B, S, nq, nkv, d = 1, 300, 4, 2, 64
+    q, k, v, do = make(B, S, nq, nkv, d, 4, "cuda", torch.bfloat16)
+    mask = MA.attention_mask(B, S, device="cuda")
+    clean = run(q, k, v, do, mask, softcap=30.0)
+    q[:, cut:] *= 16
+    k[:, cut:] *= 16
+    got = run(q, k, v, do, mask, softcap=30.0)
+    for n in (0, 1):  # (dk and dv gather from later rows)
+        assert torch.equal(got[n][:, :cut], clean[n][:, :cut])

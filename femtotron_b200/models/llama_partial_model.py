@@ -39,6 +39,7 @@ class LlamaPartialModel(nn.Module):
         self.is_first = (layer_range.start == 0) if is_first is None else is_first
         self.is_last = (layer_range.stop == n_layers) if is_last is None else is_last
         self.attn_spec = attn_spec_of(model_config)
+        self._slopes: dict[torch.device, torch.Tensor] = {}
         scale = getattr(model_config, "embed_scale", None)
         self.embed_scale = 1.0 if scale is None else float(scale)
         if self.is_first:
@@ -74,6 +75,17 @@ class LlamaPartialModel(nn.Module):
             raise ValueError(f"embed_scale is {self.embed_scale}, but the embedding multiplies its rows by {done}")
         return h * self.embed_scale if done == 1.0 else h
 
+    def _alibi_slopes(self, device: torch.device) -> torch.Tensor:
+        """The slopes of all heads, made once per device: the copy from the host waits for the stream, and a graph that is
+        being captured takes none (what is made while one is belongs to it and is not kept)."""
+        kept = self._slopes.get(device)
+        if kept is None:
+            with torch.inference_mode(False):  # kept for passes with gradients too
+                kept = MA.alibi_slopes(self.config.num_attention_heads, device)
+            if not (device.type == "cuda" and torch.cuda.is_current_stream_capturing()):
+                self._slopes[device] = kept
+        return kept
+
     def _attention(self, x: torch.Tensor, B: int, S: int, docs, prefix) -> Attention | None:
         """What attention does beyond the causal mask in this batch, or None."""
         spec = self.attn_spec or {"softcap": 0.0, "window": None, "alibi": False, "separator": None}
@@ -85,7 +97,7 @@ class LlamaPartialModel(nn.Module):
             return None
         mask = MA.attention_mask(B if docs is not None or prefix is not None else 1, S, window=spec["window"], docs=docs,
                                  prefix=prefix, device=x.device)
-        slopes = MA.alibi_slopes(self.config.num_attention_heads, x.device) if spec["alibi"] else None
+        slopes = self._alibi_slopes(x.device) if spec["alibi"] else None
         return Attention(mask, spec["softcap"], slopes)
 
     def forward(self, x: torch.Tensor, attention_mask: torch.Tensor | None = None,

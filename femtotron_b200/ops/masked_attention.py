@@ -123,10 +123,16 @@ def document_ids(input_ids: torch.Tensor, separator: int) -> torch.Tensor:
 
 def alibi_slopes(heads: int, device=None) -> torch.Tensor:
     """Slopes 2^(-8 i / n) for i = 1 ... n of the bias of distance, fp32; for a number of heads that is no
-    power of two, those of the next lower power and every other one of the next higher."""
+    power of two, those of the next lower power and every other one of the next higher.  On CUDA the host waits
+    for the stream, except while a graph is captured, which then holds a kernel per head: keep the tensor."""
     n = 2 ** int(math.log2(heads))
     slopes = [2.0 ** (-8.0 * i / n) for i in range(1, n + 1)]
     slopes += [2.0 ** (-4.0 * i / n) for i in range(1, 2 * (heads - n), 2)]
+    if device is not None and torch.device(device).type == "cuda" and torch.cuda.is_current_stream_capturing():
+        out = torch.empty(heads, dtype=torch.float32, device=device)
+        for i, s in enumerate(slopes):
+            out[i].fill_(s)
+        return out
     return torch.tensor(slopes, dtype=torch.float32, device=device)
 
 

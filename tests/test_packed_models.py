@@ -1,13 +1,17 @@
-"""Models on packed documents: the factor of the embedding wherever the embedding comes from."""
+"""Models on packed documents: the factor of the embedding wherever the embedding comes from, slopes that are made once."""
 import pytest
 import torch
 
 from femtotron_b200.models import LlamaForTraining
 from femtotron_b200.models.layer_factory import DefaultLayerFactory
 from femtotron_b200.models.parallel_plan import ParallelRule
+from femtotron_b200.ops import masked_attention as MA
 from femtotron_b200.parallel.tensor_parallel import VocabParallelEmbedding
 from femtotron_b200.training import apply_activation_checkpointing
+from common_models import full_state
 from test_packed_training import base, config, run, same  # noqa: F401
+
+gpu = pytest.mark.gpu
 
 
 def graded(model, ids):
@@ -75,3 +79,50 @@ def test_another_factor_of_the_embedding_is_refused(base):
     model.model.embed_tokens.scale = 2.0
     with pytest.raises(ValueError, match="embed_scale"):
         model(ids)
+
+
+def test_slopes_are_made_once(base, monkeypatch):
+    sd, ids, _ = base
+    made = []
+    slopes = MA.alibi_slopes
+    monkeypatch.setattr(MA, "alibi_slopes", lambda *a: made.append(a) or slopes(*a))
+    model = LlamaForTraining(config(attn_spec={"alibi": True}), dtype=torch.float32)
+    model.load_state_dict(sd)
+    with torch.no_grad():
+        first = model(ids)["logits"].clone()
+    for _ in range(2):  # what a pass without gradients made serves those with gradients
+        loss, logits, _ = graded(model, ids)
+        assert torch.equal(logits, first)
+    assert len(made) == 1 and set(model.state_dict()) == set(sd)
+
+
+@gpu
+def test_gpu_slopes_neither_wait_nor_stop_a_graph():
+    cfg = config(num_attention_heads=12, num_key_value_heads=6, hidden_size=192, intermediate_size=256,
+                 attn_spec={"alibi": True, "window": 50, "softcap": 20.0})
+    sd = {k: v.bfloat16() for k, v in full_state(cfg).items()}
+    ids = torch.randint(1, 200, (2, 150), generator=torch.Generator().manual_seed(1)).cuda()
+    model = LlamaForTraining(cfg, dtype=torch.bfloat16, device="cuda")
+    model.load_state_dict(sd)
+    with torch.no_grad():
+        want = model.model(ids)
+        torch.cuda.set_sync_debug_mode("error")
+        try:
+            got = model.model(ids)
+        finally:
+            torch.cuda.set_sync_debug_mode("default")
+        assert torch.equal(got, want)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        for kept in (True, False):  # with slopes at hand, and made in the graph
+            if not kept:
+                model.model._slopes.clear()
+            with torch.cuda.stream(side):
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph, stream=side):
+                    out = model.model(ids)
+            torch.cuda.current_stream().wait_stream(side)
+            assert bool(model.model._slopes) == kept
+            graph.replay()
+            assert torch.equal(out, want)
+        assert torch.equal(model.model(ids), want)

@@ -15,12 +15,16 @@ compute parameters of the model state dict.  Shapes come from the model configur
 which the checkpoint does not store, so the caller passes it.
 
 ``export_hf`` writes ``config.json`` + ``model.safetensors`` that
-``transformers.LlamaForCausalLM.from_pretrained`` and this package's ``ModelLoader`` read.
+``transformers.LlamaForCausalLM.from_pretrained`` and this package's ``ModelLoader`` read.  A factor of
+the embedding goes into the exported table.  What that class cannot express (capped scores, a window, a bias of
+distance, a factor on a table that the head shares) is refused, unless the directory is meant for this package
+alone.  Documents (``attn_spec``'s separator) concern packed rows, not the model, and stay in the configuration.
 The reference has no exporter (it only loads Hugging Face weights,
 femtotron/model/model_loader.py:28-104).
 """
 from __future__ import annotations
 
+import copy
 import glob
 import json
 import os
@@ -116,10 +120,33 @@ def consolidate_checkpoint(ckpt_dir: str, model_config) -> dict[str, torch.Tenso
     return out
 
 
-def export_hf(ckpt_dir: str, model_config, out_dir: str, dtype: torch.dtype = torch.bfloat16) -> str:
-    """Write `ckpt_dir`'s model as a Hugging Face directory (config.json + model.safetensors)."""
+def _beyond_llama(model_config) -> list[str]:
+    """What the model does that ``transformers.LlamaForCausalLM`` would leave out without a word."""
+    from .layers import attn_spec_of
+    spec = attn_spec_of(model_config) or {}
+    out = [f"{k}={spec[k]}" for k in ("softcap", "window", "alibi") if spec.get(k)]
+    scale = getattr(model_config, "embed_scale", None)
+    if scale not in (None, 1.0) and getattr(model_config, "tie_word_embeddings", False):
+        out.append(f"embed_scale={scale} on a tied table")
+    return out
+
+
+def export_hf(ckpt_dir: str, model_config, out_dir: str, dtype: torch.dtype = torch.bfloat16,
+              keep_attributes: bool = False) -> str:
+    """Write `ckpt_dir`'s model as a Hugging Face directory (config.json + model.safetensors).
+    `keep_attributes`: for this package alone; weights and the configuration's own attributes (attn_spec,
+    embed_scale) are written as they are."""
     from safetensors.torch import save_file
+    beyond = [] if keep_attributes else _beyond_llama(model_config)
+    if beyond:
+        raise ValueError(f"export_hf: transformers.LlamaForCausalLM does not have {', '.join(beyond)}: the exported model would "
+                         "compute other logits there (keep_attributes writes it for this package alone)")
     sd = consolidate_checkpoint(ckpt_dir, model_config)
+    scale = getattr(model_config, "embed_scale", None)
+    if scale is not None and not keep_attributes:
+        model_config = copy.deepcopy(model_config)
+        del model_config.embed_scale
+        sd["model.embed_tokens.weight"] = sd["model.embed_tokens.weight"] * float(scale)
     os.makedirs(out_dir, exist_ok=True)
     save_file({k: v.to(dtype).contiguous() for k, v in sd.items()},
               os.path.join(out_dir, "model.safetensors"), metadata={"format": "pt"})

@@ -1,8 +1,13 @@
-"""Models on packed documents: the factor of the embedding wherever the embedding comes from, slopes that are made once."""
+"""Models on packed documents: the factor of the embedding wherever the embedding comes from, slopes that are made
+once, exported models."""
+import json
+
 import pytest
 import torch
+from safetensors.torch import load_file
 
 from femtotron_b200.models import LlamaForTraining
+from femtotron_b200.models.export import export_hf
 from femtotron_b200.models.layer_factory import DefaultLayerFactory
 from femtotron_b200.models.parallel_plan import ParallelRule
 from femtotron_b200.ops import masked_attention as MA
@@ -94,6 +99,54 @@ def test_slopes_are_made_once(base, monkeypatch):
         loss, logits, _ = graded(model, ids)
         assert torch.equal(logits, first)
     assert len(made) == 1 and set(model.state_dict()) == set(sd)
+
+
+def checkpoint(path, model):
+    path.mkdir()
+    (path / "meta.json").write_text(json.dumps({"tp_size": 1, "dp_size": 1}))
+    torch.save({"optimizer": {}, "model": model.state_dict()}, path / "shard_tp0_dp0.pt")
+    return str(path)
+
+
+@pytest.mark.parametrize("attrs", [dict(embed_scale=3.0), dict(embed_scale=3.0, attn_spec={"separator": 0}), dict(embed_scale=1.0), {}])
+def test_exported_models_compute_the_same(base, tmp_path, attrs):
+    from transformers import AutoConfig, LlamaForCausalLM
+    sd, ids, _ = base
+    cfg = config(**attrs)
+    model = LlamaForTraining(cfg, dtype=torch.float32)
+    model.load_state_dict(sd)
+    out = export_hf(checkpoint(tmp_path / "ck", model), cfg, str(tmp_path / "hf"), dtype=torch.float32)
+    assert {k: getattr(cfg, k) for k in attrs} == attrs
+    with torch.no_grad():
+        want = model(ids)["logits"]  # (no separator among the ids)
+        theirs = LlamaForCausalLM.from_pretrained(out, dtype=torch.float32)(input_ids=ids).logits
+        read = AutoConfig.from_pretrained(out)
+        again = LlamaForTraining(read, dtype=torch.float32)
+        again.load_state_dict(load_file(out + "/model.safetensors"))
+        ours = again(ids)["logits"]
+    # fp32 in another order, as same()
+    assert float((theirs - want).abs().max()) < 1e-5 * float(want.abs().max())
+    assert float((ours - want).abs().max()) < 1e-5 * float(want.abs().max())
+    assert not hasattr(read, "embed_scale")
+
+
+@pytest.mark.parametrize("attrs,what", [(dict(attn_spec={"softcap": 5.0}), "softcap=5.0"), (dict(attn_spec={"window": 7}), "window=7"),
+                                        (dict(attn_spec={"alibi": True}), "alibi"),
+                                        (dict(embed_scale=3.0, tie_word_embeddings=True), "tied")])
+def test_what_llama_cannot_express_is_not_exported(base, tmp_path, attrs, what):
+    from transformers import AutoConfig
+    _, ids, _ = base
+    cfg = config(**attrs)
+    model = LlamaForTraining(cfg, dtype=torch.float32)
+    ck = checkpoint(tmp_path / "ck", model)
+    with pytest.raises(ValueError, match=what):
+        export_hf(ck, cfg, str(tmp_path / "hf"))
+    assert not (tmp_path / "hf").exists()
+    out = export_hf(ck, cfg, str(tmp_path / "own"), dtype=torch.float32, keep_attributes=True)
+    again = LlamaForTraining(AutoConfig.from_pretrained(out), dtype=torch.float32)
+    again.load_state_dict(load_file(out + "/model.safetensors"), strict=not cfg.tie_word_embeddings)
+    with torch.no_grad():
+        assert torch.equal(again(ids)["logits"], model(ids)["logits"])
 
 
 @gpu

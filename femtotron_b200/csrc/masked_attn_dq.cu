@@ -14,7 +14,7 @@ constexpr int DELTA_UNITS = 4;
 __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ BwdParams p, const Out dout) {
   const int part = threadIdx.x & 15, b = blockIdx.y;
   const uint32_t total = static_cast<uint32_t>(p.padded) * p.nq;  // of one sequence: 32-bit divisions
-  const uint32_t u0 = (blockIdx.x * 256 + threadIdx.x) / 16, step = gridDim.x * 16;
+  const uint32_t u0 = blockIdx.x * 16 + threadIdx.x / 16, step = gridDim.x * 16;  // (blocks times threads may pass 32 bits)
   uint4 x[DELTA_UNITS], l[DELTA_UNITS], y[DELTA_UNITS];
   int64_t stat[DELTA_UNITS];
   bool live[DELTA_UNITS];

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from femtotron_b200.ops import masked_attention as MA
-from test_masked_attention import make, run
+from test_masked_attention import U16, make, reference, run
 
 pytestmark = pytest.mark.gpu
 
@@ -59,3 +59,27 @@ def test_capped_scores_do_not_depend_on_later_tokens(cut):
     got = run(q, k, v, do, mask, softcap=30.0)
     for n in (0, 1):  # (dk and dv gather from later rows)
         assert torch.equal(got[n][:, :cut], clean[n][:, :cut])
+
+
+def test_row_sums_of_more_than_two_to_the_30_rows():
+    B, S, nq, nkv, d = 1, MA.MAX_TOKENS, 4104, 1, 8
+    assert S * nq > 2 ** 30
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 125e9:
+        pytest.skip("needs 125 GB of free GPU memory")
+    g = torch.Generator(device="cuda").manual_seed(0)
+
+    def some(heads):
+        return torch.empty(B, S, heads, d, device="cuda", dtype=torch.bfloat16).normal_(generator=g)
+    q, k, v, do = some(nq).requires_grad_(), some(nkv), some(nkv), some(nq)
+    docs = (torch.arange(S, device="cuda") // 64).int()[None]
+    o = MA.masked_attention(q, k, v, MA.attention_mask(B, S, docs=docs))
+    (dq,) = torch.autograd.grad(o, q, do)
+    vis = torch.ones(64, 64, dtype=torch.bool).tril()[None]
+    for first in range(S // 16 - 64, S, S // 16):  # documents all over the rows, all heads of each
+        part = [x.detach()[:, first:first + 64] for x in (q, k, v, do)]
+        want, size = reference(*part, vis, 1 / math.sqrt(d), 0.0, None)
+        x, y, z = dq[:, first:first + 64].double(), want[1], size[1]
+        assert ((x - y).abs() <= (2 * U16 + 2 ** -14) * z + U16 * y.abs()).all(), first
+    del q, k, v, do, o, dq
+    torch.cuda.empty_cache()

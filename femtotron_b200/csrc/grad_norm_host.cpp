@@ -109,6 +109,7 @@ at::Tensor dense(const at::Tensor& x) { return x.is_non_overlapping_and_dense() 
 struct Plan {
   std::vector<Item> items;
   std::vector<at::Tensor> held;                            // the copies
+  std::vector<at::Tensor> written;                         // by the kernel, of the caller's own
   std::vector<std::pair<at::Tensor, at::Tensor>> back;     // (to, from) once the kernel is done
   bool in_place;
 };
@@ -125,7 +126,9 @@ Plan plan_of(const char* op, const std::vector<at::Tensor>& xs, const std::vecto
     if (xs[i].numel() == 0) continue;
     at::Tensor src = dense(xs[i]);
     at::Tensor dst = o.is_non_overlapping_and_dense() && o.strides() == src.strides() ? o : at::Tensor();
-    if (!dst.defined()) {
+    if (dst.defined()) {
+      p.written.push_back(o);
+    } else {
       dst = p.in_place ? src : at::empty_like(src);  // in place: src is a copy already
       p.back.emplace_back(o, dst);
     }
@@ -135,6 +138,14 @@ Plan plan_of(const char* op, const std::vector<at::Tensor>& xs, const std::vecto
   }
   check_apart(op, p.items, {4, 2, 2});
   return p;
+}
+
+// Once the kernels are launched: copies go back, and autograd learns (as from the copy) that what a kernel wrote itself has
+// changed.
+void finish(const Plan& p) {
+  for (const auto& [to, from] : p.back) to.copy_(from);
+  for (const at::Tensor& x : p.written)
+    if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
 }
 
 // Launches the sums of all tables; the partial sums [blocks, n_slots].
@@ -181,7 +192,7 @@ at::Tensor grad_sumsq(const std::vector<at::Tensor>& xs, const std::vector<int64
 void grad_scale(const std::vector<at::Tensor>& xs, const at::Tensor& coef, const std::vector<at::Tensor>& outs) {
   using namespace gn;
   if (xs.empty()) return;
-  Plan p = plan_of("scale_grads", xs, outs);
+  const Plan p = plan_of("scale_grads", xs, outs);
   TORCH_CHECK(coef.scalar_type() == at::kFloat && coef.numel() == 1 && coef.device() == xs[0].device(),
               "scale_grads: the factor must be one fp32 number on the tensors' device");
   const c10::cuda::CUDAGuard g(xs[0].device());
@@ -190,13 +201,13 @@ void grad_scale(const std::vector<at::Tensor>& xs, const at::Tensor& coef, const
   const Tables tables(p.items);
   const Factor f{coef.data_ptr<float>(), nullptr, 0, 0.f, nullptr, p.in_place};
   tables.each([&](const auto& t) { C10_CUDA_CHECK(launch_scale(t, f, st)); });
-  for (auto& [to, from] : p.back) to.copy_(from);
+  finish(p);
 }
 
 at::Tensor grad_clip(const std::vector<at::Tensor>& xs, double max_norm, const std::vector<at::Tensor>& outs) {
   using namespace gn;
   TORCH_CHECK(!xs.empty(), "clip_grads: no tensors");
-  Plan p = plan_of("clip_grads", xs, outs);
+  const Plan p = plan_of("clip_grads", xs, outs);
   const c10::cuda::CUDAGuard g(xs[0].device());
   auto st = at::cuda::getCurrentCUDAStream();
   at::Tensor norm = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(xs[0].device()));
@@ -206,7 +217,7 @@ at::Tensor grad_clip(const std::vector<at::Tensor>& xs, double max_norm, const s
   const Factor f{nullptr, part.data_ptr<double>(), static_cast<int>(part.size(0)), static_cast<float>(max_norm),
                  norm.data_ptr<float>(), p.in_place};
   tables.each([&](const auto& t) { C10_CUDA_CHECK(launch_scale(t, f, st)); });
-  for (auto& [to, from] : p.back) to.copy_(from);
+  finish(p);
   return norm;
 }
 

@@ -1,5 +1,6 @@
 // Entry points of the gradient norm and clipping (grad_norm.h).
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -124,6 +125,7 @@ Plan plan_of(const char* op, const std::vector<at::Tensor>& xs, const std::vecto
     TORCH_CHECK_VALUE(o.sizes() == xs[i].sizes() && o.scalar_type() == xs[i].scalar_type() && o.device() == xs[0].device(), op,
                       ": an output of ", o.scalar_type(), " ", o.sizes(), " for ", xs[i].scalar_type(), " ", xs[i].sizes());
     if (xs[i].numel() == 0) continue;
+    at::assert_no_internal_overlap(o);
     at::Tensor src = dense(xs[i]);
     at::Tensor dst = o.is_non_overlapping_and_dense() && o.strides() == src.strides() ? o : at::Tensor();
     if (dst.defined()) {
@@ -137,6 +139,18 @@ Plan plan_of(const char* op, const std::vector<at::Tensor>& xs, const std::vecto
     p.items.push_back({src.data_ptr(), dst.data_ptr(), src.numel(), type_of(op, src), 0});
   }
   check_apart(op, p.items, {4, 2, 2});
+  // Written by a copy: as far as first addresses tell, as the columns of one matrix are no solid pieces but lie apart.
+  std::vector<std::pair<uintptr_t, uintptr_t>> solid;
+  for (const at::Tensor& x : p.written) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(x.data_ptr());
+    solid.emplace_back(a, a + x.nbytes());
+  }
+  for (const auto& [to, from] : p.back) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(to.data_ptr());
+    for (const auto& [begin, end] : solid)
+      TORCH_CHECK(a < begin || a >= end, op, ": two of the tensors written share memory");
+    solid.emplace_back(a, a + 1);
+  }
   return p;
 }
 

@@ -66,6 +66,12 @@ def sum_of_squares(tensors, slots=None, n_slots: int = 1) -> torch.Tensor:
     return out
 
 
+def _check_written(tensors) -> None:
+    for t in tensors:
+        if t.numel() and any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
+            raise RuntimeError("more than one element of a tensor that is written refers to a single memory location")
+
+
 def _scale_cpu(tensors, coef, out) -> None:
     for t, o in zip(tensors, tensors if out is None else out):
         o.copy_((t.float() * coef).to(t.dtype) if t.dtype != torch.float64 else t * coef)
@@ -86,6 +92,7 @@ def scale_grads(tensors, coef: torch.Tensor, out=None) -> None:
     if out is not None:
         _check_out("scale_grads", tensors, out)
     _check("scale_grads", tensors)
+    _check_written(tensors if out is None else out)
     _scale_cpu(tensors, coef, out)
 
 
@@ -106,6 +113,7 @@ def clip_grads(grads, max_norm: float, out=None) -> torch.Tensor:
     if not grads:
         return torch.zeros(())
     _check("clip_grads", grads)
+    _check_written(grads if out is None else out)
     norm = sum_of_squares(grads)[0].sqrt().float()
     _scale_cpu(grads, (max_norm / (norm + 1e-6)).clamp(max=1.0), out)
     return norm

@@ -1,4 +1,4 @@
-"""Clipping and scaling in place: what autograd saved is known to have changed."""
+"""Clipping and scaling in place: what autograd saved is known to have changed, and a call that is refused changes nothing."""
 import pytest
 import torch
 
@@ -30,3 +30,31 @@ def test_what_was_saved_for_a_backward_pass_is_known_to_have_changed(device, cal
         GN.sum_of_squares([x])
         GN.clip_grads([x], 1.0, out=[torch.empty_like(x)])
         assert x._version == 0
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_tensor_with_a_value_in_several_places_is_refused_before_anything_is_written(device):
+    for wide in (torch.ones(3, 1, device=device).expand(3, 4), torch.ones(1, device=device).expand(5)):
+        x = torch.full((7,), 2.0, device=device)
+        for call in (lambda: GN.clip_grads([x, wide], 1e-3), lambda: GN.scale_grads([x, wide], coef_of(x)),
+                     lambda: GN.clip_grads([x, wide], 1e-3, out=[torch.empty_like(x), wide]),
+                     lambda: GN.scale_grads([wide, x], coef_of(x), out=[wide, x])):
+            with pytest.raises(RuntimeError, match="single memory location"):
+                call()
+            assert (x == 2).all() and (wide == 1).all()
+        GN.clip_grads([x, wide], 1e-3, out=[torch.empty_like(x), torch.empty(wide.shape, device=device)])  # read, not written
+
+
+@gpu
+def test_gpu_strided_outputs_that_share_memory_are_refused():
+    base = torch.ones(8, 6, device="cuda")
+    a, b = base[:, ::2], base[:, 1::2]
+    GN.clip_grads([a, b], 1.0)  # columns in turn: nothing is shared
+    assert abs(base.norm().item() - 1) < 1e-5
+    for pair in ([a, a], [a, base[:, :5]], [base, a], [a, base]):
+        keep = base.clone()
+        with pytest.raises(RuntimeError, match="share"):
+            GN.clip_grads(pair, 1e-3)
+        with pytest.raises(RuntimeError, match="share"):
+            GN.scale_grads([torch.ones_like(x) for x in pair], coef_of(base), out=pair)
+        assert torch.equal(base, keep)

@@ -32,7 +32,7 @@ test-unit:
 		tests/test_linear_xent_ignored_rows.py tests/test_linear_xent_paths.py tests/test_linear_xent_weight_graph.py \
 		tests/test_act8_strided_rows.py tests/test_swiglu8_range.py tests/test_checkpoint8.py tests/test_mlp8_modules.py \
 		tests/test_rotary_inplace.py tests/test_rope_scaling_keys.py tests/test_one_device.py \
-		tests/test_masked_attention.py tests/test_embedding.py tests/test_grad_norm.py tests/test_grad_norm_inplace.py -q -m "not gpu"
+		tests/test_masked_attention.py tests/test_embedding.py tests/test_grad_norm.py tests/test_grad_norm_inplace.py tests/test_cpu_fp64.py -q -m "not gpu"
 
 test-race:
 	timeout $(TIMEOUT) $(PYTHON) -m pytest tests/test_protocol_model.py -q

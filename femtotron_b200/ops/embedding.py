@@ -6,7 +6,7 @@
 The gradient's sums run over the tokens in the order of the batch, in fp32, cut where the sorted list
 of tokens is cut into pieces of 32: no atomics, the same bits every time, and a frequent word takes no
 longer than rare ones.  CUDA tensors run ``csrc/embedding.cu`` (fp32, bf16 or fp16; ids int32 or int64),
-CPU tensors PyTorch.  The autograd entry point is ``functional.embedding``.
+CPU tensors PyTorch (fp64 in fp64).  The autograd entry point is ``functional.embedding``.
 
 The reference looks rows up with ``F.embedding`` and masks the ids of other shards
 (femtotron/parallel/tensor_parallel/embedding.py:57-77).
@@ -24,6 +24,11 @@ def _local(ids: torch.Tensor, words: int, vstart: int):
     return local, has
 
 
+def _wide(*types: torch.dtype) -> torch.dtype:
+    """What CPU tensors are computed in: fp32 for narrower types."""
+    return torch.float64 if torch.float64 in types else torch.float32
+
+
 def lookup(ids: torch.Tensor, table: torch.Tensor, vstart: int = 0, scale: float = 1.0) -> torch.Tensor:
     """Rows of ``table`` [words, values] times ``scale``, in its type."""
     if table.is_cuda:
@@ -31,7 +36,7 @@ def lookup(ids: torch.Tensor, table: torch.Tensor, vstart: int = 0, scale: float
     local, has = _local(ids, table.shape[0], vstart)
     out = torch.zeros(local.numel(), table.shape[1], dtype=table.dtype)
     rows = table[local[has]]
-    out[has] = rows if scale == 1.0 else (rows.float() * scale).to(table.dtype)
+    out[has] = rows if scale == 1.0 else (rows.to(_wide(table.dtype)) * scale).to(table.dtype)
     return out.view(*ids.shape, table.shape[1])
 
 
@@ -44,7 +49,7 @@ def sorted_grad(ids: torch.Tensor, dout: torch.Tensor, dst: torch.Tensor, accumu
         LAUNCHES[0] += n - 1
         return
     local, has = _local(ids, dst.shape[0], vstart)
-    g = torch.zeros(dst.shape, dtype=torch.float32)
-    g.index_add_(0, local[has], dout[has].float())
+    g = torch.zeros(dst.shape, dtype=_wide(dst.dtype, dout.dtype))
+    g.index_add_(0, local[has], dout[has].to(g.dtype))
     g = g if scale == 1.0 else g * scale
-    dst.copy_(dst.float() + g if accumulate else g)
+    dst.copy_(dst.to(g.dtype) + g if accumulate else g)

@@ -19,7 +19,7 @@ all three).  On CUDA it runs ``csrc/masked_attn*.cu`` on bf16
 tensors of any strides with a head size that is a multiple of 8 up to 128 (one that TMA does not
 take is copied first); its results and gradients are the same bits every time.  Beside the rows
 that see it, a NaN or an infinity of a token that is no padding may reach the rows of the 128-row tiles
-that it lies in or is seen from.  CPU tensors run the formulas in PyTorch.
+that it lies in or is seen from.  CPU tensors run the formulas in PyTorch (fp64 in fp64).
 
 The reference has causal attention only, inside Hugging Face's layer
 (femtotron/model/llama_partial_model.py:143-157).
@@ -149,7 +149,8 @@ def _forward_cpu(q, k, v, mask, scale, softcap, slopes):
     nkv = k.shape[2]
     vis = _visible(mask)[:, None]
     dead = mask.rows[:, :S, 1] == 0
-    qf, kf, vf = (x.float().masked_fill(dead[:, :, None, None], 0.0).transpose(1, 2) for x in (q, k, v))
+    wide = torch.promote_types(q.dtype, torch.float32)
+    qf, kf, vf = (x.to(wide).masked_fill(dead[:, :, None, None], 0.0).transpose(1, 2) for x in (q, k, v))
     kf, vf = kf.repeat_interleave(nq // nkv, 1), vf.repeat_interleave(nq // nkv, 1)
     x = qf @ kf.transpose(-1, -2) * scale
     keep = None
@@ -158,7 +159,7 @@ def _forward_cpu(q, k, v, mask, scale, softcap, slopes):
         x, keep = softcap * t, 1 - t * t
     if slopes is not None:
         i = torch.arange(S)
-        x = x - slopes.float().view(1, nq, 1, 1) * (i[:, None] - i).abs()
+        x = x - slopes.to(wide).view(1, nq, 1, 1) * (i[:, None] - i).abs()
     x = x.masked_fill(~vis, float("-inf"))
     lse = torch.logsumexp(x, -1)
     p = torch.where(vis, torch.exp(x - lse[..., None]), torch.zeros_like(x))
@@ -225,7 +226,7 @@ def _backward(q, k, v, o, low, do, lse, rows, tiles, order, slopes, meta, dq, dk
     B, S, nq, d = q.shape
     nkv = k.shape[2]
     qf, kf, vf, keep, _, p = _forward_cpu(q, k, v, mask, scale, softcap, slopes)
-    g = do.float().masked_fill((rows[:, :S, 1] == 0)[:, :, None, None], 0.0).transpose(1, 2)
+    g = do.to(p.dtype).masked_fill((rows[:, :S, 1] == 0)[:, :, None, None], 0.0).transpose(1, 2)
     dp = g @ vf.transpose(-1, -2)
     ds = p * (dp - (p * dp).sum(-1, keepdim=True))
     if keep is not None:

@@ -18,17 +18,11 @@ void xent_stats(const torch::Tensor& logits, const torch::Tensor& labels, torch:
                 int64_t vstart);
 void xent_bwd(torch::Tensor& logits, const torch::Tensor& labels, const torch::Tensor& lse,
               const torch::Tensor& grad_scale, int64_t vstart, int64_t ignore_index);
-void embed_fwd(const torch::Tensor& ids, const torch::Tensor& table, torch::Tensor& out,
-               int64_t vstart);
-void embed_bwd(const torch::Tensor& ids, const torch::Tensor& dout, torch::Tensor& dtable,
-               int64_t vstart);
 void adamw_multi(const std::vector<torch::Tensor>& params, const std::vector<torch::Tensor>& ms,
                  const std::vector<torch::Tensor>& vs, const std::vector<torch::Tensor>& grads,
                  const std::vector<torch::Tensor>& p16s, const std::vector<double>& wds,
                  double lr, double beta1, double beta2, double eps, int64_t step,
                  const c10::optional<torch::Tensor>& grad_scale);
-void sumsq_multi(const std::vector<torch::Tensor>& xs, const std::vector<int64_t>& slots,
-                 torch::Tensor& out);
 torch::Tensor symm_alloc(int64_t nbytes, int64_t device);
 torch::Tensor ipc_handle(const torch::Tensor& t);
 int64_t ipc_open(const torch::Tensor& handle, int64_t device);
@@ -133,10 +127,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("swiglu_bwd", &ft::swiglu_bwd);
   m.def("xent_stats", &ft::xent_stats);
   m.def("xent_bwd", &ft::xent_bwd);
-  m.def("embed_fwd", &ft::embed_fwd);
-  m.def("embed_bwd", &ft::embed_bwd);
   m.def("adamw_multi", &ft::adamw_multi);
-  m.def("sumsq_multi", &ft::sumsq_multi);
   m.def("symm_alloc", &ft::symm_alloc);
   m.def("ipc_handle", &ft::ipc_handle);
   m.def("ipc_open", &ft::ipc_open);

@@ -267,15 +267,6 @@ __global__ void __launch_bounds__(SMALL_NT) small_sort_kernel(const SortArgs a) 
 }
 
 // ------------------------------------------------------------------------------ sums
-template <typename T, int VEC>
-struct Row {
-  float v[VEC];
-  __device__ __forceinline__ void zero() {
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) v[k] = 0.f;
-  }
-};
-
 template <typename D, int VEC>
 __device__ __forceinline__ void put(D* d, const float (&v)[VEC], float scale, bool add) {
 #pragma unroll

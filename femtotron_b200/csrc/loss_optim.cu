@@ -1,9 +1,8 @@
 // sm_100a kernels for the model boundaries and the optimizer:
 //   * vocab-parallel cross-entropy (per-row max / sum-exp / target-logit partials, and the
 //     in-place logits -> dlogits backward), so full-vocab logits are never gathered;
-//   * vocab-parallel embedding lookup and its scatter-add backward;
 //   * multi-tensor AdamW (fp32 master, m, v; bf16 or fp32 gradient; optional bf16 param
-//     write-back) and multi-tensor sum of squares for gradient-norm clipping.
+//     write-back).
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -112,42 +111,6 @@ __global__ void __launch_bounds__(NT) xent_bwd_kernel(__nv_bfloat16* __restrict_
   }
 }
 
-// ---------------------------------------------------------------- embedding
-__global__ void embed_fwd_kernel(const int64_t* __restrict__ ids, const __nv_bfloat16* __restrict__ table,
-                                 __nv_bfloat16* __restrict__ out, int64_t T, int H, int64_t vstart,
-                                 int64_t V) {
-  const int vpr = H / 8;
-  const int64_t total = T * vpr;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total;
-       i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t t = i / vpr;
-    const int c = (i % vpr) * 8;
-    const int64_t id = ids[t] - vstart;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (id >= 0 && id < V) v = *reinterpret_cast<const uint4*>(table + id * H + c);
-    *reinterpret_cast<uint4*>(out + t * H + c) = v;
-  }
-}
-
-__global__ void embed_bwd_kernel(const int64_t* __restrict__ ids, const __nv_bfloat16* __restrict__ dout,
-                                 float* __restrict__ dtable, int64_t T, int H, int64_t vstart,
-                                 int64_t V) {
-  const int vpr = H / 8;
-  const int64_t total = T * vpr;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total;
-       i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t t = i / vpr;
-    const int c = (i % vpr) * 8;
-    const int64_t id = ids[t] - vstart;
-    if (id < 0 || id >= V) continue;
-    float v[8];
-    load8(dout + t * H + c, v);
-    float* d = dtable + id * H + c;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) atomicAdd(d + j, v[j]);
-  }
-}
-
 // ---------------------------------------------------------------- multi-tensor AdamW
 struct AdamSeg {
   float* p;             // fp32 master
@@ -231,45 +194,6 @@ __global__ void __launch_bounds__(256) adamw_kernel(const AdamSeg* __restrict__ 
   }
 }
 
-struct SqSeg {
-  const void* x;
-  int64_t n;
-  int f32;
-  int out_slot;
-};
-
-// Sum of squares per output slot (fp32 atomics into out[slot]).
-__global__ void sumsq_kernel(const SqSeg* __restrict__ segs, const int2* __restrict__ chunks,
-                             const int64_t* __restrict__ chunk_start, float* __restrict__ out,
-                             int chunk_len) {
-  const int2 ch = chunks[blockIdx.x];
-  const SqSeg s = segs[ch.x];
-  const int64_t start = chunk_start[blockIdx.x];
-  const int64_t end = min(s.n, start + chunk_len);
-  float acc = 0.f;
-  for (int64_t i = start + threadIdx.x; i < end; i += blockDim.x) {
-    const float g = s.f32 ? reinterpret_cast<const float*>(s.x)[i]
-                          : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(s.x)[i]);
-    acc += g * g;
-  }
-  acc = warp_sum(acc);
-  __shared__ float red[32];
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = acc;
-  __syncthreads();
-  if (threadIdx.x < 32) {
-    float r = threadIdx.x < blockDim.x / 32 ? red[threadIdx.x] : 0.f;
-    r = warp_sum(r);
-    if (threadIdx.x == 0) atomicAdd(out + s.out_slot, r);
-  }
-}
-
-int sm_count() {
-  int dev, sms;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return sms;
-}
-
 }  // namespace
 
 // ------------------------------------------------------------------ host entry points
@@ -299,39 +223,6 @@ void xent_bwd(torch::Tensor& logits, const torch::Tensor& labels, const torch::T
       reinterpret_cast<__nv_bfloat16*>(logits.data_ptr()), labels.data_ptr<int64_t>(),
       lse.data_ptr<float>(), grad_scale.data_ptr<float>(), V, logits.stride(0), vstart,
       ignore_index);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
-}
-
-void embed_fwd(const torch::Tensor& ids, const torch::Tensor& table, torch::Tensor& out,
-               int64_t vstart) {
-  TORCH_CHECK(ids.scalar_type() == at::kLong && ids.is_contiguous());
-  TORCH_CHECK(table.scalar_type() == at::kBFloat16 && table.is_contiguous() && out.is_contiguous());
-  const int64_t T = ids.numel();
-  const int H = table.size(1);
-  TORCH_CHECK(H % 8 == 0);
-  if (T == 0) return;
-  const c10::cuda::CUDAGuard g(ids.device());
-  const int64_t work = T * H / 8;
-  const int grid = static_cast<int>(std::min<int64_t>((work + 255) / 256, sm_count() * 16));
-  embed_fwd_kernel<<<grid, 256, 0, at::cuda::getCurrentCUDAStream()>>>(
-      ids.data_ptr<int64_t>(), reinterpret_cast<const __nv_bfloat16*>(table.data_ptr()),
-      reinterpret_cast<__nv_bfloat16*>(out.data_ptr()), T, H, vstart, table.size(0));
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
-}
-
-void embed_bwd(const torch::Tensor& ids, const torch::Tensor& dout, torch::Tensor& dtable,
-               int64_t vstart) {
-  TORCH_CHECK(dtable.scalar_type() == at::kFloat && dtable.is_contiguous());
-  TORCH_CHECK(dout.scalar_type() == at::kBFloat16 && dout.is_contiguous());
-  const int64_t T = ids.numel();
-  const int H = dtable.size(1);
-  if (T == 0) return;
-  const c10::cuda::CUDAGuard g(ids.device());
-  const int64_t work = T * H / 8;
-  const int grid = static_cast<int>(std::min<int64_t>((work + 255) / 256, sm_count() * 16));
-  embed_bwd_kernel<<<grid, 256, 0, at::cuda::getCurrentCUDAStream()>>>(
-      ids.data_ptr<int64_t>(), reinterpret_cast<const __nv_bfloat16*>(dout.data_ptr()),
-      dtable.data_ptr<float>(), T, H, vstart, dtable.size(0));
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
@@ -407,33 +298,6 @@ void adamw_multi(const std::vector<torch::Tensor>& params, const std::vector<tor
                           [&](const AdamSeg* s, const int2* c, const int64_t* o, int nc) {
                             adamw_kernel<<<nc, 256, 0, st>>>(s, c, o, h, gsp, CH);
                           });
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
-}
-
-// out[slot] += sum(x_i^2) for every tensor i assigned to `slot`.
-void sumsq_multi(const std::vector<torch::Tensor>& xs, const std::vector<int64_t>& slots,
-                 torch::Tensor& out) {
-  const size_t n = xs.size();
-  if (n == 0) return;
-  TORCH_CHECK(slots.size() == n && out.scalar_type() == at::kFloat);
-  std::vector<SqSeg> segs(n);
-  std::vector<int64_t> lens(n);
-  for (size_t i = 0; i < n; ++i) {
-    TORCH_CHECK(xs[i].is_contiguous());
-    segs[i].x = xs[i].data_ptr();
-    segs[i].n = xs[i].numel();
-    segs[i].f32 = xs[i].scalar_type() == at::kFloat ? 1 : 0;
-    segs[i].out_slot = static_cast<int>(slots[i]);
-    lens[i] = segs[i].n;
-  }
-  const c10::cuda::CUDAGuard g(xs[0].device());
-  auto st = at::cuda::getCurrentCUDAStream();
-  constexpr int CH = 1 << 16;
-  float* op = out.data_ptr<float>();
-  launch_chunked<SqSeg>(segs, lens, CH, xs[0].device(),
-                        [&](const SqSeg* s, const int2* c, const int64_t* o, int nc) {
-                          sumsq_kernel<<<nc, 512, 0, st>>>(s, c, o, op, CH);
-                        });
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 

@@ -14,7 +14,9 @@ from __future__ import annotations
 import torch
 import torch.nn.functional as F
 
+from . import embedding as E
 from .ext import native
+from .grad_norm import MAX_SLOTS, sum_of_squares
 
 
 # ------------------------------------------------------------------------------ RMSNorm
@@ -111,30 +113,14 @@ def swiglu_bwd(dh: torch.Tensor, gu: torch.Tensor, F_: int, out: torch.Tensor | 
 
 # ------------------------------------------------------------------------------ embedding
 def embed_fwd(ids: torch.Tensor, table: torch.Tensor, vstart: int) -> torch.Tensor:
-    flat = ids.reshape(-1)
-    if ids.is_cuda:
-        out = torch.empty(flat.numel(), table.shape[1], dtype=table.dtype, device=ids.device)
-        native().embed_fwd(flat.contiguous(), table, out, int(vstart))
-        return out.view(*ids.shape, table.shape[1])
-    local = flat - vstart
-    mask = (local < 0) | (local >= table.shape[0])
-    out = F.embedding(local.masked_fill(mask, 0), table)
-    out = out.masked_fill(mask[:, None], 0)
-    return out.view(*ids.shape, table.shape[1])
+    """``embedding.lookup`` without a factor."""
+    return E.lookup(ids, table, vstart)
 
 
 def embed_bwd(ids: torch.Tensor, dout: torch.Tensor, vocab_local: int, vstart: int) -> torch.Tensor:
     """Returns the fp32 table gradient [vocab_local, H]."""
-    H = dout.shape[-1]
-    flat = ids.reshape(-1)
-    d2 = dout.reshape(-1, H)
-    dtable = torch.zeros(vocab_local, H, dtype=torch.float32, device=dout.device)
-    if dout.is_cuda:
-        native().embed_bwd(flat.contiguous(), d2.contiguous(), dtable, int(vstart))
-        return dtable
-    local = flat - vstart
-    mask = (local >= 0) & (local < vocab_local)
-    dtable.index_add_(0, local[mask], d2[mask].float())
+    dtable = torch.empty(vocab_local, dout.shape[-1], dtype=torch.float32, device=dout.device)
+    E.sorted_grad(ids, dout, dtable, False, vstart)
     return dtable
 
 
@@ -205,11 +191,9 @@ def adamw_multi(params, exp_avgs, exp_avg_sqs, grads, bf16_out, weight_decays, *
 
 def sumsq_multi(tensors, slots, out: torch.Tensor) -> torch.Tensor:
     """out[slot] += sum(t^2) for each tensor t with its slot."""
-    if not tensors:
-        return out
-    if out.is_cuda:
-        native().sumsq_multi([t.contiguous() for t in tensors], [int(s) for s in slots], out)
-        return out
-    for t, s in zip(tensors, slots):
-        out[s] += t.float().pow(2).sum()
+    for s0 in range(0, out.numel() if tensors else 0, MAX_SLOTS):
+        here = [(t, s - s0) for t, s in zip(tensors, slots) if s0 <= s < s0 + MAX_SLOTS]
+        if here:
+            n = min(MAX_SLOTS, out.numel() - s0)
+            out[s0:s0 + n] += sum_of_squares(*zip(*here), n).to(out.dtype)
     return out

@@ -58,3 +58,12 @@ def test_gpu_strided_outputs_that_share_memory_are_refused():
         with pytest.raises(RuntimeError, match="share"):
             GN.scale_grads([torch.ones_like(x) for x in pair], coef_of(base), out=pair)
         assert torch.equal(base, keep)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_sums_of_squares_of_more_slots_than_a_launch_has(device):
+    from femtotron_b200.ops import kernels as K
+    out = torch.ones(11, device=device)
+    K.sumsq_multi([torch.ones(3, device=device), torch.ones(4, 2, device=device).t(), torch.ones(5, device=device).bfloat16()], [0, 9, 9], out)
+    assert out.tolist() == [4, 1, 1, 1, 1, 1, 1, 1, 1, 14, 1]
+    assert K.sumsq_multi([], [], out) is out

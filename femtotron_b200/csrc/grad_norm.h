@@ -15,7 +15,7 @@
 namespace ft {
 namespace gn {
 
-constexpr int MAX_TENSORS = 1024;  // 29 bytes of parameters each, of the 32764 that a launch has
+constexpr int MAX_TENSORS = 1024;  // 30 bytes of parameters each, of the 32764 that a launch has
 constexpr int CHUNK = 8192;        // values
 constexpr int MAX_SLOTS = 8;
 enum Type : uint8_t { F32 = 0, BF16 = 1, F16 = 2 };
@@ -44,6 +44,7 @@ struct Factor {
   float* norm;             // then the norm is written here
   bool in_place;           // a factor of 1 leaves everything as it is
 };
+static_assert(sizeof(Table<MAX_TENSORS>) + sizeof(Factor) <= 32764, "parameters of a launch");
 template <int N>
 cudaError_t launch_scale(const Table<N>& t, const Factor& f, cudaStream_t st);
 

@@ -365,15 +365,16 @@ FT_DEVICE float2 unpack_bf16x2(uint32_t v) {
 
 // Raise a kernel's dynamic shared-memory limit once per device: the attribute belongs to the
 // device's context, so a process that drives several GPUs must set it on each.  `done` is one
-// bit per device ordinal (a static of the caller, one per kernel instance).
+// bit per device ordinal (a static of the caller, one per kernel instance; host threads of several
+// devices share it).
 template <typename Kernel>
 inline void smem_attr_once(Kernel kernel, int bytes, unsigned long long& done) {
   int dev = 0;
   cudaGetDevice(&dev);
   const unsigned long long bit = 1ull << (dev & 63);
-  if (!(done & bit)) {
+  if (!(__atomic_load_n(&done, __ATOMIC_ACQUIRE) & bit)) {
     cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    done |= bit;
+    __atomic_fetch_or(&done, bit, __ATOMIC_RELEASE);
   }
 }
 

@@ -4,6 +4,7 @@
 
 #include <algorithm>
 
+#include "common.cuh"
 #include "embedding.h"
 
 namespace ft {
@@ -434,13 +435,8 @@ cudaError_t launch_clear(void* x, int64_t bytes, bool beside_sort, cudaStream_t 
 }
 
 cudaError_t launch_small_sort(const SortArgs& a, cudaStream_t st) {
-  int dev = 0;
-  static unsigned long long done = 0;  // one bit per device
-  cudaGetDevice(&dev);
-  if (!(done >> (dev & 63) & 1)) {
-    cudaFuncSetAttribute(small_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(SmallSort));
-    done |= 1ull << (dev & 63);
-  }
+  static unsigned long long done = 0;
+  smem_attr_once(small_sort_kernel, sizeof(SmallSort), done);
   small_sort_kernel<<<1, SMALL_NT, sizeof(SmallSort), st>>>(a);
   return cudaGetLastError();
 }

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from femtotron_b200.ops import masked_attention as MA
-from test_masked_attention import U16, make, reference, run
+from test_masked_attention import U16, check_gpu, make, mask_parts, reference, run
 
 pytestmark = pytest.mark.gpu
 
@@ -83,3 +83,36 @@ def test_row_sums_of_more_than_two_to_the_30_rows():
         assert ((x - y).abs() <= (2 * U16 + 2 ** -14) * z + U16 * y.abs()).all(), first
     del q, k, v, do, o, dq
     torch.cuda.empty_cache()
+
+
+SCORES = [(3.0, False), (0.0, True), (20.0, True)]
+
+
+@pytest.mark.parametrize("softcap,bias", SCORES)
+@pytest.mark.parametrize("kind", ["causal", "all", "docs both ways", "full"])
+@pytest.mark.parametrize("nq,nkv,d", [(6, 2, 64), (12, 2, 80), (8, 1, 128)])
+def test_scores_of_grouped_heads(nq, nkv, d, kind, softcap, bias):
+    check_gpu(2, 333, nq, nkv, d, kind, softcap=softcap, bias=bias, spread=2.0)
+
+
+@pytest.mark.parametrize("softcap,bias", SCORES)
+@pytest.mark.parametrize("kind", ["padded", "window", "docs both ways", "full"])
+@pytest.mark.parametrize("S,nq,nkv,d", [(2100, 8, 1, 64), (1500, 6, 1, 40), (700, 12, 2, 128)])
+def test_scores_where_blocks_share_a_group(S, nq, nkv, d, kind, softcap, bias):
+    # few key tiles: dk and dv of a key head come from several blocks and are joined
+    check_gpu(1, S, nq, nkv, d, kind, softcap=softcap, bias=bias)
+
+
+@pytest.mark.parametrize("softcap,bias", [(0.0, False), *SCORES])
+@pytest.mark.parametrize("kind", ["padded", "full"])
+@pytest.mark.parametrize("S,nq,nkv,d", [(300, 4, 2, 64), (1500, 6, 1, 40)])
+def test_packed_projections_have_the_same_bits(S, nq, nkv, d, kind, softcap, bias):
+    B = 2
+    q, k, v, do = make(B, S, nq, nkv, d, 8, "cuda", torch.bfloat16)
+    mask = MA.attention_mask(B, S, device="cuda", **{n: x.cuda() if torch.is_tensor(x) else x for n, x in mask_parts(kind, B, S, 5).items()})
+    kw = dict(softcap=softcap, slopes=MA.alibi_slopes(nq, "cuda") if bias else None)
+    want = run(q, k, v, do, mask, **kw)
+    qkv = torch.cat([q, k, v], 2).requires_grad_()
+    o = MA.masked_attention_packed(qkv, nq, nkv, mask, **kw)
+    o.backward(do)
+    assert torch.equal(o, want[0]) and torch.equal(qkv.grad, torch.cat(want[1:], 2))

@@ -9,6 +9,7 @@ from safetensors.torch import load_file
 from femtotron_b200.models import LlamaForTraining
 from femtotron_b200.models.export import export_hf
 from femtotron_b200.models.layer_factory import DefaultLayerFactory
+from femtotron_b200.models.layers import Attention
 from femtotron_b200.models.parallel_plan import ParallelRule
 from femtotron_b200.ops import masked_attention as MA
 from femtotron_b200.parallel.tensor_parallel import VocabParallelEmbedding
@@ -101,6 +102,26 @@ def test_slopes_are_made_once(base, monkeypatch):
     assert len(made) == 1 and set(model.state_dict()) == set(sd)
 
 
+@pytest.mark.parametrize("bits", [8, 16])
+def test_layer_checkpoints_keep_the_mask(base, monkeypatch, bits):
+    sd, ids, _ = base
+    docs = torch.zeros(2, 48, dtype=torch.int32)
+    docs[0, 30:] = -1
+    docs[1, 20:] = 1
+    seen = []
+    call = Attention.__call__
+    monkeypatch.setattr(Attention, "__call__", lambda self, *a: seen.append(self) or call(self, *a))
+    cfg = config(attn_spec={"window": 9, "softcap": 5.0, "alibi": True}, embed_scale=4.0)
+    want = run(cfg, sd, ids, docs=docs)
+    del seen[:]
+    got = run(cfg, sd, ids, bits=bits, docs=docs)
+    assert len(seen) == 2 * cfg.num_hidden_layers and len(set(map(id, seen))) == 1  # forward and again for the backward pass
+    assert got[0] == want[0] and torch.equal(got[1], want[1])
+    for k, g in want[2].items():
+        # 8 bits round a value by 2^-8 of its group's largest at most; two layers of six products pass that on
+        assert float((got[2][k] - g).norm()) <= (12 * 2 ** -8 if bits == 8 else 1e-6) * float(g.norm()), k
+
+
 def checkpoint(path, model):
     path.mkdir()
     (path / "meta.json").write_text(json.dumps({"tp_size": 1, "dp_size": 1}))
@@ -179,3 +200,21 @@ def test_gpu_slopes_neither_wait_nor_stop_a_graph():
             graph.replay()
             assert torch.equal(out, want)
         assert torch.equal(model.model(ids), want)
+
+
+@gpu
+@pytest.mark.parametrize("spec", [{"alibi": True}, {"alibi": True, "separator": 0, "softcap": 20.0}])
+def test_gpu_model_with_a_bias_of_distance(spec):
+    cfg = config(num_attention_heads=6, num_key_value_heads=2, hidden_size=384, intermediate_size=512, embed_scale=4.0,
+                 attn_spec=spec)
+    sd = {k: v.bfloat16().float() for k, v in full_state(cfg).items()}
+    ids = torch.randint(0, 40, (2, 150), generator=torch.Generator().manual_seed(1))
+    loss, logits, grads = run(cfg, sd, ids)
+    model = LlamaForTraining(cfg, dtype=torch.bfloat16, device="cuda")
+    model.load_state_dict(sd)
+    got = graded(model, ids.cuda())
+    # some thirty roundings of 2^-9 of two layers and the head forward, twice as many again backward
+    assert abs(got[0] - loss) < 0.02 * loss
+    assert float((got[1].float().cpu() - logits).norm() / logits.norm()) < 30 ** 0.5 * 2 ** -8
+    for k, g in grads.items():
+        assert float((got[2][k].float().cpu() - g).norm() / g.norm()) < 90 ** 0.5 * 2 ** -8, k

@@ -34,10 +34,11 @@ def lookup(ids: torch.Tensor, table: torch.Tensor, vstart: int = 0, scale: float
     if table.is_cuda:
         return native().embed_lookup(ids, table, int(vstart), float(scale))
     local, has = _local(ids, table.shape[0], vstart)
-    out = torch.zeros(local.numel(), table.shape[1], dtype=table.dtype)
-    rows = table[local[has]]
-    out[has] = rows if scale == 1.0 else (rows.to(_wide(table.dtype)) * scale).to(table.dtype)
-    return out.view(*ids.shape, table.shape[1])
+    if table.shape[0] == 0:
+        return table.new_zeros(*ids.shape, table.shape[1])
+    rows = table[local.masked_fill(~has, 0)]  # nothing here depends on the ids' values: tensors without data pass too
+    rows = rows if scale == 1.0 else (rows.to(_wide(table.dtype)) * scale).to(table.dtype)
+    return rows.masked_fill(~has[:, None], 0).view(*ids.shape, table.shape[1])
 
 
 def sorted_grad(ids: torch.Tensor, dout: torch.Tensor, dst: torch.Tensor, accumulate: bool, vstart: int = 0,

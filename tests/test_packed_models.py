@@ -122,6 +122,18 @@ def test_layer_checkpoints_keep_the_mask(base, monkeypatch, bits):
         assert float((got[2][k] - g).norm()) <= (12 * 2 ** -8 if bits == 8 else 1e-6) * float(g.norm()), k
 
 
+def test_shapes_without_data():
+    from femtotron_b200.ops import embedding as E
+    with torch.device("meta"):
+        emb = VocabParallelEmbedding(10, 4, OneRank(), dtype=torch.float32)
+        emb.scale = 3.0
+        assert emb(torch.zeros(2, 3, dtype=torch.long)).shape == (2, 3, 4)
+    # ids of other shards, a shard without words, and a table whose first row is no number
+    w = torch.tensor([[float("nan")], [2.0]])
+    assert E.lookup(torch.tensor([5, -1, 8, 6]), w, 5, 2.0)[1:].flatten().tolist() == [0.0, 0.0, 4.0]
+    assert E.lookup(torch.tensor([[5], [6]]), torch.empty(0, 7), 0).tolist() == [[[0.0] * 7]] * 2
+
+
 def checkpoint(path, model):
     path.mkdir()
     (path / "meta.json").write_text(json.dumps({"tp_size": 1, "dp_size": 1}))

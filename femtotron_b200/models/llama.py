@@ -38,7 +38,8 @@ class LlamaForTraining(nn.Module):
                 materialize_logits: bool | None = None, docs: torch.Tensor | None = None,
                 prefix: torch.Tensor | None = None) -> dict:
         """``docs`` and ``prefix``: see ``LlamaPartialModel.forward``."""
-        hidden = self.model(input_ids, docs=docs, prefix=prefix)
+        # a backbone of a user's own need not know documents where none are given
+        hidden = self.model(input_ids, **{k: v for k, v in (("docs", docs), ("prefix", prefix)) if v is not None})
         out: dict = {}
         if labels is not None:
             out["loss"] = lm_head_loss(self.lm_head, hidden, labels,

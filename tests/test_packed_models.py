@@ -134,6 +134,25 @@ def test_shapes_without_data():
     assert E.lookup(torch.tensor([[5], [6]]), torch.empty(0, 7), 0).tolist() == [[[0.0] * 7]] * 2
 
 
+def test_a_backbone_that_knows_no_documents(base):
+    sd, ids, want = base
+
+    class Backbone(torch.nn.Module):
+        def __init__(self, inner):
+            super().__init__()
+            self.inner = inner
+
+        def forward(self, input_ids):
+            return self.inner(input_ids)
+    model = LlamaForTraining(config(), dtype=torch.float32)
+    model.load_state_dict(sd)
+    model.model = Backbone(model.model)
+    with torch.no_grad():
+        assert torch.equal(model(ids)["logits"], want[1])
+        with pytest.raises(TypeError, match="docs"):
+            model(ids, docs=torch.zeros_like(ids))
+
+
 def checkpoint(path, model):
     path.mkdir()
     (path / "meta.json").write_text(json.dumps({"tp_size": 1, "dp_size": 1}))

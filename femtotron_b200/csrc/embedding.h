@@ -5,8 +5,10 @@
 // The tokens are sorted by id (stable, so equal ids stay in the order of the batch), the sorted list is cut
 // into pieces of 32, and each piece adds up its rows of dout run by run in registers.  A run inside one
 // piece goes straight to dw; one that crosses pieces leaves a partial sum per piece, and a second kernel adds
-// those up in order.  So a frequent word costs no more than a rare one, there are no atomics on values, and
-// the sum's order depends on the ids alone.
+// those up in order.  There are no atomics on values, and the sum's order depends on the ids alone.  The rows of
+// a frequent word are added by as many blocks as it has pieces, its partial sums one after the other by one: 32768 tokens added to
+// 128256 x 4096 take 251 us with words drawn evenly, 751 with one word in 90 % of the places, 783 with one in all (8192: 104, 169, 159;
+// a scatter of atomics on values: 770, 2552, 2765; 198, 646, 697).
 #pragma once
 
 #include <cuda_runtime.h>

@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(MASK_THREADS) mask_kernel(const MaskArgs a) {
 // the probabilities go over the first half of their S as bf16 pairs.  S of step j + 2 is issued behind the product of step j,
 // so one S waits while the other is worked on.  Keys leave their place with their S, values with their product: two of each do.
 // Measured (32 heads over 8, d = 128, us; in brackets one block per SM with two query tiles that shared the keys): 8192 tokens
-// in documents 159 (171), 2 x 4096 with windows of 1024 and a cap 226 (241), 16384 tokens with 8 heads over 1 448 (497), 0.75
+// in documents 159 (171), 2 x 4096 with windows of 1024 and a cap 221 (241), 16384 tokens with 8 heads over 1 448 (497), 0.75
 // of the GEMM rate.  What bounds it: the softmax's instructions, 880 clocks per step and tile at 642 of products.  There, 128
 // keys per step in halves, all waits before the products and the first keys before the block has met had been slower.
 constexpr int FWD_THREADS = 192, FWD_PRODUCER = 4, FWD_MMA = 5;

@@ -12,7 +12,8 @@ namespace ma {
 // with one buffer of 128 queries the two took turns (3320 clocks per 128 x 128 block).
 // Measured (32 heads over 8, d = 128): 8192 tokens in documents 224 us, 16384 tokens with 8 heads over 1 in 831 us (four products:
 // 0.80 of the GEMM rate).  Bound by the reads of shared memory of products with 64 columns.  10 warps on four schedulers leave 168
-// registers each; 144 are used, 167 with a cap (dp - delta before the exponentials; after them the loop spilled).
+// registers each; 146 are used, all with a cap (dp - delta before the exponentials; after
+// them the loop spilled, now only where both forms of the cap are worked out).
 constexpr int Q_STAGES = 4;
 
 struct DkvSmem {

@@ -4,8 +4,9 @@
     dw[v] = scale sum over id_t = vstart + v of dout_t
 
 The gradient's sums run over the tokens in the order of the batch, in fp32, cut where the sorted list
-of tokens is cut into pieces of 32: no atomics, the same bits every time, and a frequent word takes no
-longer than rare ones.  CUDA tensors run ``csrc/embedding.cu`` (fp32, bf16 or fp16; ids int32 or int64),
+of tokens is cut into pieces of 32: no atomics, the same bits every time.  A word's pieces are summed beside one
+another and joined one after the other, so a batch that is mostly one word takes longer (32768 tokens: three times as
+long).  CUDA tensors run ``csrc/embedding.cu`` (fp32, bf16 or fp16; ids int32 or int64),
 CPU tensors PyTorch (fp64 in fp64).  The autograd entry point is ``functional.embedding``.
 
 The reference looks rows up with ``F.embedding`` and masks the ids of other shards

@@ -15,12 +15,13 @@
   window     keys less than ``window`` tokens away
 
 ``masked_attention`` is differentiable in q, k and v (``masked_attention_packed`` in one projection that holds
-all three).  On CUDA it runs ``csrc/masked_attn*.cu`` on bf16 tensors of any strides with a head size that is a
-multiple of 8 up to 128 (one that TMA does not take is copied first); its results and gradients are the same bits
-every time, whatever stands in the places that a row does not see.  Only a NaN or an infinity of a token that
-is no padding may reach, beside the rows that see it, the rows of the 128-row tiles that it lies in or is seen from.  Between forward and backward pass it keeps q, k, v, o, what o's
-rounding to bf16 left out (as large as o) and 4 bytes per row and head.  CPU tensors run the formulas in
-PyTorch (fp64 in fp64), where such a NaN may reach any row of its sequence.
+all three).  On CUDA it runs ``csrc/masked_attn*.cu`` on bf16 tensors of any strides with a head size that is
+a multiple of 8 up to 128 (one that TMA does not take is copied first); its results and gradients are the same
+bits every time, whatever stands in the places that a row does not see.  Only a NaN or an infinity of a token
+that is no padding may reach, beside the rows that see it, the rows of the 128-row tiles that it lies in or is
+seen from.  Between forward and backward pass it keeps q, k, v, o, what o's rounding to bf16 left out (as large
+as o) and 4 bytes per row and head.  CPU tensors run the formulas in PyTorch (fp64 in fp64), where such a NaN may
+reach any row of its sequence.
 
 The reference has causal attention only, inside Hugging Face's layer
 (femtotron/model/llama_partial_model.py:143-157).

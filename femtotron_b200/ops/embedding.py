@@ -44,11 +44,16 @@ def lookup(ids: torch.Tensor, table: torch.Tensor, vstart: int = 0, scale: float
 
 def sorted_grad(ids: torch.Tensor, dout: torch.Tensor, dst: torch.Tensor, accumulate: bool, vstart: int = 0,
                 scale: float = 1.0) -> None:
-    """Store the table's gradient in ``dst`` [words, values], or add it (fp32, bf16 or fp16, rounded once)."""
+    """Store the table's gradient in ``dst`` [words, values], or add it (contiguous fp32, bf16 or fp16: rounded once;
+    others by way of an fp32 copy)."""
     dout = dout.reshape(ids.numel(), dst.shape[1])
     if dst.is_cuda:
-        n = native().embed_sorted_grad(ids, dout, dst, accumulate, int(vstart), float(scale))
+        direct = dst.is_contiguous() and dst.dtype in (torch.float32, torch.bfloat16, torch.float16)
+        to = dst if direct else torch.empty(dst.shape, dtype=torch.float32, device=dst.device)
+        n = native().embed_sorted_grad(ids, dout, to, accumulate and direct, int(vstart), float(scale))
         LAUNCHES[0] += n - 1
+        if not direct:  # a buffer of other strides or another type
+            dst.add_(to) if accumulate else dst.copy_(to)
         return
     local, has = _local(ids, dst.shape[0], vstart)
     g = torch.zeros(dst.shape, dtype=_wide(dst.dtype, dout.dtype))

@@ -153,6 +153,25 @@ def test_a_backbone_that_knows_no_documents(base):
             model(ids, docs=torch.zeros_like(ids))
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("kind", ["strided", "fp64"])
+def test_gradient_buffers_of_any_strides_and_type(device, kind):
+    from femtotron_b200.ops.functional import embedding
+    g = torch.Generator().manual_seed(0)
+    w, ids = torch.randn(9, 16, generator=g).bfloat16().to(device), torch.randint(0, 9, (40,), generator=g).to(device)
+    do = torch.randn(40, 16, generator=g).bfloat16().to(device)
+    want = torch.zeros(9, 16, dtype=torch.float64, device=device).index_add_(0, ids, do.double())
+    p = torch.nn.Parameter(w)
+    if kind == "strided":
+        p.grad = torch.zeros(16, 9, dtype=torch.bfloat16, device=device).t()
+    else:
+        p.main_grad = torch.zeros(9, 16, dtype=torch.float64, device=device)
+    got = p.grad if kind == "strided" else p.main_grad
+    for k in (1, 2):  # one rounding to bf16 of either sum; 2^-18: fp32 sums
+        embedding(ids, p).backward(do)
+        assert ((got - k * want).abs() <= (2 ** -8 * 2 * k * want.abs() if kind == "strided" else 0) + 2 ** -18 * 40 * 4).all()
+
+
 def checkpoint(path, model):
     path.mkdir()
     (path / "meta.json").write_text(json.dumps({"tp_size": 1, "dp_size": 1}))

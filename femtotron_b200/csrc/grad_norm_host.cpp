@@ -22,6 +22,8 @@ struct Item {
   uint8_t type, slot;
 };
 
+constexpr int SIZE[] = {4, 2, 2};  // bytes by Type
+
 uint8_t type_of(const char* op, const at::Tensor& x) {
   switch (x.scalar_type()) {
     case at::kFloat: return F32;
@@ -82,7 +84,7 @@ struct Tables {
 };
 
 // Memory of one call's outputs: no value may be written by two of them, nor read by another one.
-void check_apart(const char* op, const std::vector<Item>& items, const std::vector<int>& size) {
+void check_apart(const char* op, const std::vector<Item>& items) {
   struct Span {
     uintptr_t from, to;
     size_t who;
@@ -90,14 +92,14 @@ void check_apart(const char* op, const std::vector<Item>& items, const std::vect
   std::vector<Span> out;
   for (size_t i = 0; i < items.size(); ++i) {
     const uintptr_t p = reinterpret_cast<uintptr_t>(items[i].y);
-    out.push_back({p, p + items[i].n * size[items[i].type], i});
+    out.push_back({p, p + items[i].n * SIZE[items[i].type], i});
   }
   auto before = [](const Span& a, const Span& b) { return a.from < b.from; };
   if (!std::is_sorted(out.begin(), out.end(), before)) std::sort(out.begin(), out.end(), before);
   for (size_t i = 1; i < out.size(); ++i)
     TORCH_CHECK(out[i].from >= out[i - 1].to, op, ": two of the tensors written share memory");
   for (size_t i = 0; i < items.size(); ++i) {
-    const uintptr_t p = reinterpret_cast<uintptr_t>(items[i].x), e = p + items[i].n * size[items[i].type];
+    const uintptr_t p = reinterpret_cast<uintptr_t>(items[i].x), e = p + items[i].n * SIZE[items[i].type];
     auto at = std::upper_bound(out.begin(), out.end(), p, [](uintptr_t v, const Span& s) { return v < s.to; });
     for (; at != out.end() && at->from < e; ++at)
       TORCH_CHECK(at->who == i && at->from == p, op, ": a tensor written shares memory with one that is read");
@@ -110,7 +112,6 @@ at::Tensor dense(const at::Tensor& x) { return x.is_non_overlapping_and_dense() 
 struct Plan {
   std::vector<Item> items;
   std::vector<at::Tensor> held;                            // the copies
-  std::vector<at::Tensor> written;                         // by the kernel, of the caller's own
   std::vector<std::pair<at::Tensor, at::Tensor>> back;     // (to, from) once the kernel is done
   bool in_place;
 };
@@ -125,12 +126,10 @@ Plan plan_of(const char* op, const std::vector<at::Tensor>& xs, const std::vecto
     TORCH_CHECK_VALUE(o.sizes() == xs[i].sizes() && o.scalar_type() == xs[i].scalar_type() && o.device() == xs[0].device(), op,
                       ": an output of ", o.scalar_type(), " ", o.sizes(), " for ", xs[i].scalar_type(), " ", xs[i].sizes());
     if (xs[i].numel() == 0) continue;
-    at::assert_no_internal_overlap(o);
+    if (!o.is_non_overlapping_and_dense()) at::assert_no_internal_overlap(o);
     at::Tensor src = dense(xs[i]);
     at::Tensor dst = o.is_non_overlapping_and_dense() && o.strides() == src.strides() ? o : at::Tensor();
-    if (dst.defined()) {
-      p.written.push_back(o);
-    } else {
+    if (!dst.defined()) {
       dst = p.in_place ? src : at::empty_like(src);  // in place: src is a copy already
       p.back.emplace_back(o, dst);
     }
@@ -138,27 +137,24 @@ Plan plan_of(const char* op, const std::vector<at::Tensor>& xs, const std::vecto
     p.held.push_back(dst);
     p.items.push_back({src.data_ptr(), dst.data_ptr(), src.numel(), type_of(op, src), 0});
   }
-  check_apart(op, p.items, {4, 2, 2});
+  check_apart(op, p.items);
   // Written by a copy: as far as first addresses tell, as the columns of one matrix are no solid pieces but lie apart.
-  std::vector<std::pair<uintptr_t, uintptr_t>> solid;
-  for (const at::Tensor& x : p.written) {
-    const uintptr_t a = reinterpret_cast<uintptr_t>(x.data_ptr());
-    solid.emplace_back(a, a + x.nbytes());
-  }
-  for (const auto& [to, from] : p.back) {
-    const uintptr_t a = reinterpret_cast<uintptr_t>(to.data_ptr());
-    for (const auto& [begin, end] : solid)
-      TORCH_CHECK(a < begin || a >= end, op, ": two of the tensors written share memory");
-    solid.emplace_back(a, a + 1);
+  for (size_t i = 0; i < p.back.size(); ++i) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(p.back[i].first.data_ptr());
+    for (const Item& t : p.items) {
+      const uintptr_t y = reinterpret_cast<uintptr_t>(t.y);  // (or a copy's own memory, where no tensor of the caller's lies)
+      TORCH_CHECK(a < y || a >= y + t.n * SIZE[t.type], op, ": two of the tensors written share memory");
+    }
+    for (size_t k = 0; k < i; ++k)
+      TORCH_CHECK(a != reinterpret_cast<uintptr_t>(p.back[k].first.data_ptr()), op, ": two of the tensors written share memory");
   }
   return p;
 }
 
-// Once the kernels are launched: copies go back, and autograd learns (as from the copy) that what a kernel wrote itself has
-// changed.
-void finish(const Plan& p) {
+// Once the kernels are launched: copies go back, and autograd learns that what was written has changed.
+void finish(const Plan& p, const std::vector<at::Tensor>& written) {
   for (const auto& [to, from] : p.back) to.copy_(from);
-  for (const at::Tensor& x : p.written)
+  for (const at::Tensor& x : written)
     if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
 }
 
@@ -215,7 +211,7 @@ void grad_scale(const std::vector<at::Tensor>& xs, const at::Tensor& coef, const
   const Tables tables(p.items);
   const Factor f{coef.data_ptr<float>(), nullptr, 0, 0.f, nullptr, p.in_place};
   tables.each([&](const auto& t) { C10_CUDA_CHECK(launch_scale(t, f, st)); });
-  finish(p);
+  finish(p, outs.empty() ? xs : outs);
 }
 
 at::Tensor grad_clip(const std::vector<at::Tensor>& xs, double max_norm, const std::vector<at::Tensor>& outs) {
@@ -231,7 +227,7 @@ at::Tensor grad_clip(const std::vector<at::Tensor>& xs, double max_norm, const s
   const Factor f{nullptr, part.data_ptr<double>(), static_cast<int>(part.size(0)), static_cast<float>(max_norm),
                  norm.data_ptr<float>(), p.in_place};
   tables.each([&](const auto& t) { C10_CUDA_CHECK(launch_scale(t, f, st)); });
-  finish(p);
+  finish(p, outs.empty() ? xs : outs);
   return norm;
 }
 
